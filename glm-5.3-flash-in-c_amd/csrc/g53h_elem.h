@@ -1,0 +1,107 @@
+/* g53h_elem.h - elements of the operators that take several types (G53H_F32, G53H_BF16, G53H_F16):
+ * eight of them at a time to and from fp32 registers. Addresses need the alignment of one element
+ * only: gfx950 loads and stores 16 bytes at any address, and rows of odd length start anywhere.
+ */
+#ifndef G53H_ELEM_H
+#define G53H_ELEM_H
+
+#include <hip/hip_runtime.h>
+
+#include "g53h.h"
+
+typedef __bf16 g53_bf16;
+typedef _Float16 g53_f16;
+typedef float g53_v4f __attribute__((ext_vector_type(4)));
+typedef unsigned int g53_v4w __attribute__((ext_vector_type(4)));
+typedef g53_bf16 g53_v8b __attribute__((ext_vector_type(8)));
+typedef g53_f16 g53_v8h __attribute__((ext_vector_type(8)));
+
+/* The same vectors at any 2-byte address. */
+struct __attribute__((packed, aligned(2))) G53v4w_any { g53_v4w v; };
+struct __attribute__((packed, aligned(2))) G53v8b_any { g53_v8b v; };
+struct __attribute__((packed, aligned(2))) G53v8h_any { g53_v8h v; };
+struct __attribute__((packed, aligned(4))) G53v4f_any { g53_v4f v; };
+
+/* Bytes of an element of type dt, 0 if dt is none of the types. */
+static inline int g53_elem_bytes(int dt) { return dt == G53H_F32 ? 4 : (dt == G53H_BF16 || dt == G53H_F16 ? 2 : 0); }
+
+__device__ __forceinline__ void g53_load8(float (&o)[8], const float *p)
+{
+    const g53_v4f a = ((const G53v4f_any *)p)[0].v, b = ((const G53v4f_any *)p)[1].v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) { o[i] = a[i]; o[4 + i] = b[i]; }
+}
+__device__ __forceinline__ void g53_load8(float (&o)[8], const g53_bf16 *p)
+{
+    const g53_v8b a = ((const G53v8b_any *)p)->v;
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = (float)a[i];
+}
+__device__ __forceinline__ void g53_load8(float (&o)[8], const g53_f16 *p)
+{
+    const g53_v8h a = ((const G53v8h_any *)p)->v;
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = (float)a[i];
+}
+/* Stores round to the nearest value of the type, ties to even: half a step each. */
+__device__ __forceinline__ void g53_store8(float *p, const float (&v)[8])
+{
+    g53_v4f a, b;
+#pragma unroll
+    for (int i = 0; i < 4; i++) { a[i] = v[i]; b[i] = v[4 + i]; }
+    ((G53v4f_any *)p)[0].v = a;
+    ((G53v4f_any *)p)[1].v = b;
+}
+__device__ __forceinline__ void g53_store8(g53_bf16 *p, const float (&v)[8])
+{
+    g53_v8b a;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a[i] = (g53_bf16)v[i];
+    ((G53v8b_any *)p)->v = a;
+}
+__device__ __forceinline__ void g53_store8(g53_f16 *p, const float (&v)[8])
+{
+    g53_v8h a;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a[i] = (g53_f16)v[i];
+    ((G53v8h_any *)p)->v = a;
+}
+
+/* Elements c .. c + 7 of a row of n, zeros behind its end. */
+template <typename T> __device__ __forceinline__ void g53_load8_to(float (&o)[8], const T *row, int c, int n)
+{
+    if (c + 8 <= n) {
+        g53_load8(o, row + c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = c + i < n ? (float)row[c + i] : 0.0f;
+    }
+}
+template <typename T> __device__ __forceinline__ void g53_store8_to(T *row, const float (&v)[8], int c, int n)
+{
+    if (c + 8 <= n) {
+        g53_store8(row + c, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (c + i < n) row[c + i] = (T)v[i];
+    }
+}
+
+/* The sum of v over the 64 lanes of a wave, in every lane. */
+__device__ __forceinline__ float g53_wave_sum(float v)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+/* Run a kernel template over the element type that dt names: BODY sees it as E. */
+#define G53_BY_TYPE(dt, BODY)                                             \
+    do {                                                                  \
+        if ((dt) == G53H_F32) { typedef float E; BODY; }                  \
+        else if ((dt) == G53H_BF16) { typedef g53_bf16 E; BODY; }         \
+        else { typedef g53_f16 E; BODY; }                                 \
+    } while (0)
+
+#endif /* G53H_ELEM_H */

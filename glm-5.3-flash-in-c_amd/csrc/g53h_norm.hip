@@ -1,0 +1,404 @@
+/* g53h_norm.hip - the norms before and after a block, fused with the block's gate and residual
+ * scale, and their gradients.
+ *
+ *     u  = y / sqrt(mean y^2 + eps) * post        (post NULL: u = y)
+ *     h' = h + scale * gate * u
+ *     xn = h' / sqrt(mean h'^2 + eps) * next
+ *
+ * and, with rs = 1 / sqrt(mean^2 + eps) and a hat for a value times its rs,
+ *
+ *     v  = dxn next,   dH = dh' + rs(h') (v - h'^ mean(v h'^)),   dnext = sum over tokens of dxn h'^
+ *     dh = dH,   dgate = scale u dH summed over what shares the gate
+ *     du = scale gate dH,   dpost = sum over tokens of du y^
+ *     dy = rs(y) (du post - y^ mean(du post y^))
+ *
+ * Both directions are one pass over HBM: W waves hold a token's row in registers, 8 elements a lane
+ * (16 for rows above 8192), sums go over the lanes and then the waves. The next norm takes h' in fp32,
+ * before it is rounded to be stored, and the backward pass forms the same fp32 h' again from h and y.
+ * Gradients that tokens share are summed by each workgroup over its tokens in registers, written once
+ * and added up by k_norm_sum in a fixed order: no atomics, the same bits on every run.
+ */
+#include <hip/hip_runtime.h>
+
+#include "g53h.h"
+#include "g53h_elem.h"
+#include "g53h_runtime.h"
+
+#define G53_NORM_MAXH 16384
+
+struct G53NormArgs {
+    const float *post, *next;
+    const void *gate;                   /* kind 1: float [H], 2: float [T], 3: E [T][H] */
+    void *dgate;                        /* kinds 2 and 3 */
+    float *part;                        /* partial sums [groups][3][H] of dpost, dnext, dgate (kind 1) */
+    float eps, scale;
+    int T, H;
+};
+
+/* The sum of v over the W waves of a row's group; buf: two floats a wave. Every lane gets it. */
+template <int W> __device__ __forceinline__ void g53_group_sum(float &a, float &b, float (*buf)[2], int wv)
+{
+    a = g53_wave_sum(a);
+    b = g53_wave_sum(b);
+    if (W > 1) {
+        if ((threadIdx.x & 63) == 0) { buf[wv][0] = a; buf[wv][1] = b; }
+        __syncthreads();
+        a = b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) { a += buf[wv / W * W + w][0]; b += buf[wv / W * W + w][1]; }
+    }
+}
+
+/* GK: the gate's kind; Y: there is a block output (else the norm of h alone). */
+template <typename E, int W, int NV, int GK, bool Y>
+__global__ void __launch_bounds__(W < 4 ? 256 : 64 * W)
+k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
+{
+    constexpr int NW = W < 4 ? 4 : W, RB = NW / W;
+    __shared__ float buf[2][NW][2];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    long t = (wg0 + blockIdx.x) * RB + wv / W;
+    const bool live = t < a.T;
+    if (!live) t = a.T - 1;             /* rows behind the last: computed, not written */
+    const int H = a.H, c0 = ((wv % W) * 64 + lane) * 8;
+    float hv[NV][8], s = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; v++) g53_load8_to(hv[v], h + t * H, c0 + v * 512 * W, H);
+    if (Y) {
+        float yv[NV][8];
+#pragma unroll
+        for (int v = 0; v < NV; v++) g53_load8_to(yv[v], y + t * H, c0 + v * 512 * W, H);
+        float rs = 1.0f;
+        if (a.post) {
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) s = __builtin_fmaf(yv[v][i], yv[v][i], s);
+            g53_group_sum<W>(s, s2, buf[0], wv);
+            rs = 1.0f / sqrtf(s / (float)H + a.eps);
+        }
+        const float gt = a.scale * (GK == 2 ? ((const float *)a.gate)[t] : 1.0f);
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int c = c0 + v * 512 * W;
+            float pv[8], gv[8];
+            if (a.post) g53_load8_to(pv, a.post, c, H);
+            if (GK == 1) g53_load8_to(gv, (const float *)a.gate, c, H);
+            if (GK == 3) g53_load8_to(gv, (const E *)a.gate + t * H, c, H);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float u = a.post ? yv[v][i] * rs * pv[i] : yv[v][i];
+                hv[v][i] = __builtin_fmaf((GK & 1) ? gt * gv[i] : gt, u, hv[v][i]);
+            }
+            if (live) g53_store8_to(h2 + t * H, hv[v], c, H);
+        }
+    }
+    if (!xn) return;
+    s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) s = __builtin_fmaf(hv[v][i], hv[v][i], s);
+    g53_group_sum<W>(s, s2, buf[1], wv);
+    const float rs = 1.0f / sqrtf(s / (float)H + a.eps);
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int c = c0 + v * 512 * W;
+        float nv[8];
+        g53_load8_to(nv, a.next, c, H);
+#pragma unroll
+        for (int i = 0; i < 8; i++) hv[v][i] = hv[v][i] * rs * nv[i];
+        if (live) g53_store8_to(xn + t * H, hv[v], c, H);
+    }
+}
+
+/* Persistent: group g of W waves takes tokens g, g + groups, ... */
+template <typename E, int W, int NV, int GK, bool Y>
+__global__ void __launch_bounds__(W < 4 ? 256 : 64 * W)
+k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E *y, G53NormArgs a)
+{
+    constexpr int NW = W < 4 ? 4 : W, RB = NW / W;
+    __shared__ float buf[3][NW][2];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const long grp = (long)blockIdx.x * RB + wv / W, groups = (long)gridDim.x * RB;
+    const int H = a.H, c0 = ((wv % W) * 64 + lane) * 8;
+    const long rounds = (a.T + groups - 1) / groups;
+    float ap[NV][8], an[NV][8], ag[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) ap[v][i] = an[v][i] = ag[v][i] = 0.0f;
+    for (long k = 0; k < rounds; k++) {
+        long t = grp + k * groups;
+        const bool live = t < a.T;
+        if (!live) t = a.T - 1;
+        float hv[NV][8], yh[NV][8], g[NV][8], u[NV][8], rsy = 1.0f, s = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int c = c0 + v * 512 * W;
+            g53_load8_to(hv[v], h + t * H, c, H);
+            if (dh2) g53_load8_to(g[v], dh2 + t * H, c, H);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; i++) g[v][i] = 0.0f;
+        }
+        const float gt = a.scale * (GK == 2 ? ((const float *)a.gate)[t] : 1.0f);
+        float gv[NV][8];
+        if (Y) {
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int c = c0 + v * 512 * W;
+                g53_load8_to(yh[v], y + t * H, c, H);
+                if (GK == 1) g53_load8_to(gv[v], (const float *)a.gate, c, H);
+                if (GK == 3) g53_load8_to(gv[v], (const E *)a.gate + t * H, c, H);
+            }
+            if (a.post) {
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) s = __builtin_fmaf(yh[v][i], yh[v][i], s);
+                g53_group_sum<W>(s, s2, buf[0], wv);
+                rsy = 1.0f / sqrtf(s / (float)H + a.eps);
+            }
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                float pv[8];
+                if (a.post) g53_load8_to(pv, a.post, c0 + v * 512 * W, H);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    yh[v][i] *= rsy;
+                    u[v][i] = a.post ? yh[v][i] * pv[i] : yh[v][i];
+                    gv[v][i] = (GK & 1) ? gt * gv[v][i] : gt;
+                    hv[v][i] = __builtin_fmaf(gv[v][i], u[v][i], hv[v][i]);
+                }
+            }
+        }
+        if (dxn) {                      /* uniform: through the next norm into h' */
+            float d[NV][8];
+            s = s2 = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                float nv[8];
+                g53_load8_to(d[v], dxn + t * H, c0 + v * 512 * W, H);
+                g53_load8_to(nv, a.next, c0 + v * 512 * W, H);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float vi = d[v][i] * nv[i];
+                    s = __builtin_fmaf(hv[v][i], hv[v][i], s);
+                    s2 = __builtin_fmaf(vi, hv[v][i], s2);
+                }
+            }
+            g53_group_sum<W>(s, s2, buf[1], wv);
+            const float rs = 1.0f / sqrtf(s / (float)H + a.eps), mean = s2 * rs / (float)H;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                float nv[8];
+                g53_load8_to(nv, a.next, c0 + v * 512 * W, H);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float hh = hv[v][i] * rs;
+                    if (live) an[v][i] = __builtin_fmaf(d[v][i], hh, an[v][i]);
+                    g[v][i] = __builtin_fmaf(rs, __builtin_fmaf(-hh, mean, d[v][i] * nv[i]), g[v][i]);
+                }
+            }
+        }
+        if (live)
+#pragma unroll
+            for (int v = 0; v < NV; v++) g53_store8_to(dh + t * H, g[v], c0 + v * 512 * W, H);
+        if (!Y) {
+            if (W > 1) __syncthreads();
+            continue;
+        }
+        s = s2 = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int c = c0 + v * 512 * W;
+            float pv[8], dg[8];
+            if (a.post) g53_load8_to(pv, a.post, c, H);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                dg[i] = a.scale * u[v][i] * g[v][i];
+                if (GK == 1 && live) ag[v][i] += dg[i];
+                if (GK == 2) s2 += dg[i];
+                const float du = gv[v][i] * g[v][i];
+                if (live) ap[v][i] = __builtin_fmaf(du, yh[v][i], ap[v][i]);
+                g[v][i] = a.post ? du * pv[i] : du;
+                s = __builtin_fmaf(g[v][i], yh[v][i], s);
+            }
+            if (GK == 3 && live && a.dgate) g53_store8_to((E *)a.dgate + t * H, dg, c, H);
+        }
+        g53_group_sum<W>(s, s2, buf[2], wv);
+        if (GK == 2 && live && a.dgate && lane == 0 && wv % W == 0) ((float *)a.dgate)[t] = s2;
+        const float mean = s / (float)H;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            if (a.post)
+#pragma unroll
+                for (int i = 0; i < 8; i++) g[v][i] = rsy * __builtin_fmaf(-yh[v][i], mean, g[v][i]);
+            if (live) g53_store8_to(dy + t * H, g[v], c0 + v * 512 * W, H);
+        }
+        if (W > 1) __syncthreads();     /* buf is used again */
+    }
+    float *part = a.part + grp * 3 * H;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int c = c0 + v * 512 * W;
+        if (c >= H) continue;
+        if (Y) g53_store8_to(part, ap[v], c, H);
+        g53_store8_to(part + H, an[v], c, H);
+        if (GK == 1) g53_store8_to(part + 2 * H, ag[v], c, H);
+    }
+}
+
+/* out[which][c] = the groups' partial sums, added in a fixed order: 16 chains of groups, then a tree. */
+__global__ void __launch_bounds__(1024) k_norm_sum(float *dpost, float *dnext, float *dgate, const float *__restrict__ part,
+                                                   int groups, int H)
+{
+    __shared__ float buf[16][64];
+    float *out = blockIdx.y == 0 ? dpost : (blockIdx.y == 1 ? dnext : dgate);
+    if (!out) return;
+    const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (c < H)
+        for (int g = k; g < groups; g += 16) s += part[((long)g * 3 + blockIdx.y) * H + c];
+    buf[k][lane] = s;
+    __syncthreads();
+    for (int d = 8; d; d >>= 1) {
+        if (k < d) buf[k][lane] += buf[k + d][lane];
+        __syncthreads();
+    }
+    if (k == 0 && c < H) out[c] = buf[0][lane];
+}
+
+/* Waves per row: 512 elements each, twice that above 8192. */
+#define G53_NORM_BY_WIDTH(H, BODY)                                              \
+    do {                                                                        \
+        if ((H) <= 512) { constexpr int W = 1, NV = 1; BODY; }                  \
+        else if ((H) <= 1024) { constexpr int W = 2, NV = 1; BODY; }            \
+        else if ((H) <= 2048) { constexpr int W = 4, NV = 1; BODY; }            \
+        else if ((H) <= 4096) { constexpr int W = 8, NV = 1; BODY; }            \
+        else if ((H) <= 8192) { constexpr int W = 16, NV = 1; BODY; }           \
+        else { constexpr int W = 16, NV = 2; BODY; }                            \
+    } while (0)
+#define G53_NORM_BY_GATE(kind, BODY)                                            \
+    do {                                                                        \
+        if ((kind) == 0) { constexpr int GK = 0; BODY; }                        \
+        else if ((kind) == 1) { constexpr int GK = 1; BODY; }                   \
+        else if ((kind) == 2) { constexpr int GK = 2; BODY; }                   \
+        else { constexpr int GK = 3; BODY; }                                    \
+    } while (0)
+
+#define G53_NORM_WGS (1l << 21)         /* workgroups of one launch: of up to 1024 threads, counted in 32 bits */
+
+template <typename E, int W, int NV, int GK, bool Y>
+static int forward(void *h2, void *xn, const void *h, const void *y, const G53NormArgs &a)
+{
+    constexpr int NW = W < 4 ? 4 : W, RB = NW / W;
+    const long total = ((long)a.T + RB - 1) / RB;
+    for (long w0 = 0; w0 < total; w0 += G53_NORM_WGS) {
+        const unsigned wgs = (unsigned)(total - w0 < G53_NORM_WGS ? total - w0 : G53_NORM_WGS);
+        hipLaunchKernelGGL((k_block_norm<E, W, NV, GK, Y>), dim3(wgs), dim3(64 * NW), 0, g53h_stream(), (E *)h2, (E *)xn,
+                           (const E *)h, (const E *)y, a, w0);
+        G53_LAUNCHED("k_block_norm");
+    }
+    return 0;
+}
+
+template <typename E, int W, int NV, int GK, bool Y>
+static int backward(void *dh, void *dy, float *dpost, float *dnext, float *dchannel, const void *dh2, const void *dxn,
+                    const void *h, const void *y, G53NormArgs &a)
+{
+    constexpr int NW = W < 4 ? 4 : W, RB = NW / W;
+    const long need = ((long)a.T + RB - 1) / RB, most = g53h_num_cus();
+    const unsigned wgs = (unsigned)(need < most ? need : most);
+    if (wgs) {
+        a.part = (float *)g53h_op_workspace((size_t)wgs * RB * 3 * a.H * sizeof(float));
+        if (!a.part) return -1;
+        hipLaunchKernelGGL((k_block_norm_grad<E, W, NV, GK, Y>), dim3(wgs), dim3(64 * NW), 0, g53h_stream(), (E *)dh, (E *)dy,
+                           (const E *)dh2, (const E *)dxn, (const E *)h, (const E *)y, a);
+        G53_LAUNCHED("k_block_norm_grad");
+    }
+    if (dpost || dnext || dchannel) {
+        hipLaunchKernelGGL(k_norm_sum, dim3((a.H + 63) / 64, 3), dim3(1024), 0, g53h_stream(), dpost, dnext, dchannel, a.part,
+                           (int)(wgs * RB), a.H);
+        G53_LAUNCHED("k_norm_sum");
+    }
+    return 0;
+}
+
+static int norm_bad(const char *who, int T, int hidden, int dt, float eps)
+{
+    if (T < 0 || hidden < 1 || hidden > G53_NORM_MAXH || !g53_elem_bytes(dt))
+        return g53h_fail("%s: %d tokens of %d, element type %d (hidden at most %d)", who, T, hidden, dt, G53_NORM_MAXH);
+    if (!(eps > 0.0f) || eps > 1.0e30f) return g53h_fail("%s: eps %g", who, eps);
+    return 0;
+}
+
+static int block_bad(const char *who, const G53hBlockNorm *p, G53NormArgs &a)
+{
+    if (!p) return g53h_fail("%s: no parameters", who);
+    if (norm_bad(who, p->T, p->hidden, p->dt, p->eps)) return -1;
+    if (p->gate_kind < 0 || p->gate_kind > 3 || (p->gate_kind && p->T && !p->gate))
+        return g53h_fail("%s: gate kind %d%s", who, p->gate_kind, p->gate ? "" : ", no gate");
+    if (!(p->scale >= -1.0e30f && p->scale <= 1.0e30f)) return g53h_fail("%s: scale %g", who, p->scale);
+    a = G53NormArgs{p->post, p->next, p->gate, nullptr, nullptr, p->eps, p->scale, p->T, p->hidden};
+    return 0;
+}
+
+extern "C" int g53h_norm(void *xn, const void *x, const float *gain, int dt, int T, int hidden, float eps)
+{
+    if (norm_bad("g53h_norm", T, hidden, dt, eps)) return -1;
+    if (!T) return 0;
+    if (!xn || !x || !gain) return g53h_fail("g53h_norm: no rows or no gain");
+    if (g53h_ready()) return -1;
+    G53NormArgs a{nullptr, gain, nullptr, nullptr, nullptr, eps, 0.0f, T, hidden};
+    int rc;
+    G53_BY_TYPE(dt, G53_NORM_BY_WIDTH(hidden, rc = (forward<E, W, NV, 0, false>(nullptr, xn, x, nullptr, a))));
+    return rc;
+}
+
+extern "C" int g53h_norm_grad(void *dx, float *dgain, const void *dxn, const void *x, const float *gain, int dt, int T,
+                              int hidden, float eps)
+{
+    if (norm_bad("g53h_norm_grad", T, hidden, dt, eps)) return -1;
+    if (T && (!dx || !dxn || !x || !gain)) return g53h_fail("g53h_norm_grad: no rows or no gain");
+    if (g53h_ready()) return -1;
+    G53NormArgs a{nullptr, gain, nullptr, nullptr, nullptr, eps, 0.0f, T, hidden};
+    int rc;
+    G53_BY_TYPE(dt, G53_NORM_BY_WIDTH(hidden, rc = (backward<E, W, NV, 0, false>(dx, nullptr, nullptr, dgain, nullptr, nullptr,
+                                                                                  dxn, x, nullptr, a))));
+    return rc;
+}
+
+extern "C" int g53h_block_norm(void *h2, void *xn, const void *h, const void *y, const G53hBlockNorm *p)
+{
+    G53NormArgs a;
+    if (block_bad("g53h_block_norm", p, a)) return -1;
+    if (!p->T) return 0;
+    if (!h2 || !h || !y) return g53h_fail("g53h_block_norm: no rows");
+    if (xn && !p->next) return g53h_fail("g53h_block_norm: xn without its gain");
+    if (g53h_ready()) return -1;
+    int rc;
+    G53_BY_TYPE(p->dt, G53_NORM_BY_WIDTH(p->hidden, G53_NORM_BY_GATE(p->gate_kind,
+                rc = (forward<E, W, NV, GK, true>(h2, xn, h, y, a)))));
+    return rc;
+}
+
+extern "C" int g53h_block_norm_grad(void *dh, void *dy, void *dgate, float *dpost, float *dnext, const void *dh2,
+                                    const void *dxn, const void *h, const void *y, const G53hBlockNorm *p)
+{
+    G53NormArgs a;
+    if (block_bad("g53h_block_norm_grad", p, a)) return -1;
+    if (p->T && (!dh || !dy || !h || !y)) return g53h_fail("g53h_block_norm_grad: no rows");
+    if (p->T && !dh2 && !dxn) return g53h_fail("g53h_block_norm_grad: neither dh2 nor dxn");
+    if (dxn && !p->next) return g53h_fail("g53h_block_norm_grad: dxn without its gain");
+    if (g53h_ready()) return -1;
+    if (!p->post) dpost = nullptr;
+    if (!p->next) dnext = nullptr;
+    a.dgate = p->gate_kind >= 2 ? dgate : nullptr;
+    float *dchannel = p->gate_kind == 1 ? (float *)dgate : nullptr;
+    int rc;
+    G53_BY_TYPE(p->dt, G53_NORM_BY_WIDTH(p->hidden, G53_NORM_BY_GATE(p->gate_kind,
+                rc = (backward<E, W, NV, GK, true>(dh, dy, dpost, dnext, dchannel, dh2, dxn, h, y, a)))));
+    return rc;
+}

@@ -42,6 +42,9 @@ int g53h_i4_from_f8_on(uint8_t *q_d, float *steps_d, const G53hMat *src, hipStre
  * counters region, which kernels leave zeroed. */
 void       *g53h_workspace(size_t bytes);
 size_t      g53h_workspace_growth(size_t bytes);    /* what g53h_workspace(bytes) would allocate: 0 when held */
+/* A second workspace, for the operators beside the layer (sorted tokens, norms): they may run between the phases
+ * of a grouped layer, whose pass the first one holds. Grown and reused in the same way. */
+void       *g53h_op_workspace(size_t bytes);
 /* A zero-initialised region of 4096 ints that kernels use as arrival counters and flags and
  * always restore to zero before they exit. */
 int        *g53h_counters(void);

@@ -18,6 +18,8 @@ static hipEvent_t  g_ev[2] = {nullptr, nullptr};
 static int         g_ev_next = 0;
 static void       *g_ws = nullptr;
 static size_t      g_ws_bytes = 0;
+static void       *g_opws = nullptr;
+static size_t      g_opws_bytes = 0;
 static int        *g_counters = nullptr;
 static int        *g_errs = nullptr;   /* [0] k_dec_layer, [1] k_dec_tiled, [2] grouped path   */
 static unsigned   *g_mbox = nullptr;   /* host mailbox: pinned, mapped, written by kernels      */
@@ -363,26 +365,30 @@ extern "C" int g53h_mem_info(size_t *free_b, size_t *total_b)
     return 0;
 }
 
-size_t g53h_workspace_growth(size_t bytes)
+static size_t growth(size_t bytes, size_t held)
 {
-    return bytes <= g_ws_bytes ? 0 : (bytes + (bytes >> 2) + 0xfffff) & ~(size_t)0xfffff;
+    return bytes <= held ? 0 : (bytes + (bytes >> 2) + 0xfffff) & ~(size_t)0xfffff;
 }
 
-void *g53h_workspace(size_t bytes)
+static void *grown(void **ws, size_t *held, size_t bytes)
 {
-    const size_t want = g53h_workspace_growth(bytes);
-    if (!want) return g_ws;
-    if (g_ws) {
+    const size_t want = growth(bytes, *held);
+    if (!want) return *ws;
+    if (*ws) {
         if (g53h_check(hipStreamSynchronize(g_stream), "hipStreamSynchronize", __FILE__, __LINE__))
             return nullptr;
-        (void)hipFree(g_ws);
-        g_ws = nullptr;
-        g_ws_bytes = 0;
+        (void)hipFree(*ws);
+        *ws = nullptr;
+        *held = 0;
     }
-    if (g53h_check(hipMalloc(&g_ws, want), "hipMalloc(workspace)", __FILE__, __LINE__)) return nullptr;
-    g_ws_bytes = want;
-    return g_ws;
+    if (g53h_check(hipMalloc(ws, want), "hipMalloc(workspace)", __FILE__, __LINE__)) return nullptr;
+    *held = want;
+    return *ws;
 }
+
+size_t g53h_workspace_growth(size_t bytes) { return growth(bytes, g_ws_bytes); }
+void *g53h_workspace(size_t bytes) { return grown(&g_ws, &g_ws_bytes, bytes); }
+void *g53h_op_workspace(size_t bytes) { return grown(&g_opws, &g_opws_bytes, bytes); }
 
 /* ---------------------------------------------------------------- profiling ----
  * Per-kernel timing with HIP events on the compute stream: when enabled, the layer code

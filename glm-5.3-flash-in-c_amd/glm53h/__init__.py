@@ -45,6 +45,24 @@ class G53hMoeLayer(C.Structure):
                 ("block_c", C.c_int), ("tiled", C.c_int)]
 
 
+G53H_F32, G53H_BF16, G53H_F16 = 0, 1, 2
+
+
+class G53hSort(C.Structure):
+    _fields_ = [("T", C.c_int), ("topk", C.c_int), ("n_experts", C.c_int), ("offsets", C.c_void_p),
+                ("pair", C.c_void_p), ("row", C.c_void_p)]
+
+
+class G53hW4(C.Structure):
+    _fields_ = [("w", C.c_void_p), ("s", C.c_void_p), ("z", C.c_void_p), ("rows", C.c_int), ("cols", C.c_int),
+                ("group", C.c_int), ("s_dt", C.c_int)]
+
+
+class G53hBlockNorm(C.Structure):
+    _fields_ = [("T", C.c_int), ("hidden", C.c_int), ("dt", C.c_int), ("gate_kind", C.c_int), ("eps", C.c_float),
+                ("scale", C.c_float), ("post", C.c_void_p), ("next", C.c_void_p), ("gate", C.c_void_p)]
+
+
 # -------------------------------------------------------------- structs (glm53f.h) ----
 GLM53F_MAX_LAYERS = 256
 GLM53F_MAX_EOS = 8
@@ -237,6 +255,23 @@ _SIGS = {
                                       C.c_int]),
     "g53h_quant_host": (None, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_float]),
     "g53h_synth_uniform_host": (None, [C.c_void_p, C.c_size_t, C.c_uint64, C.c_uint64, C.c_float]),
+    # operators beside the layer
+    "g53h_sort_tokens": (C.c_int, [C.POINTER(G53hSort), C.c_void_p]),
+    "g53h_sorted_dispatch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hSort)]),
+    "g53h_sorted_dispatch_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hSort)]),
+    "g53h_sorted_combine": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                      C.POINTER(G53hSort)]),
+    "g53h_sorted_combine_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                           C.POINTER(G53hSort)]),
+    "g53h_mm_w4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hW4), C.c_float]),
+    "g53h_sorted_mm_w4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hSort), C.POINTER(G53hW4),
+                                    C.c_float]),
+    "g53h_norm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float]),
+    "g53h_norm_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                                 C.c_float]),
+    "g53h_block_norm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(G53hBlockNorm)]),
+    "g53h_block_norm_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(G53hBlockNorm)]),
     # drop-in (glm53f.h)
     "glm53f_mm": (None, [C.c_void_p, C.c_void_p, C.POINTER(Glm53fMat)]),
     "glm53f_i4_from_f8": (None, [C.c_void_p, C.c_void_p, C.POINTER(Glm53fMat)]),

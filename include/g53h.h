@@ -357,6 +357,84 @@ int g53h_mtile_i4(uint8_t *dst_w, float *dst_s, const uint8_t *src_w, const floa
 int g53h_mtile_i4_host(uint8_t *dst_w, float *dst_s, const uint8_t *src_w, const float *src_s, int rows, int cols,
                        int inverse);
 
+/* -------------------------------------------------- operators beside the layer ----
+ * No counterpart in the reference. What a trunk does around and inside a MoE layer, on the library's
+ * stream, so that nothing has to wait between them and g53h_moe: norms before and after the block with
+ * its gate and residual, tokens sorted by expert and back, products with 4-bit matrices of any group
+ * width; and the gradients of those that a training step differentiates. Pointers are device memory
+ * of contiguous rows, aligned to one element; activations are of one of the types below, sums are fp32,
+ * and results are rounded once. T = 0 is allowed everywhere. Arguments are checked before any work. */
+#define G53H_F32  0
+#define G53H_BF16 1
+#define G53H_F16  2
+
+/* Tokens sorted by expert. The n = T * topk pairs (t, j) of a routing, pair number t * topk + j, in
+ * order of expert and then of pair number, are the sorted rows. A pair whose expert is outside
+ * [0, n_experts) (padding: -1) is left out. T * topk < 2^31, topk 1 to 64, n_experts 1 to 1024. */
+typedef struct {
+    int  T, topk, n_experts;
+    int *offsets;        /* device [n_experts + 1]: first sorted row of each expert; the last: their number */
+    int *pair;           /* device [n]: the pair of each sorted row, -1 behind the last                     */
+    int *row;            /* device [n]: the sorted row of each pair, -1 where it is left out                */
+} G53hSort;
+/* Fills the plan's three arrays from idx_d [T][topk]. */
+int g53h_sort_tokens(const G53hSort *p, const int *idx_d);
+/* xs[row of (t, j)] = x[t]: x [T][hidden], xs [n][hidden]. Rows behind the last sorted one are left as
+ * they were. _grad: dx[t] = sum of the dxs rows of t's pairs. */
+int g53h_sorted_dispatch(void *xs_d, const void *x_d, int dt, int hidden, const G53hSort *p);
+int g53h_sorted_dispatch_grad(void *dx_d, const void *dxs_d, int dt, int hidden, const G53hSort *p);
+/* out[t] = add[t] + sum over j of w[t][j] ys[row of (t, j)], in order of j; w fp32 [T][topk]; add may be
+ * NULL, or out itself. Rows and weights of pairs left out are not read. _grad, of dout [T][hidden]:
+ * dys[row] = w dout[t] (rows behind the last left as they were; dys may be ys), dw[t][j] = the product of
+ * dout[t] and ys[row], 0 for a pair left out; add's gradient is dout. */
+int g53h_sorted_combine(void *out_d, const void *ys_d, const float *w_d, const void *add_d, int dt, int hidden,
+                        const G53hSort *p);
+int g53h_sorted_combine_grad(void *dys_d, float *dw_d, const void *dout_d, const void *ys_d, const float *w_d, int dt,
+                             int hidden, const G53hSort *p);
+
+/* A matrix of 4-bit levels with group scales: element (r, c) = s[r][c / group] * (q[r][c] - z[r][c / group]).
+ * Levels as in G53H_MAT_I4: [rows][cols / 2], the even column in the low nibble; the matrix starts at a
+ * multiple of 16 bytes. Scales [rows][groups], groups = ceil(cols / group), of type s_dt. Zero points
+ * [rows][(groups + 1) / 2], the even group in the low nibble, or NULL: 8 everywhere (with fp32 scales in
+ * groups of 64 that is G53H_MAT_I4's format). cols and group are multiples of 32. */
+typedef struct {
+    const uint8_t *w;
+    const void    *s;
+    const uint8_t *z;
+    int rows, cols, group, s_dt;
+} G53hW4;
+/* y[T][rows] = M . x[T][cols]. With swiglu_limit > 0 the matrix is gate over up (rows / 2 each) and
+ * y[T][rows / 2] their SwiGLU as g53h_swiglu's, from the fp32 sums; 0: without. Meant for few tokens:
+ * the weights are read once per 16 to 64 of them. A row of x that is not finite gives NaN. */
+int g53h_mm_w4(void *y_d, const void *x_d, int dt, int T, const G53hW4 *m, float swiglu_limit);
+/* The same over the sorted rows of a plan, each with its expert's matrix: m describes expert 0, the levels,
+ * scales and zero points of the others follow it. x: with gather the tokens [T][cols] (a row takes its pair's
+ * token), else sorted rows [n][cols]. ys [n][rows (/ 2)]; rows behind the last are left as they were. */
+int g53h_sorted_mm_w4(void *ys_d, const void *x_d, int dt, int gather, const G53hSort *p, const G53hW4 *m,
+                      float swiglu_limit);
+
+/* xn = x / sqrt(mean of x^2 + eps) * gain per row of hidden <= 16384; gain fp32 [hidden]; xn may be x.
+ * _grad: dx (may be dxn) and, where it is not NULL, dgain fp32 [hidden], from dxn and x. */
+int g53h_norm(void *xn_d, const void *x_d, const float *gain_d, int dt, int T, int hidden, float eps);
+int g53h_norm_grad(void *dx_d, float *dgain_d, const void *dxn_d, const void *x_d, const float *gain_d, int dt, int T,
+                   int hidden, float eps);
+/* After a block: u = the norm of its output y with gain post (NULL: u = y), h2 = h + scale * gate * u, and
+ * xn = the norm of h2 (before it is rounded) with gain next, the next block's input (xn NULL: not wanted).
+ * The gate by gate_kind: 0 none, 1 fp32 [hidden] per channel, 2 fp32 [T] per token, 3 [T][hidden] of type dt,
+ * as it multiplies. h2 may be h.
+ * _grad, of dh2 and dxn (either may be NULL: zero): dh (may be dh2), dy, dgate in the gate's shape and type,
+ * dpost and dnext fp32 [hidden]; dgate, dpost and dnext may be NULL. Sums over tokens are in a fixed order: the
+ * same bits on every run. */
+typedef struct {
+    int   T, hidden, dt, gate_kind;
+    float eps, scale;
+    const float *post, *next;
+    const void  *gate;
+} G53hBlockNorm;
+int g53h_block_norm(void *h2_d, void *xn_d, const void *h_d, const void *y_d, const G53hBlockNorm *p);
+int g53h_block_norm_grad(void *dh_d, void *dy_d, void *dgate_d, float *dpost_d, float *dnext_d, const void *dh2_d,
+                         const void *dxn_d, const void *h_d, const void *y_d, const G53hBlockNorm *p);
+
 /* -------------------------------------------------------- checks and inputs ---- */
 /* y[i] = expf(x[i]) by the device restatement of glibc's expf (for exhaustive checks). */
 int g53h_expf(float *y_d, const float *x_d, size_t n);

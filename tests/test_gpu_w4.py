@@ -1,0 +1,174 @@
+"""Products with 4-bit levels and group scales (g53h_mm_w4, g53h_sorted_mm_w4) against 64-bit products
+on the host. Tolerances are derived where the product is formed (op_lib.W4.product)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import glm53h
+from glm53h import check
+from op_lib import BF16, F16, F32, HALF, TINY, W4, Buf, Plan, close, enc, routing, sorted_plan, swiglu
+from test_gpu_parity import say
+
+pytestmark = pytest.mark.gpu
+LIMIT = 10.0
+
+
+@pytest.fixture(scope="module")
+def L():
+    return glm53h.init(0)
+
+
+def act_tol(y, tol, limit):
+    """What an error of tol in gate and up sums makes of the SwiGLU: |silu'| <= 1.1, |silu(g)| <= |g| + 0.3, the
+    clamps shrink distances; silu itself in fp32 is off by at most 8 roundings."""
+    g, u = np.split(y, 2, -1)
+    tg, tu = np.split(tol, 2, -1)
+    gc, uc = np.abs(np.minimum(g, limit)), np.abs(np.clip(u, -limit, limit))
+    return 1.1 * tg * (uc + tu) + (gc + 0.3) * tu + 8 * 2.0 ** -24 * (gc + 0.3) * uc
+
+
+CASES = [  # T, rows, cols, group, s_dt, zeros, swiglu
+    (1, 4096, 2048, 64, F32, False, False), (1, 1, 32, 32, F32, True, False), (2, 17, 64, 32, F16, True, False),
+    (3, 33, 96, 64, BF16, False, False), (5, 100, 160, 128, F16, True, False), (8, 64, 4096, 4096, F32, False, True),
+    (16, 1001, 2080, 32, F16, True, False), (17, 70, 480, 96, BF16, True, True), (24, 130, 1024, 128, F32, False, True),
+    (31, 34, 2016, 32, F32, True, True), (33, 48, 288, 160, F32, True, False), (64, 66, 640, 256, BF16, False, True),
+    (65, 20, 352, 64, F16, False, False), (130, 258, 224, 128, F32, True, True), (300, 40, 128, 1024, F32, True, False)]
+
+
+@pytest.mark.parametrize("T,rows,cols,group,s_dt,zeros,sw", CASES)
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_product(L, T, rows, cols, group, s_dt, zeros, sw, dt):
+    say("w4", T, rows, cols, group, s_dt, zeros, sw, dt)
+    rng = np.random.default_rng(rows + cols + T)
+    m = W4(rng, 1, rows, cols, group, s_dt, zeros)
+    x, out = Buf(rng.standard_normal((T, cols)), dt), rows // 2 if sw else rows
+    y = Buf.out((T, out), dt)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, dt, T, C.byref(m.c), LIMIT if sw else 0.0), "w4")
+    want, tol = m.product(x.val())
+    if sw:
+        want, tol = swiglu(want, LIMIT), act_tol(want, tol, LIMIT)
+    close(y.val(), want, HALF[dt] * np.abs(want) + TINY[dt] + tol)
+    if dt == F32 and cols >= 1024 and not sw:
+        # typical sums are far inside the worst case: 2^-16 of a value lost (a plane of x) would show here
+        assert np.linalg.norm(y.val() - want) < 2e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("T,rows,cols,group,s_dt,zeros,sw", [c for c in CASES if not c[-1]])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_product_of_whole_numbers_is_exact(L, T, rows, cols, group, s_dt, zeros, sw, dt):
+    """Small whole x and power-of-two scales: every partial sum fits 24 bits, so the result is the exact sum,
+    rounded once, whatever the order."""
+    say("w4, exact", T, rows, cols, group, s_dt, zeros, dt)
+    rng = np.random.default_rng(rows + cols + T + 1)
+    m = W4(rng, 1, rows, cols, group, s_dt, zeros, exact=True)
+    xv = rng.integers(-8, 9, (T, cols)).astype(float)
+    x, y = Buf(xv, dt), Buf.out((T, rows), dt)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, dt, T, C.byref(m.c), 0.0), "w4")
+    with np.errstate(over="ignore"):
+        assert np.array_equal(y.get(), enc(xv @ m.wide[0].T, dt))
+
+
+@pytest.mark.parametrize("shift", [2, 4, 6, 14])
+def test_rows_off_alignment(L, shift):
+    say("w4, x and y off by", shift)
+    rng = np.random.default_rng(shift)
+    m = W4(rng, 1, 37, 96, 32, F32, True, exact=True)
+    xv = rng.integers(-8, 9, (9, 96)).astype(float)
+    for dt in (BF16, F32) if shift == 4 else (BF16,):
+        x, y = Buf(xv, dt, shift), Buf.out((9, 37), dt, shift)
+        check(L.g53h_mm_w4(y.ptr, x.ptr, dt, 9, C.byref(m.c), 0.0), "w4")
+        assert np.array_equal(y.get(), enc(xv @ m.wide[0].T, dt))
+
+
+def test_full_range_of_fp32(L):
+    """fp32 activations from 2^-100 to 2^100: each is three planes exactly, so a column alone is off by the
+    roundings of its own few sums."""
+    say("w4, wide range")
+    rng = np.random.default_rng(8)
+    m = W4(rng, 1, 40, 64, 32, F32, True)
+    xv = np.zeros((64, 64))
+    xv[np.arange(64), np.arange(64)] = rng.uniform(1, 2, 64) * 2.0 ** rng.integers(-100, 100, 64)
+    x, y = Buf(xv, F32), Buf.out((64, 40), F32)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, F32, 64, C.byref(m.c), 0.0), "w4")
+    want, _ = m.product(x.val())
+    # three planes of (16 + q) x and of x, the surplus, the scale: ten roundings of at most 62 |x| s
+    close(y.val(), want, 10 * 2.0 ** -24 * 62 * (np.abs(x.val()) @ m.s[0].T))
+
+
+def test_other_tokens_do_not_matter(L):
+    """A token with an infinity or NaN spoils its own row only."""
+    say("w4, not finite")
+    rng = np.random.default_rng(9)
+    m = W4(rng, 1, 50, 256, 64, F32, True)
+    for dt in (F32, BF16, F16):
+        xv = rng.standard_normal((6, 256))
+        good = Buf(xv, dt)
+        xv = xv.copy()
+        xv[2, 100], xv[4, 0] = np.nan, np.inf
+        bad = Buf(xv, dt)
+        ya, yb = Buf.out((6, 50), dt), Buf.out((6, 50), dt)
+        check(L.g53h_mm_w4(ya.ptr, good.ptr, dt, 6, C.byref(m.c), 0.0), "w4")
+        check(L.g53h_mm_w4(yb.ptr, bad.ptr, dt, 6, C.byref(m.c), 0.0), "w4")
+        assert np.isnan(yb.val()[[2, 4]]).all() and np.array_equal(ya.get()[[0, 1, 3, 5]], yb.get()[[0, 1, 3, 5]])
+
+
+@pytest.mark.parametrize("T,K,NE,rows,cols,group,s_dt,zeros,sw,drop", [
+    (1, 8, 288, 64, 256, 128, BF16, False, True, 0.0), (1, 1, 1, 5, 32, 32, F32, True, False, 0.0),
+    (6, 4, 9, 40, 160, 64, F16, True, False, 0.2), (40, 6, 64, 34, 96, 32, F32, True, True, 0.1),
+    (200, 8, 5, 24, 128, 128, F32, False, False, 0.0), (70, 3, 1000, 18, 64, 64, BF16, True, False, 0.4),
+    (9, 2, 4, 10, 64, 64, F32, False, False, 1.0)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("gather", [1, 0])
+def test_sorted_products(L, T, K, NE, rows, cols, group, s_dt, zeros, sw, drop, dt, gather):
+    say("sorted w4", T, K, NE, rows, cols, group, s_dt, zeros, sw, drop, dt, gather)
+    rng = np.random.default_rng(T + K + NE)
+    idx = routing(rng, T, K, NE, drop)
+    plan, (off, pair, _) = Plan(idx, NE), sorted_plan(idx, NE)
+    n, out = off[NE], rows // 2 if sw else rows
+    m = W4(rng, NE, rows, cols, group, s_dt, zeros)
+    xv = rng.standard_normal((T if gather else T * K, cols))
+    if not gather:
+        xv[n:] = np.nan
+    x, y = Buf(xv, dt), Buf.out((T * K, out), dt)
+    check(L.g53h_sorted_mm_w4(y.ptr, x.ptr, dt, gather, plan.c, C.byref(m.c), LIMIT if sw else 0.0), "sorted w4")
+    v, got = x.val(), y.val()
+    for e in range(NE):
+        a, b = off[e], off[e + 1]
+        if a < b:
+            want, tol = m.product(v[pair[a:b] // K] if gather else v[a:b], e)
+            if sw:
+                want, tol = swiglu(want, LIMIT), act_tol(want, tol, LIMIT)
+            close(got[a:b], want, HALF[dt] * np.abs(want) + TINY[dt] + tol, e)
+    assert (y.get()[n:] == enc([77.0], dt)).all()
+
+
+def test_no_tokens(L):
+    say("w4, no tokens")
+    m = W4(np.random.default_rng(1), 1, 8, 32, 32, F32, False)
+    assert L.g53h_mm_w4(None, None, BF16, 0, C.byref(m.c), 0.0) == 0
+    off = Buf(np.zeros(2, np.int32))
+    assert L.g53h_sorted_mm_w4(None, None, BF16, 0, glm53h.G53hSort(0, 1, 1, off.ptr, None, None), C.byref(m.c), 0.0) == 0
+
+
+def test_matrix_past_2_gib(L):
+    """Stacked matrices whose levels pass 2^31 bytes: the last expert's rows are its own."""
+    say("w4, offsets past 32 bits")
+    rows, cols, NE = 1024, 32768, 140
+    one = rows * cols // 2
+    assert one * NE > 1 << 31
+    rng = np.random.default_rng(10)
+    m = W4(rng, 1, rows, cols, 128, BF16, False, exact=True)
+    w, s = glm53h.DevBuf(one * NE), glm53h.DevBuf(m.s_d.n * NE)
+    check(L.g53h_memset(w.ptr, 0x88, one * NE), "memset")                    # every level 8: zero
+    check(L.g53h_memset(s.ptr, 0x3f, m.s_d.n * NE), "memset")
+    check(L.g53h_d2d(w.ptr + one * (NE - 1), m.w_d.ptr, one), "d2d")
+    check(L.g53h_d2d(s.ptr + m.s_d.n * (NE - 1), m.s_d.ptr, m.s_d.n), "d2d")
+    idx = np.array([[NE - 1, 3], [5, NE - 1]], np.int32)
+    plan = Plan(idx, NE)
+    xv = rng.integers(-2, 3, (2, cols)).astype(float)
+    x, y = Buf(xv, BF16), Buf.out((4, rows), BF16)
+    c = glm53h.G53hW4(w.ptr, s.ptr, None, rows, cols, 128, BF16)
+    check(L.g53h_sorted_mm_w4(y.ptr, x.ptr, BF16, 1, plan.c, C.byref(c), 0.0), "sorted w4")
+    got = y.get()
+    assert (got[:2] == 0).all() and np.array_equal(got[2:], enc(xv @ m.wide[0].T, BF16))
