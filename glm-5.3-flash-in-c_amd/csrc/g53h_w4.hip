@@ -23,6 +23,10 @@
 #include "g53h_runtime.h"
 
 #define G53_W4_MAXE 1024
+#define G53_W4_MAXC (1 << 24)          /* columns: 16 rows of levels or scales stay below 2^31 bytes */
+#define G53_W4_NW 8                     /* waves of a workgroup, at most */
+#define G53_W4_LDS_MAX (150 * 1024)
+#define G53_W4_LDS (78 * 1024)          /* of its activations: two workgroups a CU */
 
 struct G53W4Args {
     const uint8_t *w;                   /* levels [n][rows][cols / 2]                        */
@@ -37,6 +41,9 @@ struct G53W4Args {
     int n_experts, topk;
     long item0;                         /* first token tile of the launch                     */
     int tiles;                          /* row tiles                                          */
+    int kw_log;                         /* log2 of the parts that a workgroup's waves split the columns into */
+    int glog;                           /* log2 of group / 32 where it is a power of two, else -1 */
+    int seg;                            /* chunks of 128 columns whose activations LDS holds  */
 };
 
 typedef unsigned int g53_v2w __attribute__((ext_vector_type(2)));
@@ -70,20 +77,18 @@ template <> __device__ __forceinline__ g53_v8h g53_w4_levels<g53_v8h>(unsigned d
                                                  ((d >> 6) & m) | o});
 }
 
-/* Eight activations from p in the levels' order, as P planes of the products' type. */
-template <typename V> __device__ __forceinline__ void g53_w4_x16(V (&o)[1], const void *p)
+/* Eight activations in the levels' order, as P planes of the products' type. */
+template <typename V> __device__ __forceinline__ void g53_w4_x(V (&o)[1], const g53_v4w (&p)[1])
 {
-    const g53_v4w v = ((const G53v4w_any *)p)->v;              /* 01 23 45 67 */
+    const g53_v4w v = p[0];                                   /* 01 23 45 67 */
     o[0] = __builtin_bit_cast(V, (g53_v4w){__builtin_amdgcn_perm(v[2], v[0], 0x05040100u),
                                            __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
                                            __builtin_amdgcn_perm(v[3], v[1], 0x05040100u),
                                            __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)});
 }
-__device__ __forceinline__ void g53_w4_x(g53_v8b (&o)[1], const g53_bf16 *p) { g53_w4_x16(o, p); }
-__device__ __forceinline__ void g53_w4_x(g53_v8h (&o)[1], const g53_f16 *p) { g53_w4_x16(o, p); }
-__device__ __forceinline__ void g53_w4_x(g53_v8b (&o)[3], const float *p)
+__device__ __forceinline__ void g53_w4_x(g53_v8b (&o)[3], const g53_v4w (&p)[2])
 {
-    const g53_v4w a = ((const G53v4w_any *)p)[0].v, b = ((const G53v4w_any *)p)[1].v;
+    const g53_v4w a = p[0], b = p[1];
     unsigned v[8];
 #pragma unroll
     for (int i = 0; i < 4; i++) { v[2 * i] = a[i]; v[2 * i + 1] = b[i]; }   /* 0 4 1 5 2 6 3 7 */
@@ -115,13 +120,6 @@ __device__ __forceinline__ void g53_turn(unsigned (&d)[4])
     d[2] = p[0]; d[3] = p[1];
 }
 
-__device__ __forceinline__ float g53_w4_scale(const G53W4Args &a, long i)
-{
-    if (a.s_dt == G53H_F32) return ((const float *)a.s)[i];
-    if (a.s_dt == G53H_BF16) return (float)((const g53_bf16 *)a.s)[i];
-    return (float)((const g53_f16 *)a.s)[i];
-}
-
 /* The token tile `item` of the sorted rows: tiles of TT rows, expert by expert. False behind the last. */
 __device__ __forceinline__ bool g53_w4_item(const G53W4Args &a, long item, int TT, int &e, int &first, int &last)
 {
@@ -151,175 +149,296 @@ __device__ __forceinline__ bool g53_w4_item(const G53W4Args &a, long item, int T
     return true;
 }
 
-/* SW: SwiGLU; the first R / 2 row tiles are gate rows, the others the same up rows. */
-template <typename E, int R, int NT, int NW, bool SW>
-__global__ void __launch_bounds__(64 * NW) k_w4(E *__restrict__ y, const E *__restrict__ x, G53W4Args a)
+/* What a wave has asked for of 128 columns: levels, scales and zero points of its row tiles as they lie. */
+template <int R> struct G53W4Chunk {
+    g53_v4w w[R];
+    unsigned s[R], z[R];
+};
+
+/* n / d for 0 <= n, by a shift where d is a power of two (log >= 0). */
+__device__ __forceinline__ int g53_quot(int n, int d, int log) { return log >= 0 ? n >> log : n / d; }
+
+/* One workgroup: up to 16 NT tokens (or sorted rows of one expert) by `out` (NW / KW) rows. Its waves are KW parts of the
+ * columns, taken in turn 128 columns each, by NW / KW groups of R row tiles. PF chunks are asked for ahead. GS: groups
+ * are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows, the others the same
+ * up rows. Columns behind the last of a chunk meet activations of zero. */
+template <typename E, int R, int NT, int PF, int GS>
+__global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2) k_w4(E *__restrict__ y, const E *__restrict__ x, G53W4Args a)
 {
     typedef typename G53W4Type<E>::V V;
     constexpr int P = G53W4Type<E>::P, TT = 16 * NT, LD = 16 * R + 4;
-    __shared__ float red[NW][TT][LD];
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int m = lane & 15, q = lane >> 4;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const bool sw = a.limit > 0.0f;
+    const int out = sw ? 8 * R : 16 * R;                     /* result rows of a wave */
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), NW = blockDim.x >> 6;
+    const int m = lane & 15, q = lane >> 4, KW = 1 << a.kw_log, kw = wv & (KW - 1), rw = wv >> a.kw_log, RW = NW >> a.kw_log;
     const long item = a.item0 + blockIdx.x / a.tiles;
     const int tile = blockIdx.x % a.tiles;
     int e = 0, first, last;
     if (a.offsets) {
         if (!g53_w4_item(a, item, TT, e, first, last)) return;
         e = __builtin_amdgcn_readfirstlane(e);
+        first = __builtin_amdgcn_readfirstlane(first);
+        last = __builtin_amdgcn_readfirstlane(last);
     } else {
         first = (int)(item * TT);
         last = a.T - first < TT ? a.T : first + TT;
     }
-    constexpr int OUT = SW ? 8 * R : 16 * R;                 /* result rows of a workgroup */
-    const int row0 = tile * OUT;
-    /* row tile r starts at this row of the matrix */
-    auto tile_row = [&](int r) { return SW ? (r < R / 2 ? row0 + 16 * r : a.half + row0 + 16 * (r - R / 2)) : row0 + 16 * r; };
-    auto tile_end = [&](int r) { return SW && r < R / 2 ? a.half : a.rows; };
-    const long wrow = a.cols / 2, mat = (long)e * a.rows, zrow = (a.groups + 1) / 2;
-    const uint8_t *wp[R];
-    long srow[R][4];
+    const int rows = last - first, row0 = (tile * RW + rw) * out;
+    /* where the row tiles begin; the lane's row in them, the last one for those behind the end */
+    const uint8_t *wb[R], *sb[R], *zb[R];
+    const int wrow = a.cols / 2, srow = a.groups * (a.s_dt == G53H_F32 ? 4 : 2), zrow = (a.groups + 1) / 2;
+    int w_of[R], s_of[R], z_of[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const int end = tile_end(r) - 1;
-        const int i = tile_row(r) + m;
-        wp[r] = a.w + (mat + (i < end ? i : end)) * wrow + q * 16;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int j = tile_row(r) + 4 * q + k;
-            srow[r][k] = mat + (j < end ? j : end);
-        }
+        const bool up = sw && r >= R / 2;
+        const int j = row0 + 16 * (up ? r - R / 2 : r), top = j < a.half ? j : a.half - 1, i = m < a.half - top ? m : a.half - top - 1;
+        const long at = (long)e * a.rows + top + (up ? a.half : 0);
+        wb[r] = a.w + at * wrow;
+        sb[r] = (const uint8_t *)a.s + at * srow;
+        zb[r] = a.z + at * zrow;
+        w_of[r] = i * wrow;
+        s_of[r] = i * srow;
+        z_of[r] = i * zrow;
     }
-    const E *xp[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        int p = first + 16 * t + m;
-        p = p < last ? p : last - 1;                          /* columns behind the last repeat it and are not written */
-        if (a.pair) p = a.pair[p] / a.topk;
-        xp[t] = x + (long)p * a.cols + q * 8;
-    }
-    g53_v4f acc[R][NT], D[R][NT], X[NT];
+    const unsigned z_mask = a.z ? 15u : 0u, z_no = a.z ? 0u : 8u;
+    g53_v4f acc[R][NT];
     const g53_v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        X[t] = zero;
+    for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int r = 0; r < R; r++) { acc[r][t] = zero; D[r][t] = zero; }
-    }
+        for (int r = 0; r < R; r++) acc[r][t] = zero;
     V ones;
 #pragma unroll
     for (int i = 0; i < 8; i++) ones[i] = 1.0f;
-    const int chunks = (a.cols + 127) / 128, per = (chunks + NW - 1) / NW;
-    const int c0 = wv * per, c1 = c0 + per < chunks ? c0 + per : chunks;
-    int g = c0 * 128 / a.group, left = (g + 1) * a.group - c0 * 128;      /* the group, and its columns to come */
-    for (int c = c0; c < c1; c++) {
+    const int chunks = (a.cols + 127) / 128;
+    typedef G53W4Chunk<R> Chunk;
+
+    /* the lane's group in chunk c: the chunk's, or that of its quarter q */
+    auto group_of = [&](int c) {
+        if (GS == 4) return g53_quot(c * 4, a.group / 32, a.glog);
+        const int g = g53_quot(c * 4 + q, a.group / 32, a.glog);
+        return g < a.groups ? g : a.groups - 1;
+    };
+    /* c behind the last chunk: that one again, never used */
+    auto load = [&](Chunk &k, int c) {
+        c = c < chunks ? c : chunks - 1;
+        const int g = group_of(c), w_at = c * 64 + q * 16, wo = w_at < wrow ? w_at : 0;
+#pragma unroll
+        for (int r = 0; r < R; r++) k.w[r] = __builtin_nontemporal_load((const g53_v4w *)(wb[r] + (unsigned)(w_of[r] + wo)));
+        if (a.s_dt == G53H_F32)
+#pragma unroll
+            for (int r = 0; r < R; r++) k.s[r] = *(const unsigned *)(sb[r] + (unsigned)(s_of[r] + g * 4));
+        else
+#pragma unroll
+            for (int r = 0; r < R; r++) k.s[r] = *(const uint16_t *)(sb[r] + (unsigned)(s_of[r] + g * 2));
+        if (a.z)
+#pragma unroll
+            for (int r = 0; r < R; r++) k.z[r] = zb[r][(unsigned)(z_of[r] + (g >> 1))];
+    };
+    const int ld = a.seg * 256 + 16;        /* bytes of a plane's row in LDS: odd sixteens, so rows start in other banks */
+    int xat[NT];                            /* the lane's token in LDS; tokens behind the last repeat it */
+#pragma unroll
+    for (int t = 0; t < NT; t++) xat[t] = (16 * t + m < rows ? 16 * t + m : rows - 1) * ld + q * 16;
+    const int plane = rows * ld;
+    /* a scale as it lies to fp32, without a branch: fp32 as it is, bf16 shifted, fp16 converted */
+    const int s_shift = a.s_dt == G53H_BF16 ? 16 : 0;
+    const unsigned s_f16 = a.s_dt == G53H_F16 ? ~0u : 0u;
+    auto use = [&](const Chunk &k, int c, int c_lds) {
         unsigned d[R][4];
-        const int steps = a.cols - c * 128 >= 128 ? 4 : (a.cols - c * 128) / 32;
+        float sc[R][4], nz[R][4];
+        const int g4 = 4 * (group_of(c) & 1);
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const g53_v4w v = q < steps ? ((const G53v4w_any *)(wp[r] + c * 64))->v : (g53_v4w){0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; i++) d[r][i] = v[i];
+            for (int i = 0; i < 4; i++) d[r][i] = k.w[r][i];
             g53_turn(d[r]);
+            const float f16 = (float)__builtin_bit_cast(g53_f16, (uint16_t)k.s[r]);
+            const unsigned f = (k.s[r] << s_shift & ~s_f16) | (__builtin_bit_cast(unsigned, f16) & s_f16);
+            const float n = -16.0f - (float)((k.z[r] >> g4 & z_mask) | z_no);
+            if (GS == 4) {
+                sc[r][3] = __builtin_bit_cast(float, f);
+                nz[r][3] = n;
+            } else {                    /* every quarter's to all lanes of the row */
+                unsigned u[4], v[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) { u[i] = f; v[i] = __builtin_bit_cast(unsigned, n); }
+                g53_turn(u);
+                g53_turn(v);
+#pragma unroll
+                for (int i = 0; i < 4; i++) { sc[r][i] = __builtin_bit_cast(float, u[i]); nz[r][i] = __builtin_bit_cast(float, v[i]); }
+            }
         }
+        g53_v4f D[R][NT], X[NT];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            if (s < steps) {
-                V b[NT][P];
+            V b[NT][P];
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    g53_w4_x(b[t], xp[t] + c * 128 + s * 32);
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int k = 0; k < P; k++) X[t] = g53_mfma(ones, b[t][k], X[t]);
+                for (int p = 0; p < P; p++) {
+                    b[t][p] = *(const V *)(lds + p * plane + xat[t] + c_lds * 256 + s * 64);
+                    X[t] = g53_mfma(b[t][p], ones, s % GS == 0 && p == 0 ? zero : X[t]);
                 }
 #pragma unroll
-                for (int r = 0; r < R; r++) {
-                    const V lv = g53_w4_levels<V>(d[r][s]);
+            for (int r = 0; r < R; r++) {
+                const V lv = g53_w4_levels<V>(d[r][s]);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int p = 0; p < P; p++) D[r][t] = g53_mfma(b[t][p], lv, s % GS == 0 && p == 0 ? zero : D[r][t]);
+            }
+            if (NT * P > 2 || GS < 4) __builtin_amdgcn_sched_barrier(0);     /* one step's activations in registers at a time */
+            if (s % GS == GS - 1)       /* a group, or what the chunk has of it */
+#pragma unroll
+                for (int r = 0; r < R; r++)
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int k = 0; k < P; k++) D[r][t] = g53_mfma(lv, b[t][k], D[r][t]);
-                }
-                left -= 32;
-                if (left == 0 || (c == c1 - 1 && s == steps - 1)) {     /* the group, or the wave's part, ends */
-#pragma unroll
-                    for (int r = 0; r < R; r++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float sc = g53_w4_scale(a, srow[r][i] * a.groups + g);
-                            const float nz = a.z ? -16.0f - (float)((a.z[srow[r][i] * zrow + (g >> 1)] >> (4 * (g & 1))) & 15)
-                                                 : -24.0f;
-#pragma unroll
-                            for (int t = 0; t < NT; t++)
-                                acc[r][t][i] = __builtin_fmaf(sc, __builtin_fmaf(nz, X[t][i], D[r][t][i]), acc[r][t][i]);
-                        }
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        X[t] = zero;
-#pragma unroll
-                        for (int r = 0; r < R; r++) D[r][t] = zero;
-                    }
-                    left = a.group;
-                    g++;
-                }
-            }
+                        for (int i = 0; i < 4; i++)
+                            acc[r][t][i] = __builtin_fmaf(sc[r][s], __builtin_fmaf(nz[r][s], X[t][i], D[r][t][i]), acc[r][t][i]);
         }
+    };
+    Chunk ring[PF];
+#pragma unroll
+    for (int i = 0; i < PF; i++) load(ring[i], kw + i * KW);
+    for (int seg0 = 0; seg0 < chunks; seg0 += a.seg) {
+        /* the segment's activations, turned into planes in the levels' order */
+        const int here = chunks - seg0 < a.seg ? chunks - seg0 : a.seg, k0 = seg0 * 128, n8 = here * 16;
+        if (seg0) __syncthreads();
+        for (int u = tid; u < rows * n8; u += 64 * NW) {
+            const int i = u / n8, c8 = u - i * n8;
+            int p = first + i;
+            if (a.pair) p = a.pair[p] / a.topk;
+            g53_v4w v[sizeof(E) / 2];
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(E) / 2; j++) {
+                v[j] = (g53_v4w){0, 0, 0, 0};
+                if (k0 + c8 * 8 < a.cols) v[j] = ((const G53v4w_any *)(x + (long)p * a.cols + k0 + c8 * 8))[j].v;
+            }
+            V b[P];
+            g53_w4_x(b, v);
+#pragma unroll
+            for (int j = 0; j < P; j++) *(V *)(lds + j * plane + i * ld + c8 * 16) = b[j];
+        }
+        __syncthreads();
+        /* Whole turns of the ring ask for the turn after them; the last of all does not, and may be short. Segments but
+         * the last are whole turns. */
+        const bool ends = seg0 + here == chunks;
+        const int until = ends ? here - PF * KW : here;
+        int i = kw;
+        for (; i < until; i += PF * KW)
+#pragma unroll
+            for (int j = 0; j < PF; j++) {
+                use(ring[j], seg0 + i + j * KW, i + j * KW);
+                load(ring[j], seg0 + i + (j + PF) * KW);
+            }
+        if (ends)
+#pragma unroll
+            for (int j = 0; j < PF; j++)
+                if (i + j * KW < here) use(ring[j], seg0 + i + j * KW, i + j * KW);
     }
+    __syncthreads();
+    float *red = (float *)lds;              /* [NW][TT][LD] */
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int t = 0; t < NT; t++) *(g53_v4f *)&red[wv][16 * t + m][16 * r + 4 * q] = acc[r][t];
-    __syncthreads();
-    for (int i = tid; i < TT * OUT; i += 64 * NW) {
-        const int t = i / OUT, r = i % OUT;
-        float v = 0.0f, u = 0.0f;
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int w = 0; w < NW; w++) {
-            v += red[w][t][r];
-            if (SW) u += red[w][t][OUT + r];
+            for (int i = 0; i < 4; i++) red[(wv * TT + 16 * t + 4 * q + i) * LD + 16 * r + m] = acc[r][t][i];
+    __syncthreads();
+    const int outs = out * RW, base = tile * outs;
+    for (int i = tid; i < rows * outs; i += 64 * NW) {
+        const int t = i / outs, o = i - t * outs, w = o / out, r = o % out;
+        float v = 0.0f, u = 0.0f;
+        for (int k = 0; k < KW; k++) {
+            v += red[((w * KW + k) * TT + t) * LD + r];
+            if (sw) u += red[((w * KW + k) * TT + t) * LD + out + r];
         }
-        if (SW) {
+        if (sw) {
             v = v > a.limit ? a.limit : v;
             u = u > a.limit ? a.limit : (u < -a.limit ? -a.limit : u);
             v = v / (1.0f + expf(-v)) * u;
         }
-        if (first + t < last && row0 + r < a.half) y[(long)(first + t) * a.half + row0 + r] = (E)v;
+        if (base + o < a.half) y[(long)(first + t) * a.half + base + o] = (E)v;
     }
 }
 
-template <typename E, int R, int NT, int NW> static int launch(void *y, const void *x, G53W4Args &a, long items)
+template <typename E, int R, int NT, int PF, int GS>
+static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const G53W4Args &a)
 {
+    static int allowed = 0;
+    if (!allowed) {
+        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, PF, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    G53_W4_LDS_MAX));
+        allowed = 1;
+    }
+    hipLaunchKernelGGL((k_w4<E, R, NT, PF, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x, a);
+    G53_LAUNCHED("k_w4");
+    return 0;
+}
+
+/* busy: token tiles that are expected to hold rows. */
+template <typename E, int R, int NT, int PF> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
+{
+    constexpr int P = G53W4Type<E>::P, TT = 16 * NT;
     const bool sw = a.limit > 0.0f;
-    const int out = sw ? 8 * R : 16 * R;
-    a.tiles = (a.half + out - 1) / out;
-    const long most = (1l << 31) / (64 * NW) / a.tiles;      /* token tiles of one launch: threads fit 32 bits */
+    const int out = sw ? 8 * R : 16 * R, chunks = (a.cols + 127) / 128, rows = a.T < TT ? a.T : TT;
+    /* While there are fewer than two workgroups a CU, they get fewer rows: their waves split the columns instead, as long
+     * as a part keeps two chunks and its share of x fits LDS, and then there are fewer waves. */
+    int k = 0, rw = G53_W4_NW;
+    while (rw > 1 && busy * ((a.half + out * rw - 1) / (out * rw)) < 2 * g53h_num_cus()) {
+        if ((4 << k) <= chunks && rows * P * ((PF << (k + 1)) * 256 + 16) <= G53_W4_LDS_MAX) k++;
+        rw /= 2;
+    }
+    const int waves = rw << k, outs = out * rw, unit = PF << k;
+    a.kw_log = k;
+    a.tiles = (a.half + outs - 1) / outs;
+    int seg = (G53_W4_LDS / (rows * P) - 16) / 256 / unit * unit;      /* chunks of x in LDS: whole turns of the ring */
+    if (seg < unit) seg = unit;
+    if (seg > chunks) seg = chunks;
+    a.seg = seg;
+    size_t lds = (size_t)rows * P * (seg * 256 + 16), red = (size_t)waves * TT * (16 * R + 4) * 4;
+    if (lds < red) lds = red;
+    const long most = (1l << 31) / (64 * G53_W4_NW) / a.tiles;      /* token tiles of one launch: threads fit 32 bits */
     if (most < 1) return g53h_fail("g53h_mm_w4: %d rows", a.rows);
     for (long i = 0; i < items; i += most) {
         a.item0 = i;
-        const dim3 grid((unsigned)((items - i < most ? items - i : most) * a.tiles)), block(64 * NW);
-        if (sw) hipLaunchKernelGGL((k_w4<E, R, NT, NW, true>), grid, block, 0, g53h_stream(), (E *)y, (const E *)x, a);
-        else hipLaunchKernelGGL((k_w4<E, R, NT, NW, false>), grid, block, 0, g53h_stream(), (E *)y, (const E *)x, a);
-        G53_LAUNCHED("k_w4");
+        const dim3 grid((unsigned)((items - i < most ? items - i : most) * a.tiles));
+        const int rc = a.group % 128 == 0 ? start<E, R, NT, PF, 4>(grid, waves, lds, y, x, a)
+                       : a.group % 64 == 0 ? start<E, R, NT, PF, 2>(grid, waves, lds, y, x, a)
+                                           : start<E, R, NT, PF, 1>(grid, waves, lds, y, x, a);
+        if (rc) return rc;
     }
     return 0;
 }
 
-/* Tokens, or sorted rows, of the busiest matrix decide the tile. */
+/* Token tiles of 16, 32 or 64: by the tokens, or by the mean rows of an expert. */
+template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
+{
+    constexpr int PF = 2;
+    const long ex = a.offsets ? (a.n_experts < a.T ? a.n_experts : a.T) : 1, mean = (a.T + ex - 1) / ex;
+    const int nt = mean <= 16 ? 1 : (mean <= 32 || sizeof(E) == 4 ? 2 : 4), TT = 16 * nt;
+    const long items = a.offsets ? a.T / TT + ex : (a.T + TT - 1) / TT, busy = ex * ((mean + TT - 1) / TT);
+    if (nt == 1) return launch<E, 2, 1, PF>(y, x, a, items, busy);
+    if constexpr (sizeof(E) == 2)
+        if (nt == 4) return launch<E, 2, 4, 2>(y, x, a, items, busy);
+    return launch<E, 2, 2, 2>(y, x, a, items, busy);
+}
+
 static int product(void *y, const void *x, int dt, G53W4Args &a)
 {
-    constexpr int NT = 1;
-    const long tiles = ((long)a.T + 16 * NT - 1) / (16 * NT);
-    const long items = a.offsets ? tiles + (a.n_experts < a.T ? a.n_experts : a.T) : tiles;
     if (g53h_ready()) return -1;
     int rc;
-    G53_BY_TYPE(dt, rc = (launch<E, 2, NT, 8>(y, x, a, items)));
+    G53_BY_TYPE(dt, rc = by_tokens<E>(y, x, a));
     return rc;
 }
 
 static int w4_bad(const char *who, const G53hW4 *m, int dt, float limit, G53W4Args &a)
 {
     if (!m || !m->w || !m->s) return g53h_fail("%s: unbound matrix", who);
-    if (m->rows < 1 || m->cols < 32 || m->cols % 32 || m->group < 32 || m->group % 32 || !g53_elem_bytes(m->s_dt))
-        return g53h_fail("%s: %d x %d levels in groups of %d, scale type %d (columns and group multiples of 32)", who, m->rows,
+    if (m->rows < 1 || m->cols < 32 || m->cols > G53_W4_MAXC || m->cols % 32 || m->group < 32 || m->group % 32 || !g53_elem_bytes(m->s_dt))
+        return g53h_fail("%s: %d x %d levels in groups of %d, scale type %d (columns and group multiples of 32, columns at most 2^24)", who, m->rows,
                          m->cols, m->group, m->s_dt);
     if (((uintptr_t)m->w & 15) || ((uintptr_t)m->s & (g53_elem_bytes(m->s_dt) - 1)))
         return g53h_fail("%s: levels must start at a multiple of 16 bytes, scales of their type", who);
@@ -334,12 +453,13 @@ static int w4_bad(const char *who, const G53hW4 *m, int dt, float limit, G53W4Ar
     a.group = m->group < m->cols ? m->group : m->cols;
     a.groups = (m->cols - 1) / a.group + 1;
     a.s_dt = m->s_dt;
+    a.glog = (a.group & (a.group - 1)) ? -1 : __builtin_ctz(a.group) - 5;
     a.limit = limit;
     a.half = limit > 0.0f ? m->rows / 2 : m->rows;
     a.offsets = a.pair = nullptr;
     a.n_experts = a.topk = 1;
     a.item0 = 0;
-    a.tiles = 0;
+    a.tiles = a.kw_log = a.seg = 0;
     return 0;
 }
 
