@@ -43,15 +43,15 @@ struct G53W4Args {
     int tiles;                          /* row tiles                                          */
     int kw_log;                         /* log2 of the parts that a workgroup's waves split the columns into */
     int glog;                           /* log2 of group / 32 where it is a power of two, else -1 */
-    int seg;                            /* chunks of 128 columns whose activations LDS holds  */
+    int seg;                            /* units of columns whose activations LDS holds       */
 };
 
 typedef unsigned int g53_v2w __attribute__((ext_vector_type(2)));
 
-template <typename E> struct G53W4Type;   /* the 16-bit type of the products, planes per value */
-template <> struct G53W4Type<float> { typedef g53_v8b V; static constexpr int P = 3; };
-template <> struct G53W4Type<g53_bf16> { typedef g53_v8b V; static constexpr int P = 1; };
-template <> struct G53W4Type<g53_f16> { typedef g53_v8h V; static constexpr int P = 1; };
+template <typename E> struct G53W4Type;   /* the 16-bit type of the products, planes per value, chunks of a unit */
+template <> struct G53W4Type<float> { typedef g53_v8b V; static constexpr int P = 3, UC = 2; };
+template <> struct G53W4Type<g53_bf16> { typedef g53_v8b V; static constexpr int P = 1, UC = 4; };
+template <> struct G53W4Type<g53_f16> { typedef g53_v8h V; static constexpr int P = 1, UC = 4; };
 
 __device__ __forceinline__ g53_v4f g53_mfma(g53_v8b a, g53_v8b b, g53_v4f c)
 {
@@ -62,20 +62,24 @@ __device__ __forceinline__ g53_v4f g53_mfma(g53_v8h a, g53_v8h b, g53_v4f c)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-/* Eight levels (nibbles 0..7 of d) as 16 + level, in the order 0 4 1 5 2 6 3 7. */
-template <typename V> __device__ __forceinline__ V g53_w4_levels(unsigned d);
-template <> __device__ __forceinline__ g53_v8b g53_w4_levels<g53_v8b>(unsigned d)
+/* Eight levels (nibbles 0..7 of d) as 16 + level, in the order 0 4 1 5 2 6 3 7. mask picks the mantissa bits, one a
+ * half; it comes in a vector register, so that and and or are one instruction (which takes one scalar and no literal). */
+template <typename V> __device__ __forceinline__ V g53_w4_levels(unsigned d, unsigned mask);
+template <> __device__ __forceinline__ g53_v8b g53_w4_levels<g53_v8b>(unsigned d, unsigned mask)
 {
-    const unsigned m = 0x00780078u, o = 0x41804180u;          /* bf16 16.0, mantissa bits 6..3 */
-    return __builtin_bit_cast(g53_v8b, (g53_v4w){((d << 3) & m) | o, ((d >> 1) & m) | o, ((d >> 5) & m) | o,
-                                                 ((d >> 9) & m) | o});
+    const unsigned o = 0x41804180u;                           /* bf16 16.0, mantissa bits 6..3 */
+    return __builtin_bit_cast(g53_v8b, (g53_v4w){((d << 3) & mask) | o, ((d >> 1) & mask) | o, ((d >> 5) & mask) | o,
+                                                 ((d >> 9) & mask) | o});
 }
-template <> __device__ __forceinline__ g53_v8h g53_w4_levels<g53_v8h>(unsigned d)
+template <> __device__ __forceinline__ g53_v8h g53_w4_levels<g53_v8h>(unsigned d, unsigned mask)
 {
-    const unsigned m = 0x03c003c0u, o = 0x4c004c00u;          /* fp16 16.0, mantissa bits 9..6 */
-    return __builtin_bit_cast(g53_v8h, (g53_v4w){((d << 6) & m) | o, ((d << 2) & m) | o, ((d >> 2) & m) | o,
-                                                 ((d >> 6) & m) | o});
+    const unsigned o = 0x4c004c00u;                           /* fp16 16.0, mantissa bits 9..6 */
+    return __builtin_bit_cast(g53_v8h, (g53_v4w){((d << 6) & mask) | o, ((d << 2) & mask) | o, ((d >> 2) & mask) | o,
+                                                 ((d >> 6) & mask) | o});
 }
+template <typename V> struct G53W4Mask;
+template <> struct G53W4Mask<g53_v8b> { static constexpr unsigned M = 0x00780078u; };
+template <> struct G53W4Mask<g53_v8h> { static constexpr unsigned M = 0x03c003c0u; };
 
 /* Eight activations in the levels' order, as P planes of the products' type. */
 template <typename V> __device__ __forceinline__ void g53_w4_x(V (&o)[1], const g53_v4w (&p)[1])
@@ -149,7 +153,8 @@ __device__ __forceinline__ bool g53_w4_item(const G53W4Args &a, long item, int T
     return true;
 }
 
-/* What a wave has asked for of 128 columns: levels, scales and zero points of its row tiles as they lie. */
+/* What a wave has asked for of 128 columns: levels of its row tiles as they lie, and, where the columns lie in several
+ * groups, their scales and zero points. */
 template <int R> struct G53W4Chunk {
     g53_v4w w[R];
     unsigned s[R], z[R];
@@ -158,15 +163,26 @@ template <int R> struct G53W4Chunk {
 /* n / d for 0 <= n, by a shift where d is a power of two (log >= 0). */
 __device__ __forceinline__ int g53_quot(int n, int d, int log) { return log >= 0 ? n >> log : n / d; }
 
+/* Every quarter's v to all lanes of its row: o[i] is quarter i's. */
+__device__ __forceinline__ void g53_spread(float (&o)[4], float v)
+{
+    unsigned u[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) u[i] = __builtin_bit_cast(unsigned, v);
+    g53_turn(u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = __builtin_bit_cast(float, u[i]);
+}
+
 /* One workgroup: up to 16 NT tokens (or sorted rows of one expert) by `out` (NW / KW) rows. Its waves are KW parts of the
- * columns, taken in turn 128 columns each, by NW / KW groups of R row tiles. PF chunks are asked for ahead. GS: groups
- * are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows, the others the same
- * up rows. Columns behind the last of a chunk meet activations of zero. */
-template <typename E, int R, int NT, int PF, int GS>
+ * columns, in units of UC x 128 taken in turn, by NW / KW groups of R row tiles. A unit's levels are asked for one unit
+ * ahead. GS: groups are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows,
+ * the others the same up rows. Columns behind the last of a unit meet activations of zero. */
+template <typename E, int R, int NT, int GS>
 __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2) k_w4(E *__restrict__ y, const E *__restrict__ x, G53W4Args a)
 {
     typedef typename G53W4Type<E>::V V;
-    constexpr int P = G53W4Type<E>::P, TT = 16 * NT, LD = 16 * R + 4;
+    constexpr int P = G53W4Type<E>::P, UC = G53W4Type<E>::UC, TT = 16 * NT, LD = 16 * R + 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const bool sw = a.limit > 0.0f;
     const int out = sw ? 8 * R : 16 * R;                     /* result rows of a wave */
@@ -201,7 +217,6 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
         s_of[r] = i * srow;
         z_of[r] = i * zrow;
     }
-    const unsigned z_mask = a.z ? 15u : 0u, z_no = a.z ? 0u : 8u;
     g53_v4f acc[R][NT];
     const g53_v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -211,62 +226,67 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     V ones;
 #pragma unroll
     for (int i = 0; i < 8; i++) ones[i] = 1.0f;
-    const int chunks = (a.cols + 127) / 128;
-    typedef G53W4Chunk<R> Chunk;
+    unsigned mask = G53W4Mask<V>::M;
+    asm volatile("" : "+v"(mask));
+    const int units = (a.cols + 128 * UC - 1) / (128 * UC);
 
-    /* the lane's group in chunk c: the chunk's, or that of its quarter q */
+    /* scales and zero points of a group, as they lie, and as they enter: s and -(16 + z) */
+    auto ask = [&](unsigned (&ks)[R], unsigned (&kz)[R], int g) {
+        if (a.s_dt == G53H_F32)
+#pragma unroll
+            for (int r = 0; r < R; r++) ks[r] = *(const unsigned *)(sb[r] + (unsigned)(s_of[r] + g * 4));
+        else
+#pragma unroll
+            for (int r = 0; r < R; r++) ks[r] = *(const uint16_t *)(sb[r] + (unsigned)(s_of[r] + g * 2));
+        if (a.z)
+#pragma unroll
+            for (int r = 0; r < R; r++) kz[r] = zb[r][(unsigned)(z_of[r] + (g >> 1))];
+    };
+    /* a scale as it lies to fp32, without a branch: fp32 as it is, bf16 shifted, fp16 converted */
+    const int s_shift = a.s_dt == G53H_BF16 ? 16 : 0;
+    const unsigned s_f16 = a.s_dt == G53H_F16 ? ~0u : 0u, z_mask = a.z ? 15u : 0u, z_no = a.z ? 0u : 8u;
+    auto scale = [&](unsigned v) {
+        const float f16 = (float)__builtin_bit_cast(g53_f16, (uint16_t)v);
+        return __builtin_bit_cast(float, (v << s_shift & ~s_f16) | (__builtin_bit_cast(unsigned, f16) & s_f16));
+    };
+    auto surplus = [&](unsigned v, int g) { return -16.0f - (float)((v >> (4 * (g & 1)) & z_mask) | z_no); };
+    /* the lane's group in chunk c: that of its quarter; in unit u: that of chunk q */
     auto group_of = [&](int c) {
-        if (GS == 4) return g53_quot(c * 4, a.group / 32, a.glog);
         const int g = g53_quot(c * 4 + q, a.group / 32, a.glog);
         return g < a.groups ? g : a.groups - 1;
     };
-    /* c behind the last chunk: that one again, never used */
+    auto unit_group = [&](int u) {
+        const int g = g53_quot((u * UC + q) * 4, a.group / 32, a.glog);
+        return g < a.groups ? g : a.groups - 1;
+    };
+    typedef G53W4Chunk<R> Chunk;
     auto load = [&](Chunk &k, int c) {
-        c = c < chunks ? c : chunks - 1;
-        const int g = group_of(c), w_at = c * 64 + q * 16, wo = w_at < wrow ? w_at : 0;
+        const int w_at = c * 64 + q * 16, wo = w_at < wrow ? w_at : 0;
 #pragma unroll
         for (int r = 0; r < R; r++) k.w[r] = __builtin_nontemporal_load((const g53_v4w *)(wb[r] + (unsigned)(w_of[r] + wo)));
-        if (a.s_dt == G53H_F32)
-#pragma unroll
-            for (int r = 0; r < R; r++) k.s[r] = *(const unsigned *)(sb[r] + (unsigned)(s_of[r] + g * 4));
-        else
-#pragma unroll
-            for (int r = 0; r < R; r++) k.s[r] = *(const uint16_t *)(sb[r] + (unsigned)(s_of[r] + g * 2));
-        if (a.z)
-#pragma unroll
-            for (int r = 0; r < R; r++) k.z[r] = zb[r][(unsigned)(z_of[r] + (g >> 1))];
+        if (GS < 4) ask(k.s, k.z, group_of(c));
     };
-    const int ld = a.seg * 256 + 16;        /* bytes of a plane's row in LDS: odd sixteens, so rows start in other banks */
+    const int ld = a.seg * (256 * UC) + 16; /* bytes of a plane's row in LDS: odd sixteens, so rows start in other banks */
     int xat[NT];                            /* the lane's token in LDS; tokens behind the last repeat it */
 #pragma unroll
-    for (int t = 0; t < NT; t++) xat[t] = (16 * t + m < rows ? 16 * t + m : rows - 1) * ld + q * 16;
+    for (int t = 0; t < NT; t++) xat[t] = (16 * t + m < rows ? 16 * t + m : rows - 1) * ld + q * (GS == 4 ? 64 : 16);
     const int plane = rows * ld;
-    /* a scale as it lies to fp32, without a branch: fp32 as it is, bf16 shifted, fp16 converted */
-    const int s_shift = a.s_dt == G53H_BF16 ? 16 : 0;
-    const unsigned s_f16 = a.s_dt == G53H_F16 ? ~0u : 0u;
-    auto use = [&](const Chunk &k, int c, int c_lds) {
+    /* sc, nz: of the chunk, GS = 4. Step s takes the columns of register s: 8 from each quarter's 32 where the chunk lies
+     * in one group, else turned to 32 in a row. */
+    auto use = [&](const Chunk &k, int c, int c_lds, const float (&sc4)[R], const float (&nz4)[R]) {
         unsigned d[R][4];
         float sc[R][4], nz[R][4];
-        const int g4 = 4 * (group_of(c) & 1);
 #pragma unroll
         for (int r = 0; r < R; r++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) d[r][i] = k.w[r][i];
-            g53_turn(d[r]);
-            const float f16 = (float)__builtin_bit_cast(g53_f16, (uint16_t)k.s[r]);
-            const unsigned f = (k.s[r] << s_shift & ~s_f16) | (__builtin_bit_cast(unsigned, f16) & s_f16);
-            const float n = -16.0f - (float)((k.z[r] >> g4 & z_mask) | z_no);
             if (GS == 4) {
-                sc[r][3] = __builtin_bit_cast(float, f);
-                nz[r][3] = n;
-            } else {                    /* every quarter's to all lanes of the row */
-                unsigned u[4], v[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) { u[i] = f; v[i] = __builtin_bit_cast(unsigned, n); }
-                g53_turn(u);
-                g53_turn(v);
-#pragma unroll
-                for (int i = 0; i < 4; i++) { sc[r][i] = __builtin_bit_cast(float, u[i]); nz[r][i] = __builtin_bit_cast(float, v[i]); }
+                sc[r][3] = sc4[r];
+                nz[r][3] = nz4[r];
+            } else {
+                g53_turn(d[r]);
+                g53_spread(sc[r], scale(k.s[r]));
+                g53_spread(nz[r], surplus(k.z[r], group_of(c)));
             }
         }
         g53_v4f D[R][NT], X[NT];
@@ -277,66 +297,103 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int p = 0; p < P; p++) {
-                    b[t][p] = *(const V *)(lds + p * plane + xat[t] + c_lds * 256 + s * 64);
+                    b[t][p] = *(const V *)(lds + p * plane + xat[t] + c_lds * 256 + s * (GS == 4 ? 16 : 64));
                     X[t] = g53_mfma(b[t][p], ones, s % GS == 0 && p == 0 ? zero : X[t]);
                 }
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                const V lv = g53_w4_levels<V>(d[r][s]);
+                const V lv = g53_w4_levels<V>(d[r][s], mask);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int p = 0; p < P; p++) D[r][t] = g53_mfma(b[t][p], lv, s % GS == 0 && p == 0 ? zero : D[r][t]);
             }
-            if (NT * P > 2 || GS < 4) __builtin_amdgcn_sched_barrier(0);     /* one step's activations in registers at a time */
+            if (NT * P > 2) __builtin_amdgcn_sched_barrier(0);     /* one step's activations in registers at a time */
             if (s % GS == GS - 1)       /* a group, or what the chunk has of it */
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
-                    for (int t = 0; t < NT; t++)
+                    for (int t = 0; t < NT; t++) {
 #pragma unroll
                         for (int i = 0; i < 4; i++)
                             acc[r][t][i] = __builtin_fmaf(sc[r][s], __builtin_fmaf(nz[r][s], X[t][i], D[r][t][i]), acc[r][t][i]);
+                        asm volatile("" : "+v"(acc[r][t]));      /* added here, not behind the next branch with D kept */
+                    }
+        }
+        __builtin_amdgcn_sched_barrier(0);      /* no work on the next chunk, which may not be there yet, before this is done */
+    };
+    Chunk ring[UC];
+    unsigned us[R], uz[R];                  /* a unit's scales, GS = 4: quarter i holds those of chunk i */
+    auto unit_scales = [&](int u, float (&sc)[R][4], float (&nz)[R][4]) {
+        if (GS < 4) return;
+        const int g = unit_group(u);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            g53_spread(sc[r], scale(us[r]));
+            g53_spread(nz[r], surplus(uz[r], g));
         }
     };
-    Chunk ring[PF];
+    if (kw < units) {
+        if (GS == 4) ask(us, uz, unit_group(kw));
 #pragma unroll
-    for (int i = 0; i < PF; i++) load(ring[i], kw + i * KW);
-    for (int seg0 = 0; seg0 < chunks; seg0 += a.seg) {
-        /* the segment's activations, turned into planes in the levels' order */
-        const int here = chunks - seg0 < a.seg ? chunks - seg0 : a.seg, k0 = seg0 * 128, n8 = here * 16;
+        for (int j = 0; j < UC; j++) load(ring[j], kw * UC + j);
+    }
+    for (int seg0 = 0; seg0 < units; seg0 += a.seg) {
+        /* the segment's activations, turned into planes in the levels' order; four to eight loads a thread in flight */
+        const int here = units - seg0 < a.seg ? units - seg0 : a.seg, k0 = seg0 * (128 * UC), n8 = here * (16 * UC);
         if (seg0) __syncthreads();
-        for (int u = tid; u < rows * n8; u += 64 * NW) {
-            const int i = u / n8, c8 = u - i * n8;
-            int p = first + i;
-            if (a.pair) p = a.pair[p] / a.topk;
-            g53_v4w v[sizeof(E) / 2];
+        for (int u0 = tid; u0 < rows * n8; u0 += 256 * NW) {
+            g53_v4w v[4][sizeof(E) / 2];
+            int at[4];
 #pragma unroll
-            for (int j = 0; j < (int)sizeof(E) / 2; j++) {
-                v[j] = (g53_v4w){0, 0, 0, 0};
-                if (k0 + c8 * 8 < a.cols) v[j] = ((const G53v4w_any *)(x + (long)p * a.cols + k0 + c8 * 8))[j].v;
+            for (int k = 0; k < 4; k++) {
+                const int u = u0 + k * 64 * NW, i = u / n8, c8 = u - i * n8;
+                at[k] = i < rows ? i * ld + c8 * 16 : -1;
+#pragma unroll
+                for (int j = 0; j < (int)sizeof(E) / 2; j++) v[k][j] = (g53_v4w){0, 0, 0, 0};
+                if (i < rows && k0 + c8 * 8 < a.cols) {
+                    int p = first + i;
+                    if (a.pair) p = a.pair[p] / a.topk;
+#pragma unroll
+                    for (int j = 0; j < (int)sizeof(E) / 2; j++)
+                        v[k][j] = ((const G53v4w_any *)(x + (long)p * a.cols + k0 + c8 * 8))[j].v;
+                }
             }
-            V b[P];
-            g53_w4_x(b, v);
 #pragma unroll
-            for (int j = 0; j < P; j++) *(V *)(lds + j * plane + i * ld + c8 * 16) = b[j];
+            for (int k = 0; k < 4; k++)
+                if (at[k] >= 0) {
+                    V b[P];
+                    g53_w4_x(b, v[k]);
+#pragma unroll
+                    for (int j = 0; j < P; j++) *(V *)(lds + j * plane + at[k]) = b[j];
+                }
         }
         __syncthreads();
-        /* Whole turns of the ring ask for the turn after them; the last of all does not, and may be short. Segments but
-         * the last are whole turns. */
-        const bool ends = seg0 + here == chunks;
-        const int until = ends ? here - PF * KW : here;
+        /* every unit asks for the wave's next one, but for the last of all; segments but the last are whole turns */
+        const bool ends = seg0 + here == units;
+        const int until = ends ? here - KW : here;
         int i = kw;
-        for (; i < until; i += PF * KW)
+        float sc[R][4], nz[R][4], sj[R], nj[R];
+        for (; i < until; i += KW) {
+            unit_scales(seg0 + i, sc, nz);
+            if (GS == 4) ask(us, uz, unit_group(seg0 + i + KW));
 #pragma unroll
-            for (int j = 0; j < PF; j++) {
-                use(ring[j], seg0 + i + j * KW, i + j * KW);
-                load(ring[j], seg0 + i + (j + PF) * KW);
+            for (int j = 0; j < UC; j++) {
+#pragma unroll
+                for (int r = 0; r < R; r++) { sj[r] = sc[r][j]; nj[r] = nz[r][j]; }
+                use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, nj);
+                load(ring[j], (seg0 + i + KW) * UC + j);
             }
-        if (ends)
+        }
+        if (ends && i < here) {
+            unit_scales(seg0 + i, sc, nz);
 #pragma unroll
-            for (int j = 0; j < PF; j++)
-                if (i + j * KW < here) use(ring[j], seg0 + i + j * KW, i + j * KW);
+            for (int j = 0; j < UC; j++) {
+#pragma unroll
+                for (int r = 0; r < R; r++) { sj[r] = sc[r][j]; nj[r] = nz[r][j]; }
+                use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, nj);
+            }
+        }
     }
     __syncthreads();
     float *red = (float *)lds;              /* [NW][TT][LD] */
@@ -364,50 +421,50 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     }
 }
 
-template <typename E, int R, int NT, int PF, int GS>
+template <typename E, int R, int NT, int GS>
 static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const G53W4Args &a)
 {
     static int allowed = 0;
     if (!allowed) {
-        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, PF, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                     G53_W4_LDS_MAX));
         allowed = 1;
     }
-    hipLaunchKernelGGL((k_w4<E, R, NT, PF, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x, a);
+    hipLaunchKernelGGL((k_w4<E, R, NT, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x, a);
     G53_LAUNCHED("k_w4");
     return 0;
 }
 
 /* busy: token tiles that are expected to hold rows. */
-template <typename E, int R, int NT, int PF> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
+template <typename E, int R, int NT> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
 {
-    constexpr int P = G53W4Type<E>::P, TT = 16 * NT;
+    constexpr int P = G53W4Type<E>::P, UC = G53W4Type<E>::UC, TT = 16 * NT;
     const bool sw = a.limit > 0.0f;
-    const int out = sw ? 8 * R : 16 * R, chunks = (a.cols + 127) / 128, rows = a.T < TT ? a.T : TT;
+    const int out = sw ? 8 * R : 16 * R, units = (a.cols + 128 * UC - 1) / (128 * UC), rows = a.T < TT ? a.T : TT;
     /* While there are fewer than two workgroups a CU, they get fewer rows: their waves split the columns instead, as long
-     * as a part keeps two chunks and its share of x fits LDS, and then there are fewer waves. */
+     * as every part has a unit and its share of x fits LDS, and then there are fewer waves. */
     int k = 0, rw = G53_W4_NW;
     while (rw > 1 && busy * ((a.half + out * rw - 1) / (out * rw)) < 2 * g53h_num_cus()) {
-        if ((4 << k) <= chunks && rows * P * ((PF << (k + 1)) * 256 + 16) <= G53_W4_LDS_MAX) k++;
+        if ((2 << k) <= units && rows * P * ((2 << k) * 256 * UC + 16) <= G53_W4_LDS_MAX) k++;
         rw /= 2;
     }
-    const int waves = rw << k, outs = out * rw, unit = PF << k;
+    const int waves = rw << k, outs = out * rw;
     a.kw_log = k;
     a.tiles = (a.half + outs - 1) / outs;
-    int seg = (G53_W4_LDS / (rows * P) - 16) / 256 / unit * unit;      /* chunks of x in LDS: whole turns of the ring */
-    if (seg < unit) seg = unit;
-    if (seg > chunks) seg = chunks;
+    int seg = (G53_W4_LDS / (rows * P) - 16) / (256 * UC) >> k << k;    /* units of x in LDS: whole turns */
+    if (seg < 1 << k) seg = 1 << k;
+    if (seg > units) seg = units;
     a.seg = seg;
-    size_t lds = (size_t)rows * P * (seg * 256 + 16), red = (size_t)waves * TT * (16 * R + 4) * 4;
+    size_t lds = (size_t)rows * P * (seg * 256 * UC + 16), red = (size_t)waves * TT * (16 * R + 4) * 4;
     if (lds < red) lds = red;
     const long most = (1l << 31) / (64 * G53_W4_NW) / a.tiles;      /* token tiles of one launch: threads fit 32 bits */
     if (most < 1) return g53h_fail("g53h_mm_w4: %d rows", a.rows);
     for (long i = 0; i < items; i += most) {
         a.item0 = i;
         const dim3 grid((unsigned)((items - i < most ? items - i : most) * a.tiles));
-        const int rc = a.group % 128 == 0 ? start<E, R, NT, PF, 4>(grid, waves, lds, y, x, a)
-                       : a.group % 64 == 0 ? start<E, R, NT, PF, 2>(grid, waves, lds, y, x, a)
-                                           : start<E, R, NT, PF, 1>(grid, waves, lds, y, x, a);
+        const int rc = a.group % 128 == 0 ? start<E, R, NT, 4>(grid, waves, lds, y, x, a)
+                       : a.group % 64 == 0 ? start<E, R, NT, 2>(grid, waves, lds, y, x, a)
+                                           : start<E, R, NT, 1>(grid, waves, lds, y, x, a);
         if (rc) return rc;
     }
     return 0;
@@ -416,14 +473,13 @@ template <typename E, int R, int NT, int PF> static int launch(void *y, const vo
 /* Token tiles of 16, 32 or 64: by the tokens, or by the mean rows of an expert. */
 template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
 {
-    constexpr int PF = 2;
     const long ex = a.offsets ? (a.n_experts < a.T ? a.n_experts : a.T) : 1, mean = (a.T + ex - 1) / ex;
     const int nt = mean <= 16 ? 1 : (mean <= 32 || sizeof(E) == 4 ? 2 : 4), TT = 16 * nt;
     const long items = a.offsets ? a.T / TT + ex : (a.T + TT - 1) / TT, busy = ex * ((mean + TT - 1) / TT);
-    if (nt == 1) return launch<E, 2, 1, PF>(y, x, a, items, busy);
+    if (nt == 1) return launch<E, 2, 1>(y, x, a, items, busy);
     if constexpr (sizeof(E) == 2)
-        if (nt == 4) return launch<E, 2, 4, 2>(y, x, a, items, busy);
-    return launch<E, 2, 2, 2>(y, x, a, items, busy);
+        if (nt == 4) return launch<E, 2, 4>(y, x, a, items, busy);
+    return launch<E, 2, 2>(y, x, a, items, busy);
 }
 
 static int product(void *y, const void *x, int dt, G53W4Args &a)
