@@ -40,7 +40,7 @@ struct G53W4Args {
     const int *pair;                    /* sorted rows taken from tokens: pair / topk, or NULL */
     int n_experts, topk;
     long item0;                         /* first token tile of the launch                     */
-    int tiles;                          /* row tiles                                          */
+    int tiles, items;                   /* row tiles, token tiles of the launch               */
     int kw_log;                         /* log2 of the parts that a workgroup's waves split the columns into */
     int glog;                           /* log2 of group / 32 where it is a power of two, else -1 */
     int seg;                            /* units of columns whose activations LDS holds       */
@@ -48,10 +48,10 @@ struct G53W4Args {
 
 typedef unsigned int g53_v2w __attribute__((ext_vector_type(2)));
 
-template <typename E> struct G53W4Type;   /* the 16-bit type of the products, planes per value, chunks of a unit */
-template <> struct G53W4Type<float> { typedef g53_v8b V; static constexpr int P = 3, UC = 2; };
-template <> struct G53W4Type<g53_bf16> { typedef g53_v8b V; static constexpr int P = 1, UC = 4; };
-template <> struct G53W4Type<g53_f16> { typedef g53_v8h V; static constexpr int P = 1, UC = 4; };
+template <typename E> struct G53W4Type;   /* the 16-bit type of the products, planes per value */
+template <> struct G53W4Type<float> { typedef g53_v8b V; static constexpr int P = 3; };
+template <> struct G53W4Type<g53_bf16> { typedef g53_v8b V; static constexpr int P = 1; };
+template <> struct G53W4Type<g53_f16> { typedef g53_v8h V; static constexpr int P = 1; };
 
 __device__ __forceinline__ g53_v4f g53_mfma(g53_v8b a, g53_v8b b, g53_v4f c)
 {
@@ -125,12 +125,16 @@ __device__ __forceinline__ void g53_turn(unsigned (&d)[4])
 }
 
 /* The token tile `item` of the sorted rows: tiles of TT rows, expert by expert. False behind the last. */
-__device__ __forceinline__ bool g53_w4_item(const G53W4Args &a, long item, int TT, int &e, int &first, int &last)
+__device__ __forceinline__ bool g53_w4_item(const int *__restrict__ offsets, int n_experts, long item, int TT, int &e, int &first, int &last)
 {
-    const int lane = threadIdx.x & 63, per = (a.n_experts + 63) / 64, e0 = lane * per;
-    int n = 0;
-    for (int i = 0; i < per; i++)
-        if (e0 + i < a.n_experts) n += (a.offsets[e0 + i + 1] - a.offsets[e0 + i] + TT - 1) / TT;
+    const int lane = threadIdx.x & 63, per = (n_experts + 63) / 64, e0 = lane * per;
+    int n = 0, from = e0 < n_experts ? offsets[e0] : 0;
+    for (int i = 0, at = from; i < per; i++)
+        if (e0 + i < n_experts) {
+            const int to = offsets[e0 + i + 1];
+            n += (to - at + TT - 1) / TT;
+            at = to;
+        }
     int incl = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -141,12 +145,13 @@ __device__ __forceinline__ bool g53_w4_item(const G53W4Args &a, long item, int T
     if (!in) return false;
     const int l = __builtin_ctzll(in);
     int skip = (int)item - __builtin_amdgcn_readlane(incl - n, l);
+    first = __builtin_amdgcn_readlane(from, l);
     for (e = l * per;; e++) {                 /* lane l's experts: one of them holds the tile */
-        first = a.offsets[e];
-        last = a.offsets[e + 1];
+        last = offsets[e + 1];
         const int tiles = (last - first + TT - 1) / TT;
         if (skip < tiles) break;
         skip -= tiles;
+        first = last;
     }
     first += skip * TT;
     last = first + TT < last ? first + TT : last;
@@ -179,20 +184,24 @@ __device__ __forceinline__ void g53_spread(float (&o)[4], float v)
  * ahead. GS: groups are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows,
  * the others the same up rows. Columns behind the last of a unit meet activations of zero. */
 template <typename E, int R, int NT, int GS>
-__global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2) k_w4(E *__restrict__ y, const E *__restrict__ x, G53W4Args a)
+__global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2) k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets, const int *__restrict__ pair, G53W4Args a)
 {
     typedef typename G53W4Type<E>::V V;
-    constexpr int P = G53W4Type<E>::P, UC = G53W4Type<E>::UC, TT = 16 * NT, LD = 16 * R + 4;
+    constexpr int P = G53W4Type<E>::P, UC = P == 3 ? R : 4, TT = 16 * NT, LD = 16 * R + 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const bool sw = a.limit > 0.0f;
     const int out = sw ? 8 * R : 16 * R;                     /* result rows of a wave */
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), NW = blockDim.x >> 6;
     const int m = lane & 15, q = lane >> 4, KW = 1 << a.kw_log, kw = wv & (KW - 1), rw = wv >> a.kw_log, RW = NW >> a.kw_log;
-    const long item = a.item0 + blockIdx.x / a.tiles;
-    const int tile = blockIdx.x % a.tiles;
+    /* Workgroups go to the 8 dies in turn. Of one matrix, eight row tiles go side by side and a row tile's token tiles
+     * after each other on one die, whose cache then holds the rows; of several, a token tile's row tiles follow each other. */
+    const unsigned eight = 8u * a.items;
+    const int tile = offsets ? blockIdx.x % a.tiles : blockIdx.x / eight * 8 + blockIdx.x % 8;
+    if (tile >= a.tiles) return;
+    const long item = a.item0 + (offsets ? blockIdx.x / a.tiles : blockIdx.x % eight / 8);
     int e = 0, first, last;
-    if (a.offsets) {
-        if (!g53_w4_item(a, item, TT, e, first, last)) return;
+    if (offsets) {
+        if (!g53_w4_item(offsets, a.n_experts, item, TT, e, first, last)) return;
         e = __builtin_amdgcn_readfirstlane(e);
         first = __builtin_amdgcn_readfirstlane(first);
         last = __builtin_amdgcn_readfirstlane(last);
@@ -261,7 +270,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     };
     typedef G53W4Chunk<R> Chunk;
     auto load = [&](Chunk &k, int c) {
-        const int w_at = c * 64 + q * 16, wo = w_at < wrow ? w_at : 0;
+        const int w_at = c * 64 + q * 16, wo = w_at < wrow ? w_at : 0;      /* behind the end: the row's start, never used */
 #pragma unroll
         for (int r = 0; r < R; r++) k.w[r] = __builtin_nontemporal_load((const g53_v4w *)(wb[r] + (unsigned)(w_of[r] + wo)));
         if (GS < 4) ask(k.s, k.z, group_of(c));
@@ -333,40 +342,56 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
             g53_spread(nz[r], surplus(uz[r], g));
         }
     };
-    if (kw < units) {
+    /* A segment's activations into LDS as planes in the levels' order, in pieces of 512 columns of a row, a wave's load;
+     * a wave asks for four at a time. */
+    typedef g53_v4w Piece[4][sizeof(E) / 2];
+    auto segment = [&](int seg0) { return units - seg0 < a.seg ? units - seg0 : a.seg; };
+    auto pieces_of = [&](int here) { return rows * ((here * (16 * UC) + 63) / 64); };
+    auto fetch = [&](Piece &v, int seg0, int p0) {
+        const int k0 = seg0 * (128 * UC), across = pieces_of(segment(seg0)) / rows;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int piece = p0 + k * NW, i = piece / across, at = k0 + ((piece - i * across) * 64 + lane) * 8;
+            const bool there = i < rows && at < a.cols;
+            int p = i < rows ? first + i : first;
+            if (pair) p = pair[p] / a.topk;
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(E) / 2; j++) {
+                v[k][j] = (g53_v4w){0, 0, 0, 0};
+                if (there) v[k][j] = ((const G53v4w_any *)(x + (long)p * a.cols + at))[j].v;
+            }
+        }
+    };
+    auto put = [&](Piece &v, int seg0, int p0) {
+        const int here = segment(seg0), across = pieces_of(here) / rows;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int piece = p0 + k * NW, i = piece / across, c8 = (piece - i * across) * 64 + lane;
+            if (i < rows && c8 < here * (16 * UC)) {
+                V b[P];
+                g53_w4_x(b, v[k]);
+#pragma unroll
+                for (int j = 0; j < P; j++) *(V *)(lds + j * plane + i * ld + c8 * 16) = b[j];
+            }
+        }
+    };
+    {   /* the first levels: behind the first activations, which LDS has to hold before */
+        Piece v;
+        fetch(v, 0, wv);
+        __builtin_amdgcn_sched_barrier(0);
         if (GS == 4) ask(us, uz, unit_group(kw));
 #pragma unroll
         for (int j = 0; j < UC; j++) load(ring[j], kw * UC + j);
+        __builtin_amdgcn_sched_barrier(0);
+        put(v, 0, wv);
     }
     for (int seg0 = 0; seg0 < units; seg0 += a.seg) {
-        /* the segment's activations, turned into planes in the levels' order; four to eight loads a thread in flight */
-        const int here = units - seg0 < a.seg ? units - seg0 : a.seg, k0 = seg0 * (128 * UC), n8 = here * (16 * UC);
+        const int here = segment(seg0), pieces = pieces_of(here);
         if (seg0) __syncthreads();
-        for (int u0 = tid; u0 < rows * n8; u0 += 256 * NW) {
-            g53_v4w v[4][sizeof(E) / 2];
-            int at[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int u = u0 + k * 64 * NW, i = u / n8, c8 = u - i * n8;
-                at[k] = i < rows ? i * ld + c8 * 16 : -1;
-#pragma unroll
-                for (int j = 0; j < (int)sizeof(E) / 2; j++) v[k][j] = (g53_v4w){0, 0, 0, 0};
-                if (i < rows && k0 + c8 * 8 < a.cols) {
-                    int p = first + i;
-                    if (a.pair) p = a.pair[p] / a.topk;
-#pragma unroll
-                    for (int j = 0; j < (int)sizeof(E) / 2; j++)
-                        v[k][j] = ((const G53v4w_any *)(x + (long)p * a.cols + k0 + c8 * 8))[j].v;
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (at[k] >= 0) {
-                    V b[P];
-                    g53_w4_x(b, v[k]);
-#pragma unroll
-                    for (int j = 0; j < P; j++) *(V *)(lds + j * plane + at[k]) = b[j];
-                }
+        for (int p0 = seg0 ? wv : wv + 4 * NW; p0 < pieces; p0 += 4 * NW) {
+            Piece v;
+            fetch(v, seg0, p0);
+            put(v, seg0, p0);
         }
         __syncthreads();
         /* every unit asks for the wave's next one, but for the last of all; segments but the last are whole turns */
@@ -404,9 +429,10 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
 #pragma unroll
             for (int i = 0; i < 4; i++) red[(wv * TT + 16 * t + 4 * q + i) * LD + 16 * r + m] = acc[r][t][i];
     __syncthreads();
-    const int outs = out * RW, base = tile * outs;
-    for (int i = tid; i < rows * outs; i += 64 * NW) {
-        const int t = i / outs, o = i - t * outs, w = o / out, r = o % out;
+    /* out and RW are powers of two */
+    const int out_log = __builtin_ctz(out), outs_log = out_log + __builtin_ctz(RW), base = tile << outs_log;
+    for (int i = tid; i < rows << outs_log; i += 64 * NW) {
+        const int t = i >> outs_log, o = i & ((1 << outs_log) - 1), w = o >> out_log, r = o & (out - 1);
         float v = 0.0f, u = 0.0f;
         for (int k = 0; k < KW; k++) {
             v += red[((w * KW + k) * TT + t) * LD + r];
@@ -430,7 +456,8 @@ static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const
                                     G53_W4_LDS_MAX));
         allowed = 1;
     }
-    hipLaunchKernelGGL((k_w4<E, R, NT, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x, a);
+    hipLaunchKernelGGL((k_w4<E, R, NT, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x,
+                       a.offsets, a.pair, a);
     G53_LAUNCHED("k_w4");
     return 0;
 }
@@ -438,13 +465,15 @@ static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const
 /* busy: token tiles that are expected to hold rows. */
 template <typename E, int R, int NT> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
 {
-    constexpr int P = G53W4Type<E>::P, UC = G53W4Type<E>::UC, TT = 16 * NT;
+    constexpr int P = G53W4Type<E>::P, UC = P == 3 ? R : 4, TT = 16 * NT;
     const bool sw = a.limit > 0.0f;
     const int out = sw ? 8 * R : 16 * R, units = (a.cols + 128 * UC - 1) / (128 * UC), rows = a.T < TT ? a.T : TT;
     /* While there are fewer than two workgroups a CU, they get fewer rows: their waves split the columns instead, as long
      * as every part has a unit and its share of x fits LDS, and then there are fewer waves. */
-    int k = 0, rw = G53_W4_NW;
-    while (rw > 1 && busy * ((a.half + out * rw - 1) / (out * rw)) < 2 * g53h_num_cus()) {
+    int k = 0, rw = units < 4 ? G53_W4_NW / 2 : G53_W4_NW;
+    for (;;) {
+        const long wgs = busy * ((a.half + out * rw - 1) / (out * rw));
+        if (rw == 1 || wgs >= 2 * g53h_num_cus() || (out * rw / 2 < 4 * rows && wgs >= g53h_num_cus() / 2)) break;
         if ((2 << k) <= units && rows * P * ((2 << k) * 256 * UC + 16) <= G53_W4_LDS_MAX) k++;
         rw /= 2;
     }
@@ -457,11 +486,12 @@ template <typename E, int R, int NT> static int launch(void *y, const void *x, G
     a.seg = seg;
     size_t lds = (size_t)rows * P * (seg * 256 * UC + 16), red = (size_t)waves * TT * (16 * R + 4) * 4;
     if (lds < red) lds = red;
-    const long most = (1l << 31) / (64 * G53_W4_NW) / a.tiles;      /* token tiles of one launch: threads fit 32 bits */
+    const long wide = a.offsets ? a.tiles : (a.tiles + 7) / 8 * 8l, most = (1l << 31) / (64 * G53_W4_NW) / wide;      /* threads of a launch fit 32 bits */
     if (most < 1) return g53h_fail("g53h_mm_w4: %d rows", a.rows);
     for (long i = 0; i < items; i += most) {
         a.item0 = i;
-        const dim3 grid((unsigned)((items - i < most ? items - i : most) * a.tiles));
+        a.items = (int)(items - i < most ? items - i : most);
+        const dim3 grid((unsigned)(a.items * wide));
         const int rc = a.group % 128 == 0 ? start<E, R, NT, 4>(grid, waves, lds, y, x, a)
                        : a.group % 64 == 0 ? start<E, R, NT, 2>(grid, waves, lds, y, x, a)
                                            : start<E, R, NT, 1>(grid, waves, lds, y, x, a);
@@ -470,16 +500,19 @@ template <typename E, int R, int NT> static int launch(void *y, const void *x, G
     return 0;
 }
 
-/* Token tiles of 16, 32 or 64: by the tokens, or by the mean rows of an expert. */
+/* Row tiles of a wave: two, so that activations read from LDS meet twice the levels, or one where two leave less than
+ * 16 waves a CU. Token tiles of 16; of 32 for fp32 with more tokens, whose three planes make the products the bound. */
 template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
 {
     const long ex = a.offsets ? (a.n_experts < a.T ? a.n_experts : a.T) : 1, mean = (a.T + ex - 1) / ex;
-    const int nt = mean <= 16 ? 1 : (mean <= 32 || sizeof(E) == 4 ? 2 : 4), TT = 16 * nt;
+    const long units = (a.cols + 511) / 512, waves = (a.rows + 31) / 32 * ex * ((mean + 15) / 16) * (units < G53_W4_NW ? units : G53_W4_NW);
+    const bool few = waves <= 16 * g53h_num_cus() && !(a.limit > 0.0f);
+    const int TT = sizeof(E) == 4 && mean > 16 && !few ? 32 : 16;
     const long items = a.offsets ? a.T / TT + ex : (a.T + TT - 1) / TT, busy = ex * ((mean + TT - 1) / TT);
-    if (nt == 1) return launch<E, 2, 1>(y, x, a, items, busy);
-    if constexpr (sizeof(E) == 2)
-        if (nt == 4) return launch<E, 2, 4>(y, x, a, items, busy);
-    return launch<E, 2, 2>(y, x, a, items, busy);
+    if (few) return launch<E, 1, 1>(y, x, a, items, busy);
+    if constexpr (sizeof(E) == 4)
+        if (TT == 32) return launch<E, 2, 2>(y, x, a, items, busy);
+    return launch<E, 2, 1>(y, x, a, items, busy);
 }
 
 static int product(void *y, const void *x, int dt, G53W4Args &a)
@@ -515,7 +548,7 @@ static int w4_bad(const char *who, const G53hW4 *m, int dt, float limit, G53W4Ar
     a.offsets = a.pair = nullptr;
     a.n_experts = a.topk = 1;
     a.item0 = 0;
-    a.tiles = a.kw_log = a.seg = 0;
+    a.tiles = a.items = a.kw_log = a.seg = 0;
     return 0;
 }
 
