@@ -67,14 +67,17 @@ __device__ __forceinline__ void g53_store8(g53_f16 *p, const float (&v)[8])
     ((G53v8h_any *)p)->v = a;
 }
 
-/* Elements c .. c + 7 of a row of n, zeros behind its end. */
+/* Elements c .. c + 7 of a row of n, zeros behind its end (where the last one is read instead: no branch). */
 template <typename T> __device__ __forceinline__ void g53_load8_to(float (&o)[8], const T *row, int c, int n)
 {
     if (c + 8 <= n) {
         g53_load8(o, row + c);
     } else {
+        T v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = c + i < n ? (float)row[c + i] : 0.0f;
+        for (int i = 0; i < 8; i++) v[i] = row[c + i < n ? c + i : n - 1];
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = c + i < n ? (float)v[i] : 0.0f;
     }
 }
 template <typename T> __device__ __forceinline__ void g53_store8_to(T *row, const float (&v)[8], int c, int n)
@@ -88,11 +91,45 @@ template <typename T> __device__ __forceinline__ void g53_store8_to(T *row, cons
     }
 }
 
-/* The sum of v over the 64 lanes of a wave, in every lane. */
+/* The same eight as they lie, for loads that are waited for later. */
+template <typename T> struct G53Raw8 { T v __attribute__((ext_vector_type(8))); };
+template <typename T> __device__ __forceinline__ void g53_raw8_to(G53Raw8<T> &o, const T *row, int c, int n)
+{
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    struct __attribute__((packed, aligned(2))) Any { V8 v; };
+    if (c + 8 <= n) {
+        o.v = ((const Any *)(row + c))->v;
+    } else {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = row[c + i < n ? c + i : n - 1];
+#pragma unroll
+        for (int i = 0; i < 8; i++) o.v[i] = c + i < n ? v[i] : (T)0.0f;
+    }
+}
+
+/* v of the lane that DPP control ctrl names, inside each row of 16 lanes. */
+template <int ctrl> __device__ __forceinline__ float g53_dpp(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true));
+}
+
+/* The sum of v over the 64 lanes of a wave, the same bits in every lane: pairs, quads and halves of a row of 16 lanes by
+ * DPP, rows and halves of the wave by register swaps, no trip through LDS. */
 __device__ __forceinline__ float g53_wave_sum(float v)
 {
+    v += g53_dpp<0xb1>(v);              /* lane ^ 1 */
+    v += g53_dpp<0x4e>(v);              /* lane ^ 2 */
+    v += g53_dpp<0x141>(v);             /* 7 - lane: the other quad of eight */
+    v += g53_dpp<0x140>(v);             /* 15 - lane: the other eight of the row */
+    typedef unsigned int V2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    for (int half = 0; half < 2; half++) {          /* the other row of two, then the other two rows */
+        const unsigned u = __builtin_bit_cast(unsigned, v);
+        const V2 p = half ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const unsigned a = p[0], b = p[1];          /* a bit cast of a vector's element takes element 0 */
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    }
     return v;
 }
 

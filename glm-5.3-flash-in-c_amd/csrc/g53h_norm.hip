@@ -30,22 +30,30 @@ struct G53NormArgs {
     const float *post, *next;
     const void *gate;                   /* kind 1: float [H], 2: float [T], 3: E [T][H] */
     void *dgate;                        /* kinds 2 and 3 */
-    float *part;                        /* partial sums [groups][3][H] of dpost, dnext, dgate (kind 1) */
+    float *part;                        /* partial sums [workgroups][3][H] of dpost, dnext, dgate (kind 1) */
     float eps, scale;
     int T, H;
 };
 
-/* The sum of v over the W waves of a row's group; buf: two floats a wave. Every lane gets it. */
-template <int W> __device__ __forceinline__ void g53_group_sum(float &a, float &b, float (*buf)[2], int wv)
+/* 1 / sqrt(v), off by one in the last place at most; v is at least eps, a normal number. */
+__device__ __forceinline__ float g53_rsq(float v) { return __builtin_amdgcn_rsqf(v); }
+
+/* Sums of N values over the W waves of a row's group, in every lane; buf: N floats a wave. */
+template <int W, int N> __device__ __forceinline__ void g53_group_sum(float (&v)[N], float (*buf)[N], int wv)
 {
-    a = g53_wave_sum(a);
-    b = g53_wave_sum(b);
-    if (W > 1) {
-        if ((threadIdx.x & 63) == 0) { buf[wv][0] = a; buf[wv][1] = b; }
-        __syncthreads();
-        a = b = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; w++) { a += buf[wv / W * W + w][0]; b += buf[wv / W * W + w][1]; }
+    for (int k = 0; k < N; k++) v[k] = g53_wave_sum(v[k]);
+    if (W > 1) {
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < N; k++) buf[wv][k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            v[k] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++) v[k] += buf[wv / W * W + w][k];
+        }
     }
 }
 
@@ -55,13 +63,13 @@ __global__ void __launch_bounds__(W < 4 ? 256 : 64 * W)
 k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
 {
     constexpr int NW = W < 4 ? 4 : W, RB = NW / W;
-    __shared__ float buf[2][NW][2];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    __shared__ float buf[2][NW][1];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     long t = (wg0 + blockIdx.x) * RB + wv / W;
     const bool live = t < a.T;
     if (!live) t = a.T - 1;             /* rows behind the last: computed, not written */
     const int H = a.H, c0 = ((wv % W) * 64 + lane) * 8;
-    float hv[NV][8], s = 0.0f, s2 = 0.0f;
+    float hv[NV][8], s[1] = {0.0f};
 #pragma unroll
     for (int v = 0; v < NV; v++) g53_load8_to(hv[v], h + t * H, c0 + v * 512 * W, H);
     if (Y) {
@@ -73,9 +81,9 @@ k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
 #pragma unroll
             for (int v = 0; v < NV; v++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) s = __builtin_fmaf(yv[v][i], yv[v][i], s);
-            g53_group_sum<W>(s, s2, buf[0], wv);
-            rs = 1.0f / sqrtf(s / (float)H + a.eps);
+                for (int i = 0; i < 8; i++) s[0] = __builtin_fmaf(yv[v][i], yv[v][i], s[0]);
+            g53_group_sum<W, 1>(s, buf[0], wv);
+            rs = g53_rsq(s[0] / (float)H + a.eps);
         }
         const float gt = a.scale * (GK == 2 ? ((const float *)a.gate)[t] : 1.0f);
 #pragma unroll
@@ -94,13 +102,13 @@ k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
         }
     }
     if (!xn) return;
-    s = 0.0f;
+    s[0] = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; v++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) s = __builtin_fmaf(hv[v][i], hv[v][i], s);
-    g53_group_sum<W>(s, s2, buf[1], wv);
-    const float rs = 1.0f / sqrtf(s / (float)H + a.eps);
+        for (int i = 0; i < 8; i++) s[0] = __builtin_fmaf(hv[v][i], hv[v][i], s[0]);
+    g53_group_sum<W, 1>(s, buf[1], wv);
+    const float rs = g53_rsq(s[0] / (float)H + a.eps);
 #pragma unroll
     for (int v = 0; v < NV; v++) {
         const int c = c0 + v * 512 * W;
@@ -112,147 +120,193 @@ k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
     }
 }
 
-/* Persistent: group g of W waves takes tokens g, g + groups, ... */
+/* Persistent: group g of W waves takes tokens g, g + groups, ...; the next token's rows are asked for before a token's sums
+ * where registers hold them (rows of up to 4096).
+ * With a = scale gate post y two rounds of sums are enough: y's squares, then, from h', its squares and its products with
+ * v and a, and a's with v and dh', from which mean(v h'^) and mean(du post y^) = rs(y) mean(a dH) follow. */
 template <typename E, int W, int NV, int GK, bool Y>
 __global__ void __launch_bounds__(W < 4 ? 256 : 64 * W)
 k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E *y, G53NormArgs a)
 {
     constexpr int NW = W < 4 ? 4 : W, RB = NW / W;
-    __shared__ float buf[3][NW][2];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    constexpr bool KEEP = NV * W <= 8;         /* gains stay in registers */
+    constexpr bool AHEAD = NV == 1;            /* and the next token's rows wait there */
+    __shared__ float buf1[2][NW][1], buf2[2][NW][5];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long grp = (long)blockIdx.x * RB + wv / W, groups = (long)gridDim.x * RB;
     const int H = a.H, c0 = ((wv % W) * 64 + lane) * 8;
     const long rounds = (a.T + groups - 1) / groups;
+    const float inv = 1.0f / (float)H;
     float ap[NV][8], an[NV][8], ag[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; v++)
 #pragma unroll
         for (int i = 0; i < 8; i++) ap[v][i] = an[v][i] = ag[v][i] = 0.0f;
-    for (long k = 0; k < rounds; k++) {
-        long t = grp + k * groups;
-        const bool live = t < a.T;
-        if (!live) t = a.T - 1;
-        float hv[NV][8], yh[NV][8], g[NV][8], u[NV][8], rsy = 1.0f, s = 0.0f, s2 = 0.0f;
+    float kp[NV][8], kn[NV][8], kg[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) { kp[v][i] = 1.0f; kn[v][i] = 0.0f; kg[v][i] = 1.0f; }
+        const int c = c0 + v * 512 * W;
+        if (KEEP) {
+            if (Y && a.post) g53_load8_to(kp[v], a.post, c, H);
+            if (dxn) g53_load8_to(kn[v], a.next, c, H);
+            if (Y && GK == 1) {
+                g53_load8_to(kg[v], (const float *)a.gate, c, H);
+#pragma unroll
+                for (int i = 0; i < 8; i++) kg[v][i] *= a.scale;
+            }
+        }
+    }
+    G53Raw8<E> rh[NV], ry[NV], rg[NV], rd[NV], rt[NV];
+    float rgate = 1.0f;
+    auto ask = [&](long t) {                         /* behind the last token: the group's own last again, not used */
+        if (t >= a.T) t = t >= groups && t - groups < a.T ? t - groups : a.T - 1;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int c = c0 + v * 512 * W;
-            g53_load8_to(hv[v], h + t * H, c, H);
-            if (dh2) g53_load8_to(g[v], dh2 + t * H, c, H);
-            else
-#pragma unroll
-                for (int i = 0; i < 8; i++) g[v][i] = 0.0f;
+            if (Y) g53_raw8_to(ry[v], y + t * H, c, H);
+            g53_raw8_to(rh[v], h + t * H, c, H);
+            if (dxn) g53_raw8_to(rd[v], dxn + t * H, c, H);
+            if (dh2) g53_raw8_to(rg[v], dh2 + t * H, c, H);
+            if (Y && GK == 3) g53_raw8_to(rt[v], (const E *)a.gate + t * H, c, H);
         }
-        const float gt = a.scale * (GK == 2 ? ((const float *)a.gate)[t] : 1.0f);
-        float gv[NV][8];
-        if (Y) {
+        if (Y && GK == 2) rgate = ((const float *)a.gate)[t];
+    };
+    if (AHEAD) ask(grp);
+    for (long k = 0; k < rounds; k++) {
+        const long t = grp + k * groups;
+        const bool live = t < a.T;
+        if (!AHEAD) ask(t);
+        const int odd = k & 1;                       /* sums of two tokens in a row lie apart: one barrier each is enough */
+        float hv[NV][8], yh[NV][8], g[NV][8], d[NV][8], gt[NV][8];
 #pragma unroll
-            for (int v = 0; v < NV; v++) {
-                const int c = c0 + v * 512 * W;
-                g53_load8_to(yh[v], y + t * H, c, H);
-                if (GK == 1) g53_load8_to(gv[v], (const float *)a.gate, c, H);
-                if (GK == 3) g53_load8_to(gv[v], (const E *)a.gate + t * H, c, H);
+        for (int v = 0; v < NV; v++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                hv[v][i] = (float)rh[v].v[i];
+                if (Y) yh[v][i] = (float)ry[v].v[i];
+                d[v][i] = dxn ? (float)rd[v].v[i] : 0.0f;
+                g[v][i] = dh2 ? (float)rg[v].v[i] : 0.0f;
+                if (Y) gt[v][i] = KEEP && GK == 1 ? kg[v][i] : a.scale * (GK == 3 ? (float)rt[v].v[i] : GK == 2 ? rgate : 1.0f);
             }
+        if (AHEAD) ask(t + groups);
+        float rsy = 1.0f;
+        if (Y) {
             if (a.post) {
+                float s[1] = {0.0f};
 #pragma unroll
                 for (int v = 0; v < NV; v++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) s = __builtin_fmaf(yh[v][i], yh[v][i], s);
-                g53_group_sum<W>(s, s2, buf[0], wv);
-                rsy = 1.0f / sqrtf(s / (float)H + a.eps);
-            }
-#pragma unroll
-            for (int v = 0; v < NV; v++) {
-                float pv[8];
-                if (a.post) g53_load8_to(pv, a.post, c0 + v * 512 * W, H);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    yh[v][i] *= rsy;
-                    u[v][i] = a.post ? yh[v][i] * pv[i] : yh[v][i];
-                    gv[v][i] = (GK & 1) ? gt * gv[v][i] : gt;
-                    hv[v][i] = __builtin_fmaf(gv[v][i], u[v][i], hv[v][i]);
-                }
+                    for (int i = 0; i < 8; i++) s[0] = __builtin_fmaf(yh[v][i], yh[v][i], s[0]);
+                g53_group_sum<W, 1>(s, buf1[odd], wv);
+                rsy = g53_rsq(s[0] * inv + a.eps);
             }
         }
-        if (dxn) {                      /* uniform: through the next norm into h' */
-            float d[NV][8];
-            s = s2 = 0.0f;
-#pragma unroll
-            for (int v = 0; v < NV; v++) {
-                float nv[8];
-                g53_load8_to(d[v], dxn + t * H, c0 + v * 512 * W, H);
-                g53_load8_to(nv, a.next, c0 + v * 512 * W, H);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float vi = d[v][i] * nv[i];
-                    s = __builtin_fmaf(hv[v][i], hv[v][i], s);
-                    s2 = __builtin_fmaf(vi, hv[v][i], s2);
-                }
-            }
-            g53_group_sum<W>(s, s2, buf[1], wv);
-            const float rs = 1.0f / sqrtf(s / (float)H + a.eps), mean = s2 * rs / (float)H;
-#pragma unroll
-            for (int v = 0; v < NV; v++) {
-                float nv[8];
-                g53_load8_to(nv, a.next, c0 + v * 512 * W, H);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float hh = hv[v][i] * rs;
-                    if (live) an[v][i] = __builtin_fmaf(d[v][i], hh, an[v][i]);
-                    g[v][i] = __builtin_fmaf(rs, __builtin_fmaf(-hh, mean, d[v][i] * nv[i]), g[v][i]);
-                }
-            }
-        }
-        if (live)
-#pragma unroll
-            for (int v = 0; v < NV; v++) g53_store8_to(dh + t * H, g[v], c0 + v * 512 * W, H);
-        if (!Y) {
-            if (W > 1) __syncthreads();
-            continue;
-        }
-        s = s2 = 0.0f;
+        /* w: v = dxn next; au: scale gate post y^, whose sum with dH is dy's mean */
+        float s[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, w[NV][8], pv[NV][8];
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int c = c0 + v * 512 * W;
-            float pv[8], dg[8];
-            if (a.post) g53_load8_to(pv, a.post, c, H);
+            float nv[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                dg[i] = a.scale * u[v][i] * g[v][i];
-                if (GK == 1 && live) ag[v][i] += dg[i];
-                if (GK == 2) s2 += dg[i];
-                const float du = gv[v][i] * g[v][i];
-                if (live) ap[v][i] = __builtin_fmaf(du, yh[v][i], ap[v][i]);
-                g[v][i] = a.post ? du * pv[i] : du;
-                s = __builtin_fmaf(g[v][i], yh[v][i], s);
+                nv[i] = kn[v][i];
+                pv[v][i] = kp[v][i];
             }
-            if (GK == 3 && live && a.dgate) g53_store8_to((E *)a.dgate + t * H, dg, c, H);
+            if (!KEEP && dxn) g53_load8_to(nv, a.next, c, H);
+            if (Y && !KEEP) {
+                if (a.post) g53_load8_to(pv[v], a.post, c, H);
+                if (GK == 1) {
+                    float gv[8];
+                    g53_load8_to(gv, (const float *)a.gate, c, H);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) gt[v][i] *= gv[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w[v][i] = d[v][i] * nv[i];
+                if (Y) {
+                    yh[v][i] *= rsy;
+                    const float u = yh[v][i] * pv[v][i], au = gt[v][i] * u;
+                    hv[v][i] = __builtin_fmaf(gt[v][i], u, hv[v][i]);
+                    s[2] = __builtin_fmaf(au, g[v][i], s[2]);
+                    s[3] = __builtin_fmaf(au, w[v][i], s[3]);
+                    s[4] = __builtin_fmaf(au, hv[v][i], s[4]);
+                }
+                s[0] = __builtin_fmaf(hv[v][i], hv[v][i], s[0]);
+                s[1] = __builtin_fmaf(w[v][i], hv[v][i], s[1]);
+            }
         }
-        g53_group_sum<W>(s, s2, buf[2], wv);
-        if (GK == 2 && live && a.dgate && lane == 0 && wv % W == 0) ((float *)a.dgate)[t] = s2;
-        const float mean = s / (float)H;
+        g53_group_sum<W, 5>(s, buf2[odd], wv);
+        const float rs = dxn ? g53_rsq(s[0] * inv + a.eps) : 0.0f, mean = s[1] * rs * inv;
+        const float meany = a.post ? (s[2] + rs * (s[3] - rs * mean * s[4])) * inv : 0.0f;
+        float gsum[1] = {0.0f};
+        if (live)
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int c = c0 + v * 512 * W;
+                float dg[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float hh = hv[v][i] * rs;
+                    an[v][i] = __builtin_fmaf(d[v][i], hh, an[v][i]);
+                    g[v][i] = __builtin_fmaf(rs, __builtin_fmaf(-hh, mean, w[v][i]), g[v][i]);
+                }
+                g53_store8_to(dh + t * H, g[v], c, H);
+                if (!Y) continue;
+                if (GK)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        dg[i] = a.scale * (yh[v][i] * pv[v][i]) * g[v][i];
+                        if (GK == 1) ag[v][i] += dg[i];
+                        if (GK == 2) gsum[0] += dg[i];
+                    }
+                if (GK == 3 && a.dgate) g53_store8_to((E *)a.dgate + t * H, dg, c, H);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float du = gt[v][i] * g[v][i];
+                    ap[v][i] = __builtin_fmaf(du, yh[v][i], ap[v][i]);
+                    g[v][i] = rsy * __builtin_fmaf(-yh[v][i], meany, du * pv[v][i]);      /* without post: du itself */
+                }
+                g53_store8_to(dy + t * H, g[v], c, H);
+            }
+        if (Y && GK == 2 && a.dgate) {
+            __shared__ float bufg[2][NW][1];
+            g53_group_sum<W, 1>(gsum, bufg[odd], wv);
+            if (live && lane == 0 && wv % W == 0) ((float *)a.dgate)[t] = gsum[0];
+        }
+    }
+    /* the sums of the workgroup's groups, added in order by the first of them, which writes them */
+    float *part = a.part + (long)blockIdx.x * 3 * H;
+    auto finish = [&](float (&v8)[NV][8], int which) {
+        if (RB > 1) {                                /* NV = 1 */
+            __shared__ float rows[RB > 1 ? NW : 1][8][64];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; i++) rows[wv][i][lane] = v8[0][i];
+            __syncthreads();
+            if (wv >= W) return;
+#pragma unroll
+            for (int r = 1; r < RB; r++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) v8[0][i] += rows[r * W + wv][i][lane];
+        }
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            if (a.post)
-#pragma unroll
-                for (int i = 0; i < 8; i++) g[v][i] = rsy * __builtin_fmaf(-yh[v][i], mean, g[v][i]);
-            if (live) g53_store8_to(dy + t * H, g[v], c0 + v * 512 * W, H);
+            const int c = c0 + v * 512 * W;
+            if (c < H) g53_store8_to(part + which * H, v8[v], c, H);
         }
-        if (W > 1) __syncthreads();     /* buf is used again */
-    }
-    float *part = a.part + grp * 3 * H;
-#pragma unroll
-    for (int v = 0; v < NV; v++) {
-        const int c = c0 + v * 512 * W;
-        if (c >= H) continue;
-        if (Y) g53_store8_to(part, ap[v], c, H);
-        g53_store8_to(part + H, an[v], c, H);
-        if (GK == 1) g53_store8_to(part + 2 * H, ag[v], c, H);
-    }
+    };
+    if (Y) finish(ap, 0);
+    finish(an, 1);
+    if (Y && GK == 1) finish(ag, 2);
 }
 
 /* out[which][c] = the groups' partial sums, added in a fixed order: 16 chains of groups, then a tree. */
-__global__ void __launch_bounds__(1024) k_norm_sum(float *dpost, float *dnext, float *dgate, const float *__restrict__ part,
-                                                   int groups, int H)
+__global__ void __launch_bounds__(1024) k_norm_sum(float *__restrict__ dpost, float *__restrict__ dnext, float *__restrict__ dgate,
+                                                   const float *__restrict__ part, int groups, int H)
 {
     __shared__ float buf[16][64];
     float *out = blockIdx.y == 0 ? dpost : (blockIdx.y == 1 ? dnext : dgate);
@@ -260,6 +314,7 @@ __global__ void __launch_bounds__(1024) k_norm_sum(float *dpost, float *dnext, f
     const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
     float s = 0.0f;
     if (c < H)
+#pragma unroll 8
         for (int g = k; g < groups; g += 16) s += part[((long)g * 3 + blockIdx.y) * H + c];
     buf[k][lane] = s;
     __syncthreads();
@@ -277,7 +332,7 @@ __global__ void __launch_bounds__(1024) k_norm_sum(float *dpost, float *dnext, f
         else if ((H) <= 1024) { constexpr int W = 2, NV = 1; BODY; }            \
         else if ((H) <= 2048) { constexpr int W = 4, NV = 1; BODY; }            \
         else if ((H) <= 4096) { constexpr int W = 8, NV = 1; BODY; }            \
-        else if ((H) <= 8192) { constexpr int W = 16, NV = 1; BODY; }           \
+        else if ((H) <= 8192) { constexpr int W = 8, NV = 2; BODY; }            \
         else { constexpr int W = 16, NV = 2; BODY; }                            \
     } while (0)
 #define G53_NORM_BY_GATE(kind, BODY)                                            \
@@ -309,10 +364,11 @@ static int backward(void *dh, void *dy, float *dpost, float *dnext, float *dchan
                     const void *h, const void *y, G53NormArgs &a)
 {
     constexpr int NW = W < 4 ? 4 : W, RB = NW / W;
-    const long need = ((long)a.T + RB - 1) / RB, most = g53h_num_cus();
-    const unsigned wgs = (unsigned)(need < most ? need : most);
+    /* eight waves a CU, all with the same number of tokens where that divides */
+    const long most = g53h_num_cus() * (W < 8 ? 2 : 1), need = ((long)a.T + RB - 1) / RB, rounds = (need + most - 1) / most;
+    const unsigned wgs = (unsigned)(need ? (need + rounds - 1) / rounds : 0);
     if (wgs) {
-        a.part = (float *)g53h_op_workspace((size_t)wgs * RB * 3 * a.H * sizeof(float));
+        a.part = (float *)g53h_op_workspace((size_t)wgs * 3 * a.H * sizeof(float));
         if (!a.part) return -1;
         hipLaunchKernelGGL((k_block_norm_grad<E, W, NV, GK, Y>), dim3(wgs), dim3(64 * NW), 0, g53h_stream(), (E *)dh, (E *)dy,
                            (const E *)dh2, (const E *)dxn, (const E *)h, (const E *)y, a);
@@ -320,7 +376,7 @@ static int backward(void *dh, void *dy, float *dpost, float *dnext, float *dchan
     }
     if (dpost || dnext || dchannel) {
         hipLaunchKernelGGL(k_norm_sum, dim3((a.H + 63) / 64, 3), dim3(1024), 0, g53h_stream(), dpost, dnext, dchannel, a.part,
-                           (int)(wgs * RB), a.H);
+                           (int)wgs, a.H);
         G53_LAUNCHED("k_norm_sum");
     }
     return 0;
@@ -330,7 +386,7 @@ static int norm_bad(const char *who, int T, int hidden, int dt, float eps)
 {
     if (T < 0 || hidden < 1 || hidden > G53_NORM_MAXH || !g53_elem_bytes(dt))
         return g53h_fail("%s: %d tokens of %d, element type %d (hidden at most %d)", who, T, hidden, dt, G53_NORM_MAXH);
-    if (!(eps > 0.0f) || eps > 1.0e30f) return g53h_fail("%s: eps %g", who, eps);
+    if (!(eps >= 1.0e-30f) || eps > 1.0e30f) return g53h_fail("%s: eps %g (1e-30 to 1e30)", who, eps);
     return 0;
 }
 
