@@ -108,6 +108,17 @@ template <typename T> __device__ __forceinline__ void g53_raw8_to(G53Raw8<T> &o,
     }
 }
 
+/* The same for rows that are read once: they need not stay in the caches. */
+template <typename T> __device__ __forceinline__ void g53_raw8_once_to(G53Raw8<T> &o, const T *row, int c, int n)
+{
+    if (c + 8 <= n && !((uintptr_t)(row + c) & 15)) {
+        typedef T V8 __attribute__((ext_vector_type(8)));
+        o.v = __builtin_nontemporal_load((const V8 *)(row + c));
+    } else {
+        g53_raw8_to(o, row, c, n);
+    }
+}
+
 /* v of the lane that DPP control ctrl names, inside each row of 16 lanes. */
 template <int ctrl> __device__ __forceinline__ float g53_dpp(float v)
 {

@@ -24,7 +24,7 @@
 #include "g53h_elem.h"
 #include "g53h_runtime.h"
 
-#define G53_SORT_SEG 8192               /* pairs of one workgroup, while there are at most G53_SORT_WGS */
+#define G53_SORT_SEG 2048               /* pairs of one workgroup, while there are at most G53_SORT_WGS */
 #define G53_SORT_WGS 128
 #define G53_SORT_MAXE 1024
 
@@ -245,16 +245,16 @@ __global__ void __launch_bounds__(256) k_combine(E *out, const E *__restrict__ y
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (add) g53_load8_to(acc, add + t * H, c, H);
     for (int j0 = 0; j0 < K; j0 += 8) {
-        float v[8][8];
+        G53Raw8<E> v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (j0 + j < K && r[j0 + j] >= 0) g53_load8_to(v[j], ys + (long)r[j0 + j] * H, c, H);
+            if (j0 + j < K && r[j0 + j] >= 0) g53_raw8_once_to(v[j], ys + (long)r[j0 + j] * H, c, H);
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (j0 + j < K && r[j0 + j] >= 0) {
                 const float wj = w ? w[t * K + j0 + j] : 1.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(wj, v[j][i], acc[i]);
+                for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(wj, (float)v[j].v[i], acc[i]);
             }
     }
     g53_store8_to(out + t * H, acc, c, H);
