@@ -9,7 +9,10 @@
  *                    lanes with the same expert, those below it are its rank. Order never depends on
  *                    timing. Routings of more than G53_SORT_SEG pairs are cut into segments, counted by
  *                    k_sort_count first; every workgroup then adds up the counts of all segments.
- *   k_dispatch       bytes of rows, 16 a thread: a token's row is read once and written topk times.
+ *   k_dispatch       bytes of rows, 16 a thread: a token's row is read once and written topk times. Written past the
+ *                    caches the rows alone leave faster (4096 tokens of 4096 bf16 to 8 experts each, with the sort and a
+ *                    combine of other rows after it: 128 us against 136), but whoever reads them next waits longer
+ *                    (dispatch and a read of its rows: 104 us against 93; 67 MB of rows: 28 against 25).
  *   k_combine        8 elements a thread: the rows of a token's pairs are all asked for before the
  *                    first is added; sums in fp32 in the order of the pairs, rounded once.
  *   k_combine_grad   one wave per pair: its weight's gradient is one sum over the wave, so nothing is
@@ -83,7 +86,8 @@ k_sort_place(int *__restrict__ offsets, int *__restrict__ pair, int *__restrict_
             for (int w = 0; w < NW; w++) here += first_of[w * NE + e];
             if (gridDim.x == 1) total = here;
             else
-                for (int b = 0; b < (int)gridDim.x; b++) {
+#pragma unroll 16
+                for (int b = 0; b < (int)gridDim.x; b++) {      /* loads of 16 segments in flight */
                     const int c = hist[(long)b * NE + e];
                     total += c;
                     before += b < (int)blockIdx.x ? c : 0;
@@ -311,12 +315,13 @@ k_combine_grad(E *dys, float *__restrict__ dw, const E *__restrict__ dout, const
     E *d = dys + r * H;
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int c = lane * 8; c < H; c += 512) {
-        float gv[8], yv[8], o[8];
+        float gv[8], o[8];
+        G53Raw8<E> yv;
         g53_load8_to(gv, g, c, H);
-        g53_load8_to(yv, y, c, H);
+        g53_raw8_once_to(yv, y, c, H);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            acc[i] = __builtin_fmaf(gv[i], yv[i], acc[i]);
+            acc[i] = __builtin_fmaf(gv[i], (float)yv.v[i], acc[i]);
             o[i] = wp * gv[i];
         }
         g53_store8_to(d, o, c, H);
