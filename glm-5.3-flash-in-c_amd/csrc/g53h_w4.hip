@@ -183,11 +183,11 @@ __device__ __forceinline__ void g53_spread(float (&o)[4], float v)
  * columns, in units of UC x 128 taken in turn, by NW / KW groups of R row tiles. A unit's levels are asked for one unit
  * ahead. GS: groups are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows,
  * the others the same up rows. Columns behind the last of a unit meet activations of zero. */
-template <typename E, int R, int NT, int GS>
+template <typename E, int R, int NT, int UC, bool ROWS, int GS>
 __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2) k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets, const int *__restrict__ pair, G53W4Args a)
 {
     typedef typename G53W4Type<E>::V V;
-    constexpr int P = G53W4Type<E>::P, UC = P == 3 ? R : 4, TT = 16 * NT, LD = 16 * R + 4;
+    constexpr int P = G53W4Type<E>::P, PM = ROWS ? 1 : P, MT = 16 * NT, TT = ROWS ? MT / P : MT, LD = 16 * R + 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const bool sw = a.limit > 0.0f;
     const int out = sw ? 8 * R : 16 * R;                     /* result rows of a wave */
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
         first = (int)(item * TT);
         last = a.T - first < TT ? a.T : first + TT;
     }
-    const int rows = last - first, row0 = (tile * RW + rw) * out;
+    const int rows = last - first, x_rows = ROWS ? P * rows : rows, row0 = (tile * RW + rw) * out;
     /* where the row tiles begin; the lane's row in them, the last one for those behind the end */
     const uint8_t *wb[R], *sb[R], *zb[R];
     const int wrow = a.cols / 2, srow = a.groups * (a.s_dt == G53H_F32 ? 4 : 2), zrow = (a.groups + 1) / 2;
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     const int ld = a.seg * (256 * UC) + 16; /* bytes of a plane's row in LDS: odd sixteens, so rows start in other banks */
     int xat[NT];                            /* the lane's token in LDS; tokens behind the last repeat it */
 #pragma unroll
-    for (int t = 0; t < NT; t++) xat[t] = (16 * t + m < rows ? 16 * t + m : rows - 1) * ld + q * (GS == 4 ? 64 : 16);
+    for (int t = 0; t < NT; t++) xat[t] = (16 * t + m < x_rows ? 16 * t + m : x_rows - 1) * ld + q * (GS == 4 ? 64 : 16);
     const int plane = rows * ld;
     /* sc, nz: of the chunk, GS = 4. Step s takes the columns of register s: 8 from each quarter's 32 where the chunk lies
      * in one group, else turned to 32 in a row. */
@@ -301,11 +301,11 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
         g53_v4f D[R][NT], X[NT];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            V b[NT][P];
+            V b[NT][PM];
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int p = 0; p < P; p++) {
+                for (int p = 0; p < PM; p++) {
                     b[t][p] = *(const V *)(lds + p * plane + xat[t] + c_lds * 256 + s * (GS == 4 ? 16 : 64));
                     X[t] = g53_mfma(b[t][p], ones, s % GS == 0 && p == 0 ? zero : X[t]);
                 }
@@ -315,9 +315,9 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int p = 0; p < P; p++) D[r][t] = g53_mfma(b[t][p], lv, s % GS == 0 && p == 0 ? zero : D[r][t]);
+                    for (int p = 0; p < PM; p++) D[r][t] = g53_mfma(b[t][p], lv, s % GS == 0 && p == 0 ? zero : D[r][t]);
             }
-            if (NT * P > 2) __builtin_amdgcn_sched_barrier(0);     /* one step's activations in registers at a time */
+            if (NT * PM > 2) __builtin_amdgcn_sched_barrier(0);     /* one step's activations in registers at a time */
             if (s % GS == GS - 1)       /* a group, or what the chunk has of it */
 #pragma unroll
                 for (int r = 0; r < R; r++)
@@ -343,14 +343,15 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
         }
     };
     /* A segment's activations into LDS as planes in the levels' order, in pieces of 512 columns of a row, a wave's load;
-     * a wave asks for four at a time. */
-    typedef g53_v4w Piece[4][sizeof(E) / 2];
+     * a wave asks for NP at a time. */
+    constexpr int NP = P == 3 && R == 2 ? 2 : 4;
+    typedef g53_v4w Piece[NP][sizeof(E) / 2];
     auto segment = [&](int seg0) { return units - seg0 < a.seg ? units - seg0 : a.seg; };
     auto pieces_of = [&](int here) { return rows * ((here * (16 * UC) + 63) / 64); };
     auto fetch = [&](Piece &v, int seg0, int p0) {
         const int k0 = seg0 * (128 * UC), across = pieces_of(segment(seg0)) / rows;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < NP; k++) {
             const int piece = p0 + k * NW, i = piece / across, at = k0 + ((piece - i * across) * 64 + lane) * 8;
             const bool there = i < rows && at < a.cols;
             int p = i < rows ? first + i : first;
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     auto put = [&](Piece &v, int seg0, int p0) {
         const int here = segment(seg0), across = pieces_of(here) / rows;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < NP; k++) {
             const int piece = p0 + k * NW, i = piece / across, c8 = (piece - i * across) * 64 + lane;
             if (i < rows && c8 < here * (16 * UC)) {
                 V b[P];
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     for (int seg0 = 0; seg0 < units; seg0 += a.seg) {
         const int here = segment(seg0), pieces = pieces_of(here);
         if (seg0) __syncthreads();
-        for (int p0 = seg0 ? wv : wv + 4 * NW; p0 < pieces; p0 += 4 * NW) {
+        for (int p0 = seg0 ? wv : wv + NP * NW; p0 < pieces; p0 += NP * NW) {
             Piece v;
             fetch(v, seg0, p0);
             put(v, seg0, p0);
@@ -421,23 +422,26 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
         }
     }
     __syncthreads();
-    float *red = (float *)lds;              /* [NW][TT][LD] */
+    float *red = (float *)lds;              /* [NW][MT][LD] */
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) red[(wv * TT + 16 * t + 4 * q + i) * LD + 16 * r + m] = acc[r][t][i];
+            for (int i = 0; i < 4; i++) red[(wv * MT + 16 * t + 4 * q + i) * LD + 16 * r + m] = acc[r][t][i];
     __syncthreads();
     /* out and RW are powers of two */
     const int out_log = __builtin_ctz(out), outs_log = out_log + __builtin_ctz(RW), base = tile << outs_log;
     for (int i = tid; i < rows << outs_log; i += 64 * NW) {
         const int t = i >> outs_log, o = i & ((1 << outs_log) - 1), w = o >> out_log, r = o & (out - 1);
         float v = 0.0f, u = 0.0f;
-        for (int k = 0; k < KW; k++) {
-            v += red[((w * KW + k) * TT + t) * LD + r];
-            if (sw) u += red[((w * KW + k) * TT + t) * LD + out + r];
-        }
+        for (int k = 0; k < KW; k++)
+#pragma unroll
+            for (int p = 0; p < (ROWS ? P : 1); p++) {
+                const float *from = red + ((w * KW + k) * MT + p * rows + t) * LD + r;
+                v += from[0];
+                if (sw) u += from[out];
+            }
         if (sw) {
             v = v > a.limit ? a.limit : v;
             u = u > a.limit ? a.limit : (u < -a.limit ? -a.limit : u);
@@ -447,25 +451,25 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     }
 }
 
-template <typename E, int R, int NT, int GS>
+template <typename E, int R, int NT, int UC, bool ROWS, int GS>
 static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const G53W4Args &a)
 {
     static int allowed = 0;
     if (!allowed) {
-        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, UC, ROWS, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                     G53_W4_LDS_MAX));
         allowed = 1;
     }
-    hipLaunchKernelGGL((k_w4<E, R, NT, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x,
+    hipLaunchKernelGGL((k_w4<E, R, NT, UC, ROWS, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x,
                        a.offsets, a.pair, a);
     G53_LAUNCHED("k_w4");
     return 0;
 }
 
 /* busy: token tiles that are expected to hold rows. */
-template <typename E, int R, int NT> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
+template <typename E, int R, int NT, int UC, bool ROWS> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
 {
-    constexpr int P = G53W4Type<E>::P, UC = P == 3 ? R : 4, TT = 16 * NT;
+    constexpr int P = G53W4Type<E>::P, TT = ROWS ? 16 * NT / P : 16 * NT;
     const bool sw = a.limit > 0.0f;
     const int out = sw ? 8 * R : 16 * R, units = (a.cols + 128 * UC - 1) / (128 * UC), rows = a.T < TT ? a.T : TT;
     /* While there are fewer than two workgroups a CU, they get fewer rows: their waves split the columns instead, as long
@@ -484,7 +488,7 @@ template <typename E, int R, int NT> static int launch(void *y, const void *x, G
     if (seg < 1 << k) seg = 1 << k;
     if (seg > units) seg = units;
     a.seg = seg;
-    size_t lds = (size_t)rows * P * (seg * 256 * UC + 16), red = (size_t)waves * TT * (16 * R + 4) * 4;
+    size_t lds = (size_t)rows * P * (seg * 256 * UC + 16), red = (size_t)waves * 16 * NT * (16 * R + 4) * 4;
     if (lds < red) lds = red;
     const long wide = a.offsets ? a.tiles : (a.tiles + 7) / 8 * 8l, most = (1l << 31) / (64 * G53_W4_NW) / wide;      /* threads of a launch fit 32 bits */
     if (most < 1) return g53h_fail("g53h_mm_w4: %d rows", a.rows);
@@ -492,27 +496,31 @@ template <typename E, int R, int NT> static int launch(void *y, const void *x, G
         a.item0 = i;
         a.items = (int)(items - i < most ? items - i : most);
         const dim3 grid((unsigned)(a.items * wide));
-        const int rc = a.group % 128 == 0 ? start<E, R, NT, 4>(grid, waves, lds, y, x, a)
-                       : a.group % 64 == 0 ? start<E, R, NT, 2>(grid, waves, lds, y, x, a)
-                                           : start<E, R, NT, 1>(grid, waves, lds, y, x, a);
+        const int rc = a.group % 128 == 0 ? start<E, R, NT, UC, ROWS, 4>(grid, waves, lds, y, x, a)
+                       : a.group % 64 == 0 ? start<E, R, NT, UC, ROWS, 2>(grid, waves, lds, y, x, a)
+                                           : start<E, R, NT, UC, ROWS, 1>(grid, waves, lds, y, x, a);
         if (rc) return rc;
     }
     return 0;
 }
 
 /* Row tiles of a wave: two, so that activations read from LDS meet twice the levels, or one where two leave less than
- * 16 waves a CU. Token tiles of 16; of 32 for fp32 with more tokens, whose three planes make the products the bound. */
+ * 16 waves a CU. Token tiles of 16. For fp32, whose products are three: up to 5 tokens put their planes side by side as 15
+ * rows of a tile, and the products are as many as bf16's; more take tiles of 16, or of 32 where there are many waves. */
 template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
 {
     const long ex = a.offsets ? (a.n_experts < a.T ? a.n_experts : a.T) : 1, mean = (a.T + ex - 1) / ex;
     const long units = (a.cols + 511) / 512, waves = (a.rows + 31) / 32 * ex * ((mean + 15) / 16) * (units < G53_W4_NW ? units : G53_W4_NW);
     const bool few = waves <= 16 * g53h_num_cus() && !(a.limit > 0.0f);
-    const int TT = sizeof(E) == 4 && mean > 16 && !few ? 32 : 16;
+    const int TT = sizeof(E) == 2 ? 16 : (mean <= 5 ? 5 : (mean > 16 && !few ? 32 : 16));
     const long items = a.offsets ? a.T / TT + ex : (a.T + TT - 1) / TT, busy = ex * ((mean + TT - 1) / TT);
-    if (few) return launch<E, 1, 1>(y, x, a, items, busy);
-    if constexpr (sizeof(E) == 4)
-        if (TT == 32) return launch<E, 2, 2>(y, x, a, items, busy);
-    return launch<E, 2, 1>(y, x, a, items, busy);
+    if constexpr (sizeof(E) == 4) {
+        if (TT == 32) return launch<E, 2, 2, 2, false>(y, x, a, items, busy);
+        if (TT == 16 && few) return launch<E, 1, 1, 1, false>(y, x, a, items, busy);
+        if (TT == 16) return launch<E, 2, 1, 2, false>(y, x, a, items, busy);
+    }
+    if (few) return launch<E, 1, 1, 4, sizeof(E) == 4>(y, x, a, items, busy);
+    return launch<E, 2, 1, 4, sizeof(E) == 4>(y, x, a, items, busy);
 }
 
 static int product(void *y, const void *x, int dt, G53W4Args &a)
