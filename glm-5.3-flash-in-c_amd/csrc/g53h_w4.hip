@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     };
     /* A segment's activations into LDS as planes in the levels' order, in pieces of 512 columns of a row, a wave's load;
      * a wave asks for NP at a time. */
-    constexpr int NP = P == 3 && R == 2 ? 2 : 4;
+    constexpr int NP = (P == 3 && R == 2) || NT > 1 ? 2 : 4;
     typedef g53_v4w Piece[NP][sizeof(E) / 2];
     auto segment = [&](int seg0) { return units - seg0 < a.seg ? units - seg0 : a.seg; };
     auto pieces_of = [&](int here) { return rows * ((here * (16 * UC) + 63) / 64); };
@@ -505,22 +505,23 @@ template <typename E, int R, int NT, int UC, bool ROWS> static int launch(void *
 }
 
 /* Row tiles of a wave: two, so that activations read from LDS meet twice the levels, or one where two leave less than
- * 16 waves a CU. Token tiles of 16. For fp32, whose products are three: up to 5 tokens put their planes side by side as 15
- * rows of a tile, and the products are as many as bf16's; more take tiles of 16, or of 32 where there are many waves. */
+ * 16 waves a CU (4096 x 2048 by one token in bf16: 4.8 us against 5.9). Token tiles of 16, or of 32 for more tokens of
+ * many waves, which then turn levels into floats half as often (16384 x 4096 by 128 tokens: 44 us against 50; fp32: 57
+ * against 71). For fp32, whose products are three, up to 5 tokens put their planes side by side as 15 rows of a tile, and
+ * the products are as many as bf16's (16384 x 4096 by one token: 14.5 us against 16.4). */
 template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
 {
+    constexpr bool F32 = sizeof(E) == 4;
     const long ex = a.offsets ? (a.n_experts < a.T ? a.n_experts : a.T) : 1, mean = (a.T + ex - 1) / ex;
     const long units = (a.cols + 511) / 512, waves = (a.rows + 31) / 32 * ex * ((mean + 15) / 16) * (units < G53_W4_NW ? units : G53_W4_NW);
     const bool few = waves <= 16 * g53h_num_cus() && !(a.limit > 0.0f);
-    const int TT = sizeof(E) == 2 ? 16 : (mean <= 5 ? 5 : (mean > 16 && !few ? 32 : 16));
+    const int TT = F32 && mean <= 5 ? 5 : (mean > 16 && !few ? 32 : 16);
     const long items = a.offsets ? a.T / TT + ex : (a.T + TT - 1) / TT, busy = ex * ((mean + TT - 1) / TT);
-    if constexpr (sizeof(E) == 4) {
-        if (TT == 32) return launch<E, 2, 2, 2, false>(y, x, a, items, busy);
-        if (TT == 16 && few) return launch<E, 1, 1, 1, false>(y, x, a, items, busy);
-        if (TT == 16) return launch<E, 2, 1, 2, false>(y, x, a, items, busy);
-    }
-    if (few) return launch<E, 1, 1, 4, sizeof(E) == 4>(y, x, a, items, busy);
-    return launch<E, 2, 1, 4, sizeof(E) == 4>(y, x, a, items, busy);
+    if (TT == 32) return launch<E, 2, 2, 2, false>(y, x, a, items, busy);
+    if constexpr (F32)
+        if (TT == 16) return few ? launch<E, 1, 1, 1, false>(y, x, a, items, busy) : launch<E, 2, 1, 2, false>(y, x, a, items, busy);
+    if (few) return launch<E, 1, 1, 4, F32>(y, x, a, items, busy);
+    return launch<E, 2, 1, 4, F32>(y, x, a, items, busy);
 }
 
 static int product(void *y, const void *x, int dt, G53W4Args &a)
