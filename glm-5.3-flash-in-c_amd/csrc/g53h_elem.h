@@ -119,6 +119,15 @@ template <typename T> __device__ __forceinline__ void g53_raw8_once_to(G53Raw8<T
     }
 }
 
+/* The loads into o are waited for here. Stores count as loads do, so a wait behind them would be for them too. */
+template <typename T> __device__ __forceinline__ void g53_arrived(G53Raw8<T> &o)
+{
+    typedef unsigned int Words __attribute__((ext_vector_type(sizeof(o.v) / 4)));
+    Words w = __builtin_bit_cast(Words, o.v);
+    asm volatile("" : "+v"(w));
+    o.v = __builtin_bit_cast(decltype(o.v), w);
+}
+
 /* v of the lane that DPP control ctrl names, inside each row of 16 lanes. */
 template <int ctrl> __device__ __forceinline__ float g53_dpp(float v)
 {

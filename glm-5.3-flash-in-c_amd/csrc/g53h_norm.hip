@@ -13,7 +13,7 @@
  *     dy = rs(y) (du post - y^ mean(du post y^))
  *
  * Both directions are one pass over HBM: W waves hold a token's row in registers, 8 elements a lane
- * (16 for rows above 8192), sums go over the lanes and then the waves. The next norm takes h' in fp32,
+ * (16 for rows above 4096), sums go over the lanes and then the waves. The next norm takes h' in fp32,
  * before it is rounded to be stored, and the backward pass forms the same fp32 h' again from h and y.
  * Gradients that tokens share are summed by each workgroup over its tokens in registers, written once
  * and added up by k_norm_sum in a fixed order: no atomics, the same bits on every run.
@@ -30,7 +30,7 @@ struct G53NormArgs {
     const float *post, *next;
     const void *gate;                   /* kind 1: float [H], 2: float [T], 3: E [T][H] */
     void *dgate;                        /* kinds 2 and 3 */
-    float *part;                        /* partial sums [workgroups][3][H] of dpost, dnext, dgate (kind 1) */
+    float *part;                        /* partial sums [workgroups][2][H] of dpost over scale and channel's gate, and dnext */
     float eps, scale;
     int T, H;
 };
@@ -122,8 +122,9 @@ k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
 
 /* Persistent: group g of W waves takes tokens g, g + groups, ...; the next token's rows are asked for before a token's sums
  * where registers hold them (rows of up to 4096).
- * With a = scale gate post y two rounds of sums are enough: y's squares, then, from h', its squares and its products with
- * v and a, and a's with v and dh', from which mean(v h'^) and mean(du post y^) = rs(y) mean(a dH) follow. */
+ * With k = scale gate post two rounds of sums are enough: y's squares, then h''s squares and its products with v and k y^,
+ * and k y^'s with v and dh', from which mean(v h'^) and mean(du post y^) = mean(k y^ dH) follow. Where the gate is the same for
+ * all tokens (kinds 0 and 1), A = sum over tokens of y^ dH gives dpost = scale gate A and dgate = scale post A. */
 template <typename E, int W, int NV, int GK, bool Y>
 __global__ void __launch_bounds__(W < 4 ? 256 : 64 * W)
 k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E *y, G53NormArgs a)
@@ -137,26 +138,32 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
     const int H = a.H, c0 = ((wv % W) * 64 + lane) * 8;
     const long rounds = (a.T + groups - 1) / groups;
     const float inv = 1.0f / (float)H;
-    float ap[NV][8], an[NV][8], ag[NV][8];
+    float ap[NV][8], an[NV][8];
+    float kp[NV][8], kn[NV][8];                /* scale gate post, or scale post for kinds 2 and 3; next */
+    auto gains = [&](int v) {
+        const int c = c0 + v * 512 * W;
 #pragma unroll
-    for (int v = 0; v < NV; v++)
+        for (int i = 0; i < 8; i++) { kp[v][i] = a.scale; kn[v][i] = 0.0f; }
+        if (dxn) g53_load8_to(kn[v], a.next, c, H);
+        if (Y) {
+            float t[8];
+            if (a.post) {
+                g53_load8_to(t, a.post, c, H);
 #pragma unroll
-        for (int i = 0; i < 8; i++) ap[v][i] = an[v][i] = ag[v][i] = 0.0f;
-    float kp[NV][8], kn[NV][8], kg[NV][8];
+                for (int i = 0; i < 8; i++) kp[v][i] *= t[i];
+            }
+            if (GK == 1) {
+                g53_load8_to(t, (const float *)a.gate, c, H);
+#pragma unroll
+                for (int i = 0; i < 8; i++) kp[v][i] *= t[i];
+            }
+        }
+    };
 #pragma unroll
     for (int v = 0; v < NV; v++) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) { kp[v][i] = 1.0f; kn[v][i] = 0.0f; kg[v][i] = 1.0f; }
-        const int c = c0 + v * 512 * W;
-        if (KEEP) {
-            if (Y && a.post) g53_load8_to(kp[v], a.post, c, H);
-            if (dxn) g53_load8_to(kn[v], a.next, c, H);
-            if (Y && GK == 1) {
-                g53_load8_to(kg[v], (const float *)a.gate, c, H);
-#pragma unroll
-                for (int i = 0; i < 8; i++) kg[v][i] *= a.scale;
-            }
-        }
+        for (int i = 0; i < 8; i++) ap[v][i] = an[v][i] = 0.0f;
+        if (KEEP) gains(v);
     }
     G53Raw8<E> rh[NV], ry[NV], rg[NV], rd[NV], rt[NV];
     float rgate = 1.0f;
@@ -174,12 +181,13 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
         if (Y && GK == 2) rgate = ((const float *)a.gate)[t];
     };
     if (AHEAD) ask(grp);
-    for (long k = 0; k < rounds; k++) {
-        const long t = grp + k * groups;
+    for (long r = 0; r < rounds; r++) {
+        const long t = grp + r * groups;
         const bool live = t < a.T;
         if (!AHEAD) ask(t);
-        const int odd = k & 1;                       /* sums of two tokens in a row lie apart: one barrier each is enough */
-        float hv[NV][8], yh[NV][8], g[NV][8], d[NV][8], gt[NV][8];
+        const int odd = r & 1;                       /* sums of two tokens in a row lie apart: one barrier each is enough */
+        float hv[NV][8], yh[NV][8], g[NV][8], d[NV][8], w[NV][8], gt[NV][8];
+        const float tgate = rgate;
 #pragma unroll
         for (int v = 0; v < NV; v++)
 #pragma unroll
@@ -188,52 +196,35 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
                 if (Y) yh[v][i] = (float)ry[v].v[i];
                 d[v][i] = dxn ? (float)rd[v].v[i] : 0.0f;
                 g[v][i] = dh2 ? (float)rg[v].v[i] : 0.0f;
-                if (Y) gt[v][i] = KEEP && GK == 1 ? kg[v][i] : a.scale * (GK == 3 ? (float)rt[v].v[i] : GK == 2 ? rgate : 1.0f);
+                if (Y && GK == 3) gt[v][i] = (float)rt[v].v[i];
             }
         if (AHEAD) ask(t + groups);
         float rsy = 1.0f;
-        if (Y) {
-            if (a.post) {
-                float s[1] = {0.0f};
+        if (Y && a.post) {
+            float s[1] = {0.0f};
 #pragma unroll
-                for (int v = 0; v < NV; v++)
+            for (int v = 0; v < NV; v++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) s[0] = __builtin_fmaf(yh[v][i], yh[v][i], s[0]);
-                g53_group_sum<W, 1>(s, buf1[odd], wv);
-                rsy = g53_rsq(s[0] * inv + a.eps);
-            }
+                for (int i = 0; i < 8; i++) s[0] = __builtin_fmaf(yh[v][i], yh[v][i], s[0]);
+            g53_group_sum<W, 1>(s, buf1[odd], wv);
+            rsy = g53_rsq(s[0] * inv + a.eps);
         }
-        /* w: v = dxn next; au: scale gate post y^, whose sum with dH is dy's mean */
-        float s[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, w[NV][8], pv[NV][8];
+        /* the factor of y^ in h', of dH in dy */
+        auto factor = [&](int v, int i) { return GK < 2 ? kp[v][i] : kp[v][i] * (GK == 2 ? tgate : gt[v][i]); };
+        float s[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            const int c = c0 + v * 512 * W;
-            float nv[8];
+            if (!KEEP) gains(v);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                nv[i] = kn[v][i];
-                pv[v][i] = kp[v][i];
-            }
-            if (!KEEP && dxn) g53_load8_to(nv, a.next, c, H);
-            if (Y && !KEEP) {
-                if (a.post) g53_load8_to(pv[v], a.post, c, H);
-                if (GK == 1) {
-                    float gv[8];
-                    g53_load8_to(gv, (const float *)a.gate, c, H);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) gt[v][i] *= gv[i];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                w[v][i] = d[v][i] * nv[i];
+                w[v][i] = d[v][i] * kn[v][i];
                 if (Y) {
                     yh[v][i] *= rsy;
-                    const float u = yh[v][i] * pv[v][i], au = gt[v][i] * u;
-                    hv[v][i] = __builtin_fmaf(gt[v][i], u, hv[v][i]);
-                    s[2] = __builtin_fmaf(au, g[v][i], s[2]);
-                    s[3] = __builtin_fmaf(au, w[v][i], s[3]);
-                    s[4] = __builtin_fmaf(au, hv[v][i], s[4]);
+                    const float u = factor(v, i) * yh[v][i];
+                    hv[v][i] += u;
+                    s[2] = __builtin_fmaf(u, g[v][i], s[2]);
+                    s[3] = __builtin_fmaf(u, w[v][i], s[3]);
+                    s[4] = __builtin_fmaf(u, hv[v][i], s[4]);
                 }
                 s[0] = __builtin_fmaf(hv[v][i], hv[v][i], s[0]);
                 s[1] = __builtin_fmaf(w[v][i], hv[v][i], s[1]);
@@ -241,8 +232,17 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
         }
         g53_group_sum<W, 5>(s, buf2[odd], wv);
         const float rs = dxn ? g53_rsq(s[0] * inv + a.eps) : 0.0f, mean = s[1] * rs * inv;
-        const float meany = a.post ? (s[2] + rs * (s[3] - rs * mean * s[4])) * inv : 0.0f;
+        const float to_y = a.post ? -rsy * (s[2] + rs * (s[3] - rs * mean * s[4])) * inv : 0.0f;
         float gsum[1] = {0.0f};
+        if (AHEAD)                                   /* the next token's rows, before this one's stores */
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                g53_arrived(rh[v]);
+                if (Y) g53_arrived(ry[v]);
+                if (dxn) g53_arrived(rd[v]);
+                if (dh2) g53_arrived(rg[v]);
+                if (Y && GK == 3) g53_arrived(rt[v]);
+            }
         if (live)
 #pragma unroll
             for (int v = 0; v < NV; v++) {
@@ -256,20 +256,19 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
                 }
                 g53_store8_to(dh + t * H, g[v], c, H);
                 if (!Y) continue;
-                if (GK)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        dg[i] = a.scale * (yh[v][i] * pv[v][i]) * g[v][i];
-                        if (GK == 1) ag[v][i] += dg[i];
-                        if (GK == 2) gsum[0] += dg[i];
-                    }
-                if (GK == 3 && a.dgate) g53_store8_to((E *)a.dgate + t * H, dg, c, H);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float du = gt[v][i] * g[v][i];
-                    ap[v][i] = __builtin_fmaf(du, yh[v][i], ap[v][i]);
-                    g[v][i] = rsy * __builtin_fmaf(-yh[v][i], meany, du * pv[v][i]);      /* without post: du itself */
+                    if (GK < 2) {
+                        ap[v][i] = __builtin_fmaf(yh[v][i], g[v][i], ap[v][i]);
+                    } else {
+                        const float yg = yh[v][i] * g[v][i];
+                        ap[v][i] = __builtin_fmaf(GK == 2 ? tgate : gt[v][i], yg, ap[v][i]);
+                        dg[i] = kp[v][i] * yg;
+                        gsum[0] += dg[i];
+                    }
+                    g[v][i] = __builtin_fmaf(to_y, yh[v][i], rsy * (factor(v, i) * g[v][i]));      /* without post: du itself */
                 }
+                if (GK == 3 && a.dgate) g53_store8_to((E *)a.dgate + t * H, dg, c, H);
                 g53_store8_to(dy + t * H, g[v], c, H);
             }
         if (Y && GK == 2 && a.dgate) {
@@ -279,7 +278,7 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
         }
     }
     /* the sums of the workgroup's groups, added in order by the first of them, which writes them */
-    float *part = a.part + (long)blockIdx.x * 3 * H;
+    float *part = a.part + (long)blockIdx.x * 2 * H;
     auto finish = [&](float (&v8)[NV][8], int which) {
         if (RB > 1) {                                /* NV = 1 */
             __shared__ float rows[RB > 1 ? NW : 1][8][64];
@@ -301,28 +300,36 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
     };
     if (Y) finish(ap, 0);
     finish(an, 1);
-    if (Y && GK == 1) finish(ag, 2);
 }
 
-/* out[which][c] = the groups' partial sums, added in a fixed order: 16 chains of groups, then a tree. */
+/* Column c of the workgroups' partial sums, added in a fixed order: 32 chains, then a tree. The first give dpost and the
+ * gradient of a gate by channel (scale and the other's value times the sum; the gate by token or element is in it already),
+ * the second dnext. */
 __global__ void __launch_bounds__(1024) k_norm_sum(float *__restrict__ dpost, float *__restrict__ dnext, float *__restrict__ dgate,
-                                                   const float *__restrict__ part, int groups, int H)
+                                                   const float *__restrict__ post, const float *__restrict__ gate,
+                                                   const float *__restrict__ part, float scale, int parts, int H)
 {
-    __shared__ float buf[16][64];
-    float *out = blockIdx.y == 0 ? dpost : (blockIdx.y == 1 ? dnext : dgate);
-    if (!out) return;
-    const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    __shared__ float buf[32][32];
+    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, which = blockIdx.y;
+    if (which ? !dnext : !dpost && !dgate) return;
     float s = 0.0f;
     if (c < H)
 #pragma unroll 8
-        for (int g = k; g < groups; g += 16) s += part[((long)g * 3 + blockIdx.y) * H + c];
+        for (int g = k; g < parts; g += 32) s += part[((long)g * 2 + which) * H + c];
     buf[k][lane] = s;
     __syncthreads();
-    for (int d = 8; d; d >>= 1) {
+    for (int d = 16; d; d >>= 1) {
         if (k < d) buf[k][lane] += buf[k + d][lane];
         __syncthreads();
     }
-    if (k == 0 && c < H) out[c] = buf[0][lane];
+    if (k || c >= H) return;
+    s = buf[0][lane];
+    if (which) {
+        dnext[c] = s;
+        return;
+    }
+    if (dpost) dpost[c] = scale * (gate ? gate[c] : 1.0f) * s;
+    if (dgate) dgate[c] = scale * (post ? post[c] : 1.0f) * s;
 }
 
 /* Waves per row: 512 elements each, twice that above 8192. */
@@ -368,15 +375,15 @@ static int backward(void *dh, void *dy, float *dpost, float *dnext, float *dchan
     const long most = g53h_num_cus() * (W < 8 ? 2 : 1), need = ((long)a.T + RB - 1) / RB, rounds = (need + most - 1) / most;
     const unsigned wgs = (unsigned)(need ? (need + rounds - 1) / rounds : 0);
     if (wgs) {
-        a.part = (float *)g53h_op_workspace((size_t)wgs * 3 * a.H * sizeof(float));
+        a.part = (float *)g53h_op_workspace((size_t)wgs * 2 * a.H * sizeof(float));
         if (!a.part) return -1;
         hipLaunchKernelGGL((k_block_norm_grad<E, W, NV, GK, Y>), dim3(wgs), dim3(64 * NW), 0, g53h_stream(), (E *)dh, (E *)dy,
                            (const E *)dh2, (const E *)dxn, (const E *)h, (const E *)y, a);
         G53_LAUNCHED("k_block_norm_grad");
     }
     if (dpost || dnext || dchannel) {
-        hipLaunchKernelGGL(k_norm_sum, dim3((a.H + 63) / 64, 3), dim3(1024), 0, g53h_stream(), dpost, dnext, dchannel, a.part,
-                           (int)wgs, a.H);
+        hipLaunchKernelGGL(k_norm_sum, dim3((a.H + 31) / 32, 2), dim3(1024), 0, g53h_stream(), dpost, dnext, dchannel, a.post,
+                           GK == 1 ? (const float *)a.gate : nullptr, a.part, a.scale, (int)wgs, a.H);
         G53_LAUNCHED("k_norm_sum");
     }
     return 0;
