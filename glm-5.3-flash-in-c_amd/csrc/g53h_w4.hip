@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     auto load = [&](Chunk &k, int c) {
         const int w_at = c * 64 + q * 16, wo = w_at < wrow ? w_at : 0;      /* behind the end: the row's start, never used */
 #pragma unroll
-        for (int r = 0; r < R; r++) k.w[r] = __builtin_nontemporal_load((const g53_v4w *)(wb[r] + (unsigned)(w_of[r] + wo)));
+        for (int r = 0; r < R; r++) k.w[r] = *(const g53_v4w *)(wb[r] + (unsigned)(w_of[r] + wo));
         if (GS < 4) ask(k.s, k.z, group_of(c));
     };
     const int ld = a.seg * (256 * UC) + 16; /* bytes of a plane's row in LDS: odd sixteens, so rows start in other banks */
