@@ -183,7 +183,7 @@ __device__ __forceinline__ void g53_spread(float (&o)[4], float v)
  * columns, in units of UC x 128 taken in turn, by NW / KW groups of R row tiles. A unit's levels are asked for one unit
  * ahead. GS: groups are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows,
  * the others the same up rows. Columns behind the last of a unit meet activations of zero. */
-template <typename E, int R, int NT, int UC, bool ROWS, int GS>
+template <typename E, int R, int NT, int UC, bool ROWS, bool LINES, int GS>
 __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2) k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets, const int *__restrict__ pair, G53W4Args a)
 {
     typedef typename G53W4Type<E>::V V;
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     /* where the row tiles begin; the lane's row in them, the last one for those behind the end */
     const uint8_t *wb[R], *sb[R], *zb[R];
     const int wrow = a.cols / 2, srow = a.groups * (a.s_dt == G53H_F32 ? 4 : 2), zrow = (a.groups + 1) / 2;
-    int w_of[R], s_of[R], z_of[R];
+    int w_of[R][2], s_of[R], z_of[R];       /* the rows that the lane loads; the row m whose scales it takes */
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const bool up = sw && r >= R / 2;
@@ -222,7 +222,12 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
         wb[r] = a.w + at * wrow;
         sb[r] = (const uint8_t *)a.s + at * srow;
         zb[r] = a.z + at * zrow;
-        w_of[r] = i * wrow;
+        const int end = a.half - top - 1;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int j8 = LINES ? (m & 7) + 8 * b : m;
+            w_of[r][b] = (j8 < end ? j8 : end) * wrow;
+        }
         s_of[r] = i * srow;
         z_of[r] = i * zrow;
     }
@@ -269,11 +274,33 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
         return g < a.groups ? g : a.groups - 1;
     };
     typedef G53W4Chunk<R> Chunk;
-    auto load = [&](Chunk &k, int c) {
-        const int w_at = c * 64 + q * 16, wo = w_at < wrow ? w_at : 0;      /* behind the end: the row's start, never used */
+    /* Levels of a chunk, 16 rows x 64 bytes a load, or (LINES) of two: a load takes whole lines then, 8 rows x 128 bytes,
+     * the first chunk's quarter q in lanes m < 8 of its rows and the second's in lanes m >= 8, until `pass` gives each lane
+     * its row of both; such lines are not kept in the caches, where half lines wait for their other half. */
+    constexpr int PAIR = LINES ? 2 : 1;
+    auto load = [&](Chunk *k, int c) {
+        const int w_at = c * 64 + (LINES ? (m >> 3) * 64 : 0) + q * 16, wo = w_at < wrow ? w_at : 0;   /* behind the end: not used */
 #pragma unroll
-        for (int r = 0; r < R; r++) k.w[r] = *(const g53_v4w *)(wb[r] + (unsigned)(w_of[r] + wo));
-        if (GS < 4) ask(k.s, k.z, group_of(c));
+        for (int b = 0; b < PAIR; b++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const g53_v4w *from = (const g53_v4w *)(wb[r] + (unsigned)(w_of[r][b] + wo));
+                k[b].w[r] = LINES ? __builtin_nontemporal_load(from) : *from;
+            }
+        if (GS < 4)
+#pragma unroll
+            for (int b = 0; b < PAIR; b++) ask(k[b].s, k[b].z, group_of(c + b));
+    };
+    auto pass = [&](Chunk *k) {
+        if (LINES)
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {       /* by 8 lanes of 16: rows 8..15 of the first, 0..7 of the second */
+                    const int u = (int)k[0].w[r][i], v = (int)k[PAIR - 1].w[r][i];
+                    k[0].w[r][i] = (unsigned)__builtin_amdgcn_update_dpp(u, v, 0x128, 0xf, 0xc, false);
+                    k[PAIR - 1].w[r][i] = (unsigned)__builtin_amdgcn_update_dpp(v, u, 0x128, 0xf, 0x3, false);
+                }
     };
     const int ld = a.seg * (256 * UC) + 16; /* bytes of a plane's row in LDS: odd sixteens, so rows start in other banks */
     int xat[NT];                            /* the lane's token in LDS; tokens behind the last repeat it */
@@ -382,7 +409,7 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
         __builtin_amdgcn_sched_barrier(0);
         if (GS == 4) ask(us, uz, unit_group(kw));
 #pragma unroll
-        for (int j = 0; j < UC; j++) load(ring[j], kw * UC + j);
+        for (int j = 0; j < UC; j += PAIR) load(ring + j, kw * UC + j);
         __builtin_amdgcn_sched_barrier(0);
         put(v, 0, wv);
     }
@@ -405,16 +432,18 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
             if (GS == 4) ask(us, uz, unit_group(seg0 + i + KW));
 #pragma unroll
             for (int j = 0; j < UC; j++) {
+                if (j % PAIR == 0) pass(ring + j);
 #pragma unroll
                 for (int r = 0; r < R; r++) { sj[r] = sc[r][j]; nj[r] = nz[r][j]; }
                 use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, nj);
-                load(ring[j], (seg0 + i + KW) * UC + j);
+                if (j % PAIR == PAIR - 1) load(ring + j - (PAIR - 1), (seg0 + i + KW) * UC + j - (PAIR - 1));
             }
         }
         if (ends && i < here) {
             unit_scales(seg0 + i, sc, nz);
 #pragma unroll
             for (int j = 0; j < UC; j++) {
+                if (j % PAIR == 0) pass(ring + j);
 #pragma unroll
                 for (int r = 0; r < R; r++) { sj[r] = sc[r][j]; nj[r] = nz[r][j]; }
                 use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, nj);
@@ -451,23 +480,23 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     }
 }
 
-template <typename E, int R, int NT, int UC, bool ROWS, int GS>
+template <typename E, int R, int NT, int UC, bool ROWS, bool LINES, int GS>
 static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const G53W4Args &a)
 {
     static int allowed = 0;
     if (!allowed) {
-        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, UC, ROWS, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, UC, ROWS, LINES, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                     G53_W4_LDS_MAX));
         allowed = 1;
     }
-    hipLaunchKernelGGL((k_w4<E, R, NT, UC, ROWS, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x,
+    hipLaunchKernelGGL((k_w4<E, R, NT, UC, ROWS, LINES, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x,
                        a.offsets, a.pair, a);
     G53_LAUNCHED("k_w4");
     return 0;
 }
 
 /* busy: token tiles that are expected to hold rows. */
-template <typename E, int R, int NT, int UC, bool ROWS> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
+template <typename E, int R, int NT, int UC, bool ROWS, bool LINES = false> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
 {
     constexpr int P = G53W4Type<E>::P, TT = ROWS ? 16 * NT / P : 16 * NT;
     const bool sw = a.limit > 0.0f;
@@ -496,9 +525,9 @@ template <typename E, int R, int NT, int UC, bool ROWS> static int launch(void *
         a.item0 = i;
         a.items = (int)(items - i < most ? items - i : most);
         const dim3 grid((unsigned)(a.items * wide));
-        const int rc = a.group % 128 == 0 ? start<E, R, NT, UC, ROWS, 4>(grid, waves, lds, y, x, a)
-                       : a.group % 64 == 0 ? start<E, R, NT, UC, ROWS, 2>(grid, waves, lds, y, x, a)
-                                           : start<E, R, NT, UC, ROWS, 1>(grid, waves, lds, y, x, a);
+        const int rc = a.group % 128 == 0 ? start<E, R, NT, UC, ROWS, LINES, 4>(grid, waves, lds, y, x, a)
+                       : a.group % 64 == 0 ? start<E, R, NT, UC, ROWS, LINES, 2>(grid, waves, lds, y, x, a)
+                                           : start<E, R, NT, UC, ROWS, LINES, 1>(grid, waves, lds, y, x, a);
         if (rc) return rc;
     }
     return 0;
@@ -508,7 +537,10 @@ template <typename E, int R, int NT, int UC, bool ROWS> static int launch(void *
  * 16 waves a CU (4096 x 2048 by one token in bf16: 4.8 us against 5.9). Token tiles of 16, or of 32 for more tokens of
  * many waves, which then turn levels into floats half as often (16384 x 4096 by 128 tokens: 44 us against 50; fp32: 57
  * against 71). For fp32, whose products are three, up to 5 tokens put their planes side by side as 15 rows of a tile, and
- * the products are as many as bf16's (16384 x 4096 by one token: 14.5 us against 16.4). */
+ * the products are as many as bf16's (16384 x 4096 by one token: 14.5 us against 16.4). Long rows of a matrix that one
+ * token tile meets are loaded in whole lines (65536 x 4096 by 5 tokens: 27.3 us against 30.7; eight gate/up matrices of
+ * 4096 x 4096 by one token 16.3 against 17.2); short rows, or rows that further tiles read again, in half lines (64 matrices
+ * of 2048 x 1024 by 64 tokens 20.8 against 22.4, 2048 x 2048 by 256 tokens 58 against 70). */
 template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
 {
     constexpr bool F32 = sizeof(E) == 4;
@@ -521,6 +553,7 @@ template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
     if constexpr (F32)
         if (TT == 16) return few ? launch<E, 1, 1, 1, false>(y, x, a, items, busy) : launch<E, 2, 1, 2, false>(y, x, a, items, busy);
     if (few) return launch<E, 1, 1, 4, F32>(y, x, a, items, busy);
+    if (mean <= TT && units >= 4) return launch<E, 2, 1, 4, F32, true>(y, x, a, items, busy);
     return launch<E, 2, 1, 4, F32>(y, x, a, items, busy);
 }
 
