@@ -325,7 +325,10 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
                 g53_spread(nz[r], surplus(k.z[r], group_of(c)));
             }
         }
-        g53_v4f D[R][NT], X[NT];
+        /* the upper planes of fp32 apart from the lower ones: what a sum of the surplus' size rounds away is rounded once
+         * a product instead of three times */
+        constexpr int DP = PM == 3 ? 2 : 1;
+        g53_v4f D[R][NT][DP], X[NT][DP];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             V b[NT][PM];
@@ -333,8 +336,9 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int p = 0; p < PM; p++) {
+                    g53_v4f &to = X[t][p ? DP - 1 : 0];
                     b[t][p] = *(const V *)(lds + p * plane + xat[t] + c_lds * 256 + s * (GS == 4 ? 16 : 64));
-                    X[t] = g53_mfma(b[t][p], ones, s % GS == 0 && p == 0 ? zero : X[t]);
+                    to = g53_mfma(b[t][p], ones, s % GS == 0 && p < 2 ? zero : to);
                 }
 #pragma unroll
             for (int r = 0; r < R; r++) {
@@ -342,7 +346,10 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int p = 0; p < PM; p++) D[r][t] = g53_mfma(b[t][p], lv, s % GS == 0 && p == 0 ? zero : D[r][t]);
+                    for (int p = 0; p < PM; p++) {
+                        g53_v4f &to = D[r][t][p ? DP - 1 : 0];
+                        to = g53_mfma(b[t][p], lv, s % GS == 0 && p < 2 ? zero : to);
+                    }
             }
             if (NT * PM > 2) __builtin_amdgcn_sched_barrier(0);     /* one step's activations in registers at a time */
             if (s % GS == GS - 1)       /* a group, or what the chunk has of it */
@@ -351,8 +358,11 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            acc[r][t][i] = __builtin_fmaf(sc[r][s], __builtin_fmaf(nz[r][s], X[t][i], D[r][t][i]), acc[r][t][i]);
+                        for (int i = 0; i < 4; i++) {
+                            float v = __builtin_fmaf(nz[r][s], X[t][0][i], D[r][t][0][i]);
+                            if (DP == 2) v += __builtin_fmaf(nz[r][s], X[t][DP - 1][i], D[r][t][DP - 1][i]);
+                            acc[r][t][i] = __builtin_fmaf(sc[r][s], v, acc[r][t][i]);
+                        }
                         asm volatile("" : "+v"(acc[r][t]));      /* added here, not behind the next branch with D kept */
                     }
         }
