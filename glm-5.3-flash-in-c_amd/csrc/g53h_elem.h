@@ -67,11 +67,15 @@ __device__ __forceinline__ void g53_store8(g53_f16 *p, const float (&v)[8])
     ((G53v8h_any *)p)->v = a;
 }
 
-/* Elements c .. c + 7 of a row of n, zeros behind its end (where the last one is read instead: no branch). */
+/* Elements c .. c + 7 of a row of n, zeros behind its end: a lane whose eight all lie there reads nothing, one that meets
+ * the end reads the last element in their place, without a branch. */
 template <typename T> __device__ __forceinline__ void g53_load8_to(float (&o)[8], const T *row, int c, int n)
 {
     if (c + 8 <= n) {
         g53_load8(o, row + c);
+    } else if (c >= n) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = 0.0f;
     } else {
         T v[8];
 #pragma unroll
@@ -99,6 +103,9 @@ template <typename T> __device__ __forceinline__ void g53_raw8_to(G53Raw8<T> &o,
     struct __attribute__((packed, aligned(2))) Any { V8 v; };
     if (c + 8 <= n) {
         o.v = ((const Any *)(row + c))->v;
+    } else if (c >= n) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) o.v[i] = (T)0.0f;
     } else {
         T v[8];
 #pragma unroll

@@ -24,6 +24,7 @@
 
 #define G53_W4_MAXE 1024
 #define G53_W4_MAXC (1 << 24)          /* columns: 16 rows of levels or scales stay below 2^31 bytes */
+#define G53_W4_MAXR (1 << 30)
 #define G53_W4_NW 8                     /* waves of a workgroup, at most */
 #define G53_W4_LDS_MAX (150 * 1024)
 #define G53_W4_LDS (78 * 1024)          /* of its activations: two workgroups a CU */
@@ -125,14 +126,15 @@ __device__ __forceinline__ void g53_turn(unsigned (&d)[4])
 }
 
 /* The token tile `item` of the sorted rows: tiles of TT rows, expert by expert. False behind the last. */
-__device__ __forceinline__ bool g53_w4_item(const int *__restrict__ offsets, int n_experts, long item, int TT, int &e, int &first, int &last)
+__device__ __forceinline__ bool g53_w4_item(const int *__restrict__ offsets, int n_experts, long item, int TT,
+                                            int &e, int &first, int &last)
 {
     const int lane = threadIdx.x & 63, per = (n_experts + 63) / 64, e0 = lane * per;
     int n = 0, from = e0 < n_experts ? offsets[e0] : 0;
     for (int i = 0, at = from; i < per; i++)
         if (e0 + i < n_experts) {
             const int to = offsets[e0 + i + 1];
-            n += (to - at + TT - 1) / TT;
+            n += (int)((unsigned)(to - at + TT - 1) / TT);
             at = to;
         }
     int incl = n;
@@ -148,13 +150,13 @@ __device__ __forceinline__ bool g53_w4_item(const int *__restrict__ offsets, int
     first = __builtin_amdgcn_readlane(from, l);
     for (e = l * per;; e++) {                 /* lane l's experts: one of them holds the tile */
         last = offsets[e + 1];
-        const int tiles = (last - first + TT - 1) / TT;
+        const int tiles = (int)((unsigned)(last - first + TT - 1) / TT);
         if (skip < tiles) break;
         skip -= tiles;
         first = last;
     }
     first += skip * TT;
-    last = first + TT < last ? first + TT : last;
+    last = last - first > TT ? first + TT : last;
     return true;
 }
 
@@ -184,7 +186,8 @@ __device__ __forceinline__ void g53_spread(float (&o)[4], float v)
  * ahead. GS: groups are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows,
  * the others the same up rows. Columns behind the last of a unit meet activations of zero. */
 template <typename E, int R, int NT, int UC, bool ROWS, bool LINES, int GS>
-__global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2) k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets, const int *__restrict__ pair, G53W4Args a)
+__global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2)
+k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets, const int *__restrict__ pair, G53W4Args a)
 {
     typedef typename G53W4Type<E>::V V;
     constexpr int P = G53W4Type<E>::P, PM = ROWS ? 1 : P, MT = 16 * NT, TT = ROWS ? MT / P : MT, LD = 16 * R + 4;
@@ -192,7 +195,8 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
     const bool sw = a.limit > 0.0f;
     const int out = sw ? 8 * R : 16 * R;                     /* result rows of a wave */
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), NW = blockDim.x >> 6;
-    const int m = lane & 15, q = lane >> 4, KW = 1 << a.kw_log, kw = wv & (KW - 1), rw = wv >> a.kw_log, RW = NW >> a.kw_log;
+    const int m = lane & 15, q = lane >> 4;
+    const int KW = 1 << a.kw_log, kw = wv & (KW - 1), rw = wv >> a.kw_log, RW = NW >> a.kw_log;
     /* Workgroups go to the 8 dies in turn. Of one matrix, eight row tiles go side by side and a row tile's token tiles
      * after each other on one die, whose cache then holds the rows; of several, a token tile's row tiles follow each other. */
     const unsigned eight = 8u * a.items;
@@ -217,7 +221,8 @@ __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const bool up = sw && r >= R / 2;
-        const int j = row0 + 16 * (up ? r - R / 2 : r), top = j < a.half ? j : a.half - 1, i = m < a.half - top ? m : a.half - top - 1;
+        const int j = row0 + 16 * (up ? r - R / 2 : r), top = j < a.half ? j : a.half - 1;
+        const int i = m < a.half - top ? m : a.half - top - 1;
         const long at = (long)e * a.rows + top + (up ? a.half : 0);
         wb[r] = a.w + at * wrow;
         sb[r] = (const uint8_t *)a.s + at * srow;
@@ -506,7 +511,8 @@ static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const
 }
 
 /* busy: token tiles that are expected to hold rows. */
-template <typename E, int R, int NT, int UC, bool ROWS, bool LINES = false> static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
+template <typename E, int R, int NT, int UC, bool ROWS, bool LINES = false>
+static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
 {
     constexpr int P = G53W4Type<E>::P, TT = ROWS ? 16 * NT / P : 16 * NT;
     const bool sw = a.limit > 0.0f;
@@ -529,8 +535,8 @@ template <typename E, int R, int NT, int UC, bool ROWS, bool LINES = false> stat
     a.seg = seg;
     size_t lds = (size_t)rows * P * (seg * 256 * UC + 16), red = (size_t)waves * 16 * NT * (16 * R + 4) * 4;
     if (lds < red) lds = red;
-    const long wide = a.offsets ? a.tiles : (a.tiles + 7) / 8 * 8l, most = (1l << 31) / (64 * G53_W4_NW) / wide;      /* threads of a launch fit 32 bits */
-    if (most < 1) return g53h_fail("g53h_mm_w4: %d rows", a.rows);
+    /* threads of a launch fit 32 bits: of 2^30 rows a workgroup has 256 */
+    const long wide = a.offsets ? a.tiles : (a.tiles + 7) / 8 * 8l, most = (1l << 31) / (64 * G53_W4_NW) / wide;
     for (long i = 0; i < items; i += most) {
         a.item0 = i;
         a.items = (int)(items - i < most ? items - i : most);
@@ -555,13 +561,15 @@ template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
 {
     constexpr bool F32 = sizeof(E) == 4;
     const long ex = a.offsets ? (a.n_experts < a.T ? a.n_experts : a.T) : 1, mean = (a.T + ex - 1) / ex;
-    const long units = (a.cols + 511) / 512, waves = (a.rows + 31) / 32 * ex * ((mean + 15) / 16) * (units < G53_W4_NW ? units : G53_W4_NW);
+    const long units = (a.cols + 511) / 512;
+    const long waves = (a.rows + 31) / 32 * ex * ((mean + 15) / 16) * (units < G53_W4_NW ? units : G53_W4_NW);
     const bool few = waves <= 16 * g53h_num_cus() && !(a.limit > 0.0f);
     const int TT = F32 && mean <= 5 ? 5 : (mean > 16 && !few ? 32 : 16);
-    const long items = a.offsets ? a.T / TT + ex : (a.T + TT - 1) / TT, busy = ex * ((mean + TT - 1) / TT);
+    const long items = a.offsets ? a.T / TT + ex : (a.T - 1) / TT + 1, busy = ex * ((mean + TT - 1) / TT);
     if (TT == 32) return launch<E, 2, 2, 2, false>(y, x, a, items, busy);
     if constexpr (F32)
-        if (TT == 16) return few ? launch<E, 1, 1, 1, false>(y, x, a, items, busy) : launch<E, 2, 1, 2, false>(y, x, a, items, busy);
+        if (TT == 16)
+            return few ? launch<E, 1, 1, 1, false>(y, x, a, items, busy) : launch<E, 2, 1, 2, false>(y, x, a, items, busy);
     if (few) return launch<E, 1, 1, 4, F32>(y, x, a, items, busy);
     if (mean <= TT && units >= 4) return launch<E, 2, 1, 4, F32, true>(y, x, a, items, busy);
     return launch<E, 2, 1, 4, F32>(y, x, a, items, busy);
@@ -578,9 +586,10 @@ static int product(void *y, const void *x, int dt, G53W4Args &a)
 static int w4_bad(const char *who, const G53hW4 *m, int dt, float limit, G53W4Args &a)
 {
     if (!m || !m->w || !m->s) return g53h_fail("%s: unbound matrix", who);
-    if (m->rows < 1 || m->cols < 32 || m->cols > G53_W4_MAXC || m->cols % 32 || m->group < 32 || m->group % 32 || !g53_elem_bytes(m->s_dt))
-        return g53h_fail("%s: %d x %d levels in groups of %d, scale type %d (columns and group multiples of 32, columns at most 2^24)", who, m->rows,
-                         m->cols, m->group, m->s_dt);
+    if (m->rows < 1 || m->rows > G53_W4_MAXR || m->cols < 32 || m->cols > G53_W4_MAXC || m->cols % 32 || m->group < 32 ||
+        m->group % 32 || !g53_elem_bytes(m->s_dt))
+        return g53h_fail("%s: %d x %d levels in groups of %d, scale type %d (columns and group multiples of 32, at most 2^24 "
+                         "columns of 2^30 rows)", who, m->rows, m->cols, m->group, m->s_dt);
     if (((uintptr_t)m->w & 15) || ((uintptr_t)m->s & (g53_elem_bytes(m->s_dt) - 1)))
         return g53h_fail("%s: levels must start at a multiple of 16 bytes, scales of their type", who);
     if (!g53_elem_bytes(dt)) return g53h_fail("%s: element type %d", who, dt);

@@ -380,7 +380,7 @@ typedef struct {
 /* Fills the plan's three arrays from idx_d [T][topk]. */
 int g53h_sort_tokens(const G53hSort *p, const int *idx_d);
 /* xs[row of (t, j)] = x[t]: x [T][hidden], xs [n][hidden]. Rows behind the last sorted one are left as
- * they were. _grad: dx[t] = sum of the dxs rows of t's pairs. */
+ * they were. _grad: dx[t] = sum of the dxs rows of t's pairs. hidden at most 2^30. */
 int g53h_sorted_dispatch(void *xs_d, const void *x_d, int dt, int hidden, const G53hSort *p);
 int g53h_sorted_dispatch_grad(void *dx_d, const void *dxs_d, int dt, int hidden, const G53hSort *p);
 /* out[t] = add[t] + sum over j of w[t][j] ys[row of (t, j)], in order of j; w fp32 [T][topk]; add may be
@@ -405,7 +405,9 @@ typedef struct {
 } G53hW4;
 /* y[T][rows] = M . x[T][cols]. With swiglu_limit > 0 the matrix is gate over up (rows / 2 each) and
  * y[T][rows / 2] their SwiGLU as g53h_swiglu's, from the fp32 sums; 0: without. Meant for few tokens:
- * the weights are read once per 16 to 64 of them. A row of x that is not finite gives NaN. */
+ * the levels go to the matrix cores once per 16 or 32 of them (fp32: 5 where there are no more). Products
+ * are exact and sums fp32; a row of x whose |x| times 31 leaves fp32 in a group's sum, or that is not
+ * finite, gives NaN, and fp32 values below 2^-109 lose low bits. At most 2^24 columns of 2^30 rows. */
 int g53h_mm_w4(void *y_d, const void *x_d, int dt, int T, const G53hW4 *m, float swiglu_limit);
 /* The same over the sorted rows of a plan, each with its expert's matrix: m describes expert 0, the levels,
  * scales and zero points of the others follow it. x: with gather the tokens [T][cols] (a row takes its pair's
@@ -413,8 +415,8 @@ int g53h_mm_w4(void *y_d, const void *x_d, int dt, int T, const G53hW4 *m, float
 int g53h_sorted_mm_w4(void *ys_d, const void *x_d, int dt, int gather, const G53hSort *p, const G53hW4 *m,
                       float swiglu_limit);
 
-/* xn = x / sqrt(mean of x^2 + eps) * gain per row of hidden <= 16384; gain fp32 [hidden]; xn may be x.
- * _grad: dx (may be dxn) and, where it is not NULL, dgain fp32 [hidden], from dxn and x. */
+/* xn = x / sqrt(mean of x^2 + eps) * gain per row of hidden <= 16384; gain fp32 [hidden]; eps 1e-30 to
+ * 1e30; xn may be x. _grad: dx (may be dxn) and, where it is not NULL, dgain fp32 [hidden], from dxn and x. */
 int g53h_norm(void *xn_d, const void *x_d, const float *gain_d, int dt, int T, int hidden, float eps);
 int g53h_norm_grad(void *dx_d, float *dgain_d, const void *dxn_d, const void *x_d, const float *gain_d, int dt, int T,
                    int hidden, float eps);
@@ -422,9 +424,9 @@ int g53h_norm_grad(void *dx_d, float *dgain_d, const void *dxn_d, const void *x_
  * xn = the norm of h2 (before it is rounded) with gain next, the next block's input (xn NULL: not wanted).
  * The gate by gate_kind: 0 none, 1 fp32 [hidden] per channel, 2 fp32 [T] per token, 3 [T][hidden] of type dt,
  * as it multiplies. h2 may be h.
- * _grad, of dh2 and dxn (either may be NULL: zero): dh (may be dh2), dy, dgate in the gate's shape and type,
- * dpost and dnext fp32 [hidden]; dgate, dpost and dnext may be NULL. Sums over tokens are in a fixed order: the
- * same bits on every run. */
+ * _grad, of dh2 and dxn (one of them may be NULL: zero): dh (may be dh2), dy, dgate in the gate's shape and
+ * type, dpost (with post) and dnext (with next) fp32 [hidden]; dgate, dpost and dnext may be NULL. Sums over
+ * tokens are in a fixed order: the same bits on every run. */
 typedef struct {
     int   T, hidden, dt, gate_kind;
     float eps, scale;

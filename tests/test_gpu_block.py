@@ -8,8 +8,10 @@ import numpy as np
 import pytest
 
 import glm53h
-from glm53h import check
-from op_lib import BF16, F16, F32, HALF, W4, Buf, Plan, block, dec, enc, swiglu
+import glm53h.synth as S
+from glm53h import DevBuf, check
+from op_lib import BF16, F16, F32, HALF, W4, Buf, Plan, block, dec, enc, sorted_plan, swiglu
+from test_gpu_grouped import run
 from test_gpu_parity import say
 
 pytestmark = pytest.mark.gpu
@@ -109,3 +111,33 @@ def test_training_step(L):
         diff = (loss(*up) - loss(*down)) / (2 * e)
         # e^2 of third derivatives of order one, 64-bit rounding / e, and fp32 gradients of some 800 terms
         assert abs(diff - (grad * d).sum()) < 1e-4 * (1 + abs(diff)), i
+
+
+def test_between_the_phases_of_a_grouped_layer(L):
+    """The operators have a workspace of their own: a grouped layer that is begun, with them in between, ends as without."""
+    say("operators inside a grouped pass")
+    sp = S.LayerSpec(E=512, I=512, NE=8, K=4, router_sigma=0.02)
+    T = 700
+    layer = S.DeviceLayer.build(sp)
+    x = S.x_host(sp, T, batch=6)
+    want, wi, ww = run(layer, x, 1, "g53h_moe_grouped")
+    assert T <= L.g53h_grouped_max_tokens(C.byref(layer.layer))
+    rng = np.random.default_rng(7)
+    xd, od, id_, wd = DevBuf.from_array(x), DevBuf(x.nbytes), DevBuf.from_array(wi), DevBuf.from_array(ww)
+    h, d, g = (Buf(rng.standard_normal(s), F32) for s in ((T, 512), (T, 512), (512,)))
+    dx, dg = Buf.out((T, 512), F32), Buf.out(512, F32)
+
+    def others():
+        plan = Plan(np.repeat(wi, 8, 0), sp.NE)              # 22400 pairs: segments, whose counts lie in a workspace
+        check(L.g53h_norm_grad(dx.ptr, dg.ptr, d.ptr, h.ptr, g.ptr, F32, T, 512, EPS), "norm_grad")
+        return plan
+
+    check(L.g53h_grouped_begin(xd.ptr, T, C.byref(layer.layer), id_.ptr), "begin")
+    first = others()
+    check(L.g53h_grouped_batch(C.byref(layer.layer)), "batch")
+    second = others()
+    check(L.g53h_grouped_end(od.ptr, wd.ptr), "end")
+    assert L.g53h_grouped_errors() == 0
+    assert np.array_equal(od.download(np.uint32).reshape(x.shape), want.view(np.uint32))
+    for plan in (first, second):
+        assert all(np.array_equal(a, b) for a, b in zip(plan.arrays(), sorted_plan(np.repeat(wi, 8, 0), sp.NE)))

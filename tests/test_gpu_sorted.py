@@ -41,6 +41,18 @@ def test_sort_one_expert_or_none(L, T, K, NE, fill):
         assert np.array_equal(g, w)
 
 
+@pytest.mark.parametrize("n", [63, 64, 65, 1023, 1024, 1025, 2048, 2049])
+@pytest.mark.parametrize("NE", [1, 255, 256, 1024])
+def test_sort_at_the_edges_of_its_kernels(L, n, NE):
+    say("sort, edges", n, NE)
+    rng = np.random.default_rng(n + NE)
+    idx = routing(rng, n, 1, NE, 0.2)
+    idx[-1] = NE - 1                                      # the last pair is there, and one just past the experts is not
+    idx[0] = NE
+    for g, w in zip(Plan(idx, NE).arrays(), sorted_plan(idx, NE)):
+        assert np.array_equal(g, w)
+
+
 def test_sort_no_tokens(L):
     say("sort, no tokens")
     off = Buf(np.full(10, -7, np.int32))

@@ -96,6 +96,36 @@ def test_full_range_of_fp32(L):
     close(y.val(), want, 10 * 2.0 ** -24 * 62 * (np.abs(x.val()) @ m.s[0].T))
 
 
+def test_smallest_fp16_activations(L):
+    """fp16 values below the normal range enter as they are: multiples of 2^-24, with sums that fit 24 bits, exactly."""
+    say("w4, fp16 below its normal range")
+    rng = np.random.default_rng(13)
+    m = W4(rng, 1, 24, 96, 32, F32, True, exact=True)
+    for T in (1, 20):
+        xv = rng.integers(-8, 9, (T, 96)) * 2.0 ** -24
+        x, y = Buf(xv, F16), Buf.out((T, 24), F16)
+        assert np.array_equal(x.val(), xv)
+        check(L.g53h_mm_w4(y.ptr, x.ptr, F16, T, C.byref(m.c), 0.0), "w4")
+        assert np.array_equal(y.get(), enc(xv @ m.wide[0].T, F16))
+
+
+@pytest.mark.parametrize("T", [1, 5, 6, 33])
+def test_fp32_error_stays_that_of_one_sum(L, T):
+    """fp32 products of short rows, in two groups of 128: x of size 1, levels even over 0..15, zero point 8. A group's D, the
+    sum of (16 + level) x, has an rms of 24 sqrt(128) = 272 and is added up in 4 steps, each off by up to 2^-15 (a sum in
+    [256, 512) that is cut, not rounded): 2^-15 / sqrt(3) rms. X, the sum of x, has 11.3 and counts 24 times: 24 x 2^-20 /
+    sqrt(3). Together sqrt(4) sqrt(1.76e-5^2 + 1.32e-5^2) = 4.4e-5 of a group whose own rms is sqrt(128) x 4.6 = 52:
+    8.5e-7, and the spread of a norm over 512 rows allows two fifths more. The lower planes add 2^-8 of it where their
+    products have sums of their own; in one sum with the upper ones they would each be cut at its size: sqrt(3) as much."""
+    say("w4, fp32 error", T)
+    rng = np.random.default_rng(14 + T)
+    m = W4(rng, 1, 512, 256, 128, F32, False)
+    x, y = Buf(rng.standard_normal((T, 256)), F32), Buf.out((T, 512), F32)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, F32, T, C.byref(m.c), 0.0), "w4")
+    want = x.val() @ m.wide[0].T
+    assert np.linalg.norm(y.val() - want) < 1.2e-6 * np.linalg.norm(want)
+
+
 def test_other_tokens_do_not_matter(L):
     """A token with an infinity or NaN spoils its own row only."""
     say("w4, not finite")

@@ -99,6 +99,17 @@ def test_norms_without_rows(L):
     refused(L, L.g53h_block_norm_grad(P, P, P, P, P, None, None, P, P, norm()), "neither")
 
 
+def test_sizes_past_the_limits(L):
+    for d in (dict(rows=(1 << 30) + 1), dict(cols=(1 << 24) + 32), dict(rows=-64), dict(cols=-128), dict(group=-32)):
+        refused(L, L.g53h_mm_w4(P, P, 1, 1, w4(**d), 0.0), "levels")
+        refused(L, L.g53h_sorted_mm_w4(P, P, 1, 0, plan(), w4(**d), 0.0), "levels")
+    refused(L, L.g53h_sorted_dispatch(P, P, 0, (1 << 30) + 1, plan()), "hidden")
+    refused(L, L.g53h_sorted_combine(P, P, P, None, 0, (1 << 30) + 1, plan()), "hidden")
+    for eps in (9e-31, 2e30):
+        refused(L, L.g53h_norm(P, P, P, 1, 2, 64, eps), "eps")
+        refused(L, L.g53h_block_norm(P, P, P, P, norm(eps=eps)), "eps")
+
+
 def test_struct_sizes():
     assert C.sizeof(glm53h.G53hSort) == 40
     assert C.sizeof(glm53h.G53hW4) == 40
