@@ -30,9 +30,9 @@ struct G53NormArgs {
     const float *post, *next;
     const void *gate;                   /* kind 1: float [H], 2: float [T], 3: E [T][H] */
     void *dgate;                        /* kinds 2 and 3 */
-    float *part;                        /* partial sums [workgroups][2][H] of dpost over scale and channel's gate, and dnext */
+    float *part;                        /* partial sums [workgroups][2][pitch] of dpost over scale and channel's gate, and dnext */
     float eps, scale;
-    int T, H;
+    int T, H, pitch;                    /* H up to a multiple of 32 */
 };
 
 /* 1 / sqrt(v), off by one in the last place at most; v is at least eps, a normal number. */
@@ -278,7 +278,7 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
         }
     }
     /* the sums of the workgroup's groups, added in order by the first of them, which writes them */
-    float *part = a.part + (long)blockIdx.x * 2 * H;
+    float *part = a.part + (long)blockIdx.x * 2 * a.pitch;
     auto finish = [&](float (&v8)[NV][8], int which) {
         if (RB > 1) {                                /* NV = 1 */
             __shared__ float rows[RB > 1 ? NW : 1][8][64];
@@ -295,41 +295,47 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int c = c0 + v * 512 * W;
-            if (c < H) g53_store8_to(part + which * H, v8[v], c, H);
+            if (c < a.pitch) g53_store8(part + which * a.pitch + c, v8[v]);    /* zeros behind H */
         }
     };
     if (Y) finish(ap, 0);
     finish(an, 1);
 }
 
-/* Column c of the workgroups' partial sums, added in a fixed order: 32 chains, then a tree. The first give dpost and the
- * gradient of a gate by channel (scale and the other's value times the sum; the gate by token or element is in it already),
- * the second dnext. */
-__global__ void __launch_bounds__(1024) k_norm_sum(float *__restrict__ dpost, float *__restrict__ dnext, float *__restrict__ dgate,
-                                                   const float *__restrict__ post, const float *__restrict__ gate,
-                                                   const float *__restrict__ part, float scale, int parts, int H)
+/* 32 columns of the workgroups' partial sums, added in a fixed order: 32 chains, four columns a lane, then a tree. The
+ * first sums give dpost and the gradient of a gate by channel (scale and the other's value times the sum; the gate by
+ * token or element is in it already), the second dnext. */
+__global__ void __launch_bounds__(256) k_norm_sum(float *__restrict__ dpost, float *__restrict__ dnext, float *__restrict__ dgate,
+                                                  const float *__restrict__ post, const float *__restrict__ gate,
+                                                  const float *__restrict__ part, float scale, int parts, int H, int pitch)
 {
-    __shared__ float buf[32][32];
-    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, which = blockIdx.y;
+    __shared__ g53_v4f buf[4][8];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, which = blockIdx.y;
     if (which ? !dnext : !dpost && !dgate) return;
-    float s = 0.0f;
-    if (c < H)
+    const float *from = part + which * pitch + blockIdx.x * 32 + (lane & 7) * 4;
+    g53_v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-        for (int g = k; g < parts; g += 32) s += part[((long)g * 2 + which) * H + c];
-    buf[k][lane] = s;
-    __syncthreads();
-    for (int d = 16; d; d >>= 1) {
-        if (k < d) buf[k][lane] += buf[k + d][lane];
-        __syncthreads();
+    for (int g = wv * 8 + (lane >> 3); g < parts; g += 32) {
+        const g53_v4f v = *(const g53_v4f *)(from + (long)g * 2 * pitch);
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] += v[i];
     }
-    if (k || c >= H) return;
-    s = buf[0][lane];
+#pragma unroll
+    for (int d = 8; d < 64; d <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] += __shfl_xor(s[i], d);
+    if (lane < 8) buf[wv][lane] = s;
+    __syncthreads();
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x >= 32 || c >= H) return;
+    const float *b = (const float *)buf + threadIdx.x;
+    const float t = (b[0] + b[32]) + (b[64] + b[96]);
     if (which) {
-        dnext[c] = s;
+        dnext[c] = t;
         return;
     }
-    if (dpost) dpost[c] = scale * (gate ? gate[c] : 1.0f) * s;
-    if (dgate) dgate[c] = scale * (post ? post[c] : 1.0f) * s;
+    if (dpost) dpost[c] = scale * (gate ? gate[c] : 1.0f) * t;
+    if (dgate) dgate[c] = scale * (post ? post[c] : 1.0f) * t;
 }
 
 /* Waves per row: 512 elements each, twice that above 8192. */
@@ -375,15 +381,15 @@ static int backward(void *dh, void *dy, float *dpost, float *dnext, float *dchan
     const long most = g53h_num_cus() * (W < 8 ? 2 : 1), need = ((long)a.T + RB - 1) / RB, rounds = (need + most - 1) / most;
     const unsigned wgs = (unsigned)(need ? (need + rounds - 1) / rounds : 0);
     if (wgs) {
-        a.part = (float *)g53h_op_workspace((size_t)wgs * 2 * a.H * sizeof(float));
+        a.part = (float *)g53h_op_workspace((size_t)wgs * 2 * a.pitch * sizeof(float));
         if (!a.part) return -1;
         hipLaunchKernelGGL((k_block_norm_grad<E, W, NV, GK, Y>), dim3(wgs), dim3(64 * NW), 0, g53h_stream(), (E *)dh, (E *)dy,
                            (const E *)dh2, (const E *)dxn, (const E *)h, (const E *)y, a);
         G53_LAUNCHED("k_block_norm_grad");
     }
     if (dpost || dnext || dchannel) {
-        hipLaunchKernelGGL(k_norm_sum, dim3((a.H + 31) / 32, 2), dim3(1024), 0, g53h_stream(), dpost, dnext, dchannel, a.post,
-                           GK == 1 ? (const float *)a.gate : nullptr, a.part, a.scale, (int)wgs, a.H);
+        hipLaunchKernelGGL(k_norm_sum, dim3(a.pitch / 32, 2), dim3(256), 0, g53h_stream(), dpost, dnext, dchannel, a.post,
+                           GK == 1 ? (const float *)a.gate : nullptr, a.part, a.scale, (int)wgs, a.H, a.pitch);
         G53_LAUNCHED("k_norm_sum");
     }
     return 0;
@@ -404,7 +410,7 @@ static int block_bad(const char *who, const G53hBlockNorm *p, G53NormArgs &a)
     if (p->gate_kind < 0 || p->gate_kind > 3 || (p->gate_kind && p->T && !p->gate))
         return g53h_fail("%s: gate kind %d%s", who, p->gate_kind, p->gate ? "" : ", no gate");
     if (!(p->scale >= -1.0e30f && p->scale <= 1.0e30f)) return g53h_fail("%s: scale %g", who, p->scale);
-    a = G53NormArgs{p->post, p->next, p->gate, nullptr, nullptr, p->eps, p->scale, p->T, p->hidden};
+    a = G53NormArgs{p->post, p->next, p->gate, nullptr, nullptr, p->eps, p->scale, p->T, p->hidden, (p->hidden + 31) & ~31};
     return 0;
 }
 
@@ -414,7 +420,7 @@ extern "C" int g53h_norm(void *xn, const void *x, const float *gain, int dt, int
     if (!T) return 0;
     if (!xn || !x || !gain) return g53h_fail("g53h_norm: no rows or no gain");
     if (g53h_ready()) return -1;
-    G53NormArgs a{nullptr, gain, nullptr, nullptr, nullptr, eps, 0.0f, T, hidden};
+    G53NormArgs a{nullptr, gain, nullptr, nullptr, nullptr, eps, 0.0f, T, hidden, (hidden + 31) & ~31};
     int rc;
     G53_BY_TYPE(dt, G53_NORM_BY_WIDTH(hidden, rc = (forward<E, W, NV, 0, false>(nullptr, xn, x, nullptr, a))));
     return rc;
@@ -426,7 +432,7 @@ extern "C" int g53h_norm_grad(void *dx, float *dgain, const void *dxn, const voi
     if (norm_bad("g53h_norm_grad", T, hidden, dt, eps)) return -1;
     if (T && (!dx || !dxn || !x || !gain)) return g53h_fail("g53h_norm_grad: no rows or no gain");
     if (g53h_ready()) return -1;
-    G53NormArgs a{nullptr, gain, nullptr, nullptr, nullptr, eps, 0.0f, T, hidden};
+    G53NormArgs a{nullptr, gain, nullptr, nullptr, nullptr, eps, 0.0f, T, hidden, (hidden + 31) & ~31};
     int rc;
     G53_BY_TYPE(dt, G53_NORM_BY_WIDTH(hidden, rc = (backward<E, W, NV, 0, false>(dx, nullptr, nullptr, dgain, nullptr, nullptr,
                                                                                   dxn, x, nullptr, a))));
