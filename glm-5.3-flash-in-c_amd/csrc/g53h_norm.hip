@@ -70,12 +70,27 @@ k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
     if (!live) t = a.T - 1;             /* rows behind the last: computed, not written */
     const int H = a.H, c0 = ((wv % W) * 64 + lane) * 8;
     float hv[NV][8], s[1] = {0.0f};
+    float pv[NV][8], gv[NV][8], nv[NV][8];
+    constexpr bool EARLY = NV == 1;     /* gains are asked for with the rows */
+    auto gains = [&](int v) {
+        const int c = c0 + v * 512 * W;
+        if (Y && a.post) g53_load8_to(pv[v], a.post, c, H);
+        if (Y && GK == 1) g53_load8_to(gv[v], (const float *)a.gate, c, H);
+        if (Y && GK == 3) g53_load8_to(gv[v], (const E *)a.gate + t * H, c, H);
+    };
+    auto next = [&](int v) {
+        if (xn) g53_load8_to(nv[v], a.next, c0 + v * 512 * W, H);
+    };
 #pragma unroll
     for (int v = 0; v < NV; v++) g53_load8_to(hv[v], h + t * H, c0 + v * 512 * W, H);
     if (Y) {
         float yv[NV][8];
 #pragma unroll
         for (int v = 0; v < NV; v++) g53_load8_to(yv[v], y + t * H, c0 + v * 512 * W, H);
+        if (EARLY) {
+            gains(0);
+            next(0);
+        }
         float rs = 1.0f;
         if (a.post) {
 #pragma unroll
@@ -89,17 +104,16 @@ k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int c = c0 + v * 512 * W;
-            float pv[8], gv[8];
-            if (a.post) g53_load8_to(pv, a.post, c, H);
-            if (GK == 1) g53_load8_to(gv, (const float *)a.gate, c, H);
-            if (GK == 3) g53_load8_to(gv, (const E *)a.gate + t * H, c, H);
+            if (!EARLY) gains(v);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float u = a.post ? yv[v][i] * rs * pv[i] : yv[v][i];
-                hv[v][i] = __builtin_fmaf((GK & 1) ? gt * gv[i] : gt, u, hv[v][i]);
+                const float u = a.post ? yv[v][i] * rs * pv[v][i] : yv[v][i];
+                hv[v][i] = __builtin_fmaf((GK & 1) ? gt * gv[v][i] : gt, u, hv[v][i]);
             }
             if (live) g53_store8_to(h2 + t * H, hv[v], c, H);
         }
+    } else if (EARLY) {
+        next(0);
     }
     if (!xn) return;
     s[0] = 0.0f;
@@ -112,10 +126,9 @@ k_block_norm(E *h2, E *xn, const E *h, const E *y, G53NormArgs a, long wg0)
 #pragma unroll
     for (int v = 0; v < NV; v++) {
         const int c = c0 + v * 512 * W;
-        float nv[8];
-        g53_load8_to(nv, a.next, c, H);
+        if (!EARLY) next(v);
 #pragma unroll
-        for (int i = 0; i < 8; i++) hv[v][i] = hv[v][i] * rs * nv[i];
+        for (int i = 0; i < 8; i++) hv[v][i] = hv[v][i] * rs * nv[v][i];
         if (live) g53_store8_to(xn + t * H, hv[v], c, H);
     }
 }
@@ -142,29 +155,15 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
     float kp[NV][8], kn[NV][8];                /* scale gate post, or scale post for kinds 2 and 3; next */
     auto gains = [&](int v) {
         const int c = c0 + v * 512 * W;
+        float gv[8];                                 /* all asked for before the first is used */
 #pragma unroll
-        for (int i = 0; i < 8; i++) { kp[v][i] = a.scale; kn[v][i] = 0.0f; }
+        for (int i = 0; i < 8; i++) { kp[v][i] = 1.0f; kn[v][i] = 0.0f; }
         if (dxn) g53_load8_to(kn[v], a.next, c, H);
-        if (Y) {
-            float t[8];
-            if (a.post) {
-                g53_load8_to(t, a.post, c, H);
+        if (Y && a.post) g53_load8_to(kp[v], a.post, c, H);
+        if (Y && GK == 1) g53_load8_to(gv, (const float *)a.gate, c, H);
 #pragma unroll
-                for (int i = 0; i < 8; i++) kp[v][i] *= t[i];
-            }
-            if (GK == 1) {
-                g53_load8_to(t, (const float *)a.gate, c, H);
-#pragma unroll
-                for (int i = 0; i < 8; i++) kp[v][i] *= t[i];
-            }
-        }
+        for (int i = 0; i < 8; i++) kp[v][i] *= Y && GK == 1 ? a.scale * gv[i] : a.scale;
     };
-#pragma unroll
-    for (int v = 0; v < NV; v++) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) ap[v][i] = an[v][i] = 0.0f;
-        if (KEEP) gains(v);
-    }
     G53Raw8<E> rh[NV], ry[NV], rg[NV], rd[NV], rt[NV];
     float rgate = 1.0f;
     auto ask = [&](long t) {                         /* behind the last token: the group's own last again, not used */
@@ -181,6 +180,12 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
         if (Y && GK == 2) rgate = ((const float *)a.gate)[t];
     };
     if (AHEAD) ask(grp);
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) ap[v][i] = an[v][i] = 0.0f;
+        if (KEEP) gains(v);
+    }
     for (long r = 0; r < rounds; r++) {
         const long t = grp + r * groups;
         const bool live = t < a.T;
