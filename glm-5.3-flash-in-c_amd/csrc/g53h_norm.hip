@@ -13,7 +13,7 @@
  *     dy = rs(y) (du post - y^ mean(du post y^))
  *
  * Both directions are one pass over HBM: W waves hold a token's row in registers, 8 elements a lane
- * (16 for rows above 4096), sums go over the lanes and then the waves. The next norm takes h' in fp32,
+ * (16 for rows above 4096, 32 above 8192), sums go over the lanes and then the waves. The next norm takes h' in fp32,
  * before it is rounded to be stored, and the backward pass forms the same fp32 h' again from h and y.
  * Gradients that tokens share are summed by each workgroup over its tokens in registers, written once
  * and added up by k_norm_sum in a fixed order: no atomics, the same bits on every run.
@@ -143,8 +143,8 @@ __global__ void __launch_bounds__(W < 4 ? 256 : 64 * W)
 k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E *y, G53NormArgs a)
 {
     constexpr int NW = W < 4 ? 4 : W, RB = NW / W;
-    constexpr bool KEEP = NV * W <= 8;         /* gains stay in registers */
-    constexpr bool AHEAD = NV == 1;            /* and the next token's rows wait there */
+    constexpr bool KEEP = NV == 1;             /* gains stay in registers, and the next token's rows wait there */
+    constexpr bool HELD = NV < 4;               /* sums over tokens too; of rows above 8192 they are in LDS */
     __shared__ float buf1[2][NW][1], buf2[2][NW][5];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long grp = (long)blockIdx.x * RB + wv / W, groups = (long)gridDim.x * RB;
@@ -152,6 +152,23 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
     const long rounds = (a.T + groups - 1) / groups;
     const float inv = 1.0f / (float)H;
     float ap[NV][8], an[NV][8];
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    float *sums = (float *)lds + threadIdx.x * 4;    /* [2][NV][2][threads][4], HELD false */
+    auto at = [&](int which, int v, int b) { return (g53_v4f *)(sums + ((which * NV + v) * 2 + b) * (64 * NW * 4)); };
+    auto add = [&](float (&to)[NV][8], int which, int v, const float (&p)[8], const float (&q)[8]) {   /* of p q */
+        if (HELD) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) to[v][i] = __builtin_fmaf(p[i], q[i], to[v][i]);
+        } else {
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                g53_v4f o = *at(which, v, b);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(p[4 * b + i], q[4 * b + i], o[i]);
+                *at(which, v, b) = o;
+            }
+        }
+    };
     float kp[NV][8], kn[NV][8];                /* scale gate post, or scale post for kinds 2 and 3; next */
     auto gains = [&](int v) {
         const int c = c0 + v * 512 * W;
@@ -179,31 +196,38 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
         }
         if (Y && GK == 2) rgate = ((const float *)a.gate)[t];
     };
-    if (AHEAD) ask(grp);
+    if (KEEP) ask(grp);
 #pragma unroll
     for (int v = 0; v < NV; v++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) ap[v][i] = an[v][i] = 0.0f;
+        if (!HELD)
+#pragma unroll
+            for (int k = 0; k < 4; k++) *at(k >> 1, v, k & 1) = (g53_v4f){0.0f, 0.0f, 0.0f, 0.0f};
         if (KEEP) gains(v);
     }
     for (long r = 0; r < rounds; r++) {
         const long t = grp + r * groups;
         const bool live = t < a.T;
-        if (!AHEAD) ask(t);
+        if (!KEEP) ask(t);
         const int odd = r & 1;                       /* sums of two tokens in a row lie apart: one barrier each is enough */
-        float hv[NV][8], yh[NV][8], g[NV][8], d[NV][8], w[NV][8], gt[NV][8];
+        float hv[NV][8], yh[NV][8], g_[NV][8], d_[NV][8], w[NV][8], gt_[NV][8];
         const float tgate = rgate;
+        /* dh', dxn and the gate of the element: in fp32 where the next token's take their place, else as they came */
+        auto g = [&](int v, int i) { return KEEP ? g_[v][i] : dh2 ? (float)rg[v].v[i] : 0.0f; };
+        auto d = [&](int v, int i) { return KEEP ? d_[v][i] : dxn ? (float)rd[v].v[i] : 0.0f; };
+        auto gt = [&](int v, int i) { return KEEP ? gt_[v][i] : (float)rt[v].v[i]; };
 #pragma unroll
         for (int v = 0; v < NV; v++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 hv[v][i] = (float)rh[v].v[i];
                 if (Y) yh[v][i] = (float)ry[v].v[i];
-                d[v][i] = dxn ? (float)rd[v].v[i] : 0.0f;
-                g[v][i] = dh2 ? (float)rg[v].v[i] : 0.0f;
-                if (Y && GK == 3) gt[v][i] = (float)rt[v].v[i];
+                if (KEEP) d_[v][i] = dxn ? (float)rd[v].v[i] : 0.0f;
+                if (KEEP) g_[v][i] = dh2 ? (float)rg[v].v[i] : 0.0f;
+                if (KEEP && Y && GK == 3) gt_[v][i] = (float)rt[v].v[i];
             }
-        if (AHEAD) ask(t + groups);
+        if (KEEP) ask(t + groups);
         float rsy = 1.0f;
         if (Y && a.post) {
             float s[1] = {0.0f};
@@ -215,19 +239,19 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
             rsy = g53_rsq(s[0] * inv + a.eps);
         }
         /* the factor of y^ in h', of dH in dy */
-        auto factor = [&](int v, int i) { return GK < 2 ? kp[v][i] : kp[v][i] * (GK == 2 ? tgate : gt[v][i]); };
+        auto factor = [&](int v, int i) { return GK < 2 ? kp[v][i] : kp[v][i] * (GK == 2 ? tgate : gt(v, i)); };
         float s[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             if (!KEEP) gains(v);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                w[v][i] = d[v][i] * kn[v][i];
+                w[v][i] = d(v, i) * kn[v][i];
                 if (Y) {
                     yh[v][i] *= rsy;
                     const float u = factor(v, i) * yh[v][i];
                     hv[v][i] += u;
-                    s[2] = __builtin_fmaf(u, g[v][i], s[2]);
+                    s[2] = __builtin_fmaf(u, g(v, i), s[2]);
                     s[3] = __builtin_fmaf(u, w[v][i], s[3]);
                     s[4] = __builtin_fmaf(u, hv[v][i], s[4]);
                 }
@@ -239,7 +263,7 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
         const float rs = dxn ? g53_rsq(s[0] * inv + a.eps) : 0.0f, mean = s[1] * rs * inv;
         const float to_y = a.post ? -rsy * (s[2] + rs * (s[3] - rs * mean * s[4])) * inv : 0.0f;
         float gsum[1] = {0.0f};
-        if (AHEAD)                                   /* the next token's rows, before this one's stores */
+        if (KEEP)                                   /* the next token's rows, before this one's stores */
 #pragma unroll
             for (int v = 0; v < NV; v++) {
                 g53_arrived(rh[v]);
@@ -252,29 +276,36 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
 #pragma unroll
             for (int v = 0; v < NV; v++) {
                 const int c = c0 + v * 512 * W;
-                float dg[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float hh = hv[v][i] * rs;
-                    an[v][i] = __builtin_fmaf(d[v][i], hh, an[v][i]);
-                    g[v][i] = __builtin_fmaf(rs, __builtin_fmaf(-hh, mean, w[v][i]), g[v][i]);
+                float dg[8], dv[8], o[8];
+                if (!KEEP) {                         /* converted again, not kept in fp32 */
+                    if (dxn) g53_arrived(rd[v]);
+                    if (dh2) g53_arrived(rg[v]);
+                    if (Y && GK == 3) g53_arrived(rt[v]);
                 }
-                g53_store8_to(dh + t * H, g[v], c, H);
-                if (!Y) continue;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    if (GK < 2) {
-                        ap[v][i] = __builtin_fmaf(yh[v][i], g[v][i], ap[v][i]);
-                    } else {
-                        const float yg = yh[v][i] * g[v][i];
-                        ap[v][i] = __builtin_fmaf(GK == 2 ? tgate : gt[v][i], yg, ap[v][i]);
+                    hv[v][i] *= rs;
+                    dv[i] = d(v, i);
+                    o[i] = __builtin_fmaf(rs, __builtin_fmaf(-hv[v][i], mean, w[v][i]), g(v, i));
+                }
+                add(an, 1, v, dv, hv[v]);
+                g53_store8_to(dh + t * H, o, c, H);
+                if (!Y) continue;
+                if (GK < 2) add(ap, 0, v, yh[v], o);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (GK >= 2) {
+                        const float yg = yh[v][i] * o[i];
+                        dv[i] = GK == 2 ? tgate : gt(v, i);
                         dg[i] = kp[v][i] * yg;
                         gsum[0] += dg[i];
+                        hv[v][i] = yg;
                     }
-                    g[v][i] = __builtin_fmaf(to_y, yh[v][i], rsy * (factor(v, i) * g[v][i]));      /* without post: du itself */
+                    o[i] = __builtin_fmaf(to_y, yh[v][i], rsy * (factor(v, i) * o[i]));      /* without post: du itself */
                 }
+                if (GK >= 2) add(ap, 0, v, dv, hv[v]);
                 if (GK == 3 && a.dgate) g53_store8_to((E *)a.dgate + t * H, dg, c, H);
-                g53_store8_to(dy + t * H, g[v], c, H);
+                g53_store8_to(dy + t * H, o, c, H);
             }
         if (Y && GK == 2 && a.dgate) {
             __shared__ float bufg[2][NW][1];
@@ -285,6 +316,11 @@ k_block_norm_grad(E *dh, E *dy, const E *dh2, const E *dxn, const E *h, const E 
     /* the sums of the workgroup's groups, added in order by the first of them, which writes them */
     float *part = a.part + (long)blockIdx.x * 2 * a.pitch;
     auto finish = [&](float (&v8)[NV][8], int which) {
+        if (!HELD)
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) v8[v][i] = (*at(which, v, i >> 2))[i & 3];
         if (RB > 1) {                                /* NV = 1 */
             __shared__ float rows[RB > 1 ? NW : 1][8][64];
             __syncthreads();
@@ -343,7 +379,8 @@ __global__ void __launch_bounds__(256) k_norm_sum(float *__restrict__ dpost, flo
     if (dgate) dgate[c] = scale * (post ? post[c] : 1.0f) * t;
 }
 
-/* Waves per row: 512 elements each, twice that above 8192. */
+/* Waves per row: 512 elements each up to 4096, then eight with more. Of 16 the gradient's registers do not hold the rows
+ * (1024 x 8192 bf16: 82 us against 38; 512 x 16384, sums in registers: 155 against 93). */
 #define G53_NORM_BY_WIDTH(H, BODY)                                              \
     do {                                                                        \
         if ((H) <= 512) { constexpr int W = 1, NV = 1; BODY; }                  \
@@ -351,7 +388,7 @@ __global__ void __launch_bounds__(256) k_norm_sum(float *__restrict__ dpost, flo
         else if ((H) <= 2048) { constexpr int W = 4, NV = 1; BODY; }            \
         else if ((H) <= 4096) { constexpr int W = 8, NV = 1; BODY; }            \
         else if ((H) <= 8192) { constexpr int W = 8, NV = 2; BODY; }            \
-        else { constexpr int W = 16, NV = 2; BODY; }                            \
+        else { constexpr int W = 8, NV = 4; BODY; }                             \
     } while (0)
 #define G53_NORM_BY_GATE(kind, BODY)                                            \
     do {                                                                        \
@@ -385,10 +422,17 @@ static int backward(void *dh, void *dy, float *dpost, float *dnext, float *dchan
     /* eight waves a CU, all with the same number of tokens where that divides */
     const long most = g53h_num_cus() * (W < 8 ? 2 : 1), need = ((long)a.T + RB - 1) / RB, rounds = (need + most - 1) / most;
     const unsigned wgs = (unsigned)(need ? (need + rounds - 1) / rounds : 0);
+    constexpr size_t lds = NV < 4 ? 0 : (size_t)4 * NV * 64 * NW * sizeof(g53_v4f);
     if (wgs) {
+        static int allowed = 0;
+        if (lds && !allowed) {
+            G53_TRY(hipFuncSetAttribute((const void *)k_block_norm_grad<E, W, NV, GK, Y>,
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+            allowed = 1;
+        }
         a.part = (float *)g53h_op_workspace((size_t)wgs * 2 * a.pitch * sizeof(float));
         if (!a.part) return -1;
-        hipLaunchKernelGGL((k_block_norm_grad<E, W, NV, GK, Y>), dim3(wgs), dim3(64 * NW), 0, g53h_stream(), (E *)dh, (E *)dy,
+        hipLaunchKernelGGL((k_block_norm_grad<E, W, NV, GK, Y>), dim3(wgs), dim3(64 * NW), lds, g53h_stream(), (E *)dh, (E *)dy,
                            (const E *)dh2, (const E *)dxn, (const E *)h, (const E *)y, a);
         G53_LAUNCHED("k_block_norm_grad");
     }
