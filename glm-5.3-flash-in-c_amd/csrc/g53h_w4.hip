@@ -162,9 +162,10 @@ __device__ __forceinline__ bool g53_w4_item(const int *__restrict__ offsets, int
 
 /* What a wave has asked for of 128 columns: levels of its row tiles as they lie, and, where the columns lie in several
  * groups, their scales and zero points. */
-template <int R> struct G53W4Chunk {
+template <int R, int X> struct G53W4Chunk {
     g53_v4w w[R];
     unsigned s[R], z[R];
+    g53_v4w x[4][X];                    /* and of its activations, where LDS does not hold them: 8 columns a step */
 };
 
 /* n / d for 0 <= n, by a shift where d is a power of two (log >= 0). */
@@ -185,7 +186,7 @@ __device__ __forceinline__ void g53_spread(float (&o)[4], float v)
  * columns, in units of UC x 128 taken in turn, by NW / KW groups of R row tiles. A unit's levels are asked for one unit
  * ahead. GS: groups are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows,
  * the others the same up rows. Columns behind the last of a unit meet activations of zero. */
-template <typename E, int R, int NT, int UC, bool ROWS, bool LINES, int GS>
+template <typename E, int R, int NT, int UC, bool ROWS, bool LINES, bool DIRECT, int GS>
 __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2)
 k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets, const int *__restrict__ pair, G53W4Args a)
 {
@@ -278,7 +279,13 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
         const int g = g53_quot((u * UC + q) * 4, a.group / 32, a.glog);
         return g < a.groups ? g : a.groups - 1;
     };
-    typedef G53W4Chunk<R> Chunk;
+    constexpr int XW = sizeof(E) / 2;       /* 16-byte words of 8 activations */
+    typedef G53W4Chunk<R, XW> Chunk;
+    const E *xr = x;                        /* DIRECT: the lane's token */
+    if (DIRECT) {
+        const int i = first + (m < rows ? m : rows - 1), t = pair ? pair[i] / a.topk : i;
+        xr = x + (long)t * a.cols + q * (GS == 4 ? 32 : 8);
+    }
     /* Levels of a chunk, 16 rows x 64 bytes a load, or (LINES) of two: a load takes whole lines then, 8 rows x 128 bytes,
      * the first chunk's quarter q in lanes m < 8 of its rows and the second's in lanes m >= 8, until `pass` gives each lane
      * its row of both; such lines are not kept in the caches, where half lines wait for their other half. */
@@ -295,6 +302,16 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
         if (GS < 4)
 #pragma unroll
             for (int b = 0; b < PAIR; b++) ask(k[b].s, k[b].z, group_of(c + b));
+        if (DIRECT)
+#pragma unroll
+            for (int b = 0; b < PAIR; b++)
+#pragma unroll
+                for (int s = 0; s < 4; s++) {   /* columns behind the last: the row's first, made zero in `use` */
+                    const int at = (c + b) * 128 + s * (GS == 4 ? 8 : 32);
+                    const bool in = (GS == 4 ? (c + b) * 128 + q * 32 : at) < a.cols;
+#pragma unroll
+                    for (int j = 0; j < XW; j++) k[b].x[s][j] = ((const G53v4w_any *)(xr + (in ? at : 0)))[j].v;
+                }
     };
     auto pass = [&](Chunk *k) {
         if (LINES)
@@ -337,12 +354,24 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             V b[NT][PM];
+            if (DIRECT) {
+                V o[P];
+                g53_v4w v[XW];
+                const bool in = c * 128 + (GS == 4 ? q : s) * 32 < a.cols;
+#pragma unroll
+                for (int j = 0; j < XW; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[j][i] = in ? k.x[s][j][i] : 0u;
+                g53_w4_x(o, v);
+#pragma unroll
+                for (int p = 0; p < PM; p++) b[0][p] = o[p];
+            }
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int p = 0; p < PM; p++) {
                     g53_v4f &to = X[t][p ? DP - 1 : 0];
-                    b[t][p] = *(const V *)(lds + p * plane + xat[t] + c_lds * 256 + s * (GS == 4 ? 16 : 64));
+                    if (!DIRECT) b[t][p] = *(const V *)(lds + p * plane + xat[t] + c_lds * 256 + s * (GS == 4 ? 16 : 64));
                     to = g53_mfma(b[t][p], ones, s % GS == 0 && p < 2 ? zero : to);
                 }
 #pragma unroll
@@ -420,23 +449,25 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
     };
     {   /* the first levels: behind the first activations, which LDS has to hold before */
         Piece v;
-        fetch(v, 0, wv);
+        if (!DIRECT) fetch(v, 0, wv);
         __builtin_amdgcn_sched_barrier(0);
         if (GS == 4) ask(us, uz, unit_group(kw));
 #pragma unroll
         for (int j = 0; j < UC; j += PAIR) load(ring + j, kw * UC + j);
         __builtin_amdgcn_sched_barrier(0);
-        put(v, 0, wv);
+        if (!DIRECT) put(v, 0, wv);
     }
     for (int seg0 = 0; seg0 < units; seg0 += a.seg) {
         const int here = segment(seg0), pieces = pieces_of(here);
-        if (seg0) __syncthreads();
-        for (int p0 = seg0 ? wv : wv + NP * NW; p0 < pieces; p0 += NP * NW) {
-            Piece v;
-            fetch(v, seg0, p0);
-            put(v, seg0, p0);
+        if (!DIRECT) {
+            if (seg0) __syncthreads();
+            for (int p0 = seg0 ? wv : wv + NP * NW; p0 < pieces; p0 += NP * NW) {
+                Piece v;
+                fetch(v, seg0, p0);
+                put(v, seg0, p0);
+            }
+            __syncthreads();
         }
-        __syncthreads();
         /* every unit asks for the wave's next one, but for the last of all; segments but the last are whole turns */
         const bool ends = seg0 + here == units;
         const int until = ends ? here - KW : here;
@@ -495,23 +526,23 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
     }
 }
 
-template <typename E, int R, int NT, int UC, bool ROWS, bool LINES, int GS>
+template <typename E, int R, int NT, int UC, bool ROWS, bool LINES, bool DIRECT, int GS>
 static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const G53W4Args &a)
 {
     static int allowed = 0;
     if (!allowed) {
-        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, UC, ROWS, LINES, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, UC, ROWS, LINES, DIRECT, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                     G53_W4_LDS_MAX));
         allowed = 1;
     }
-    hipLaunchKernelGGL((k_w4<E, R, NT, UC, ROWS, LINES, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x,
+    hipLaunchKernelGGL((k_w4<E, R, NT, UC, ROWS, LINES, DIRECT, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x,
                        a.offsets, a.pair, a);
     G53_LAUNCHED("k_w4");
     return 0;
 }
 
 /* busy: token tiles that are expected to hold rows. */
-template <typename E, int R, int NT, int UC, bool ROWS, bool LINES = false>
+template <typename E, int R, int NT, int UC, bool ROWS, bool LINES = false, bool DIRECT = false>
 static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
 {
     constexpr int P = G53W4Type<E>::P, TT = ROWS ? 16 * NT / P : 16 * NT;
@@ -522,18 +553,19 @@ static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
     int k = 0, rw = units < 4 ? G53_W4_NW / 2 : G53_W4_NW;
     for (;;) {
         const long wgs = busy * ((a.half + out * rw - 1) / (out * rw));
-        if (rw == 1 || wgs >= 2 * g53h_num_cus() || (out * rw / 2 < 4 * rows && wgs >= g53h_num_cus() / 2)) break;
-        if ((2 << k) <= units && rows * P * ((2 << k) * 256 * UC + 16) <= G53_W4_LDS_MAX) k++;
+        if (rw == 1 || wgs >= 2 * g53h_num_cus() || (!DIRECT && out * rw / 2 < 4 * rows && wgs >= g53h_num_cus() / 2)) break;
+        if ((2 << k) <= units && (DIRECT || rows * P * ((2 << k) * 256 * UC + 16) <= G53_W4_LDS_MAX)) k++;
         rw /= 2;
     }
+    if (DIRECT && (rw > 1 || (busy * ((a.half + out - 1) / out) << k) > 8 * g53h_num_cus())) return 1;
     const int waves = rw << k, outs = out * rw;
     a.kw_log = k;
     a.tiles = (a.half + outs - 1) / outs;
     int seg = (G53_W4_LDS / (rows * P) - 16) / (256 * UC) >> k << k;    /* units of x in LDS: whole turns */
     if (seg < 1 << k) seg = 1 << k;
-    if (seg > units) seg = units;
+    if (seg > units || DIRECT) seg = units;
     a.seg = seg;
-    size_t lds = (size_t)rows * P * (seg * 256 * UC + 16), red = (size_t)waves * 16 * NT * (16 * R + 4) * 4;
+    size_t lds = DIRECT ? 0 : (size_t)rows * P * (seg * 256 * UC + 16), red = (size_t)waves * 16 * NT * (16 * R + 4) * 4;
     if (lds < red) lds = red;
     /* threads of a launch fit 32 bits: of 2^30 rows a workgroup has 256 */
     const long wide = a.offsets ? a.tiles : (a.tiles + 7) / 8 * 8l, most = (1l << 31) / (64 * G53_W4_NW) / wide;
@@ -541,9 +573,9 @@ static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
         a.item0 = i;
         a.items = (int)(items - i < most ? items - i : most);
         const dim3 grid((unsigned)(a.items * wide));
-        const int rc = a.group % 128 == 0 ? start<E, R, NT, UC, ROWS, LINES, 4>(grid, waves, lds, y, x, a)
-                       : a.group % 64 == 0 ? start<E, R, NT, UC, ROWS, LINES, 2>(grid, waves, lds, y, x, a)
-                                           : start<E, R, NT, UC, ROWS, LINES, 1>(grid, waves, lds, y, x, a);
+        const int rc = a.group % 128 == 0 ? start<E, R, NT, UC, ROWS, LINES, DIRECT, 4>(grid, waves, lds, y, x, a)
+                       : a.group % 64 == 0 ? start<E, R, NT, UC, ROWS, LINES, DIRECT, 2>(grid, waves, lds, y, x, a)
+                                           : start<E, R, NT, UC, ROWS, LINES, DIRECT, 1>(grid, waves, lds, y, x, a);
         if (rc) return rc;
     }
     return 0;
@@ -567,6 +599,10 @@ template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
     const int TT = F32 && mean <= 5 ? 5 : (mean > 16 && !few ? 32 : 16);
     const long items = a.offsets ? a.T / TT + ex : (a.T - 1) / TT + 1, busy = ex * ((mean + TT - 1) / TT);
     if (TT == 32) return launch<E, 2, 2, 2, false>(y, x, a, items, busy);
+    if (few && TT == 16) {
+        const int rc = launch<E, 1, 1, F32 ? 1 : 2, false, false, true>(y, x, a, items, busy);
+        if (rc <= 0) return rc;
+    }
     if constexpr (F32)
         if (TT == 16)
             return few ? launch<E, 1, 1, 1, false>(y, x, a, items, busy) : launch<E, 2, 1, 2, false>(y, x, a, items, busy);
