@@ -11,10 +11,19 @@
  * is the value exactly (8 + 8 + 8 mantissa bits, by truncation).
  *
  * A wave owns R tiles of 16 rows and NT tiles of 16 tokens over a part of the columns and steps by 128
- * columns: one 16-byte load per lane and row tile (16 rows x 64 bytes), turned so that each of the
- * four products of 32 columns covers consecutive columns (v_permlane32_swap and v_permlane16_swap
- * exchange the lanes' quarters with the four registers), so groups of any multiple of 32 end between
- * products. The NW waves of a workgroup split the columns and add up through LDS.
+ * columns: one 16-byte load per lane and row tile (16 rows x 64 bytes, or 8 rows x whole lines of 128).
+ * Where a chunk of 128 columns lies in one group, each of its four products takes 8 columns of every
+ * lane quarter's 32; in groups of 32, 64 or 96 the registers are turned so that a product covers 32
+ * columns in a row and groups end between products (v_permlane32_swap and v_permlane16_swap exchange the
+ * lanes' quarters with the four registers). The NW waves of a workgroup split the columns and add up
+ * through LDS, which also holds the activations, turned into planes once a workgroup, except for small
+ * matrices, whose waves each load theirs.
+ *
+ * By few tokens the levels' bytes bound it: 65536 x 4096 by 5 fp16 tokens 27.3 us, 5.1 TB/s (a plain
+ * read stream of as many bytes: 23 to 26); eight gate/up matrices of 4096 x 4096 by one token 16.3 us,
+ * 4.2 TB/s with a launch and the search of a row's expert in it. Small matrices are a launch and three
+ * trips to memory (4096 x 2048 by one token 4.5 us), many tokens the vector work of turning levels into
+ * floats beside the products (16384 x 4096 by 128 bf16 tokens 41 us, 420 TFLOP/s).
  */
 #include <hip/hip_runtime.h>
 
@@ -185,7 +194,8 @@ __device__ __forceinline__ void g53_spread(float (&o)[4], float v)
 /* One workgroup: up to 16 NT tokens (or sorted rows of one expert) by `out` (NW / KW) rows. Its waves are KW parts of the
  * columns, in units of UC x 128 taken in turn, by NW / KW groups of R row tiles. A unit's levels are asked for one unit
  * ahead. GS: groups are multiples of GS x 32 columns (4, 2 or 1). With SwiGLU the first R / 2 row tiles are gate rows,
- * the others the same up rows. Columns behind the last of a unit meet activations of zero. */
+ * the others the same up rows. Columns behind the last of a unit meet activations of zero. DIRECT (R = NT = 1): a wave
+ * loads its activations a unit ahead into registers, from the caches, and LDS only adds up. */
 template <typename E, int R, int NT, int UC, bool ROWS, bool LINES, bool DIRECT, int GS>
 __global__ void __launch_bounds__(64 * G53_W4_NW, NT * G53W4Type<E>::P <= 3 ? 4 : 2)
 k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets, const int *__restrict__ pair, G53W4Args a)
@@ -588,7 +598,12 @@ static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
  * the products are as many as bf16's (16384 x 4096 by one token: 14.5 us against 16.4). Long rows of a matrix that one
  * token tile meets are loaded in whole lines (65536 x 4096 by 5 tokens: 27.3 us against 30.7; eight gate/up matrices of
  * 4096 x 4096 by one token 16.3 against 17.2); short rows, or rows that further tiles read again, in half lines (64 matrices
- * of 2048 x 1024 by 64 tokens 20.8 against 22.4, 2048 x 2048 by 256 tokens 58 against 70). */
+ * of 2048 x 1024 by 64 tokens 20.8 against 22.4, 2048 x 2048 by 256 tokens 58 against 70).
+ * Small matrices, of at most 8 waves a CU that share no activations, load them without LDS, which takes a trip to memory
+ * and a barrier out of a call that is little else: 1001 x 2080 by 24 tokens in fp32 7.7 us against 10.5, 4096 x 4096 by 8
+ * in bf16 7.6 against 11.0, one expert's 1024 x 1024 by one 4.6 against 5.1; of more waves the caches' rate bounds them
+ * (6000 x 4096 by 8 tokens in bf16 10.2 against 7.9). Up to 5 fp32 tokens do so where a wave has at most two chunks
+ * (256 x 512 by one 4.5 against 5.0; 4096 x 4096 by one 8.6 against 6.1). */
 template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
 {
     constexpr bool F32 = sizeof(E) == 4;
@@ -597,10 +612,12 @@ template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
     const long waves = (a.rows + 31) / 32 * ex * ((mean + 15) / 16) * (units < G53_W4_NW ? units : G53_W4_NW);
     const bool few = waves <= 16 * g53h_num_cus() && !(a.limit > 0.0f);
     const int TT = F32 && mean <= 5 ? 5 : (mean > 16 && !few ? 32 : 16);
-    const long items = a.offsets ? a.T / TT + ex : (a.T - 1) / TT + 1, busy = ex * ((mean + TT - 1) / TT);
+    auto items_of = [&](int tt) { return a.offsets ? a.T / tt + ex : (a.T - 1) / tt + 1l; };
+    auto busy_of = [&](int tt) { return ex * ((mean + tt - 1) / tt); };
+    const long items = items_of(TT), busy = busy_of(TT);
     if (TT == 32) return launch<E, 2, 2, 2, false>(y, x, a, items, busy);
-    if (few && TT == 16) {
-        const int rc = launch<E, 1, 1, F32 ? 1 : 2, false, false, true>(y, x, a, items, busy);
+    if (few && (TT == 16 || a.cols <= 2048)) {
+        const int rc = launch<E, 1, 1, F32 ? 1 : 2, false, false, true>(y, x, a, items_of(16), busy_of(16));
         if (rc <= 0) return rc;
     }
     if constexpr (F32)
