@@ -22,7 +22,7 @@
  * By few tokens the levels' bytes bound it: 65536 x 4096 by 5 fp16 tokens 27.3 us, 5.1 TB/s (a plain
  * read stream of as many bytes: 23 to 26); eight gate/up matrices of 4096 x 4096 by one token 16.3 us,
  * 4.2 TB/s with a launch and the search of a row's expert in it. Small matrices are a launch and three
- * trips to memory (4096 x 2048 by one token 4.5 us), many tokens the vector work of turning levels into
+ * trips to memory (4096 x 2048 by one token 4.3 us), many tokens the vector work of turning levels into
  * floats beside the products (16384 x 4096 by 128 bf16 tokens 41 us, 420 TFLOP/s).
  */
 #include <hip/hip_runtime.h>
@@ -169,8 +169,8 @@ __device__ __forceinline__ bool g53_w4_item(const int *__restrict__ offsets, int
     return true;
 }
 
-/* What a wave has asked for of 128 columns: levels of its row tiles as they lie, and, where the columns lie in several
- * groups, their scales and zero points. */
+/* What a wave has asked for of 128 columns: levels of its row tiles as they lie, and, where they are not asked for by unit,
+ * scales and zero points. */
 template <int R, int X> struct G53W4Chunk {
     g53_v4w w[R];
     unsigned s[R], z[R];
@@ -280,13 +280,19 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
         return __builtin_bit_cast(float, (v << s_shift & ~s_f16) | (__builtin_bit_cast(unsigned, f16) & s_f16));
     };
     auto surplus = [&](unsigned v, int g) { return -16.0f - (float)((v >> (4 * (g & 1)) & z_mask) | z_no); };
-    /* the lane's group in chunk c: that of its quarter; in unit u: that of chunk q */
+    /* the lane's group in chunk c: that of its quarter; in unit u: that of chunk q's half h (of NH halves) */
+    constexpr int NH = GS == 4 ? 1 : 2;
+    /* Scales are asked for by unit: by chunk they are as many requests to the vector cache as the levels (16384 x 4096 in
+     * groups of 64 by one bf16 token 15.0 us against 11.8, 64 matrices of 2048 x 1024 by 64 tokens 21.2 against 18.5). Not
+     * those of groups of 32, whose registers would be too many, nor where fp32's three products wait for no scale (4096 x
+     * 4096 by 64 tokens 30.9 us against 32.9 by unit). */
+    constexpr bool UNIT = GS == 4 || (GS == 2 && UC > 1 && PM == 1);
     auto group_of = [&](int c) {
         const int g = g53_quot(c * 4 + q, a.group / 32, a.glog);
         return g < a.groups ? g : a.groups - 1;
     };
-    auto unit_group = [&](int u) {
-        const int g = g53_quot((u * UC + q) * 4, a.group / 32, a.glog);
+    auto unit_group = [&](int u, int h) {
+        const int g = g53_quot((u * UC + q) * 4 + 2 * h, a.group / 32, a.glog);
         return g < a.groups ? g : a.groups - 1;
     };
     constexpr int XW = sizeof(E) / 2;       /* 16-byte words of 8 activations */
@@ -309,7 +315,7 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
                 const g53_v4w *from = (const g53_v4w *)(wb[r] + (unsigned)(w_of[r][b] + wo));
                 k[b].w[r] = LINES ? __builtin_nontemporal_load(from) : *from;
             }
-        if (GS < 4)
+        if (!UNIT)
 #pragma unroll
             for (int b = 0; b < PAIR; b++) ask(k[b].s, k[b].z, group_of(c + b));
         if (DIRECT)
@@ -339,20 +345,23 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
 #pragma unroll
     for (int t = 0; t < NT; t++) xat[t] = (16 * t + m < x_rows ? 16 * t + m : x_rows - 1) * ld + q * (GS == 4 ? 64 : 16);
     const int plane = rows * ld;
-    /* sc, nz: of the chunk, GS = 4. Step s takes the columns of register s: 8 from each quarter's 32 where the chunk lies
+    /* sc4, nz4: of the chunk's halves, where UNIT. Step s takes the columns of register s: 8 from each quarter's 32 where the chunk lies
      * in one group, else turned to 32 in a row. */
-    auto use = [&](const Chunk &k, int c, int c_lds, const float (&sc4)[R], const float (&nz4)[R]) {
+    auto use = [&](const Chunk &k, int c, int c_lds, const float (&sc4)[R][NH], const float (&nz4)[R][NH]) {
         unsigned d[R][4];
         float sc[R][4], nz[R][4];
 #pragma unroll
         for (int r = 0; r < R; r++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) d[r][i] = k.w[r][i];
-            if (GS == 4) {
-                sc[r][3] = sc4[r];
-                nz[r][3] = nz4[r];
+            if (GS < 4) g53_turn(d[r]);
+            if (UNIT) {
+#pragma unroll
+                for (int h = 0; h < NH; h++) {
+                    sc[r][GS * (h + 1) - 1] = sc4[r][h];
+                    nz[r][GS * (h + 1) - 1] = nz4[r][h];
+                }
             } else {
-                g53_turn(d[r]);
                 g53_spread(sc[r], scale(k.s[r]));
                 g53_spread(nz[r], surplus(k.z[r], group_of(c)));
             }
@@ -413,15 +422,24 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
         __builtin_amdgcn_sched_barrier(0);      /* no work on the next chunk, which may not be there yet, before this is done */
     };
     Chunk ring[UC];
-    unsigned us[R], uz[R];                  /* a unit's scales, GS = 4: quarter i holds those of chunk i */
-    auto unit_scales = [&](int u, float (&sc)[R][4], float (&nz)[R][4]) {
-        if (GS < 4) return;
-        const int g = unit_group(u);
+    /* a unit's scales, where UNIT: quarter i holds those of chunk i */
+    unsigned us[NH][R], uz[NH][R];
+    auto ask_unit = [&](int u) {
+        if (UNIT)
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            g53_spread(sc[r], scale(us[r]));
-            g53_spread(nz[r], surplus(uz[r], g));
-        }
+            for (int h = 0; h < NH; h++) ask(us[h], uz[h], unit_group(u, h));
+    };
+    auto unit_scales = [&](int u, float (&sc)[NH][R][4], float (&nz)[NH][R][4]) {
+        if (UNIT)
+#pragma unroll
+            for (int h = 0; h < NH; h++) {
+                const int g = unit_group(u, h);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    g53_spread(sc[h][r], scale(us[h][r]));
+                    g53_spread(nz[h][r], surplus(uz[h][r], g));
+                }
+            }
     };
     /* A segment's activations into LDS as planes in the levels' order, in pieces of 512 columns of a row, a wave's load;
      * a wave asks for NP at a time. */
@@ -461,7 +479,7 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
         Piece v;
         if (!DIRECT) fetch(v, 0, wv);
         __builtin_amdgcn_sched_barrier(0);
-        if (GS == 4) ask(us, uz, unit_group(kw));
+        ask_unit(kw);
 #pragma unroll
         for (int j = 0; j < UC; j += PAIR) load(ring + j, kw * UC + j);
         __builtin_amdgcn_sched_barrier(0);
@@ -482,15 +500,17 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
         const bool ends = seg0 + here == units;
         const int until = ends ? here - KW : here;
         int i = kw;
-        float sc[R][4], nz[R][4], sj[R], nj[R];
+        float sc[NH][R][4], nz[NH][R][4], sj[R][NH], nj[R][NH];
         for (; i < until; i += KW) {
             unit_scales(seg0 + i, sc, nz);
-            if (GS == 4) ask(us, uz, unit_group(seg0 + i + KW));
+            ask_unit(seg0 + i + KW);
 #pragma unroll
             for (int j = 0; j < UC; j++) {
                 if (j % PAIR == 0) pass(ring + j);
 #pragma unroll
-                for (int r = 0; r < R; r++) { sj[r] = sc[r][j]; nj[r] = nz[r][j]; }
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int h = 0; h < NH; h++) { sj[r][h] = sc[h][r][j]; nj[r][h] = nz[h][r][j]; }
                 use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, nj);
                 if (j % PAIR == PAIR - 1) load(ring + j - (PAIR - 1), (seg0 + i + KW) * UC + j - (PAIR - 1));
             }
@@ -501,7 +521,9 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
             for (int j = 0; j < UC; j++) {
                 if (j % PAIR == 0) pass(ring + j);
 #pragma unroll
-                for (int r = 0; r < R; r++) { sj[r] = sc[r][j]; nj[r] = nz[r][j]; }
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int h = 0; h < NH; h++) { sj[r][h] = sc[h][r][j]; nj[r][h] = nz[h][r][j]; }
                 use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, nj);
             }
         }
