@@ -153,7 +153,8 @@ __device__ __forceinline__ float g53_wave_sum(float v)
 #pragma unroll
     for (int half = 0; half < 2; half++) {          /* the other row of two, then the other two rows */
         const unsigned u = __builtin_bit_cast(unsigned, v);
-        const V2 p = half ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const V2 p = half ? __builtin_amdgcn_permlane32_swap(u, u, false, false)
+                          : __builtin_amdgcn_permlane16_swap(u, u, false, false);
         const unsigned a = p[0], b = p[1];          /* a bit cast of a vector's element takes element 0 */
         v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
     }

@@ -17,6 +17,11 @@
  * before it is rounded to be stored, and the backward pass forms the same fp32 h' again from h and y.
  * Gradients that tokens share are summed by each workgroup over its tokens in registers, written once
  * and added up by k_norm_sum in a fixed order: no atomics, the same bits on every run.
+ *
+ * Both are bound by HBM once there are many tokens: forward 8192 x 4096 bf16 with a gate per channel 55.5 us,
+ * 4.8 TB/s, backward 4096 x 4096 44 us, 4.6 TB/s with the sums' launch (4 us). A gradient of few tokens is
+ * latency: two launches, a workgroup a CU that meets memory, two sums over its waves and one barrier each per
+ * token, and as many bytes of partial sums as of two rows a workgroup (1025 x 4096: 14 us and 4, floor 10.6).
  */
 #include <hip/hip_runtime.h>
 

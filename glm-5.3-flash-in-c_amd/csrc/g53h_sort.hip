@@ -2,28 +2,27 @@
  * expert (a stable counting sort), the copy of every token's row to its experts' rows, the weighted
  * sum back, and the gradients of both.
  *
- *   k_sort_place     a pair's row is offsets[its expert] + the number of earlier pairs of the same
- *                    expert. A workgroup counts its pairs per wave and expert in LDS, turns the counts
- *                    into first rows by a prefix sum over the experts and the waves, and then walks its
- *                    pairs in order, 64 at a time: a ballot per bit of the expert gives each lane the
- *                    lanes with the same expert, those below it are its rank. Order never depends on
- *                    timing. Routings of more than G53_SORT_SEG pairs are cut into segments, counted by
- *                    k_sort_count first; every workgroup then adds up the counts of all segments.
- *                    One launch's time and two trips to memory: 2.4 us for 64 pairs and fewer, 7 us
- *                    for the 32768 pairs of 4096 tokens, in two launches.
- *   k_dispatch       bytes of rows, 16 a thread: a token's row is read once and written topk times.
- *                    4096 tokens of 4096 bf16 to 8 experts each: 302 MB, 62 us, 4.9 TB/s. Written past
- *                    the caches the rows alone leave faster (with the sort and a combine of other rows
- *                    after it 128 us against 136), but whoever reads them next waits longer (dispatch and
- *                    a read of its rows: 104 us against 93; 67 MB of rows: 28 against 25).
- *   k_combine        8 elements a thread: the rows of a token's pairs are all asked for before the
- *                    first is added; sums in fp32 in the order of the pairs, rounded once. The same
- *                    tokens: 302 MB, 64 us, 4.7 TB/s, what a copy of 4 GiB reaches.
- *   k_combine_grad   one wave per pair: its weight's gradient is one sum over the wave, so nothing is
- *                    exchanged between waves; the waves of a workgroup mostly share a token, whose
- *                    gradient row they read from the vector cache. 2048 tokens: 285 MB, 60 us, 4.7 TB/s.
+ * k_sort_place: a pair's row is offsets[its expert] + the number of earlier pairs of the same expert. A
+ * workgroup counts its pairs per wave and expert in LDS, turns the counts into first rows by a prefix sum
+ * over the experts and the waves, and then walks its pairs in order, 64 at a time: a ballot per bit of the
+ * expert gives each lane the lanes with the same expert, those below it are its rank. Order never depends on
+ * timing. Routings of more than G53_SORT_SEG pairs are cut into segments, counted by k_sort_count first;
+ * every workgroup then adds up the counts of all segments. Latency: 2.6 us for 64 pairs and fewer
+ * (k_sort_few), 4.9 + 7.8 for 32768 pairs of 288 experts in 16 segments.
  *
- * All but the sort are bound by HBM.
+ * k_sorted_dispatch: bytes of rows, 16 a thread; a token's row is read once and written topk times. 4096
+ * tokens of 4096 bf16 to 8 experts each, 302 MB: 55 us, 5.5 TB/s, bound by HBM. Written past the caches the
+ * rows alone leave faster (with the sort and a combine of other rows after it 128 us against 136), but
+ * whoever reads them next waits longer (dispatch and a read of its rows 104 us against 93; 67 MB of rows 28
+ * against 25).
+ *
+ * k_sorted_combine: 8 elements a thread; the rows of a token's pairs are all asked for before the first is
+ * added; sums in fp32 in the order of the pairs, rounded once. The same tokens, 302 MB: 67 us, 4.5 TB/s, a
+ * large copy's rate.
+ *
+ * k_sorted_combine_grad: one wave per pair. Its weight's gradient is one sum over the wave, so nothing is
+ * exchanged between waves; the waves of a workgroup mostly share a token, whose gradient row they read from
+ * the vector cache. 2048 of these tokens, 285 MB: 63 us, 4.5 TB/s.
  */
 #include <hip/hip_runtime.h>
 
@@ -208,7 +207,8 @@ extern "C" int g53h_sort_tokens(const G53hSort *p, const int *idx)
     int *hist = nullptr;
     static int allowed = 0;             /* 1024 experts: 64 KB of counts and a little more */
     if (!allowed) {
-        G53_TRY(hipFuncSetAttribute((const void *)k_sort_place<16>, hipFuncAttributeMaxDynamicSharedMemorySize, 16 * G53_SORT_MAXE * 4));
+        G53_TRY(hipFuncSetAttribute((const void *)k_sort_place<16>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    16 * G53_SORT_MAXE * 4));
         allowed = 1;
     }
     if (wgs > 1) {
@@ -229,7 +229,7 @@ extern "C" int g53h_sort_tokens(const G53hSort *p, const int *idx)
 
 /* --------------------------------------------------------------------- dispatch ---- */
 /* nb bytes a row; a workgroup copies 4 KB of one token's row to its topk rows. */
-__global__ void __launch_bounds__(256) k_dispatch(uint8_t *__restrict__ xs, const uint8_t *__restrict__ x,
+__global__ void __launch_bounds__(256) k_sorted_dispatch(uint8_t *__restrict__ xs, const uint8_t *__restrict__ x,
                                                   const int *__restrict__ row, long nb, int K, int chunks, long wg0)
 {
     const long wg = wg0 + blockIdx.x;
@@ -271,9 +271,9 @@ extern "C" int g53h_sorted_dispatch(void *xs, const void *x, int dt, int hidden,
     const long total = (long)p->T * chunks;
     for (long w0 = 0; w0 < total; w0 += G53_LAUNCH_WGS) {
         const unsigned wgs = (unsigned)(total - w0 < G53_LAUNCH_WGS ? total - w0 : G53_LAUNCH_WGS);
-        hipLaunchKernelGGL(k_dispatch, dim3(wgs), dim3(256), 0, g53h_stream(), (uint8_t *)xs, (const uint8_t *)x, p->row, nb,
+        hipLaunchKernelGGL(k_sorted_dispatch, dim3(wgs), dim3(256), 0, g53h_stream(), (uint8_t *)xs, (const uint8_t *)x, p->row, nb,
                            p->topk, chunks, w0);
-        G53_LAUNCHED("k_dispatch");
+        G53_LAUNCHED("k_sorted_dispatch");
     }
     return 0;
 }
@@ -281,7 +281,7 @@ extern "C" int g53h_sorted_dispatch(void *xs, const void *x, int dt, int hidden,
 /* ---------------------------------------------------------------------- combine ---- */
 /* out[t] = add[t] + sum over the token's pairs of w times their row; w NULL: 1, add NULL: 0. */
 template <typename E>
-__global__ void __launch_bounds__(256) k_combine(E *out, const E *__restrict__ ys, const float *__restrict__ w,
+__global__ void __launch_bounds__(256) k_sorted_combine(E *out, const E *__restrict__ ys, const float *__restrict__ w,
                                                  const E *add, const int *__restrict__ row, int H, int K, int chunks,
                                                  long wg0)
 {
@@ -316,9 +316,9 @@ static int combine(const char *who, void *out, const void *ys, const float *w, c
     const long total = (long)p->T * chunks;
     for (long w0 = 0; w0 < total; w0 += G53_LAUNCH_WGS) {
         const unsigned wgs = (unsigned)(total - w0 < G53_LAUNCH_WGS ? total - w0 : G53_LAUNCH_WGS);
-        G53_BY_TYPE(dt, hipLaunchKernelGGL(k_combine<E>, dim3(wgs), dim3(256), 0, g53h_stream(), (E *)out, (const E *)ys, w,
+        G53_BY_TYPE(dt, hipLaunchKernelGGL(k_sorted_combine<E>, dim3(wgs), dim3(256), 0, g53h_stream(), (E *)out, (const E *)ys, w,
                                            (const E *)add, p->row, hidden, p->topk, chunks, w0));
-        G53_LAUNCHED("k_combine");
+        G53_LAUNCHED("k_sorted_combine");
     }
     return 0;
 }
@@ -343,7 +343,7 @@ extern "C" int g53h_sorted_dispatch_grad(void *dx, const void *dxs, int dt, int 
 /* One wave per pair: dys of its row, dw of the pair. */
 template <typename E>
 __global__ void __launch_bounds__(256)
-k_combine_grad(E *dys, float *__restrict__ dw, const E *__restrict__ dout, const E *ys, const float *__restrict__ w,
+k_sorted_combine_grad(E *dys, float *__restrict__ dw, const E *__restrict__ dout, const E *ys, const float *__restrict__ w,
                const int *__restrict__ row, int H, int K, long n, long wg0)
 {
     const int lane = threadIdx.x & 63;
@@ -384,9 +384,9 @@ extern "C" int g53h_sorted_combine_grad(void *dys, float *dw, const void *dout, 
     const long n = (long)p->T * p->topk, total = (n + 3) / 4;
     for (long w0 = 0; w0 < total; w0 += G53_LAUNCH_WGS) {
         const unsigned wgs = (unsigned)(total - w0 < G53_LAUNCH_WGS ? total - w0 : G53_LAUNCH_WGS);
-        G53_BY_TYPE(dt, hipLaunchKernelGGL(k_combine_grad<E>, dim3(wgs), dim3(256), 0, g53h_stream(), (E *)dys, dw,
+        G53_BY_TYPE(dt, hipLaunchKernelGGL(k_sorted_combine_grad<E>, dim3(wgs), dim3(256), 0, g53h_stream(), (E *)dys, dw,
                                            (const E *)dout, (const E *)ys, w, p->row, hidden, p->topk, n, w0));
-        G53_LAUNCHED("k_combine_grad");
+        G53_LAUNCHED("k_sorted_combine_grad");
     }
     return 0;
 }

@@ -307,7 +307,8 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
      * its row of both; such lines are not kept in the caches, where half lines wait for their other half. */
     constexpr int PAIR = LINES ? 2 : 1;
     auto load = [&](Chunk *k, int c) {
-        const int w_at = c * 64 + (LINES ? (m >> 3) * 64 : 0) + q * 16, wo = w_at < wrow ? w_at : 0;   /* behind the end: not used */
+        const int w_at = c * 64 + (LINES ? (m >> 3) * 64 : 0) + q * 16;
+        const int wo = w_at < wrow ? w_at : 0;      /* behind the end: not used */
 #pragma unroll
         for (int b = 0; b < PAIR; b++)
 #pragma unroll
@@ -345,8 +346,8 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
 #pragma unroll
     for (int t = 0; t < NT; t++) xat[t] = (16 * t + m < x_rows ? 16 * t + m : x_rows - 1) * ld + q * (GS == 4 ? 64 : 16);
     const int plane = rows * ld;
-    /* sc4, nz4: of the chunk's halves, where UNIT. Step s takes the columns of register s: 8 from each quarter's 32 where the chunk lies
-     * in one group, else turned to 32 in a row. */
+    /* sc4, nz4: of the chunk's halves, where UNIT. Step s takes the columns of register s: 8 from each quarter's 32 where
+     * the chunk lies in one group, else turned to 32 in a row. */
     auto use = [&](const Chunk &k, int c, int c_lds, const float (&sc4)[R][NH], const float (&nz4)[R][NH]) {
         unsigned d[R][4];
         float sc[R][4], nz[R][4];
@@ -563,12 +564,12 @@ static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const
 {
     static int allowed = 0;
     if (!allowed) {
-        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, UC, ROWS, LINES, DIRECT, GS>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                    G53_W4_LDS_MAX));
+        G53_TRY(hipFuncSetAttribute((const void *)k_w4<E, R, NT, UC, ROWS, LINES, DIRECT, GS>,
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, G53_W4_LDS_MAX));
         allowed = 1;
     }
-    hipLaunchKernelGGL((k_w4<E, R, NT, UC, ROWS, LINES, DIRECT, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y, (const E *)x,
-                       a.offsets, a.pair, a);
+    hipLaunchKernelGGL((k_w4<E, R, NT, UC, ROWS, LINES, DIRECT, GS>), grid, dim3(64 * waves), lds, g53h_stream(), (E *)y,
+                       (const E *)x, a.offsets, a.pair, a);
     G53_LAUNCHED("k_w4");
     return 0;
 }
