@@ -69,6 +69,64 @@ def test_product_of_whole_numbers_is_exact(L, T, rows, cols, group, s_dt, zeros,
         assert np.array_equal(y.get(), enc(xv @ m.wide[0].T, dt))
 
 
+@pytest.mark.parametrize("T", [1, 3, 12, 40])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (64, True), (96, True), (128, True), (192, False)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_matrices_of_many_rows_are_exact(L, T, group, zeros, dt):
+    """A matrix that fills the card, whose waves take two row tiles and, for few tokens, whole lines: 16 copies of 1040
+    rows, whole numbers as above."""
+    say("w4, many rows", T, group, zeros, dt)
+    rng = np.random.default_rng(group + T)
+    rows, cols, n = 1040, 4096, 16
+    m = W4(rng, 1, rows, cols, group, BF16, zeros, exact=True)
+    parts = [glm53h.DevBuf(b.n * n) if b else None for b in (m.w_d, m.s_d, m.z_d)]
+    for big, b in zip(parts, (m.w_d, m.s_d, m.z_d)):
+        for k in range(n if b else 0):
+            check(L.g53h_d2d(big.ptr + k * b.n, b.ptr, b.n), "d2d")
+    c = glm53h.G53hW4(parts[0].ptr, parts[1].ptr, parts[2].ptr if zeros else None, rows * n, cols, group, BF16)
+    xv = rng.integers(-2, 3, (T, cols)).astype(float)
+    x, y = Buf(xv, dt), Buf.out((T, rows * n), dt)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, dt, T, C.byref(c), 0.0), "w4")
+    with np.errstate(over="ignore"):
+        assert np.array_equal(y.get(), np.tile(enc(xv @ m.wide[0].T, dt), (1, n)))
+
+
+@pytest.mark.parametrize("T,rows,cols,group,zeros", [(2, 50, 2080, 32, True), (16, 34, 2112, 64, True), (5, 66, 2304, 96, False),
+                                                     (9, 20, 4096, 192, True), (3, 130, 608, 64, False), (14, 36, 1600, 32, True)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_swiglu_of_few_tokens(L, T, rows, cols, group, zeros, dt):
+    say("w4, swiglu", T, rows, cols, group, zeros, dt)
+    rng = np.random.default_rng(rows + cols)
+    m = W4(rng, 1, rows, cols, group, F16, zeros)
+    x, y = Buf(rng.standard_normal((T, cols)), dt), Buf.out((T, rows // 2), dt)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, dt, T, C.byref(m.c), LIMIT), "w4")
+    sums, tol = m.product(x.val())
+    want, tol = swiglu(sums, LIMIT), act_tol(sums, tol, LIMIT)
+    close(y.val(), want, HALF[dt] * np.abs(want) + TINY[dt] + tol)
+
+
+def test_a_matrix_of_the_int4_experts(L):
+    """A G53H_MAT_I4 matrix (quantised by the library) as it lies: against the engine's own product with it. Both are
+    within the worst case of an fp32 sum of the 64-bit product: 512 products, group sums and their sum, each addition
+    off by 2^-24 of at most 62 (levels as they enter) sum |x| s."""
+    say("w4, int4 experts' format")
+    rng = np.random.default_rng(21)
+    rows, cols, T = 256, 512, 3
+    codes = rng.integers(0, 256, (rows, cols)).astype(np.uint8)
+    codes[(codes & 0x7f) == 0x7f] = 0                            # no NaN
+    w, s = Buf(codes), Buf(rng.uniform(0.5, 1.5, (2, 4)), F32)
+    q, steps = Buf(np.zeros((rows, cols // 2), np.uint8)), Buf(np.zeros((rows, cols // 64)), F32)
+    f8 = glm53h.G53hMat(w.ptr, s.ptr, rows, cols, 128, 128, 4, 0)
+    check(L.g53h_i4_from_f8(q.ptr, steps.ptr, C.byref(f8)), "g53h_i4_from_f8")
+    i4 = glm53h.G53hMat(q.ptr, steps.ptr, rows, cols, 1, 64, cols // 64, 4)                # G53H_MAT_I4
+    x, ya, yb = Buf(rng.standard_normal((T, cols)), F32), Buf.out((T, rows), F32), Buf.out((T, rows), F32)
+    check(L.g53h_mm_f8(ya.ptr, x.ptr, T, C.byref(i4)), "g53h_mm_f8")
+    check(L.g53h_mm_w4(yb.ptr, x.ptr, F32, T, C.byref(glm53h.G53hW4(q.ptr, steps.ptr, None, rows, cols, 64, F32)), 0.0), "w4")
+    size = np.abs(x.val()) @ np.repeat(steps.val(), 64, 1).T
+    close(yb.val(), ya.val(), 2 * (2 * 512 + 40) * 2.0 ** -24 * 62 * size)
+    assert np.abs(ya.val()).max() > 0
+
+
 @pytest.mark.parametrize("shift", [2, 4, 6, 14])
 def test_rows_off_alignment(L, shift):
     say("w4, x and y off by", shift)
