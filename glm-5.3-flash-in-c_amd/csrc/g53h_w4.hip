@@ -23,7 +23,7 @@
  * read stream of as many bytes: 23 to 26); eight gate/up matrices of 4096 x 4096 by one token 16.3 us,
  * 4.2 TB/s with a launch and the search of a row's expert in it. Small matrices are a launch and three
  * trips to memory (4096 x 2048 by one token 4.3 us), many tokens the vector work of turning levels into
- * floats beside the products (16384 x 4096 by 128 bf16 tokens 41 us, 420 TFLOP/s).
+ * floats beside the products (16384 x 4096 by 128 bf16 tokens 44 us, 390 TFLOP/s).
  */
 #include <hip/hip_runtime.h>
 
@@ -574,21 +574,30 @@ static int start(dim3 grid, int waves, size_t lds, void *y, const void *x, const
     return 0;
 }
 
-/* busy: token tiles that are expected to hold rows. */
+/* busy: token tiles that are expected to hold rows, mean: rows of an expert. */
 template <typename E, int R, int NT, int UC, bool ROWS, bool LINES = false, bool DIRECT = false>
-static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
+static int launch(void *y, const void *x, G53W4Args &a, long items, long busy, long mean)
 {
     constexpr int P = G53W4Type<E>::P, TT = ROWS ? 16 * NT / P : 16 * NT;
     const bool sw = a.limit > 0.0f;
     const int out = sw ? 8 * R : 16 * R, units = (a.cols + 128 * UC - 1) / (128 * UC), rows = a.T < TT ? a.T : TT;
-    /* While there are fewer than two workgroups a CU, they get fewer rows: their waves split the columns instead, as long
-     * as every part has a unit and its share of x fits LDS, and then there are fewer waves. */
+    /* A workgroup's eight waves are rw groups of rows by 2^k parts of the columns. For the fewest tokens, whose levels are all
+     * there is to wait for, the fewest rows that leave two workgroups a CU. Else a workgroup takes the time that its
+     * activations need on their way to LDS, as of 5 rows each, and its rows', and the CUs take workgroups in rounds (8192 x
+     * 4096 by 64 bf16 tokens: 256 workgroups 18.4 us, 512 20.6, 128 28.9; 6000 x 4096 by 16: 188 10.8, 375 16.8). */
     int k = 0, rw = units < 4 ? G53_W4_NW / 2 : G53_W4_NW;
-    for (;;) {
-        const long wgs = busy * ((a.half + out * rw - 1) / (out * rw));
-        if (rw == 1 || wgs >= 2 * g53h_num_cus() || (!DIRECT && out * rw / 2 < 4 * rows && wgs >= g53h_num_cus() / 2)) break;
-        if ((2 << k) <= units && (DIRECT || rows * P * ((2 << k) * 256 * UC + 16) <= G53_W4_LDS_MAX)) k++;
-        rw /= 2;
+    const int each = mean < rows ? (int)mean : rows;
+    long least = 0;
+    for (int i = 0, r = rw;; r /= 2) {
+        const long wgs = busy * ((a.half + out * r - 1) / (out * r)), slots = g53h_num_cus() * (G53_W4_NW / (r << i));
+        const long cost = (wgs + slots - 1) / slots * (G53_W4_NW / (r << i)) * (5 * each + out * r);
+        if (DIRECT || rows <= 5 || !least || cost < least) {
+            least = cost;
+            rw = r;
+            k = i;
+        }
+        if (r == 1 || ((DIRECT || rows <= 5) && wgs >= 2 * g53h_num_cus())) break;
+        if ((2 << i) <= units && (DIRECT || rows * P * ((2 << i) * 256 * UC + 16) <= G53_W4_LDS_MAX)) i++;
     }
     if (DIRECT && (rw > 1 || (busy * ((a.half + out - 1) / out) << k) > 8 * g53h_num_cus())) return 1;
     const int waves = rw << k, outs = out * rw;
@@ -615,9 +624,9 @@ static int launch(void *y, const void *x, G53W4Args &a, long items, long busy)
 }
 
 /* Row tiles of a wave: two, so that activations read from LDS meet twice the levels, or one where two leave less than
- * 16 waves a CU (4096 x 2048 by one token in bf16: 4.8 us against 5.9). Token tiles of 16, or of 32 for more tokens of
- * many waves, which then turn levels into floats half as often (16384 x 4096 by 128 tokens: 44 us against 50; fp32: 57
- * against 71). For fp32, whose products are three, up to 5 tokens put their planes side by side as 15 rows of a tile, and
+ * 16 waves a CU (4096 x 2048 by one token in bf16: 4.8 us against 5.9). Token tiles of 16, or of 32 for more tokens
+ * where they leave 32 waves a CU, which then turn levels into floats half as often (16384 x 4096 by 128 tokens: 43 us
+ * against 48; 8192 x 4096 by 64, of fewer waves, 22 against 18). For fp32, whose products are three, up to 5 tokens put their planes side by side as 15 rows of a tile, and
  * the products are as many as bf16's (16384 x 4096 by one token: 14.5 us against 16.4). Long rows of a matrix that one
  * token tile meets are loaded in whole lines (65536 x 4096 by 5 tokens: 27.3 us against 30.7; eight gate/up matrices of
  * 4096 x 4096 by one token 16.3 against 17.2); short rows, or rows that further tiles read again, in half lines (64 matrices
@@ -634,21 +643,23 @@ template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
     const long units = (a.cols + 511) / 512;
     const long waves = (a.rows + 31) / 32 * ex * ((mean + 15) / 16) * (units < G53_W4_NW ? units : G53_W4_NW);
     const bool few = waves <= 16 * g53h_num_cus() && !(a.limit > 0.0f);
-    const int TT = F32 && mean <= 5 ? 5 : (mean > 16 && !few ? 32 : 16);
+    const long waves32 = (a.rows + 31) / 32 * ex * ((mean + 31) / 32) * (units < G53_W4_NW ? units : G53_W4_NW);
+    const bool many = waves32 >= 32 * g53h_num_cus();
+    const int TT = F32 && mean <= 5 ? 5 : (mean > 16 && many ? 32 : 16);
     auto items_of = [&](int tt) { return a.offsets ? a.T / tt + ex : (a.T - 1) / tt + 1l; };
     auto busy_of = [&](int tt) { return ex * ((mean + tt - 1) / tt); };
     const long items = items_of(TT), busy = busy_of(TT);
-    if (TT == 32) return launch<E, 2, 2, 2, false>(y, x, a, items, busy);
+    if (TT == 32) return launch<E, 2, 2, 2, false>(y, x, a, items, busy, mean);
     if (few && (TT == 16 || a.cols <= 2048)) {
-        const int rc = launch<E, 1, 1, F32 ? 1 : 2, false, false, true>(y, x, a, items_of(16), busy_of(16));
+        const int rc = launch<E, 1, 1, F32 ? 1 : 2, false, false, true>(y, x, a, items_of(16), busy_of(16), mean);
         if (rc <= 0) return rc;
     }
     if constexpr (F32)
         if (TT == 16)
-            return few ? launch<E, 1, 1, 1, false>(y, x, a, items, busy) : launch<E, 2, 1, 2, false>(y, x, a, items, busy);
-    if (few) return launch<E, 1, 1, 4, F32>(y, x, a, items, busy);
-    if (mean <= TT && units >= 4) return launch<E, 2, 1, 4, F32, true>(y, x, a, items, busy);
-    return launch<E, 2, 1, 4, F32>(y, x, a, items, busy);
+            return few ? launch<E, 1, 1, 1, false>(y, x, a, items, busy, mean) : launch<E, 2, 1, 2, false>(y, x, a, items, busy, mean);
+    if (few) return launch<E, 1, 1, 4, F32>(y, x, a, items, busy, mean);
+    if (mean <= TT && units >= 4) return launch<E, 2, 1, 4, F32, true>(y, x, a, items, busy, mean);
+    return launch<E, 2, 1, 4, F32>(y, x, a, items, busy, mean);
 }
 
 static int product(void *y, const void *x, int dt, G53W4Args &a)
