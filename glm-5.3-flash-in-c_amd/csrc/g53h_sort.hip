@@ -289,21 +289,26 @@ __global__ void __launch_bounds__(256) k_sorted_combine(E *out, const E *__restr
     const long t = wg / chunks;
     const int c = ((int)(wg % chunks) * 256 + threadIdx.x) * 8;
     if (c >= H) return;
-    const int *r = row + t * K;
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (add) g53_load8_to(acc, add + t * H, c, H);
     for (int j0 = 0; j0 < K; j0 += 8) {
         G53Raw8<E> v[8];
+        int r[8];
+        float wj[8];                    /* asked for with the rows' places, not behind the rows */
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const long at = t * K + (j0 + j < K ? j0 + j : K - 1);
+            r[j] = j0 + j < K ? row[at] : -1;
+            wj[j] = w ? w[at] : 1.0f;
+        }
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (j0 + j < K && r[j0 + j] >= 0) g53_raw8_once_to(v[j], ys + (long)r[j0 + j] * H, c, H);
+            if (r[j] >= 0) g53_raw8_once_to(v[j], ys + (long)r[j] * H, c, H);
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (j0 + j < K && r[j0 + j] >= 0) {
-                const float wj = w ? w[t * K + j0 + j] : 1.0f;
+            if (r[j] >= 0)
 #pragma unroll
-                for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(wj, (float)v[j].v[i], acc[i]);
-            }
+                for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(wj[j], (float)v[j].v[i], acc[i]);
     }
     g53_store8_to(out + t * H, acc, c, H);
 }

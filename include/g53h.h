@@ -384,7 +384,7 @@ int g53h_sort_tokens(const G53hSort *p, const int *idx_d);
 int g53h_sorted_dispatch(void *xs_d, const void *x_d, int dt, int hidden, const G53hSort *p);
 int g53h_sorted_dispatch_grad(void *dx_d, const void *dxs_d, int dt, int hidden, const G53hSort *p);
 /* out[t] = add[t] + sum over j of w[t][j] ys[row of (t, j)], in order of j; w fp32 [T][topk]; add may be
- * NULL, or out itself. Rows and weights of pairs left out are not read. _grad, of dout [T][hidden]:
+ * NULL, or out itself. Weights of pairs left out do not count. _grad, of dout [T][hidden]:
  * dys[row] = w dout[t] (rows behind the last left as they were; dys may be ys), dw[t][j] = the product of
  * dout[t] and ys[row], 0 for a pair left out; add's gradient is dout. */
 int g53h_sorted_combine(void *out_d, const void *ys_d, const float *w_d, const void *add_d, int dt, int hidden,
