@@ -231,6 +231,29 @@ def test_sorted_products(L, T, K, NE, rows, cols, group, s_dt, zeros, sw, drop, 
     assert (y.get()[n:] == enc([77.0], dt)).all()
 
 
+@pytest.mark.parametrize("T,K,NE,expert,rows,cols", [(100, 2, 40, 39, 48, 256), (333, 1, 1000, 0, 40, 96), (70, 64, 64, 5, 16, 64),
+                                                     (300, 3, 300, 299, 544, 2048)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_one_expert_takes_all(L, T, K, NE, expert, rows, cols, dt):
+    """Every pair of every token the same expert, the others nothing: exact, whole numbers, and the same bits again."""
+    say("sorted w4, one expert", T, K, NE, expert, rows, cols, dt)
+    rng = np.random.default_rng(T)
+    m = W4(rng, 1, rows, cols, 32, F32, True, exact=True)
+    w, s, z = (glm53h.DevBuf(b.n * NE) for b in (m.w_d, m.s_d, m.z_d))
+    for big, b in ((w, m.w_d), (s, m.s_d), (z, m.z_d)):
+        check(L.g53h_memset(big.ptr, 0xff, b.n * NE), "memset")   # NaN scales elsewhere
+        check(L.g53h_d2d(big.ptr + b.n * expert, b.ptr, b.n), "d2d")
+    plan = Plan(np.full((T, K), expert, np.int32), NE)
+    xv = rng.integers(-2, 3, (T, cols)).astype(float)
+    x = Buf(xv, dt)
+    c = glm53h.G53hW4(w.ptr, s.ptr, z.ptr, rows, cols, 32, F32)
+    want = np.repeat(enc(xv @ m.wide[0].T, dt), K, 0)
+    for _ in range(2):
+        y = Buf.out((T * K, rows), dt)
+        check(L.g53h_sorted_mm_w4(y.ptr, x.ptr, dt, 1, plan.c, C.byref(c), 0.0), "sorted w4")
+        assert np.array_equal(y.get(), want)
+
+
 def test_no_tokens(L):
     say("w4, no tokens")
     m = W4(np.random.default_rng(1), 1, 8, 32, 32, F32, False)
