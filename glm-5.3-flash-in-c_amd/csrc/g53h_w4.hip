@@ -581,22 +581,23 @@ static int launch(void *y, const void *x, G53W4Args &a, long items, long busy, l
     constexpr int P = G53W4Type<E>::P, TT = ROWS ? 16 * NT / P : 16 * NT;
     const bool sw = a.limit > 0.0f;
     const int out = sw ? 8 * R : 16 * R, units = (a.cols + 128 * UC - 1) / (128 * UC), rows = a.T < TT ? a.T : TT;
-    /* A workgroup's eight waves are rw groups of rows by 2^k parts of the columns. For the fewest tokens, whose levels are all
-     * there is to wait for, the fewest rows that leave two workgroups a CU. Else a workgroup takes the time that its
-     * activations need on their way to LDS, as of 5 rows each, and its rows', and the CUs take workgroups in rounds (8192 x
-     * 4096 by 64 bf16 tokens: 256 workgroups 18.4 us, 512 20.6, 128 28.9; 6000 x 4096 by 16: 188 10.8, 375 16.8). */
+    /* A workgroup's eight waves are rw groups of rows by 2^k parts of the columns. A workgroup takes the time that its
+     * activations need on their way to LDS, as of 5 rows each, and its rows', and the CUs take workgroups in rounds: 8192 x
+     * 4096 by 64 bf16 tokens 256 workgroups 18.4 us, 512 20.6, 128 28.9; 6000 x 4096 by 16: 188 10.8, 375 16.8; by 5 fp32
+     * tokens 8192 x 4096: 256 9.1, 512 14.8. DIRECT has no activations in LDS to share: the fewest rows that leave two
+     * workgroups a CU. */
     int k = 0, rw = units < 4 ? G53_W4_NW / 2 : G53_W4_NW;
     const int each = mean < rows ? (int)mean : rows;
     long least = 0;
     for (int i = 0, r = rw;; r /= 2) {
         const long wgs = busy * ((a.half + out * r - 1) / (out * r)), slots = g53h_num_cus() * (G53_W4_NW / (r << i));
         const long cost = (wgs + slots - 1) / slots * (G53_W4_NW / (r << i)) * (5 * each + out * r);
-        if (DIRECT || rows <= 5 || !least || cost < least) {
+        if (DIRECT || !least || cost < least) {
             least = cost;
             rw = r;
             k = i;
         }
-        if (r == 1 || ((DIRECT || rows <= 5) && wgs >= 2 * g53h_num_cus())) break;
+        if (r == 1 || (DIRECT && wgs >= 2 * g53h_num_cus())) break;
         if ((2 << i) <= units && (DIRECT || rows * P * ((2 << i) * 256 * UC + 16) <= G53_W4_LDS_MAX)) i++;
     }
     if (DIRECT && (rw > 1 || (busy * ((a.half + out - 1) / out) << k) > 8 * g53h_num_cus())) return 1;
