@@ -19,8 +19,8 @@
  * through LDS, which also holds the activations, turned into planes once a workgroup, except for small
  * matrices, whose waves each load theirs.
  *
- * By few tokens the levels' bytes bound it: 65536 x 4096 by 5 fp16 tokens 27.3 us, 5.1 TB/s (a plain
- * read stream of as many bytes: 23 to 26); eight gate/up matrices of 4096 x 4096 by one token 16.3 us,
+ * By few tokens the levels' bytes bound it: 65536 x 4096 by 5 fp16 tokens 28.8 us, 4.9 TB/s (a plain
+ * read stream of as many bytes: 23 to 26); eight gate/up matrices of 4096 x 4096 by one token 16.5 us,
  * 4.2 TB/s with a launch and the search of a row's expert in it. Small matrices are a launch and three
  * trips to memory (4096 x 2048 by one token 4.3 us), many tokens the vector work of turning levels into
  * floats beside the products (16384 x 4096 by 128 bf16 tokens 44 us, 390 TFLOP/s).
