@@ -3,12 +3,21 @@
  *
  *     y[t][r] = sum over groups g of  s[r][g] * sum over c in g of (q[r][c] - z[r][g]) x[t][c]
  *
- * Levels go to the matrix cores as they are, without a multiplication: level q becomes the 16-bit
- * float 16 + q (its four bits are the top bits of the mantissa of 2^4), one shift and one and-or per
- * two levels, exact in bf16 and fp16. What was added comes off per group: with X = the group's sum of
- * x (one product with a matrix of ones, shared by all row tiles), the group adds s (D - (16 + z) X).
- * Products are exact in fp32 and summed in fp32; fp32 activations enter as three bf16 planes whose sum
- * is the value exactly (8 + 8 + 8 mantissa bits, by truncation).
+ * Levels go to the matrix cores as whole numbers, exact in bf16 and fp16, and the scale joins a group's
+ * sum. With fp32 and fp16 activations they go as q - z. A sum of (16 + q) x, which takes less work to
+ * form, is many times the result where x has a mean or one large value, and its roundings stay when
+ * (16 + z) X comes off, X the group's sum of x: fp32 x = N(1, 1) by weights around 0, 4096 columns, 3e-6
+ * of the result's norm off against 1e-7 of q - z and 4e-7 of a plain fp32 sum; 2^13 in one column
+ * 1e-4 of the rows in which its level is z, against 1e-7. (65536 x 4096 by 5 fp16 tokens 29.5 us against
+ * 28.8, 16384 x 4096 by one in fp32 11.3 against 9.8.) fp16: the level's four bits are the top bits of
+ * the mantissa of 2^4, and a packed subtraction takes 16 + z off two levels. fp32 activations enter as
+ * three bf16 planes whose sum is the value exactly (8 + 8 + 8 mantissa bits, by truncation), and their
+ * levels, since bf16 has no packed subtraction, as four bytes less z, then fp32, whose upper halves are
+ * bf16. With bf16 activations levels go as q, two by one conversion of bytes that are e4m3 codes of
+ * q 2^-9, and z X comes off, X by one product with ones that all row tiles share: roundings are those of
+ * sums of (q + z) s |x|, 2^-24 each, below a result that keeps 2^-9 of itself (with 2^13 in one column 1
+ * of 150 results is not the nearest bf16, with 16 + q 1 of 70; q - z as with fp32: 65536 x 4096 by one
+ * token 33.4 us against 26.7). Products are exact and sums fp32.
  *
  * A wave owns R tiles of 16 rows and NT tiles of 16 tokens over a part of the columns and steps by 128
  * columns: one 16-byte load per lane and row tile (16 rows x 64 bytes, or 8 rows x whole lines of 128).
@@ -72,40 +81,91 @@ __device__ __forceinline__ g53_v4f g53_mfma(g53_v8h a, g53_v8h b, g53_v4f c)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-/* Eight levels (nibbles 0..7 of d) as 16 + level, in the order 0 4 1 5 2 6 3 7. mask picks the mantissa bits, one a
- * half; it comes in a vector register, so that and and or are one instruction (which takes one scalar and no literal). */
-template <typename V> __device__ __forceinline__ V g53_w4_levels(unsigned d, unsigned mask);
-template <> __device__ __forceinline__ g53_v8b g53_w4_levels<g53_v8b>(unsigned d, unsigned mask)
+/* What takes a zero point z off levels, for g53_w4_levels: in each byte 128 - z (fp32), in each half -(16 + z) as fp16;
+ * bf16: -z, which takes it off the sum. */
+template <typename E> __device__ __forceinline__ unsigned g53_w4_zero(unsigned z);
+template <> __device__ __forceinline__ unsigned g53_w4_zero<float>(unsigned z)
 {
-    const unsigned o = 0x41804180u;                           /* bf16 16.0, mantissa bits 6..3 */
-    return __builtin_bit_cast(g53_v8b, (g53_v4w){((d << 3) & mask) | o, ((d >> 1) & mask) | o, ((d >> 5) & mask) | o,
-                                                 ((d >> 9) & mask) | o});
+    return __builtin_amdgcn_perm(0u, 128u - z, 0u);
 }
-template <> __device__ __forceinline__ g53_v8h g53_w4_levels<g53_v8h>(unsigned d, unsigned mask)
+template <> __device__ __forceinline__ unsigned g53_w4_zero<g53_f16>(unsigned z)
 {
+    return __builtin_amdgcn_perm(0u, 0xcc00u | z << 6, 0x01000100u);
+}
+template <> __device__ __forceinline__ unsigned g53_w4_zero<g53_bf16>(unsigned z)
+{
+    return __builtin_bit_cast(unsigned, -(float)z);
+}
+
+/* Eight levels (nibbles 0..7 of d) in the order 0 2 1 3 4 6 5 7, or 0 4 1 5 2 6 3 7 for fp16, less their zero point but for
+ * bf16. mask picks mantissa bits, one half each; it comes in a vector register, so that and and or are one instruction
+ * (which takes one scalar and no literal). */
+template <typename E> __device__ __forceinline__ typename G53W4Type<E>::V g53_w4_levels(unsigned d, unsigned mask, unsigned zero);
+template <> __device__ __forceinline__ g53_v8b g53_w4_levels<float>(unsigned d, unsigned, unsigned zero)
+{
+    /* bytes q + 128 - z, no carry between them, then q - z as signed bytes: even levels, odd levels */
+    const unsigned even = ((d & 0x0f0f0f0fu) + zero) ^ 0x80808080u, odd = ((d >> 4 & 0x0f0f0f0fu) + zero) ^ 0x80808080u;
+    g53_v4w o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const unsigned b = (i & 1 ? odd : even) >> 16 * (i >> 1);
+        const float low = (float)(int)(int8_t)b, high = (float)(int)(int8_t)(b >> 8);
+        o[i] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, high), __builtin_bit_cast(unsigned, low), 0x07060302u);
+    }
+    return __builtin_bit_cast(g53_v8b, o);
+}
+template <> __device__ __forceinline__ g53_v8b g53_w4_levels<g53_bf16>(unsigned d, unsigned, unsigned)
+{
+    /* e4m3 codes 0 to 15 are multiples of 2^-9, those below the normal range and the first octave */
+    const unsigned even = d & 0x0f0f0f0fu, odd = d >> 4 & 0x0f0f0f0fu;
+    typedef g53_bf16 V2 __attribute__((ext_vector_type(2)));
+    const V2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false);
+    const V2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true);
+    return (g53_v8b){a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
+}
+template <> __device__ __forceinline__ g53_v8h g53_w4_levels<g53_f16>(unsigned d, unsigned mask, unsigned zero)
+{
+    typedef g53_f16 V2 __attribute__((ext_vector_type(2)));
     const unsigned o = 0x4c004c00u;                           /* fp16 16.0, mantissa bits 9..6 */
-    return __builtin_bit_cast(g53_v8h, (g53_v4w){((d << 6) & mask) | o, ((d << 2) & mask) | o, ((d >> 2) & mask) | o,
-                                                 ((d >> 6) & mask) | o});
+    g53_v4w v = {((d << 6) & mask) | o, ((d << 2) & mask) | o, ((d >> 2) & mask) | o, ((d >> 6) & mask) | o};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const unsigned w = v[i];
+        v[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(V2, w) + __builtin_bit_cast(V2, zero));
+    }
+    return __builtin_bit_cast(g53_v8h, v);
 }
-template <typename V> struct G53W4Mask;
-template <> struct G53W4Mask<g53_v8b> { static constexpr unsigned M = 0x00780078u; };
-template <> struct G53W4Mask<g53_v8h> { static constexpr unsigned M = 0x03c003c0u; };
 
 /* Eight activations in the levels' order, as P planes of the products' type. */
-template <typename V> __device__ __forceinline__ void g53_w4_x(V (&o)[1], const g53_v4w (&p)[1])
+__device__ __forceinline__ void g53_w4_x(g53_v8b (&o)[1], const g53_v4w (&p)[1])
 {
     const g53_v4w v = p[0];                                   /* 01 23 45 67 */
-    o[0] = __builtin_bit_cast(V, (g53_v4w){__builtin_amdgcn_perm(v[2], v[0], 0x05040100u),
-                                           __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
-                                           __builtin_amdgcn_perm(v[3], v[1], 0x05040100u),
-                                           __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)});
+    o[0] = __builtin_bit_cast(g53_v8b, (g53_v4w){__builtin_amdgcn_perm(v[1], v[0], 0x05040100u),
+                                                 __builtin_amdgcn_perm(v[1], v[0], 0x07060302u),
+                                                 __builtin_amdgcn_perm(v[3], v[2], 0x05040100u),
+                                                 __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)});
+}
+/* fp16: where one is not finite, the first pair takes a NaN, and with it the row's results. (What is 0 times each, summed up:
+ * 0, or a NaN whose upper half is one of fp16. fp32's second plane does it, infinity less itself, and bf16's sum of x.) */
+__device__ __forceinline__ void g53_w4_x(g53_v8h (&o)[1], const g53_v4w (&p)[1])
+{
+    typedef g53_f16 V2 __attribute__((ext_vector_type(2)));
+    const g53_v4w v = p[0];                                   /* 01 23 45 67 */
+    float none = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const unsigned w = v[i];
+        none = __builtin_amdgcn_fdot2(__builtin_bit_cast(V2, w), (V2){0.0f, 0.0f}, none, false);
+    }
+    o[0] = __builtin_bit_cast(g53_v8h, (g53_v4w){__builtin_amdgcn_perm(v[2], v[0], 0x05040100u) | __builtin_bit_cast(unsigned, none),
+                                                 __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
+                                                 __builtin_amdgcn_perm(v[3], v[1], 0x05040100u),
+                                                 __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)});
 }
 __device__ __forceinline__ void g53_w4_x(g53_v8b (&o)[3], const g53_v4w (&p)[2])
 {
     const g53_v4w a = p[0], b = p[1];
-    unsigned v[8];
-#pragma unroll
-    for (int i = 0; i < 4; i++) { v[2 * i] = a[i]; v[2 * i + 1] = b[i]; }   /* 0 4 1 5 2 6 3 7 */
+    unsigned v[8] = {a[0], a[2], a[1], a[3], b[0], b[2], b[1], b[3]};        /* 0 2 1 3 4 6 5 7 */
 #pragma unroll
     for (int k = 0; k < 3; k++) {
         g53_v4w h;
@@ -181,12 +241,16 @@ template <int R, int X> struct G53W4Chunk {
 __device__ __forceinline__ int g53_quot(int n, int d, int log) { return log >= 0 ? n >> log : n / d; }
 
 /* Every quarter's v to all lanes of its row: o[i] is quarter i's. */
+__device__ __forceinline__ void g53_spread(unsigned (&o)[4], unsigned v)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = v;
+    g53_turn(o);
+}
 __device__ __forceinline__ void g53_spread(float (&o)[4], float v)
 {
     unsigned u[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) u[i] = __builtin_bit_cast(unsigned, v);
-    g53_turn(u);
+    g53_spread(u, __builtin_bit_cast(unsigned, v));
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = __builtin_bit_cast(float, u[i]);
 }
@@ -253,14 +317,14 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int r = 0; r < R; r++) acc[r][t] = zero;
-    V ones;
+    V ones;                             /* bf16: for the sums of x */
 #pragma unroll
     for (int i = 0; i < 8; i++) ones[i] = 1.0f;
-    unsigned mask = G53W4Mask<V>::M;
+    unsigned mask = 0x03c003c0u;
     asm volatile("" : "+v"(mask));
     const int units = (a.cols + 128 * UC - 1) / (128 * UC);
 
-    /* scales and zero points of a group, as they lie, and as they enter: s and -(16 + z) */
+    /* scales and zero points of a group, as they lie, and as they enter */
     auto ask = [&](unsigned (&ks)[R], unsigned (&kz)[R], int g) {
         if (a.s_dt == G53H_F32)
 #pragma unroll
@@ -279,7 +343,7 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
         const float f16 = (float)__builtin_bit_cast(g53_f16, (uint16_t)v);
         return __builtin_bit_cast(float, (v << s_shift & ~s_f16) | (__builtin_bit_cast(unsigned, f16) & s_f16));
     };
-    auto surplus = [&](unsigned v, int g) { return -16.0f - (float)((v >> (4 * (g & 1)) & z_mask) | z_no); };
+    auto zero_of = [&](unsigned v, int g) { return g53_w4_zero<E>((v >> (4 * (g & 1)) & z_mask) | z_no); };
     /* the lane's group in chunk c: that of its quarter; in unit u: that of chunk q's half h (of NH halves) */
     constexpr int NH = GS == 4 ? 1 : 2;
     /* Scales are asked for by unit: by chunk they are as many requests to the vector cache as the levels (16384 x 4096 in
@@ -346,11 +410,11 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
 #pragma unroll
     for (int t = 0; t < NT; t++) xat[t] = (16 * t + m < x_rows ? 16 * t + m : x_rows - 1) * ld + q * (GS == 4 ? 64 : 16);
     const int plane = rows * ld;
-    /* sc4, nz4: of the chunk's halves, where UNIT. Step s takes the columns of register s: 8 from each quarter's 32 where
+    /* sc4, zr4: of the chunk's halves, where UNIT. Step s takes the columns of register s: 8 from each quarter's 32 where
      * the chunk lies in one group, else turned to 32 in a row. */
-    auto use = [&](const Chunk &k, int c, int c_lds, const float (&sc4)[R][NH], const float (&nz4)[R][NH]) {
-        unsigned d[R][4];
-        float sc[R][4], nz[R][4];
+    auto use = [&](const Chunk &k, int c, int c_lds, const float (&sc4)[R][NH], const unsigned (&zr4)[R][NH]) {
+        unsigned d[R][4], zr[R][4];
+        float sc[R][4];
 #pragma unroll
         for (int r = 0; r < R; r++) {
 #pragma unroll
@@ -360,17 +424,18 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
 #pragma unroll
                 for (int h = 0; h < NH; h++) {
                     sc[r][GS * (h + 1) - 1] = sc4[r][h];
-                    nz[r][GS * (h + 1) - 1] = nz4[r][h];
+#pragma unroll
+                    for (int i = 0; i < GS; i++) zr[r][GS * h + i] = zr4[r][h];
                 }
             } else {
                 g53_spread(sc[r], scale(k.s[r]));
-                g53_spread(nz[r], surplus(k.z[r], group_of(c)));
+                g53_spread(zr[r], zero_of(k.z[r], group_of(c)));
             }
         }
-        /* the upper planes of fp32 apart from the lower ones: what a sum of the surplus' size rounds away is rounded once
-         * a product instead of three times */
+        /* the upper planes of fp32 apart from the lower ones, whose roundings are 2^-8 of theirs then */
         constexpr int DP = PM == 3 ? 2 : 1;
-        g53_v4f D[R][NT][DP], X[NT][DP];
+        constexpr bool SUM = __is_same(E, g53_bf16);    /* zero points come off the sums, with x's */
+        g53_v4f D[R][NT][DP], X[NT];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             V b[NT][PM];
@@ -390,13 +455,12 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int p = 0; p < PM; p++) {
-                    g53_v4f &to = X[t][p ? DP - 1 : 0];
                     if (!DIRECT) b[t][p] = *(const V *)(lds + p * plane + xat[t] + c_lds * 256 + s * (GS == 4 ? 16 : 64));
-                    to = g53_mfma(b[t][p], ones, s % GS == 0 && p < 2 ? zero : to);
+                    if (SUM) X[t] = g53_mfma(b[t][p], ones, s % GS == 0 ? zero : X[t]);
                 }
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                const V lv = g53_w4_levels<V>(d[r][s], mask);
+                const V lv = g53_w4_levels<E>(d[r][s], mask, zr[r][s]);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -413,8 +477,9 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
                     for (int t = 0; t < NT; t++) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            float v = __builtin_fmaf(nz[r][s], X[t][0][i], D[r][t][0][i]);
-                            if (DP == 2) v += __builtin_fmaf(nz[r][s], X[t][DP - 1][i], D[r][t][DP - 1][i]);
+                            float v = D[r][t][0][i];
+                            if (SUM) v = __builtin_fmaf(__builtin_bit_cast(float, zr[r][s]), X[t][i], v);
+                            if (DP == 2) v += D[r][t][DP - 1][i];
                             acc[r][t][i] = __builtin_fmaf(sc[r][s], v, acc[r][t][i]);
                         }
                         asm volatile("" : "+v"(acc[r][t]));      /* added here, not behind the next branch with D kept */
@@ -430,7 +495,7 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
 #pragma unroll
             for (int h = 0; h < NH; h++) ask(us[h], uz[h], unit_group(u, h));
     };
-    auto unit_scales = [&](int u, float (&sc)[NH][R][4], float (&nz)[NH][R][4]) {
+    auto unit_scales = [&](int u, float (&sc)[NH][R][4], unsigned (&zr)[NH][R][4]) {
         if (UNIT)
 #pragma unroll
             for (int h = 0; h < NH; h++) {
@@ -438,7 +503,7 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     g53_spread(sc[h][r], scale(us[h][r]));
-                    g53_spread(nz[h][r], surplus(uz[h][r], g));
+                    g53_spread(zr[h][r], zero_of(uz[h][r], g));
                 }
             }
     };
@@ -501,9 +566,10 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
         const bool ends = seg0 + here == units;
         const int until = ends ? here - KW : here;
         int i = kw;
-        float sc[NH][R][4], nz[NH][R][4], sj[R][NH], nj[R][NH];
+        float sc[NH][R][4], sj[R][NH];
+        unsigned zr[NH][R][4], zj[R][NH];
         for (; i < until; i += KW) {
-            unit_scales(seg0 + i, sc, nz);
+            unit_scales(seg0 + i, sc, zr);
             ask_unit(seg0 + i + KW);
 #pragma unroll
             for (int j = 0; j < UC; j++) {
@@ -511,21 +577,21 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
-                    for (int h = 0; h < NH; h++) { sj[r][h] = sc[h][r][j]; nj[r][h] = nz[h][r][j]; }
-                use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, nj);
+                    for (int h = 0; h < NH; h++) { sj[r][h] = sc[h][r][j]; zj[r][h] = zr[h][r][j]; }
+                use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, zj);
                 if (j % PAIR == PAIR - 1) load(ring + j - (PAIR - 1), (seg0 + i + KW) * UC + j - (PAIR - 1));
             }
         }
         if (ends && i < here) {
-            unit_scales(seg0 + i, sc, nz);
+            unit_scales(seg0 + i, sc, zr);
 #pragma unroll
             for (int j = 0; j < UC; j++) {
                 if (j % PAIR == 0) pass(ring + j);
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
-                    for (int h = 0; h < NH; h++) { sj[r][h] = sc[h][r][j]; nj[r][h] = nz[h][r][j]; }
-                use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, nj);
+                    for (int h = 0; h < NH; h++) { sj[r][h] = sc[h][r][j]; zj[r][h] = zr[h][r][j]; }
+                use(ring[j], (seg0 + i) * UC + j, i * UC + j, sj, zj);
             }
         }
     }

@@ -406,8 +406,9 @@ typedef struct {
 /* y[T][rows] = M . x[T][cols]. With swiglu_limit > 0 the matrix is gate over up (rows / 2 each) and
  * y[T][rows / 2] their SwiGLU as g53h_swiglu's, from the fp32 sums; 0: without. Meant for few tokens:
  * the levels go to the matrix cores once per 16 or 32 of them (fp32: 5 where there are no more). Products
- * are exact and sums fp32; a row of x whose |x| times 31 leaves fp32 in a group's sum, or that is not
- * finite, gives NaN, and fp32 values below 2^-109 lose low bits. At most 2^24 columns of 2^30 rows. */
+ * are exact and sums fp32, of (q - z) x in a group, with bf16 x of q x less z times that of x. A row of x
+ * that is not finite gives NaN, one whose |x| times 15 leaves fp32 in a group's sum infinities or NaN, and
+ * fp32 values below 2^-109 lose low bits. At most 2^24 columns of 2^30 rows. */
 int g53h_mm_w4(void *y_d, const void *x_d, int dt, int T, const G53hW4 *m, float swiglu_limit);
 /* The same over the sorted rows of a plan, each with its expert's matrix: m describes expert 0, the levels,
  * scales and zero points of the others follow it. x: with gather the tokens [T][cols] (a row takes its pair's

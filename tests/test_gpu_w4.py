@@ -283,3 +283,121 @@ def test_matrix_past_2_gib(L):
     check(L.g53h_sorted_mm_w4(y.ptr, x.ptr, BF16, 1, plan.c, C.byref(c), 0.0), "sorted w4")
     got = y.get()
     assert (got[:2] == 0).all() and np.array_equal(got[2:], enc(xv @ m.wide[0].T, BF16))
+
+
+def tight(m, x, dt, e=0):
+    """x times matrix e, and what its sums may be off: a product is one of at most min(group, 128) of a partial sum, partial
+    sums join the row's as often as the columns hold groups' pieces of 32 to 128, and then up to eight waves' and three
+    planes' are added. Every addition is off by at most 2^-23 of the sum of its products' sizes (the matrix cores may cut
+    what does not fit, which is a whole step). Levels enter as q - z, exactly; with bf16 as q, and z times the sum of x comes
+    off: sizes are (q + z) |x| then."""
+    depth = min(m.group, 128) + -(-x.shape[1] // min(m.group, 32 if m.group % 64 else 64 if m.group % 128 else 128)) + 16
+    size = (m.lv[e] + m.z[e]) * m.s[e] if dt == BF16 else np.abs(m.wide[e])
+    return x @ m.wide[e].T, depth * 2.0 ** -23 * (np.abs(x) @ size.T)
+
+
+def centred(rng, m, zeros):
+    """Levels as a quantiser makes them of N(0, 1) weights: the largest of a group 6 or 7 from its zero point, 6 to 9 or 8."""
+    n, rows, cols = m.lv.shape
+    gs = -(-cols // m.group)
+    w = rng.standard_normal((n, rows, cols))
+    top = np.repeat(np.abs(w).reshape(n, rows, gs, m.group).max(3), m.group, 2)
+    if zeros:
+        z = rng.integers(6, 10, (n, rows, gs + gs % 2)).astype(np.uint8)
+        m.z = np.repeat(z[..., :gs], m.group, 2).astype(np.int64)
+        m.z_d = Buf(z[..., 0::2] | (z[..., 1::2] << 4))
+    levels(m, np.round(w / top * (6 if zeros else 7)).astype(np.int64) + m.z)
+
+
+def levels(m, lv):
+    m.lv, m.wide = lv, (lv - m.z) * m.s
+    m.w_d = Buf((lv[..., 0::2] | (lv[..., 1::2] << 4)).astype(np.uint8))
+
+
+def copies(L, m, n):
+    """The arrays of n copies of m's rows below each other."""
+    parts = [glm53h.DevBuf(b.n * n) if b else None for b in (m.w_d, m.s_d, m.z_d)]
+    for big, b in zip(parts, (m.w_d, m.s_d, m.z_d)):
+        for k in range(n if b else 0):
+            check(L.g53h_d2d(big.ptr + k * b.n, b.ptr, b.n), "d2d")
+    return parts
+
+
+PATHS = [(1, 1), (5, 1), (6, 1), (24, 1), (1, 32), (5, 32), (12, 32), (40, 32)]   # tokens, copies of 520 rows
+
+
+@pytest.mark.parametrize("T,n", PATHS)
+@pytest.mark.parametrize("group,zeros", [(128, False), (128, True), (64, True), (32, True)])
+@pytest.mark.parametrize("mean", [1.0, 10.0])
+def test_fp32_error_whatever_the_mean(L, T, n, group, zeros, mean):
+    """fp32 products of x = N(mean, 1) with weights around 0 are as near as a plain fp32 sum. Of 1024 columns a chunk of 128 is added in four
+    steps, each off by at most a step (2^-23) of its partial sum, whose norm over the rows is at most sqrt(k / 4) of the
+    chunk's at step k: 3.07 together; chunks' errors are independent, so the row's is 3.07 x 2^-23 = 3.7e-7 of its norm.
+    Eight waves' sums and the chunks before them are added with half a step each of sqrt(j / 8): 5.9 x 2^-24 = 3.5e-7; a
+    step's lower planes are 2^-8 of it. 7.2e-7 of the result's norm, and the spread of a norm over 512 rows makes 9e-7.
+    (Groups of 32 and 64 trade steps of the first kind for as many of the second.)"""
+    say("w4, fp32 error", T, n, group, zeros, mean)
+    rng = np.random.default_rng(T + group)
+    m = W4(rng, 1, 520, 1024, group, F32, zeros)
+    centred(rng, m, zeros)
+    parts = copies(L, m, n)
+    x, y = Buf(rng.normal(mean, 1.0, (T, 1024)), F32), Buf.out((T, 520 * n), F32)
+    c = glm53h.G53hW4(*[b.ptr if b else None for b in parts], 520 * n, 1024, group, F32)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, F32, T, C.byref(c), 0.0), "w4")
+    want = x.val() @ m.wide[0].T
+    got = y.val().reshape(T, n, 520)
+    assert (got == got[:, :1]).all()
+    off = np.linalg.norm(got[:, 0] - want) / np.linalg.norm(want)
+    say("off by", off)
+    assert off < 9e-7
+
+
+@pytest.mark.parametrize("T,n", PATHS)
+@pytest.mark.parametrize("group,zeros", [(128, False), (128, True), (96, True), (64, True), (32, False)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_a_large_value_that_a_level_makes_zero(L, T, n, group, zeros, dt):
+    """One column of x is 2^13 to 2^30 times the others, and its levels are the zero point: it adds nothing, nor do its
+    roundings in fp32 and fp16, where the bound is that of the other columns."""
+    say("w4, large value", T, n, group, zeros, dt)
+    rng = np.random.default_rng(T + group)
+    m = W4(rng, 1, 520, 1024, group, F32, zeros)
+    at = 700
+    lv = m.lv.copy()
+    lv[:, :, at] = m.z[:, :, at]
+    levels(m, lv)
+    parts = copies(L, m, n)
+    xv = rng.standard_normal((T, 1024))
+    xv[:, at] = {F32: 2.0 ** 30, F16: 2.0 ** 15, BF16: 2.0 ** 13}[dt]
+    x, y = Buf(xv, dt), Buf.out((T, 520 * n), dt)
+    c = glm53h.G53hW4(*[b.ptr if b else None for b in parts], 520 * n, 1024, group, F32)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, dt, T, C.byref(c), 0.0), "w4")
+    want, tol = tight(m, x.val(), dt)
+    got = y.val().reshape(T, n, 520)
+    assert (got == got[:, :1]).all()
+    close(got[:, 0], want, HALF[dt] * np.abs(want) + TINY[dt] + tol)
+
+
+@pytest.mark.parametrize("T,n", PATHS)
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_a_value_that_is_not_finite_in_any_place(L, T, n, dt):
+    """An infinity or NaN at any of 1024 columns makes all of its token's results NaN, and no other token's."""
+    say("w4, not finite in any place", T, n, dt)
+    rng = np.random.default_rng(T)
+    m = W4(rng, 1, 520, 1024, 64, F32, True)
+    parts = copies(L, m, n)
+    c = glm53h.G53hW4(*[b.ptr if b else None for b in parts], 520 * n, 1024, 64, F32)
+    xv = rng.standard_normal((T, 1024))
+    x, ya, yb = Buf(xv, dt), Buf.out((T, 520 * n), dt), Buf.out((T, 520 * n), dt)
+    check(L.g53h_mm_w4(ya.ptr, x.ptr, dt, T, C.byref(c), 0.0), "w4")
+    good, size = ya.get(), x.n // x.shape[0] // 1024
+    for k, (at, bad) in enumerate([(0, np.inf), (1, -np.inf), (6, np.nan), (39, -np.inf), (514, np.inf), (1023, np.inf)]):
+        t = k % T
+        one = Buf(np.array([bad]), dt)
+        check(L.g53h_d2d(x.ptr + (t * 1024 + at) * size, one.ptr, size), "d2d")
+        check(L.g53h_mm_w4(yb.ptr, x.ptr, dt, T, C.byref(c), 0.0), "w4")
+        got = yb.val()
+        assert np.isnan(got[t]).all(), (at, bad)
+        rest = [i for i in range(T) if i != t]
+        assert np.array_equal(yb.get()[rest], good[rest])
+        one = Buf(xv[t, at:at + 1], dt)
+        check(L.g53h_d2d(x.ptr + (t * 1024 + at) * size, one.ptr, size), "d2d")
