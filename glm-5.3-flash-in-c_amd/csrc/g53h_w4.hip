@@ -676,8 +676,10 @@ static int launch(void *y, const void *x, G53W4Args &a, long items, long busy, l
     a.seg = seg;
     size_t lds = DIRECT ? 0 : (size_t)rows * P * (seg * 256 * UC + 16), red = (size_t)waves * 16 * NT * (16 * R + 4) * 4;
     if (lds < red) lds = red;
-    /* threads of a launch fit 32 bits: of 2^30 rows a workgroup has 256 */
-    const long wide = a.offsets ? a.tiles : (a.tiles + 7) / 8 * 8l, most = (1l << 31) / (64 * G53_W4_NW) / wide;
+    /* threads of a launch, 64 a wave, fit 32 bits: waves are as many as groups of rows (rw) where rows pass 2^29, so 2^30
+     * rows are 2^31 threads at least, of 32 rows a wave */
+    const long wide = a.offsets ? a.tiles : (a.tiles + 7) / 8 * 8l, most = (1l << 31) / (64 * waves) / wide;
+    if (most < 1) return g53h_fail("4-bit product: %d rows in workgroups of %d rows and %d waves", a.rows, outs, waves);
     for (long i = 0; i < items; i += most) {
         a.item0 = i;
         a.items = (int)(items - i < most ? items - i : most);

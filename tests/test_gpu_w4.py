@@ -7,7 +7,7 @@ import pytest
 
 import glm53h
 from glm53h import check
-from op_lib import BF16, F16, F32, HALF, TINY, W4, Buf, Plan, close, enc, routing, sorted_plan, swiglu
+from op_lib import BF16, F16, F32, HALF, TINY, W4, Buf, Plan, close, dec, enc, routing, sorted_plan, swiglu
 from test_gpu_parity import say
 
 pytestmark = pytest.mark.gpu
@@ -401,3 +401,35 @@ def test_a_value_that_is_not_finite_in_any_place(L, T, n, dt):
         assert np.array_equal(yb.get()[rest], good[rest])
         one = Buf(xv[t, at:at + 1], dt)
         check(L.g53h_d2d(x.ptr + (t * 1024 + at) * size, one.ptr, size), "d2d")
+
+
+@pytest.mark.parametrize("rows,limit", [((1 << 29) + 4096, 0.0), (1 << 30, 0.0), (1 << 30, LIMIT)])
+def test_as_many_rows_as_there_may_be(L, rows, limit):
+    """2^30 rows of 32 columns, 16 GiB of levels: copies of 4096 rows of whole numbers. (With SwiGLU: all copies alike, and
+    the first one within its tolerance.)"""
+    say("w4, many rows", rows, limit)
+    rng = np.random.default_rng(17)
+    m = W4(rng, 1, 4096, 32, 32, BF16, False, exact=True)
+    parts = []
+    for b in (m.w_d, m.s_d):
+        big, have = glm53h.DevBuf(b.n // 4096 * rows), b.n
+        check(L.g53h_d2d(big.ptr, b.ptr, b.n), "d2d")
+        while have < big.nbytes:                                   # twice as much at a time
+            more = min(have, big.nbytes - have)
+            check(L.g53h_d2d(big.ptr + have, big.ptr, more), "d2d")
+            have += more
+        parts.append(big)
+    c = glm53h.G53hW4(parts[0].ptr, parts[1].ptr, None, rows, 32, 32, BF16)
+    x, out = Buf(rng.integers(-2, 3, (1, 32)).astype(float), BF16), rows // 2 if limit else rows
+    y = glm53h.DevBuf(2 * out)
+    check(L.g53h_memset(y.ptr, 0xff, 2 * out), "memset")           # NaN
+    check(L.g53h_mm_w4(y.ptr, x.ptr, BF16, 1, C.byref(c), limit), "w4")
+    got = y.download(np.uint16).reshape(-1, 4096)
+    assert (got == got[0]).all()
+    sums, tol = tight(m, x.val(), BF16)
+    if limit:
+        both, tol = np.concatenate((sums, sums), 1), np.concatenate((tol, tol), 1)    # gate and up rows are alike
+        want, tol = swiglu(both, limit), act_tol(both, tol, limit)
+        close(dec(got[:1], BF16), want, HALF[BF16] * np.abs(want) + TINY[BF16] + tol)
+    else:
+        assert np.array_equal(got[:1], enc(sums, BF16))
