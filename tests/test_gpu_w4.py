@@ -433,3 +433,23 @@ def test_as_many_rows_as_there_may_be(L, rows, limit):
         close(dec(got[:1], BF16), want, HALF[BF16] * np.abs(want) + TINY[BF16] + tol)
     else:
         assert np.array_equal(got[:1], enc(sums, BF16))
+
+
+@pytest.mark.parametrize("T,rows,cols,group,s_dt,zeros,sw", CASES)
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_product_within_the_roundings_of_its_own_products(L, T, rows, cols, group, s_dt, zeros, sw, dt):
+    """The bound counts |q - z| s |x| (bf16: q + z) and no more than 128 products a partial sum, so that a wrong wide group
+    shows, with and without SwiGLU; and the whole is within half a step of the type and, for the sums, 2^-19."""
+    say("w4, tight", T, rows, cols, group, s_dt, zeros, sw, dt)
+    rng = np.random.default_rng(rows + cols + T + 2)
+    m = W4(rng, 1, rows, cols, group, s_dt, zeros)
+    x, out = Buf(rng.standard_normal((T, cols)), dt), rows // 2 if sw else rows
+    y = Buf.out((T, out), dt)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, dt, T, C.byref(m.c), LIMIT if sw else 0.0), "w4")
+    want, tol = tight(m, x.val(), dt)
+    if sw:
+        want, tol = swiglu(want, LIMIT), act_tol(want, tol, LIMIT)
+    got = y.val()
+    close(got, want, HALF[dt] * np.abs(want) + TINY[dt] + tol)
+    if out * T >= 100:
+        assert np.linalg.norm(got - want) <= (HALF[dt] + 2.0 ** -19) * np.linalg.norm(want)
