@@ -453,3 +453,81 @@ def test_product_within_the_roundings_of_its_own_products(L, T, rows, cols, grou
     close(got, want, HALF[dt] * np.abs(want) + TINY[dt] + tol)
     if out * T >= 100:
         assert np.linalg.norm(got - want) <= (HALF[dt] + 2.0 ** -19) * np.linalg.norm(want)
+
+
+class Stacked:
+    """NE matrices of `n` copies of a tile of rows of their own: the tiles (W4) on the host, all of it on the device. With
+    halves, gate over up: n copies of the tile's upper half of rows, then n of its lower half."""
+
+    def __init__(self, L, rng, NE, tile, n, cols, group, s_dt, zeros, exact, halves=False):
+        self.m = m = W4(rng, NE, tile, cols, group, s_dt, zeros, exact=exact)
+        self.rows, parts = tile * n, []
+        for b in (m.w_d, m.s_d, m.z_d):
+            if b is None:
+                parts.append(None)
+                continue
+            big, one = glm53h.DevBuf(b.n * n), b.n // NE                    # bytes of a tile
+            piece = one // 2 if halves else one
+            for e in range(NE):
+                for h in range(2 if halves else 1):
+                    for k in range(n):
+                        check(L.g53h_d2d(big.ptr + (e * n * one) + (h * n + k) * piece, b.ptr + e * one + h * piece, piece), "d2d")
+            parts.append(big)
+        self.parts = parts
+        self.c = glm53h.G53hW4(parts[0].ptr, parts[1].ptr, parts[2].ptr if zeros else None, tile * n, cols, group, s_dt)
+
+
+@pytest.mark.parametrize("counts", [[40, 70, 0, 55, 33, 64, 47, 51], [1, 200, 0, 0, 31, 32, 33, 63]])
+@pytest.mark.parametrize("gather", [1, 0])
+@pytest.mark.parametrize("group,zeros,sw", [(128, True, False), (32, False, False), (64, True, True), (96, True, True)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_large_experts_of_many_rows(L, counts, gather, group, zeros, sw, dt):
+    """A batch over eight large matrices, which go by 32 rows at a time: experts of uneven rows, some with none, some that end
+    at a tile's end or one row behind it, tokens without an expert between them. Whole numbers are exact; with SwiGLU within
+    the roundings of its sums."""
+    say("sorted w4, large experts", counts, gather, group, zeros, sw, dt)
+    rng = np.random.default_rng(group + sum(counts))
+    NE, cols, tile, n = 8, 2112, 208, 20
+    m = Stacked(L, rng, NE, tile, n, cols, group, BF16, zeros, not sw, halves=sw)
+    flat = np.concatenate([np.full(k, e) for e, k in enumerate(counts)] + [np.full(9, -1)]).astype(np.int32)
+    flat = rng.permutation(flat)
+    K = 2 if len(flat) % 2 == 0 else 1
+    idx = flat.reshape(-1, K)
+    plan, (off, pair, _) = Plan(idx, NE), sorted_plan(idx, NE)
+    last, out = off[NE], m.rows // 2 if sw else m.rows
+    xv = rng.standard_normal((len(idx) if gather else flat.size, cols)) if sw else rng.integers(
+        -2, 3, (len(idx) if gather else flat.size, cols)).astype(float)
+    if not gather:
+        xv[last:] = np.nan
+    x, y = Buf(xv, dt), Buf.out((flat.size, out), dt)
+    check(L.g53h_sorted_mm_w4(y.ptr, x.ptr, dt, gather, plan.c, C.byref(m.c), LIMIT if sw else 0.0), "sorted w4")
+    v, got = x.val(), y.get()
+    assert (got[last:] == enc([77.0], dt)).all()
+    got = got[:last].reshape(last, n, -1)
+    assert (got == got[:, :1]).all()                                        # copies alike
+    for e in range(NE):
+        a, b = off[e], off[e + 1]
+        if a < b:
+            want, tol = tight(m.m, v[pair[a:b] // K] if gather else v[a:b], dt, e)
+            if sw:
+                want, tol = swiglu(want, LIMIT), act_tol(want, tol, LIMIT)
+                close(dec(got[a:b, 0], dt), want, HALF[dt] * np.abs(want) + TINY[dt] + tol, e)
+            else:
+                assert np.array_equal(got[a:b, 0], enc(want, dt)), e
+
+
+@pytest.mark.parametrize("T", [33, 40, 64])
+@pytest.mark.parametrize("group,zeros", [(128, True), (64, False), (32, True)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_swiglu_of_a_large_matrix_and_many_tokens(L, T, group, zeros, dt):
+    say("w4, swiglu of a large matrix", T, group, zeros, dt)
+    rng = np.random.default_rng(T + group)
+    m = Stacked(L, rng, 1, 1040, 16, 4096, group, F16, zeros, False, halves=True)
+    x, y = Buf(rng.standard_normal((T, 4096)), dt), Buf.out((T, 8320), dt)
+    check(L.g53h_mm_w4(y.ptr, x.ptr, dt, T, C.byref(m.c), LIMIT), "w4")
+    got = y.val().reshape(T, 16, 520)
+    assert (got == got[:, :1]).all()
+    sums, tol = tight(m.m, x.val(), dt)
+    want, tol = swiglu(sums, LIMIT), act_tol(sums, tol, LIMIT)
+    close(got[:, 0], want, HALF[dt] * np.abs(want) + TINY[dt] + tol)
+    assert np.linalg.norm(got[:, 0] - want) <= (HALF[dt] + 2.0 ** -19) * np.linalg.norm(want)
