@@ -28,11 +28,13 @@
  * through LDS, which also holds the activations, turned into planes once a workgroup, except for small
  * matrices, whose waves each load theirs.
  *
- * By few tokens the levels' bytes bound it: 65536 x 4096 by 5 fp16 tokens 28.8 us, 4.9 TB/s (a plain
+ * By few tokens the levels' bytes bound it: 65536 x 4096 by 5 fp16 tokens 29.5 us, 4.8 TB/s (a plain
  * read stream of as many bytes: 23 to 26); eight gate/up matrices of 4096 x 4096 by one token 16.5 us,
- * 4.2 TB/s with a launch and the search of a row's expert in it. Small matrices are a launch and three
- * trips to memory (4096 x 2048 by one token 4.3 us), many tokens the vector work of turning levels into
- * floats beside the products (16384 x 4096 by 128 bf16 tokens 44 us, 390 TFLOP/s).
+ * 4.2 TB/s with a launch and the search of a row's expert in it. Matrices of 10 to 40 MB leave part of
+ * the card idle at their start and end (9000 x 8192 by 5 tokens 18.1 us, 2.1 TB/s). Small ones are a
+ * launch and three trips to memory (4096 x 2048 by one token 4.2 us), many tokens the vector work of
+ * turning levels into floats beside the products (16384 x 4096 by 128 bf16 tokens 45 us, 380 TFLOP/s).
+ * fp32 has the most of it: by few tokens it bounds whole streams too (65536 x 4096 by one 34 us).
  */
 #include <hip/hip_runtime.h>
 
@@ -347,10 +349,10 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
     /* the lane's group in chunk c: that of its quarter; in unit u: that of chunk q's half h (of NH halves) */
     constexpr int NH = GS == 4 ? 1 : 2;
     /* Scales are asked for by unit: by chunk they are as many requests to the vector cache as the levels (16384 x 4096 in
-     * groups of 64 by one bf16 token 15.0 us against 11.8, 64 matrices of 2048 x 1024 by 64 tokens 21.2 against 18.5). Not
-     * those of groups of 32, whose registers would be too many, nor where fp32's three products wait for no scale (4096 x
-     * 4096 by 64 tokens 30.9 us against 32.9 by unit). */
-    constexpr bool UNIT = GS == 4 || (GS == 2 && UC > 1 && PM == 1);
+     * groups of 64 by one bf16 token 16.0 us against 12.2, by 5 fp16 tokens 16.6 against 12.8, 64 matrices of 2048 x 1024 by
+     * 64 tokens 21.5 against 18.1; 4096 x 4096 by 64 fp32 tokens 30.6 either way). Not those of groups of 32, whose registers
+     * would be too many. */
+    constexpr bool UNIT = GS == 4 || (GS == 2 && UC > 1);
     auto group_of = [&](int c) {
         const int g = g53_quot(c * 4 + q, a.group / 32, a.glog);
         return g < a.groups ? g : a.groups - 1;
@@ -649,9 +651,11 @@ static int launch(void *y, const void *x, G53W4Args &a, long items, long busy, l
     const int out = sw ? 8 * R : 16 * R, units = (a.cols + 128 * UC - 1) / (128 * UC), rows = a.T < TT ? a.T : TT;
     /* A workgroup's eight waves are rw groups of rows by 2^k parts of the columns. A workgroup takes the time that its
      * activations need on their way to LDS, as of 5 rows each, and its rows', and the CUs take workgroups in rounds: 8192 x
-     * 4096 by 64 bf16 tokens 256 workgroups 18.4 us, 512 20.6, 128 28.9; 6000 x 4096 by 16: 188 10.8, 375 16.8; by 5 fp32
-     * tokens 8192 x 4096: 256 9.1, 512 14.8. DIRECT has no activations in LDS to share: the fewest rows that leave two
-     * workgroups a CU. */
+     * 4096 by 64 bf16 tokens 256 workgroups 18.8 us, 512 20.4, 128 28.5; 6000 x 4096 by 16: 188 11.0, 375 16.6; by 5 fp32
+     * tokens 8192 x 4096: 256 9.9, 512 15.6. An expert's rows count as `mean`, all experts' alike, since the host does not know
+     * them: uneven ones can do better by other parts (512 rows of each of 16 experts by 64 tokens 10.8, by twice the rows a
+     * workgroup 9.0), and so can some single matrices (24576 x 2048 gate/up by one 11.9, by a quarter 10.8). DIRECT has no
+     * activations in LDS to share: the fewest rows that leave two workgroups a CU. */
     int k = 0, rw = units < 4 ? G53_W4_NW / 2 : G53_W4_NW;
     const int each = mean < rows ? (int)mean : rows;
     long least = 0;
@@ -693,18 +697,21 @@ static int launch(void *y, const void *x, G53W4Args &a, long items, long busy, l
 }
 
 /* Row tiles of a wave: two, so that activations read from LDS meet twice the levels, or one where two leave less than
- * 16 waves a CU (4096 x 2048 by one token in bf16: 4.8 us against 5.9). Token tiles of 16, or of 32 for more tokens
- * where they leave 32 waves a CU, which then turn levels into floats half as often (16384 x 4096 by 128 tokens: 43 us
- * against 48; 8192 x 4096 by 64, of fewer waves, 22 against 18). For fp32, whose products are three, up to 5 tokens put their planes side by side as 15 rows of a tile, and
- * the products are as many as bf16's (16384 x 4096 by one token: 14.5 us against 16.4). Long rows of a matrix that one
- * token tile meets are loaded in whole lines (65536 x 4096 by 5 tokens: 27.3 us against 30.7; eight gate/up matrices of
- * 4096 x 4096 by one token 16.3 against 17.2); short rows, or rows that further tiles read again, in half lines (64 matrices
- * of 2048 x 1024 by 64 tokens 20.8 against 22.4, 2048 x 2048 by 256 tokens 58 against 70).
+ * 16 waves a CU (4096 x 2048 by one token in bf16, both with LDS: 5.6 us against 8.0). Token tiles of 16, or of 32 for more
+ * tokens where they leave 32 waves a CU, which then turn levels into floats half as often (16384 x 4096 by 128 tokens in
+ * bf16 45.4 us against 48.2, in fp16 44.6 against 50.0; 8192 x 4096 by 64, of fewer waves, 21.7 against 18.5; in fp32, whose
+ * waves take twice the registers then, 8192 x 4096 by 128 in groups of 64 54 against 66, but 16384 x 4096 by 128 90 against
+ * 81 and 64 gate/up experts of 2048 x 2048 by 256 tokens 141 against 100).
+ * For fp32, whose products are three, up to 5 tokens put their planes side by side as 15 rows of a tile, and
+ * the products are as many as bf16's (16384 x 4096 by one token: 11.4 us against 18.0). Long rows of a matrix that one
+ * token tile meets are loaded in whole lines (65536 x 4096 by 5 fp16 tokens: 30.0 us against 33.3; eight gate/up matrices of
+ * 4096 x 4096 by one token 17.0 against 18.5); short rows, or rows that further tiles read again, in half lines (64 matrices
+ * of 2048 x 1024 by 64 tokens 17.9 against 18.4, 8192 x 4096 by 64 18.5 against 18.9).
  * Small matrices, of at most 8 waves a CU that share no activations, load them without LDS, which takes a trip to memory
- * and a barrier out of a call that is little else: 1001 x 2080 by 24 tokens in fp32 7.7 us against 10.5, 4096 x 4096 by 8
- * in bf16 7.6 against 11.0, one expert's 1024 x 1024 by one 4.6 against 5.1; of more waves the caches' rate bounds them
- * (6000 x 4096 by 8 tokens in bf16 10.2 against 7.9). Up to 5 fp32 tokens do so where a wave has at most two chunks
- * (256 x 512 by one 4.5 against 5.0; 4096 x 4096 by one 8.6 against 6.1). */
+ * and a barrier out of a call that is little else: 4096 x 2048 by one token in bf16 4.2 us against 5.6, 1001 x 2080 by 24 in
+ * fp32 7.2 against 10.2, one expert's 1024 x 1024 by one 4.0 against 5.0; of more waves the caches' rate bounds them
+ * (4096 x 4096 by 8 tokens in bf16 6.4 either way, 6000 x 4096 10.2 against 8.0). Up to 5 fp32 tokens do so where a wave has
+ * at most two chunks (256 x 512 by one 3.5 against 4.4; 4096 x 4096 by one 8.6 against 6.5). */
 template <typename E> static int by_tokens(void *y, const void *x, G53W4Args &a)
 {
     constexpr bool F32 = sizeof(E) == 4;
