@@ -14,7 +14,8 @@
  *
  * Both directions are one pass over HBM: W waves hold a token's row in registers, 8 elements a lane
  * (16 for rows above 4096, 32 above 8192), sums go over the lanes and then the waves. The next norm takes h' in fp32,
- * before it is rounded to be stored, and the backward pass forms the same fp32 h' again from h and y.
+ * before it is rounded to be stored, and the backward pass forms that h' again from h and y, with roundings of its own
+ * (a last bit of fp32 may differ).
  * Gradients that tokens share are summed by each workgroup over its tokens in registers, written once
  * and added up by k_norm_sum in a fixed order: no atomics, the same bits on every run.
  *
@@ -22,6 +23,8 @@
  * 4.8 TB/s, backward 4096 x 4096 44 us, 4.6 TB/s with the sums' launch (4 us). A gradient of few tokens is
  * latency: two launches, a workgroup a CU that meets memory, two sums over its waves and one barrier each per
  * token, and as many bytes of partial sums as of two rows a workgroup (1025 x 4096: 14 us and 4, floor 10.6).
+ * Gradients with a block output spill above 4096 wide: 10 to 42 registers up to 8192 (1024 x 8192 bf16: 40 us,
+ * floor 21), 158 to 324 above (512 x 16384: 92, floor 21); without one, 4 in fp32 above 8192 (22, floor 10.6, in bf16).
  */
 #include <hip/hip_runtime.h>
 

@@ -8,7 +8,7 @@
  * expert gives each lane the lanes with the same expert, those below it are its rank. Order never depends on
  * timing. Routings of more than G53_SORT_SEG pairs are cut into segments, counted by k_sort_count first;
  * every workgroup then adds up the counts of all segments. Latency: 2.6 us for 64 pairs and fewer
- * (k_sort_few), 4.9 + 7.8 for 32768 pairs of 288 experts in 16 segments.
+ * (k_sort_few), 4.6 + 7.7 for 32768 pairs of 288 experts in 16 segments, each waited for.
  *
  * k_sorted_dispatch: bytes of rows, 16 a thread; a token's row is read once and written topk times. 4096
  * tokens of 4096 bf16 to 8 experts each, 302 MB: 55 us, 5.5 TB/s, bound by HBM. Written past the caches the
@@ -146,7 +146,7 @@ k_sort_place(int *__restrict__ offsets, int *__restrict__ pair, int *__restrict_
 }
 
 /* Up to 64 pairs: a lane holds a pair's key and meets every other; experts count the keys below them. No LDS, no barrier:
- * one token's 8 pairs of 288 experts in 2.4 us, a launch's own time, against 4.1 by counting. */
+ * one token's 8 pairs of 288 experts in 2.6 us, a launch's own time, against 4.1 by counting. */
 __global__ void __launch_bounds__(256) k_sort_few(int *__restrict__ offsets, int *__restrict__ pair, int *__restrict__ row,
                                                   const int *__restrict__ idx, int n, int NE)
 {

@@ -359,7 +359,8 @@ int g53h_mtile_i4_host(uint8_t *dst_w, float *dst_s, const uint8_t *src_w, const
 
 /* -------------------------------------------------- operators beside the layer ----
  * No counterpart in the reference. What a trunk does around and inside a MoE layer, on the library's
- * stream, so that nothing has to wait between them and g53h_moe: norms before and after the block with
+ * stream, so that nothing has to wait between them and, in fp32, g53h_router and g53h_moe, which take no
+ * other type (a caller of bf16 or fp16 rows converts the layer's x itself): norms before and after the block with
  * its gate and residual, tokens sorted by expert and back, products with 4-bit matrices of any group
  * width; and the gradients of those that a training step differentiates. Pointers are device memory
  * of contiguous rows, aligned to one element; activations are of one of the types below, sums are fp32,
@@ -417,7 +418,8 @@ int g53h_sorted_mm_w4(void *ys_d, const void *x_d, int dt, int gather, const G53
                       float swiglu_limit);
 
 /* xn = x / sqrt(mean of x^2 + eps) * gain per row of hidden <= 16384; gain fp32 [hidden]; eps 1e-30 to
- * 1e30; xn may be x. _grad: dx (may be dxn) and, where it is not NULL, dgain fp32 [hidden], from dxn and x. */
+ * 1e30; xn may be x. Squares are summed in fp32: a row whose sum leaves it gives zeros (|x| of 1e19 / sqrt(hidden)
+ * and more may). _grad: dx (may be dxn) and, where it is not NULL, dgain fp32 [hidden], from dxn and x. */
 int g53h_norm(void *xn_d, const void *x_d, const float *gain_d, int dt, int T, int hidden, float eps);
 int g53h_norm_grad(void *dx_d, float *dgain_d, const void *dxn_d, const void *x_d, const float *gain_d, int dt, int T,
                    int hidden, float eps);
