@@ -9,12 +9,12 @@
  * (16 + z) X comes off, X the group's sum of x: fp32 x = N(1, 1) by weights around 0, 4096 columns, 3e-6
  * of the result's norm off against 1e-7 of q - z and 4e-7 of a plain fp32 sum; 2^13 in one column
  * 1e-4 of the rows in which its level is z, against 1e-7. (65536 x 4096 by 5 fp16 tokens 29.5 us against
- * 28.8, 16384 x 4096 by one in fp32 11.3 against 9.8.) fp16: the level's four bits are the top bits of
- * the mantissa of 2^4, and a packed subtraction takes 16 + z off two levels. fp32 activations enter as
- * three bf16 planes whose sum is the value exactly (8 + 8 + 8 mantissa bits, by truncation), and their
- * levels, since bf16 has no packed subtraction, as four bytes less z, then fp32, whose upper halves are
- * bf16. With bf16 activations levels go as q, two by one conversion of bytes that are e4m3 codes of
- * q 2^-9, and z X comes off, X by one product with ones that all row tiles share: roundings are those of
+ * 28.8, 16384 x 4096 by one in fp32 11.3 against 9.8.) fp16: one conversion takes two levels, as e4m3 codes
+ * of q 2^-9, and one packed subtraction z off them. fp32 activations enter as three bf16 planes whose sum
+ * is the value exactly (8 + 8 + 8 mantissa bits, by truncation), and their levels, since bf16 has no
+ * packed subtraction, as four bytes less z, then fp32, whose upper halves are bf16. With bf16 activations
+ * levels go as q and z X comes off, X by one product with ones that all row tiles share: roundings are
+ * those of
  * sums of (q + z) s |x|, 2^-24 each, below a result that keeps 2^-9 of itself (with 2^13 in one column 1
  * of 150 results is not the nearest bf16, with 16 + q 1 of 70; q - z as with fp32: 65536 x 4096 by one
  * token 33.4 us against 26.7). Products are exact and sums fp32.
@@ -83,27 +83,19 @@ __device__ __forceinline__ g53_v4f g53_mfma(g53_v8h a, g53_v8h b, g53_v4f c)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-/* What takes a zero point z off levels, for g53_w4_levels: in each byte 128 - z (fp32), in each half -(16 + z) as fp16;
- * bf16: -z, which takes it off the sum. */
-template <typename E> __device__ __forceinline__ unsigned g53_w4_zero(unsigned z);
-template <> __device__ __forceinline__ unsigned g53_w4_zero<float>(unsigned z)
+/* What takes a zero point z off levels, for g53_w4_levels: in each byte 128 - z (fp32), in each half -z as fp16; bf16: -z,
+ * which takes it off the sum. */
+template <typename E> __device__ __forceinline__ unsigned g53_w4_zero(unsigned z)
 {
-    return __builtin_amdgcn_perm(0u, 128u - z, 0u);
-}
-template <> __device__ __forceinline__ unsigned g53_w4_zero<g53_f16>(unsigned z)
-{
-    return __builtin_amdgcn_perm(0u, 0xcc00u | z << 6, 0x01000100u);
-}
-template <> __device__ __forceinline__ unsigned g53_w4_zero<g53_bf16>(unsigned z)
-{
-    return __builtin_bit_cast(unsigned, -(float)z);
+    if constexpr (__is_same(E, float)) return __builtin_amdgcn_perm(0u, 128u - z, 0u);
+    if constexpr (__is_same(E, g53_bf16)) return __builtin_bit_cast(unsigned, -(float)z);
+    return __builtin_amdgcn_perm(0u, __builtin_bit_cast(unsigned short, (g53_f16)(short)-(int)z), 0x01000100u);
 }
 
-/* Eight levels (nibbles 0..7 of d) in the order 0 2 1 3 4 6 5 7, or 0 4 1 5 2 6 3 7 for fp16, less their zero point but for
- * bf16. mask picks mantissa bits, one half each; it comes in a vector register, so that and and or are one instruction
- * (which takes one scalar and no literal). */
-template <typename E> __device__ __forceinline__ typename G53W4Type<E>::V g53_w4_levels(unsigned d, unsigned mask, unsigned zero);
-template <> __device__ __forceinline__ g53_v8b g53_w4_levels<float>(unsigned d, unsigned, unsigned zero)
+/* Eight levels (nibbles 0..7 of d) in the order 0 2 1 3 4 6 5 7, less their zero point but for bf16. e4m3 codes 0 to 15,
+ * those below the normal range and the first octave, are multiples of 2^-9, so a conversion takes two levels. */
+template <typename E> __device__ __forceinline__ typename G53W4Type<E>::V g53_w4_levels(unsigned d, unsigned zero);
+template <> __device__ __forceinline__ g53_v8b g53_w4_levels<float>(unsigned d, unsigned zero)
 {
     /* bytes q + 128 - z, no carry between them, then q - z as signed bytes: even levels, odd levels */
     const unsigned even = ((d & 0x0f0f0f0fu) + zero) ^ 0x80808080u, odd = ((d >> 4 & 0x0f0f0f0fu) + zero) ^ 0x80808080u;
@@ -116,53 +108,49 @@ template <> __device__ __forceinline__ g53_v8b g53_w4_levels<float>(unsigned d, 
     }
     return __builtin_bit_cast(g53_v8b, o);
 }
-template <> __device__ __forceinline__ g53_v8b g53_w4_levels<g53_bf16>(unsigned d, unsigned, unsigned)
+template <> __device__ __forceinline__ g53_v8b g53_w4_levels<g53_bf16>(unsigned d, unsigned)
 {
-    /* e4m3 codes 0 to 15 are multiples of 2^-9, those below the normal range and the first octave */
-    const unsigned even = d & 0x0f0f0f0fu, odd = d >> 4 & 0x0f0f0f0fu;
     typedef g53_bf16 V2 __attribute__((ext_vector_type(2)));
-    const V2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false);
-    const V2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true);
+    const unsigned even = d & 0x0f0f0f0fu, odd = d >> 4 & 0x0f0f0f0fu;
+    const V2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false);
+    const V2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false);
+    const V2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true);
+    const V2 e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true);
     return (g53_v8b){a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
 }
-template <> __device__ __forceinline__ g53_v8h g53_w4_levels<g53_f16>(unsigned d, unsigned mask, unsigned zero)
+template <> __device__ __forceinline__ g53_v8h g53_w4_levels<g53_f16>(unsigned d, unsigned zero)
 {
     typedef g53_f16 V2 __attribute__((ext_vector_type(2)));
-    const unsigned o = 0x4c004c00u;                           /* fp16 16.0, mantissa bits 9..6 */
-    g53_v4w v = {((d << 6) & mask) | o, ((d << 2) & mask) | o, ((d >> 2) & mask) | o, ((d >> 6) & mask) | o};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const unsigned w = v[i];
-        v[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(V2, w) + __builtin_bit_cast(V2, zero));
-    }
-    return __builtin_bit_cast(g53_v8h, v);
+    const unsigned even = d & 0x0f0f0f0fu, odd = d >> 4 & 0x0f0f0f0fu;
+    const V2 z = __builtin_bit_cast(V2, zero);
+    const V2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, false) + z;
+    const V2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, false) + z;
+    const V2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, true) + z;
+    const V2 e = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, true) + z;
+    return (g53_v8h){a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
 }
 
-/* Eight activations in the levels' order, as P planes of the products' type. */
-__device__ __forceinline__ void g53_w4_x(g53_v8b (&o)[1], const g53_v4w (&p)[1])
+/* Eight activations in the levels' order, as P planes of the products' type. fp16: where one is not finite, the first pair
+ * takes a NaN, and with it the row's results. (What is 0 times each, summed up: 0, or a NaN whose upper half is one of fp16.
+ * fp32's second plane does it, infinity less itself, and bf16's sum of x.) */
+template <typename V> __device__ __forceinline__ void g53_w4_x(V (&o)[1], const g53_v4w (&p)[1])
 {
     const g53_v4w v = p[0];                                   /* 01 23 45 67 */
-    o[0] = __builtin_bit_cast(g53_v8b, (g53_v4w){__builtin_amdgcn_perm(v[1], v[0], 0x05040100u),
-                                                 __builtin_amdgcn_perm(v[1], v[0], 0x07060302u),
-                                                 __builtin_amdgcn_perm(v[3], v[2], 0x05040100u),
-                                                 __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)});
-}
-/* fp16: where one is not finite, the first pair takes a NaN, and with it the row's results. (What is 0 times each, summed up:
- * 0, or a NaN whose upper half is one of fp16. fp32's second plane does it, infinity less itself, and bf16's sum of x.) */
-__device__ __forceinline__ void g53_w4_x(g53_v8h (&o)[1], const g53_v4w (&p)[1])
-{
-    typedef g53_f16 V2 __attribute__((ext_vector_type(2)));
-    const g53_v4w v = p[0];                                   /* 01 23 45 67 */
-    float none = 0.0f;
+    unsigned none = 0u;
+    if constexpr (__is_same(V, g53_v8h)) {
+        typedef g53_f16 V2 __attribute__((ext_vector_type(2)));
+        float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const unsigned w = v[i];
-        none = __builtin_amdgcn_fdot2(__builtin_bit_cast(V2, w), (V2){0.0f, 0.0f}, none, false);
+        for (int i = 0; i < 4; i++) {
+            const unsigned w = v[i];
+            sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(V2, w), (V2){0.0f, 0.0f}, sum, false);
+        }
+        none = __builtin_bit_cast(unsigned, sum);
     }
-    o[0] = __builtin_bit_cast(g53_v8h, (g53_v4w){__builtin_amdgcn_perm(v[2], v[0], 0x05040100u) | __builtin_bit_cast(unsigned, none),
-                                                 __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
-                                                 __builtin_amdgcn_perm(v[3], v[1], 0x05040100u),
-                                                 __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)});
+    o[0] = __builtin_bit_cast(V, (g53_v4w){__builtin_amdgcn_perm(v[1], v[0], 0x05040100u) | none,
+                                           __builtin_amdgcn_perm(v[1], v[0], 0x07060302u),
+                                           __builtin_amdgcn_perm(v[3], v[2], 0x05040100u),
+                                           __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)});
 }
 __device__ __forceinline__ void g53_w4_x(g53_v8b (&o)[3], const g53_v4w (&p)[2])
 {
@@ -322,8 +310,6 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
     V ones;                             /* bf16: for the sums of x */
 #pragma unroll
     for (int i = 0; i < 8; i++) ones[i] = 1.0f;
-    unsigned mask = 0x03c003c0u;
-    asm volatile("" : "+v"(mask));
     const int units = (a.cols + 128 * UC - 1) / (128 * UC);
 
     /* scales and zero points of a group, as they lie, and as they enter */
@@ -462,7 +448,7 @@ k_w4(E *__restrict__ y, const E *__restrict__ x, const int *__restrict__ offsets
                 }
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                const V lv = g53_w4_levels<E>(d[r][s], mask, zr[r][s]);
+                const V lv = g53_w4_levels<E>(d[r][s], zr[r][s]);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
