@@ -8,7 +8,7 @@
  * expert gives each lane the lanes with the same expert, those below it are its rank. Order never depends on
  * timing. Routings of more than G53_SORT_SEG pairs are cut into segments, counted by k_sort_count first;
  * every workgroup then adds up the counts of all segments. Latency: 2.6 us for 64 pairs and fewer
- * (k_sort_few), 4.6 + 7.7 for 32768 pairs of 288 experts in 16 segments, each waited for.
+ * (k_sort_few), 4.8 + 7.8 for 32768 pairs of 288 experts in 16 segments (9.7 in a row of sorts).
  *
  * k_sorted_dispatch: bytes of rows, 16 a thread; a token's row is read once and written topk times. 4096
  * tokens of 4096 bf16 to 8 experts each, 302 MB: 55 us, 5.5 TB/s, bound by HBM. Written past the caches the
@@ -17,12 +17,12 @@
  * against 25).
  *
  * k_sorted_combine: 8 elements a thread; the rows of a token's pairs are all asked for before the first is
- * added; sums in fp32 in the order of the pairs, rounded once. The same tokens, 302 MB: 67 us, 4.5 TB/s, a
+ * added; sums in fp32 in the order of the pairs, rounded once. The same tokens, 302 MB: 68 us, 4.4 TB/s, a
  * large copy's rate.
  *
  * k_sorted_combine_grad: one wave per pair. Its weight's gradient is one sum over the wave, so nothing is
  * exchanged between waves; the waves of a workgroup mostly share a token, whose gradient row they read from
- * the vector cache. 2048 of these tokens, 285 MB: 63 us, 4.5 TB/s.
+ * the vector cache. 2048 of these tokens, 285 MB: 64 us, 4.5 TB/s.
  */
 #include <hip/hip_runtime.h>
 
