@@ -531,3 +531,24 @@ def test_swiglu_of_a_large_matrix_and_many_tokens(L, T, group, zeros, dt):
     want, tol = swiglu(sums, LIMIT), act_tol(sums, tol, LIMIT)
     close(got[:, 0], want, HALF[dt] * np.abs(want) + TINY[dt] + tol)
     assert np.linalg.norm(got[:, 0] - want) <= (HALF[dt] + 2.0 ** -19) * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_more_tokens_than_one_launch_takes(L, dt):
+    """2^25 tokens and some, whose tiles are more than a launch's threads: copies of 4096 tokens of whole numbers."""
+    say("w4, many tokens", dt)
+    rng = np.random.default_rng(18)
+    T, cols, rows = (1 << 25) + 3 * 4096, 32, 16
+    m = W4(rng, 1, rows, cols, 32, F32, True, exact=True)
+    one = Buf(rng.integers(-2, 3, (4096, cols)).astype(float), dt)
+    x, have = glm53h.DevBuf(one.n // 4096 * T), one.n
+    check(L.g53h_d2d(x.ptr, one.ptr, one.n), "d2d")
+    while have < x.nbytes:
+        more = min(have, x.nbytes - have)
+        check(L.g53h_d2d(x.ptr + have, x.ptr, more), "d2d")
+        have += more
+    want = enc(one.val() @ m.wide[0].T, dt)
+    y = glm53h.DevBuf(want.nbytes // 4096 * T)
+    check(L.g53h_memset(y.ptr, 0xff, y.nbytes), "memset")                    # NaN
+    check(L.g53h_mm_w4(y.ptr, x.ptr, dt, T, C.byref(m.c), 0.0), "w4")
+    assert (y.download(want.dtype).reshape(-1, 4096, rows) == want).all()
