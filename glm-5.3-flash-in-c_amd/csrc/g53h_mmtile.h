@@ -1,0 +1,277 @@
+/* g53h_mmtile.h - tiles of matrix products that stream their operands through LDS, for the products of sorted rows
+ * (g53h_emm.hip) and of microscaled matrices (g53h_mx4.hip).
+ *
+ * A workgroup of WR x WC waves owns a tile of BM x BN results; each of its waves MT x NT tiles of 16 x 16. It takes the
+ * summed dimension in chunks: 128 bytes of every operand row where a row holds the summed elements side by side
+ * ("along": x and W forward), or as many of its rows where they lie across ("across": W for the rows' gradient, both
+ * operands of the matrices'). Either way a chunk is 128 bytes for each of the tile's rows or columns, and moves in
+ * pieces of 16 bytes, 64 a wave and instruction, straight to LDS (global_load_lds) into a ring of slots. The loads are
+ * inline assembly, and waits count them by hand: the compiler would wait for every load to LDS before any LDS read.
+ *
+ * LDS places. Along: row r is 128 bytes, piece u of it at u ^ (r % 8), so the 16 rows that a fragment read meets lie in
+ * all banks. Across: a row of the chunk holds the tile's columns, piece u at u ^ f(k): the rows that a transposing read
+ * (ds_read_b64_tr_b16: 4 rows x 16 columns for 16 lanes) or a read of fp32 columns meets in one go lie in all banks.
+ */
+#ifndef G53H_MMTILE_H
+#define G53H_MMTILE_H
+
+#include <hip/hip_runtime.h>
+
+#include "g53h.h"
+#include "g53h_elem.h"
+
+typedef float g53_v4f_mm __attribute__((ext_vector_type(4)));
+typedef short g53_v4s __attribute__((ext_vector_type(4)));
+typedef g53_v4s __attribute__((address_space(3))) *G53LdsTr;
+
+static __device__ const g53_v4w g53_nothing = {0, 0, 0, 0};     /* what a load behind an operand's end reads */
+
+/* A value every lane reads alike from memory that no kernel of this launch writes: a scalar load. */
+template <class V> __device__ __forceinline__ V g53_uniform_load(const V *p)
+{
+    return *(const __attribute__((address_space(4))) V *)(uintptr_t)p;
+}
+
+/* 16 bytes per lane from p to LDS byte lds + 16 * lane. M0 holds the LDS address and is written ahead of the load. */
+__device__ __forceinline__ void g53_to_lds(const uint8_t *p, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+/* At most n loads of the wave are on their way behind this; then every wave of the workgroup gets here. */
+template <int n> __device__ __forceinline__ void g53_loads_left()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
+}
+__device__ __forceinline__ void g53_meet()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+/* p / topk for a pair number p (below 2^31) by a product: mul = ceil(2^(31 + l) / topk), shift = 31 + l, l = the bits of
+ * topk - 1. */
+struct G53Div {
+    uint32_t mul;
+    int shift;
+};
+static inline G53Div g53_div_of(int d)
+{
+    int l = 0;
+    while ((1 << l) < d) l++;
+    return {(uint32_t)(((1ull << (31 + l)) + (unsigned)d - 1) / (unsigned)d), 31 + l};
+}
+__device__ __forceinline__ int g53_div(int p, G53Div d) { return (int)((uint64_t)(uint32_t)p * d.mul >> d.shift); }
+
+/* Rows [first, last) of expert e: the tile `item / across` in the experts' order, tiles of TM rows; n the tile across.
+ * Items are dealt to the 8 dies in runs of up to 32, about what a die has in work at a time, so that its cache serves a
+ * tile's operands to the others of the run. Within an expert eight tiles of rows go with each tile across. False
+ * where the launch has no item for the workgroup. */
+struct G53Item {
+    int e, first, last, n;
+};
+__device__ __forceinline__ bool g53_tile_item(const int *__restrict__ offsets, int NE, int TM, int across, long wg,
+                                              G53Item &it)
+{
+    const int lane = threadIdx.x & 63, per = (NE + 63) / 64, e0 = lane * per;
+    int n = 0, from = e0 < NE ? offsets[e0] : 0;
+    for (int i = 0, at = from; i < per; i++)
+        if (e0 + i < NE) {
+            const int to = offsets[e0 + i + 1];
+            n += (int)((unsigned)(to - at + TM - 1) / TM);
+            at = to;
+        }
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+    }
+    const long total = (long)__builtin_amdgcn_readlane(incl, 63) * across;
+    const int run = total >= 256 ? 32 : total >= 16 ? (int)(total / 8) : 1;
+    const long i = wg >> 3, item = ((i / run) * 8 + (wg & 7)) * run + i % run;
+    if (item >= total) return false;
+    const unsigned long long in = __ballot((long)incl * across > item);
+    const int l = __builtin_ctzll(in);
+    long left = item - (long)__builtin_amdgcn_readlane(incl - n, l) * across;
+    int first = __builtin_amdgcn_readlane(from, l), last, e = l * per, tiles;
+    for (;; e++) {                      /* lane l's experts: one of them holds the item */
+        last = g53_uniform_load(offsets + e + 1);
+        tiles = (int)((unsigned)(last - first + TM - 1) / TM);
+        if (left < (long)tiles * across) break;
+        left -= (long)tiles * across;
+        first = last;
+    }
+    const long eight = 8l * across;
+    const int g = (int)(left / eight), in_g = (int)(left % eight), of = tiles - 8 * g < 8 ? tiles - 8 * g : 8;
+    const int t = 8 * g + in_g % of;
+    it.n = __builtin_amdgcn_readfirstlane(in_g / of);
+    it.e = __builtin_amdgcn_readfirstlane(e);
+    it.first = __builtin_amdgcn_readfirstlane(first + t * TM);
+    it.last = __builtin_amdgcn_readfirstlane(last - it.first > TM ? it.first + TM : last);
+    return true;
+}
+
+/* Where a lane's 16 bytes of a chunk come from, and how many of them there are (16 and more: all, 0 and less: none). */
+struct G53Piece {
+    const uint8_t *p;
+    long n;
+};
+/* The piece in registers, zeros behind its end, at any alignment of its elements (of type E). */
+template <typename E> __device__ __forceinline__ g53_v4w g53_piece(const G53Piece &s)
+{
+    if (s.n >= 16) return ((const G53v4w_any *)s.p)->v;
+    g53_v4w o = {0, 0, 0, 0};
+    if (s.n > 0) {
+        const E *p = (const E *)s.p;
+        constexpr int N = 16 / sizeof(E);
+        const int n = (int)s.n / (int)sizeof(E);
+        E v[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = i < n ? p[i] : (E)0.0f;
+        __builtin_memcpy(&o, v, 16);
+    }
+    return o;
+}
+
+/* The 16-bit type of the products and the planes of a value. fp32 enters as three bf16 planes, each the rounded rest of
+ * those before it: with 8 bits a plane and at most half a step left by each, the three hold every bit of the value
+ * (above 2^-109; and values that round past bf16's largest, from 3.39e38, count as infinite). Of the nine products
+ * of two values' planes six are taken: the others are below 2^-26 of the value's product together. */
+template <typename E> struct G53Mm;
+template <> struct G53Mm<float> { typedef g53_v8b V; static constexpr int P = 3; };
+template <> struct G53Mm<g53_bf16> { typedef g53_v8b V; static constexpr int P = 1; };
+template <> struct G53Mm<g53_f16> { typedef g53_v8h V; static constexpr int P = 1; };
+
+__device__ __forceinline__ g53_v4f g53_mm(g53_v8b a, g53_v8b b, g53_v4f c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ g53_v4f g53_mm(g53_v8h a, g53_v8h b, g53_v4f c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+template <typename E> struct G53Frag { typename G53Mm<E>::V v[G53Mm<E>::P]; };
+
+__device__ __forceinline__ void g53_planes(G53Frag<float> &o, const float (&v)[8])
+{
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = v[i];
+#pragma unroll
+    for (int p = 0; p < 3; p++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const g53_bf16 h = (g53_bf16)r[i];
+            o.v[p][i] = h;
+            if (p < 2) r[i] -= (float)h;          /* exact */
+        }
+}
+template <typename E> __device__ __forceinline__ g53_v4f g53_mm(const G53Frag<E> &a, const G53Frag<E> &b, g53_v4f c)
+{
+    if constexpr (G53Mm<E>::P == 3) {
+        c = g53_mm(a.v[2], b.v[0], c);
+        c = g53_mm(a.v[1], b.v[1], c);
+        c = g53_mm(a.v[0], b.v[2], c);
+        c = g53_mm(a.v[1], b.v[0], c);
+        c = g53_mm(a.v[0], b.v[1], c);
+        return g53_mm(a.v[0], b.v[0], c);
+    } else {
+        return g53_mm(a.v[0], b.v[0], c);
+    }
+}
+
+/* Fragments of 32 summed elements (lane (m, q) = (lane % 16, lane / 16): row m, elements 8 q .. 8 q + 7) from a chunk
+ * at LDS address `at`, whose rows start at row0 (a multiple of 16), tile t of 16 rows, step j of 32 elements. */
+template <typename E> struct G53Along {
+    int at[2];
+    __device__ __forceinline__ void setup(int row0)
+    {
+        const int m = threadIdx.x & 15, q = threadIdx.x >> 4 & 3;
+        const int u = sizeof(E) == 4 ? 2 * q : q;
+        at[0] = (row0 + m) * 128 + ((u ^ (m & 7)) << 4);
+        at[1] = sizeof(E) == 4 ? (row0 + m) * 128 + (((u + 1) ^ (m & 7)) << 4) : at[0] ^ 64;
+    }
+    __device__ __forceinline__ void read(G53Frag<E> &o, const uint8_t *lds, int t, int j) const
+    {
+        if constexpr (sizeof(E) == 4) {
+            const g53_v4f a = *(const g53_v4f *)(lds + at[0] + t * 2048), b = *(const g53_v4f *)(lds + at[1] + t * 2048);
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { v[i] = a[i]; v[4 + i] = b[i]; }
+            g53_planes(o, v);
+        } else {
+            o.v[0] = *(const typename G53Mm<E>::V *)(lds + at[j] + t * 2048);
+        }
+    }
+};
+/* The same from a chunk of rows of R columns each, whose columns start at col0: NT tiles of 16. */
+template <typename E, int R, int NT> struct G53Across {
+    static constexpr int RB = R * sizeof(E), U = RB / 16;         /* bytes and pieces of a row */
+    int at[NT];
+    static __device__ __forceinline__ int place(int k)
+    {
+        return (sizeof(E) == 4 ? 4 * (k >> 3 & 3) : 2 * ((k & 3) | (k >> 3 & 1) << 2)) & (U - 1);
+    }
+    __device__ __forceinline__ void setup(int col0)
+    {
+        const int m = threadIdx.x & 15, q = threadIdx.x >> 4 & 3;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int c = col0 + 16 * t;
+            if (sizeof(E) == 4) {
+                const int k = 8 * q, u = (c + m) >> 2;
+                at[t] = k * RB + ((u ^ place(k)) << 4) + (m & 3) * 4;
+            } else {
+                const int k = 8 * q + (m >> 2), u = (c >> 3) + (m >> 1 & 1);
+                at[t] = k * RB + ((u ^ place(k)) << 4) + (m & 1) * 8;
+            }
+        }
+    }
+    __device__ __forceinline__ void read(G53Frag<E> &o, const uint8_t *lds, int t, int j) const
+    {
+        if constexpr (sizeof(E) == 4) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = *(const float *)(lds + at[t] + i * RB);
+            g53_planes(o, v);
+        } else {
+            const g53_v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((G53LdsTr)(lds + at[t] + j * 32 * RB));
+            const g53_v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((G53LdsTr)(lds + at[t] + (j * 32 + 4) * RB));
+            o.v[0] = __builtin_bit_cast(typename G53Mm<E>::V, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+/* Four neighbours of a row, those below `n` columns of them; rounded once. old: added to what is there. */
+template <typename O> __device__ __forceinline__ void g53_store4(O *row, long c, long n, g53_v4f v, bool old)
+{
+    typedef O V4 __attribute__((ext_vector_type(4)));
+    struct __attribute__((packed, aligned(2))) Any { V4 v; };
+    if (c + 4 <= n) {
+        V4 o;
+        if (old) {
+            const V4 was = ((const Any *)(row + c))->v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] += (float)was[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = (O)v[i];
+        ((Any *)(row + c))->v = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (c + i < n) row[c + i] = (O)(old ? v[i] + (float)row[c + i] : v[i]);
+    }
+}
+
+/* The clamped SwiGLU, as g53h_swiglu's. */
+__device__ __forceinline__ float g53_swiglu1(float g, float u, float limit)
+{
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : (u < -limit ? -limit : u);
+    return g / (1.0f + expf(-g)) * u;
+}
+
+#endif /* G53H_MMTILE_H */

@@ -266,6 +266,11 @@ _SIGS = {
     "g53h_mm_w4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hW4), C.c_float]),
     "g53h_sorted_mm_w4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hSort), C.POINTER(G53hW4),
                                     C.c_float]),
+    "g53h_sorted_mm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hSort), C.c_void_p, C.c_int,
+                                 C.c_int, C.c_float]),
+    "g53h_sorted_mm_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                      C.POINTER(G53hSort), C.c_void_p, C.c_int, C.c_int]),
+    "g53h_sorted_swiglu_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hSort), C.c_float]),
     "g53h_norm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float]),
     "g53h_norm_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                  C.c_float]),

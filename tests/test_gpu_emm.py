@@ -1,0 +1,259 @@
+"""Products of sorted rows with their experts' matrices, and their gradients, against 64 bits on the host: whole numbers,
+whose sums are exact in fp32, to the bit, and normal values within the roundings of their sums."""
+import numpy as np
+import pytest
+
+import glm53h
+from glm53h import DevBuf, check
+from op_lib import BF16, F16, F32, HALF, TINY, Buf, Plan, close, dec, enc, routing, sorted_plan, swiglu
+from test_gpu_parity import say
+
+pytestmark = pytest.mark.gpu
+LIMIT = 2.0
+
+
+@pytest.fixture(scope="module")
+def L():
+    return glm53h.init(0)
+
+
+def rounded(a, dt):
+    return dec(enc(a, dt), dt)
+
+
+def values(rng, shape, dt, whole, scale=1.0):
+    """Whole numbers of -3 to 3, or normal values of the type."""
+    return rng.integers(-3, 4, shape).astype(np.float64) if whole else rounded(scale * rng.standard_normal(shape), dt)
+
+
+def off(n, size, y, dt, whole, limit_slope=1.0):
+    """What sums of n products in fp32, in any order, and the rounding to the type may be off by: every addition at
+    most 2^-23 (a matrix core may cut instead of rounding) of the sum of the sizes; fp32 values' products 2^-24 each
+    besides (2^-26 left out by the planes, doubled for the two roundings of planes)."""
+    if whole:
+        return HALF[dt] * np.abs(y) + TINY[dt]
+    return limit_slope * (n + 32 + 6 * n / 32) * 2.0 ** -23 * size + HALF[dt] * np.abs(y) + TINY[dt]
+
+
+# (T, K, NE, rows, cols): single tokens, tiles cut in every way, odd sizes, experts without rows, one that takes all
+SIZES = [(1, 1, 1, 1, 1), (1, 4, 16, 64, 64), (5, 2, 3, 30, 40), (33, 3, 7, 130, 72), (70, 1, 1, 258, 200), (129, 2, 4, 136, 8),
+         (64, 4, 300, 48, 96), (300, 2, 2, 66, 333), (17, 2, 5, 514, 301)]
+
+
+def cases():
+    for i, s in enumerate(SIZES):
+        for dt in (BF16, F16, F32):
+            yield s + (dt, i % 2, (i // 2 + dt) % 2, (i + dt) % 3 == 0)
+
+
+@pytest.mark.parametrize("T,K,NE,rows,cols,dt,gather,sw,shifted", cases())
+def test_forward(L, T, K, NE, rows, cols, dt, gather, sw, shifted):
+    say("forward", T, K, NE, rows, cols, dt, gather, sw, shifted)
+    rng = np.random.default_rng(T + rows)
+    rows += rows % 2 if sw else 0
+    idx = routing(rng, T, K, NE, 0.2)
+    idx[rng.random((T, K)) < 0.1] = NE                       # outside
+    offsets, pair, _ = sorted_plan(idx, NE)
+    n, used, out = T * K, offsets[NE], rows // 2 if sw else rows
+    shift = (2 if dt != F32 else 4) if shifted else 0
+    plan = Plan(idx, NE)
+    for whole in (True, False):
+        xv = values(rng, (T if gather else n, cols), dt, whole)
+        wv = values(rng, (NE, rows, cols), dt, whole, 0.1)
+        x, w = Buf(xv, dt, shift), Buf(wv, dt, shift)
+        ys, gu = Buf.out((n, out), dt, shift), Buf.out((n, rows), dt, shift)
+        check(L.g53h_sorted_mm(ys.ptr, gu.ptr if sw else None, x.ptr, dt, gather, plan.c, w.ptr, rows, cols, LIMIT if sw else 0.0))
+        ref, size, act = np.full((n, rows), 77.0), np.zeros((n, rows)), np.full((n, out), 77.0)
+        for e in range(NE):
+            r = slice(offsets[e], offsets[e + 1])
+            xe = xv[pair[r] // K] if gather else xv[r]
+            ref[r], size[r] = xe @ wv[e].T, np.abs(xe) @ np.abs(wv[e]).T
+        tol = off(cols, size, ref, dt, whole)
+        tol[used:] = 0
+        if not sw:
+            close(ys.val(), ref, tol, whole)
+            continue
+        close(gu.val(), ref, tol, ("gu", whole))
+        act[:used] = swiglu(ref[:used], LIMIT)
+        # |d silu| <= 1.1 and |up| <= limit, |silu| <= limit and slope 1: sums of both; expf and the division 4 steps
+        sums = off(cols, size, ref, F32, whole)
+        ta = np.zeros((n, out))
+        ta[:used] = (1.1 * LIMIT * (sums[:used, :out] + sums[:used, out:]) + (4 * 2.0 ** -23 + HALF[dt]) * np.abs(act[:used]) + TINY[dt]) * 1.01
+        close(ys.val(), act, ta, ("act", whole))
+
+
+@pytest.mark.parametrize("T,K,NE,rows,cols,dt,gather,w32,shifted", cases())
+def test_gradients(L, T, K, NE, rows, cols, dt, gather, w32, shifted):
+    say("gradients", T, K, NE, rows, cols, dt, gather, w32, shifted)
+    rng = np.random.default_rng(T + cols)
+    idx = routing(rng, T, K, NE, 0.2)
+    if NE > 1:
+        idx[idx == 1] = -1                                   # an expert without rows
+    offsets, pair, _ = sorted_plan(idx, NE)
+    n, used, wt = T * K, offsets[NE], F32 if w32 else dt
+    shift = (2 if dt != F32 else 4) if shifted else 0
+    plan = Plan(idx, NE)
+    for whole in (True, False):
+        xv = values(rng, (T if gather else n, cols), dt, whole)
+        wv, dv = values(rng, (NE, rows, cols), dt, whole, 0.1), values(rng, (n, rows), dt, whole)
+        old = values(rng, (NE, rows, cols), wt, whole)
+        x, w, d = Buf(xv, dt, shift), Buf(wv, dt, shift), Buf(dv, dt, shift)
+        dx, dw, da = Buf.out((n, cols), dt, shift), Buf.out((NE, rows, cols), wt), Buf(old, wt)
+        check(L.g53h_sorted_mm_grad(dx.ptr, dw.ptr, wt, 0, d.ptr, x.ptr, dt, gather, plan.c, w.ptr, rows, cols))
+        check(L.g53h_sorted_mm_grad(None, da.ptr, wt, 1, d.ptr, x.ptr, dt, gather, plan.c, None, rows, cols))
+        rx, sx = np.full((n, cols), 77.0), np.zeros((n, cols))
+        rw, sz, many = np.zeros((NE, rows, cols)), np.zeros((NE, rows, cols)), np.zeros((NE, 1, 1))
+        for e in range(NE):
+            r = slice(offsets[e], offsets[e + 1])
+            xe = xv[pair[r] // K] if gather else xv[r]
+            rx[r], sx[r] = dv[r] @ wv[e], np.abs(dv[r]) @ np.abs(wv[e])
+            rw[e], sz[e], many[e] = dv[r].T @ xe, np.abs(dv[r]).T @ np.abs(xe), r.stop - r.start
+        tol = off(rows, sx, rx, dt, whole)
+        tol[used:] = 0
+        close(dx.val(), rx, tol, ("dx", whole))
+        close(dw.val(), rw, off(many, sz, rw, wt, whole), ("dw", whole))
+        close(da.val(), old + rw, off(many + 1, sz + np.abs(old), old + rw, wt, whole), ("added", whole))
+        again = Buf.out((n, cols), dt, shift)
+        check(L.g53h_sorted_mm_grad(again.ptr, None, wt, 0, d.ptr, None, dt, gather, plan.c, w.ptr, rows, cols))
+        assert np.array_equal(again.get(), dx.get())
+
+
+@pytest.mark.parametrize("T,K,inter,dt", [(1, 1, 1, F32), (5, 2, 33, BF16), (9, 3, 2056, F16), (30, 4, 128, F32), (7, 1, 4099, BF16)])
+def test_swiglu_grad(L, T, K, inter, dt):
+    say("swiglu_grad", T, K, inter, dt)
+    rng = np.random.default_rng(inter)
+    NE, n = 6, T * K
+    idx = routing(rng, T, K, NE, 0.2)
+    idx[0, 0] = 1
+    used = sorted_plan(idx, NE)[0][NE]
+    gv = rounded(2.0 * rng.standard_normal((n, 2 * inter)), dt)
+    gv[0, :: max(1, inter // 7)] = LIMIT                     # at the limit: inside
+    gv[n // 2, inter:] = -LIMIT
+    gv[n - 1, 0] = -100.0                                    # exp of it overflows
+    dv = rounded(rng.standard_normal((n, inter)), dt)
+    gu, d, plan = Buf(gv, dt), Buf(dv, dt), Plan(idx, NE)
+    out = Buf.out((n, 2 * inter), dt)
+    check(L.g53h_sorted_swiglu_grad(out.ptr, d.ptr, gu.ptr, dt, inter, plan.c, LIMIT))
+    g, u = gv[:, :inter], gv[:, inter:]
+    gc, uc = np.minimum(g, LIMIT), np.clip(u, -LIMIT, LIMIT)
+    s = 1.0 / (1.0 + np.exp(-gc))
+    want = np.concatenate([np.where(g <= LIMIT, dv * uc * s * (1 + gc * (1 - s)), 0),
+                           np.where(np.abs(u) <= LIMIT, dv * gc * s, 0)], 1)
+    # ten operations of half a step each; 1 - s and 1 + gc (1 - s) are off by steps of their parts
+    size = np.concatenate([np.abs(dv * uc) * s * (1 + np.abs(gc)), np.abs(dv * gc) * s], 1)
+    # below 2^-126 fp32 has steps of 2^-149: s, formed by an exponential and a division, is off by half of one each, and
+    # enters as s d u (1 + g) and s d g
+    deep = 2.0 ** -149 * np.concatenate([np.abs(dv * uc) * (1 + np.abs(gc)), np.abs(dv * gc)], 1)
+    tol = 16 * 2.0 ** -24 * size + deep + HALF[dt] * np.abs(want) + TINY[dt]
+    want[used:], tol[used:] = 77.0, 0
+    close(out.val(), want, tol)
+    check(L.g53h_sorted_swiglu_grad(gu.ptr, d.ptr, gu.ptr, dt, inter, plan.c, LIMIT))      # in place
+    assert np.array_equal(gu.get()[:used], out.get()[:used]) and np.array_equal(gu.get()[used:], enc(gv, dt)[used:])
+    # against differences, away from the limits
+    e = 1e-6
+    f = lambda v: swiglu(v, LIMIT)                           # noqa: E731
+    near = np.abs(np.abs(gv) - LIMIT) < 1e-4
+    for half in (0, 1):
+        step = np.zeros_like(gv)
+        step[:, half * inter:(half + 1) * inter] = e
+        diff = dv * (f(gv + step) - f(gv - step)) / (2 * e)
+        part = slice(half * inter, (half + 1) * inter)
+        ok = ~near[:used, part]
+        assert (np.abs(diff[:used] - want[:used, part])[ok] <= 1e-8 * (1 + np.abs(dv[:used])[ok]) * 8).all()
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+def test_values_that_are_not_finite_stay_in_their_rows(L, dt):
+    say("not finite", dt)
+    rng = np.random.default_rng(3)
+    T, NE, rows, cols = 40, 3, 70, 96
+    idx = routing(rng, T, 1, NE)
+    offsets, pair, row = sorted_plan(idx, NE)
+    xv, wv = values(rng, (T, cols), dt, True), values(rng, (NE, rows, cols), dt, True)
+    dv = values(rng, (T, rows), dt, True)
+    xv[7, 3], xv[20, 95], dv[row[7], 5] = np.inf, np.nan, np.nan
+    x, w, d, plan = Buf(xv, dt), Buf(wv, dt), Buf(dv, dt), Plan(idx, NE)
+    ys, dx = Buf.out((T, rows), dt), Buf.out((T, cols), dt)
+    check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, dt, 1, plan.c, w.ptr, rows, cols, 0.0))
+    check(L.g53h_sorted_mm_grad(dx.ptr, None, dt, 0, d.ptr, None, dt, 1, plan.c, w.ptr, rows, cols))
+    y, g = ys.val(), dx.val()
+    for r in range(T):
+        t = pair[r]
+        e = idx[t, 0]
+        if t in (7, 20):
+            assert not np.isfinite(y[r][wv[e][:, 3 if t == 7 else 95] != 0]).any()
+        else:
+            assert np.array_equal(y[r], rounded(wv[e] @ xv[t], dt))
+        if t == 7:
+            assert np.isnan(g[r]).all()
+        else:
+            assert np.array_equal(g[r], rounded(dv[r] @ wv[e], dt))
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+def test_nothing_to_do(L, dt):
+    say("nothing", dt)
+    rows, cols, NE = 40, 24, 4
+    w = Buf(np.ones((NE, rows, cols)), dt)
+    dw = Buf.out((NE, rows, cols), dt)
+    plan = Plan(np.full((3, 2), -1, np.int32), NE)           # no pair has an expert
+    x, ys, d = Buf(np.full((3, cols), np.nan), dt), Buf.out((6, rows), dt), Buf(np.full((6, rows), np.nan), dt)
+    dx = Buf.out((6, cols), dt)
+    check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, dt, 1, plan.c, w.ptr, rows, cols, 0.0))
+    check(L.g53h_sorted_mm_grad(dx.ptr, dw.ptr, dt, 0, d.ptr, x.ptr, dt, 1, plan.c, w.ptr, rows, cols))
+    assert (ys.val() == 77).all() and (dx.val() == 77).all() and (dw.val() == 0).all()
+    none = Plan(np.zeros((0, 2), np.int32), NE)              # no tokens at all
+    dw = Buf.out((NE, rows, cols), dt)
+    check(L.g53h_sorted_mm(None, None, None, dt, 1, none.c, None, rows, cols, 0.0))
+    check(L.g53h_sorted_swiglu_grad(None, None, None, dt, rows // 2, none.c, 1.0))
+    check(L.g53h_sorted_mm_grad(None, dw.ptr, dt, 0, None, None, dt, 1, none.c, None, rows, cols))
+    assert (dw.val() == 0).all()
+    check(L.g53h_sorted_mm_grad(None, dw.ptr, dt, 1, None, None, dt, 1, none.c, None, rows, cols))
+    assert (dw.val() == 0).all()
+
+
+def test_offsets_past_32_bits(L):
+    """Results and matrices whose bytes and elements pass 2^32: the last ones are right."""
+    say("large")
+    rng = np.random.default_rng(5)
+    T, K, NE, rows, cols = 70000, 8, 2, 8000, 64             # ys: 4.48e9 elements
+    n = T * K
+    idx = np.tile(np.array([0, 0, 0, 0, 1, 1, 1, 1], np.int32), (T, 1))
+    xv, wv = values(rng, (T, cols), BF16, True), values(rng, (NE, rows, cols), BF16, True)
+    x, w, plan = Buf(xv, BF16), Buf(wv, BF16), Plan(idx, NE)
+    ys = DevBuf(2 * n * rows)
+    check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, BF16, 1, plan.c, w.ptr, rows, cols, 0.0))
+    offsets, pair, _ = sorted_plan(idx, NE)
+    for r in (0, n // 2 - 1, n // 2, (1 << 32) // rows, (1 << 31) // rows, n - 1):
+        got = dec(ys.download(np.uint16, rows, 2 * r * rows), BF16)
+        assert np.array_equal(got, rounded(wv[int(r >= n // 2)] @ xv[pair[r] // K], BF16)), r
+    # the rows' gradient reads them again: of the last rows, whole numbers once more
+    last = values(rng, (8, rows), BF16, True)
+    L.g53h_memset(ys.ptr, 0, ys.nbytes)
+    bits = enc(last, BF16)
+    check(L.g53h_h2d(ys.ptr + 2 * (n - 8) * rows, bits.ctypes.data, bits.nbytes))
+    dx, dw = DevBuf(2 * n * cols), Buf.out((NE, rows, cols), F32)
+    check(L.g53h_sorted_mm_grad(dx.ptr, dw.ptr, F32, 0, ys.ptr, x.ptr, BF16, 1, plan.c, w.ptr, rows, cols))
+    got = dec(dx.download(np.uint16, 8 * cols, 2 * (n - 8) * cols), BF16).reshape(8, cols)
+    assert np.array_equal(got, rounded(last @ wv[1], BF16))
+    assert np.array_equal(dw.val()[1], last.T @ xv[pair[n - 8:] // K]) and not dw.val()[0].any()
+
+
+def test_matrices_past_32_bits(L):
+    say("large matrices")
+    rng = np.random.default_rng(6)
+    NE, rows, cols, T = 20, 8192, 16400, 3                   # 2.7e9 elements, 5.4e9 bytes
+    one = values(rng, (rows, cols), F16, True)
+    w = DevBuf(2 * NE * rows * cols)
+    bits = enc(one, F16)
+    check(L.g53h_h2d(w.ptr + 2 * (NE - 1) * rows * cols, bits.ctypes.data, bits.nbytes))
+    idx = np.full((T, 1), NE - 1, np.int32)
+    xv, dv, plan = values(rng, (T, cols), F16, True), values(rng, (T, rows), F16, True), Plan(idx, NE)
+    x, d, ys, dx = Buf(xv, F16), Buf(dv, F16), Buf.out((T, rows), F16), Buf.out((T, cols), F16)
+    check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, F16, 1, plan.c, w.ptr, rows, cols, 0.0))
+    check(L.g53h_sorted_mm_grad(dx.ptr, None, F16, 0, d.ptr, None, F16, 1, plan.c, w.ptr, rows, cols))
+    assert np.array_equal(ys.val(), rounded(xv @ one.T, F16)) and np.array_equal(dx.val(), rounded(dv @ one, F16))
+    check(L.g53h_sorted_mm_grad(None, w.ptr, F16, 0, d.ptr, x.ptr, F16, 1, plan.c, None, rows, cols))
+    at = (NE - 1) * rows * cols
+    assert np.array_equal(dec(w.download(np.float16, rows * cols, 2 * at), F16).reshape(rows, cols), dv.T @ xv)
+    assert not w.download(np.uint16, 1 << 20, 2 * (at - (1 << 20))).any()

@@ -114,3 +114,38 @@ def test_struct_sizes():
     assert C.sizeof(glm53h.G53hSort) == 40
     assert C.sizeof(glm53h.G53hW4) == 40
     assert C.sizeof(glm53h.G53hBlockNorm) == 48
+
+
+@pytest.mark.parametrize("bad", [dict(T=-1), dict(topk=0), dict(topk=65), dict(NE=0), dict(NE=1025), dict(T=1 << 28, topk=8),
+                                 dict(offsets=None), dict(pair=None)])
+def test_expert_products_plans(L, bad):
+    refused(L, L.g53h_sorted_mm(P, None, P, 1, 0, plan(**bad), P, 8, 8, 0.0), "g53h_sorted_mm", "plan")
+    refused(L, L.g53h_sorted_mm_grad(P, P, 0, 0, P, P, 1, 0, plan(**bad), P, 8, 8), "g53h_sorted_mm_grad", "plan")
+    refused(L, L.g53h_sorted_swiglu_grad(P, P, P, 1, 8, plan(**bad), 1.0), "g53h_sorted_swiglu_grad", "plan")
+
+
+def test_expert_products(L):
+    for dt in (-1, 3):
+        refused(L, L.g53h_sorted_mm(P, None, P, dt, 0, plan(), P, 8, 8, 0.0), "element type")
+        refused(L, L.g53h_sorted_mm_grad(P, P, 0, 0, P, P, dt, 0, plan(), P, 8, 8), "element type")
+        refused(L, L.g53h_sorted_swiglu_grad(P, P, P, dt, 8, plan(), 1.0), "element type")
+    for rows, cols in ((0, 8), (8, 0), (-8, 8), ((1 << 24) + 1, 8), (8, (1 << 24) + 1)):
+        refused(L, L.g53h_sorted_mm(P, None, P, 1, 0, plan(), P, rows, cols, 0.0), "matrices")
+        refused(L, L.g53h_sorted_mm_grad(P, P, 0, 0, P, P, 1, 0, plan(), P, rows, cols), "matrices")
+    for limit in (-1.0, float("nan"), float("inf")):
+        refused(L, L.g53h_sorted_mm(P, None, P, 1, 0, plan(), P, 8, 8, limit), "limit")
+        refused(L, L.g53h_sorted_swiglu_grad(P, P, P, 1, 8, plan(), limit), "limit")
+    refused(L, L.g53h_sorted_swiglu_grad(P, P, P, 1, 8, plan(), 0.0), "limit")
+    refused(L, L.g53h_sorted_swiglu_grad(P, P, P, 1, 0, plan(), 1.0), "matrices")
+    refused(L, L.g53h_sorted_mm(P, None, P, 1, 0, plan(), P, 7, 8, 1.0), "SwiGLU")
+    refused(L, L.g53h_sorted_mm(P, P, P, 1, 0, plan(), P, 8, 8, 0.0), "without SwiGLU")
+    refused(L, L.g53h_sorted_mm(None, None, P, 1, 0, plan(), P, 8, 8, 0.0), "no rows")
+    refused(L, L.g53h_sorted_mm(P, None, P, 1, 0, plan(), None, 8, 8, 0.0), "no matrices")
+    refused(L, L.g53h_sorted_mm(P, None, P + 1, 1, 0, plan(), P, 8, 8, 0.0), "multiples of an element")
+    refused(L, L.g53h_sorted_mm_grad(None, None, 0, 0, P, P, 1, 0, plan(), P, 8, 8), "neither")
+    refused(L, L.g53h_sorted_mm_grad(P, P, 2, 0, P, P, 1, 0, plan(), P, 8, 8), "of type 2")
+    refused(L, L.g53h_sorted_mm_grad(P, None, 0, 0, None, P, 1, 0, plan(), P, 8, 8), "no rows")
+    refused(L, L.g53h_sorted_mm_grad(P, None, 0, 0, P, P, 1, 0, plan(), None, 8, 8), "no matrices")
+    refused(L, L.g53h_sorted_mm_grad(None, P, 0, 0, P, None, 1, 0, plan(), P, 8, 8), "no rows")
+    refused(L, L.g53h_sorted_mm_grad(None, P + 2, 0, 0, P, P, 1, 0, plan(), P, 8, 8), "multiples of an element")
+    refused(L, L.g53h_sorted_swiglu_grad(P, None, P, 1, 8, plan(), 1.0), "no rows")
