@@ -1,0 +1,382 @@
+/* g53h_mx4.hip - microscaled 4-bit matrices: E2M1 levels with one power of two for 32 columns of a row, the block format of
+ * the scaled matrix instructions. Quantisation of rows and back, and products of two such matrices, of one matrix
+ * (g53h_mm_mx4) or of the matrix of each sorted row's expert (g53h_sorted_mm_mx4).
+ *
+ *     y[t][r] = sum over blocks b of  2^(xs[t][b] + s[r][b] - 254) * sum over c in b of xq[t][c] q[r][c]
+ *
+ * Levels and scales go to v_mfma_scale_f32_16x16x128_f8f6f4 as they lie: lane (m, q) takes the 32 levels, 16 bytes, of
+ * row m and block q of four, and their scale. Products and scales are exact; sums are fp32.
+ */
+#include <hip/hip_runtime.h>
+
+#include "g53h.h"
+#include "g53h_elem.h"
+#include "g53h_mmtile.h"
+#include "g53h_runtime.h"
+
+#define G53_MX_MAXE 1024
+#define G53_MX_MAXC (1 << 24)
+#define G53_MX_WGS (1l << 22)           /* workgroups of a launch: its threads are counted in 32 bits */
+
+typedef int g53_v8i __attribute__((ext_vector_type(8)));
+struct __attribute__((packed, aligned(1))) G53v4w_byte { g53_v4w v; };
+
+/* ---------------------------------------------------------------- quantisation ---- */
+/* Eight columns a lane, a block in four: its largest size by DPP, the scale's exponent that of the largest value less 2
+ * (6 is 1.5 * 2^2), so that levels reach 4 to 8 and those above 6 count as 6. A block with a value that is not finite has
+ * the scale 255, NaN, and levels of zero. */
+template <typename E>
+__global__ void __launch_bounds__(256) k_mx4_quant(uint8_t *__restrict__ w, uint8_t *__restrict__ s, const E *__restrict__ x,
+                                                   long eights, long wg0)
+{
+    const long i = (wg0 + blockIdx.x) * 256 + threadIdx.x;      /* rows are whole blocks: one run of eights */
+    if (i >= eights) return;
+    float v[8];
+    g53_load8(v, x + i * 8);
+    unsigned top = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const unsigned u = __builtin_bit_cast(unsigned, v[k]) & 0x7fffffffu;
+        top = u > top ? u : top;
+    }
+    unsigned o = __builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true);      /* lane ^ 1 */
+    top = o > top ? o : top;
+    o = __builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true);               /* lane ^ 2 */
+    top = o > top ? o : top;
+    const int e = (int)(top >> 23);
+    const int b = e == 255 ? 255 : e > 2 ? e - 2 : 0;
+    /* by 2^(127 - b), exactly: levels */
+    const float up = __builtin_bit_cast(float, (unsigned)(254 - b) << 23);
+    unsigned q = 0;
+#define G53_PAIR(k) q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[2 * k] * up, v[2 * k + 1] * up, 1.0f, k)
+    G53_PAIR(0); G53_PAIR(1); G53_PAIR(2); G53_PAIR(3);
+#undef G53_PAIR
+    if (b == 255) q = 0;
+    ((unsigned *)w)[i] = q;
+    if (!(threadIdx.x & 3)) s[i >> 2] = (uint8_t)b;
+}
+
+template <typename E>
+__global__ void __launch_bounds__(256) k_mx4_dequant(E *__restrict__ x, const uint8_t *__restrict__ w, const uint8_t *__restrict__ s,
+                                                     long eights, long wg0)
+{
+    const long i = (wg0 + blockIdx.x) * 256 + threadIdx.x;
+    if (i >= eights) return;
+    const unsigned q = ((const unsigned *)w)[i], b = s[i >> 2];
+    const float up = __builtin_bit_cast(float, b == 0 ? 1u << 22 : b == 255 ? 0x7fc00000u : b << 23);
+    float v[8];
+#define G53_PAIR(k)                                                                       \
+    do {                                                                                  \
+        const auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, k);              \
+        v[2 * k] = p[0] * up;                                                             \
+        v[2 * k + 1] = p[1] * up;                                                         \
+    } while (0)
+    G53_PAIR(0); G53_PAIR(1); G53_PAIR(2); G53_PAIR(3);
+#undef G53_PAIR
+    g53_store8(x + i * 8, v);
+}
+
+/* -------------------------------------------------------------------- products ---- */
+struct G53MxArgs {
+    const uint8_t *x, *xs;              /* levels [T][cols / 2] and scales [T][cols / 32] */
+    const uint8_t *w, *s;               /* [NE][rows][cols / 2], [NE][rows][cols / 32]     */
+    const int *offsets, *pair;          /* NULL: one matrix; x is sorted rows              */
+    void *out;
+    int NE, T, rows, cols, half;
+    float limit;
+    int across;
+    G53Div topk;
+    long wg0;
+};
+
+/* One tile: 256 columns a chunk, the scales of two chunks a time. */
+template <typename E, int WR, int WC, int MT, int NT, int NS>
+__global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
+{
+    constexpr int NW = WR * WC, BM = 16 * MT * WR, BN = 16 * NT * WC, SLOT = (BM + BN) * 128, SEG = (BM + BN) * 16;
+    constexpr int IA = BM / (8 * NW), IB = BN / (8 * NW), IS = (BM + BN + 64 * NW - 1) / (64 * NW);
+    static_assert(IA * 8 * NW == BM && IB * 8 * NW == BN && NS == 2, "whole instructions");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wv / WC, wc = wv % WC;
+    const bool sw = a.limit > 0.0f;
+    const int cut = sw ? BN / 2 : BN;
+    G53Item it;
+    const long wg = a.wg0 + blockIdx.x;
+    if (a.offsets) {
+        if (!g53_tile_item(a.offsets, a.NE, BM, a.across, wg, it)) return;
+    } else {
+        const long item = wg / a.across;
+        if (item * BM >= a.T) return;
+        it.e = 0;
+        it.n = (int)(wg % a.across);
+        it.first = (int)(item * BM);
+        it.last = a.T - it.first > BM ? it.first + BM : a.T;
+    }
+    const int n0 = it.n * cut, live = it.last - it.first, rb = a.cols / 2, sb = a.cols / 32;
+    const int chunks = (rb + 127) / 128, segs = (chunks + 1) / 2;
+    const long e0 = (long)it.e * a.rows;
+    auto x_row = [&](int r) -> long {
+        const int s = it.first + (r < live ? r : live - 1);
+        return a.pair ? g53_div(a.pair[s], a.topk) : s;
+    };
+    auto w_row = [&](int r) -> long {
+        int at = n0 + r, up = 0;
+        if (sw) {                       /* a wave's first half of tiles: gate, the others: up */
+            const int t = r / 16 % NT;
+            up = t >= NT / 2;
+            at = n0 + r / (16 * NT) * (8 * NT) + (up ? t - NT / 2 : t) * 16 + r % 16;
+        }
+        at = at < a.half ? at : a.half - 1;
+        return e0 + at + (up ? a.half : 0);
+    };
+    const int u8 = (lane & 7) ^ (lane >> 3);
+    const uint8_t *pa[IA], *pb[IB], *ps[IS];
+#pragma unroll
+    for (int i = 0; i < IA; i++) pa[i] = a.x + x_row((i * NW + wv) * 8 + (lane >> 3)) * rb + u8 * 16;
+#pragma unroll
+    for (int i = 0; i < IB; i++) pb[i] = a.w + w_row((i * NW + wv) * 8 + (lane >> 3)) * rb + u8 * 16;
+#pragma unroll
+    for (int i = 0; i < IS; i++) {
+        const int r = i * 64 * NW + tid;
+        ps[i] = r < BM ? a.xs + x_row(r) * sb : a.s + w_row(r - BM < BN ? r - BM : BN - 1) * sb;
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    auto ask = [&](int c, int slot) {
+        const uint32_t to = lds0 + slot * SLOT + wv * 1024;
+        const bool in = c * 128 + u8 * 16 < rb;
+#pragma unroll
+        for (int i = 0; i < IA; i++) g53_to_lds(in ? pa[i] + (long)c * 128 : (const uint8_t *)&g53_nothing, to + i * NW * 1024);
+#pragma unroll
+        for (int i = 0; i < IB; i++)
+            g53_to_lds(in ? pb[i] + (long)c * 128 : (const uint8_t *)&g53_nothing, to + BM * 128 + i * NW * 1024);
+    };
+    /* A row's 16 scales of a segment, each quarter's four side by side. */
+    g53_v4w rs[IS];
+    auto fetch = [&](int seg) {
+        const int n = sb - seg * 16;
+#pragma unroll
+        for (int i = 0; i < IS; i++) {
+            const uint8_t *p = ps[i] + (long)seg * 16;
+            if (n >= 16) rs[i] = ((const G53v4w_byte *)p)->v;
+            else
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    unsigned v = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v |= 4 * k + j < n ? (unsigned)p[4 * k + j] << 8 * j : 0u;
+                    rs[i][k] = v;
+                }
+        }
+    };
+    uint8_t *const lds_s = lds + NS * SLOT;
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < IS; i++) {
+            const int r = i * 64 * NW + tid;
+            const unsigned l0 = __builtin_amdgcn_perm(rs[i][1], rs[i][0], 0x05010400u), l1 = __builtin_amdgcn_perm(rs[i][1], rs[i][0], 0x07030602u);
+            const unsigned h0 = __builtin_amdgcn_perm(rs[i][3], rs[i][2], 0x05010400u), h1 = __builtin_amdgcn_perm(rs[i][3], rs[i][2], 0x07030602u);
+            const g53_v4w o = {__builtin_amdgcn_perm(h0, l0, 0x05040100u), __builtin_amdgcn_perm(h0, l0, 0x07060302u),
+                               __builtin_amdgcn_perm(h1, l1, 0x05040100u), __builtin_amdgcn_perm(h1, l1, 0x07060302u)};
+            if (r < BM + BN) *(g53_v4w *)(lds_s + buf * SEG + r * 16) = o;
+        }
+    };
+    const int m = lane & 15, q = lane >> 4;
+    const int fa = (wr * 16 * MT + m) * 128 + ((q ^ (m & 7)) << 4), fb = BM * 128 + (wc * 16 * NT + m) * 128 + ((q ^ (m & 7)) << 4);
+    const int sa = (wr * 16 * MT + m) * 16 + 4 * q, sbt = (BM + wc * 16 * NT + m) * 16 + 4 * q;
+    g53_v4f acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[i][t] = (g53_v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    auto frag = [&](const uint8_t *p) {
+        const g53_v4w v = *(const g53_v4w *)p;
+        return (g53_v8i){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+    };
+    auto multiply = [&](int slot, int c) {
+        const uint8_t *l = lds + slot * SLOT, *ls = lds_s + (c >> 1 & 1) * SEG;
+        const int sh = (c & 1) * 16;
+        int wsc[NT], xsc[MT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) wsc[t] = *(const int *)(ls + sbt + t * 256) >> sh;
+#pragma unroll
+        for (int i = 0; i < MT; i++) xsc[i] = *(const int *)(ls + sa + i * 256) >> sh;
+#define G53_MX_STEP(j)                                                                                                   \
+    do {                                                                                                                 \
+        g53_v8i b[NT];                                                                                                   \
+        _Pragma("unroll") for (int t = 0; t < NT; t++) b[t] = frag(l + (fb ^ (j) * 64) + t * 2048);                      \
+        _Pragma("unroll") for (int i = 0; i < MT; i++) {                                                                 \
+            const g53_v8i v = frag(l + (fa ^ (j) * 64) + i * 2048);                                                      \
+            _Pragma("unroll") for (int t = 0; t < NT; t++) acc[i][t] =                                                   \
+                __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[t], v, acc[i][t], 4, 4, j, wsc[t], j, xsc[i]);        \
+        }                                                                                                                \
+    } while (0)
+        G53_MX_STEP(0);
+        G53_MX_STEP(1);
+#undef G53_MX_STEP
+    };
+    fetch(0);
+    put(0);
+    ask(0, 0);
+    for (int c = 0; c < chunks; c++) {
+        g53_loads_left<0>();
+        g53_meet();
+        /* the next segment's scales: asked for with its first chunk's time to spare, put before more loads are asked for */
+        const int seg = c >> 1;
+        if ((c & 1) && seg + 1 < segs) put(seg + 1 & 1);
+        if (!(c & 1) && seg + 1 < segs) fetch(seg + 1);
+        if (c + 1 < chunks) ask(c + 1, c + 1 & 1);
+        multiply(c & 1, c);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int r = (wr * MT + i) * 16 + m;
+        if (r >= live) continue;
+        E *row = (E *)a.out + (long)(it.first + r) * a.half;
+        if (!sw) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) g53_store4(row, n0 + (wc * NT + t) * 16 + 4 * q, a.half, acc[i][t], false);
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT / 2; t++) {
+                g53_v4f v;
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = g53_swiglu1(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
+                g53_store4(row, n0 + (wc * NT / 2 + t) * 16 + 4 * q, a.half, v, false);
+            }
+        }
+    }
+}
+
+template <typename E, int WR, int WC, int MT, int NT, int NS> static int launch(G53MxArgs a, long n)
+{
+    constexpr int BM = 16 * MT * WR, BN = 16 * NT * WC;
+    constexpr size_t LDS = (size_t)NS * (BM + BN) * 128 + 2 * (BM + BN) * 16;
+    static int allowed = 0;
+    if (!allowed) {
+        G53_TRY(hipFuncSetAttribute((const void *)k_mx4<E, WR, WC, MT, NT, NS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
+        allowed = 1;
+    }
+    const int cut = a.limit > 0.0f ? BN / 2 : BN;
+    a.across = (a.half + cut - 1) / cut;
+    long wgs = ((n + BM - 1) / BM) * a.across;
+    if (a.offsets) {
+        const long items = (n / BM + (a.NE < n ? a.NE : n)) * a.across;
+        wgs = (items + 7) / 8 * 8 + (items < 8 ? 8 : items < 256 ? (items + 7) / 8 * 8 : 256);      /* whole runs on every die */
+    }
+    for (long w0 = 0; w0 < wgs; w0 += G53_MX_WGS) {
+        a.wg0 = w0;
+        const dim3 grid((unsigned)(wgs - w0 < G53_MX_WGS ? wgs - w0 : G53_MX_WGS));
+        hipLaunchKernelGGL((k_mx4<E, WR, WC, MT, NT, NS>), grid, dim3(64 * WR * WC), LDS, g53h_stream(), a);
+        G53_LAUNCHED("k_mx4");
+    }
+    return 0;
+}
+
+/* --------------------------------------------------------------------- the calls ---- */
+static int mx_bad(const char *who, const G53hMx4 *m)
+{
+    if (!m) return g53h_fail("%s: no matrix", who);
+    if (m->rows < 0 || m->cols < 32 || m->cols > G53_MX_MAXC || m->cols % 32)
+        return g53h_fail("%s: %d x %d levels (columns a multiple of 32, at most 2^24)", who, m->rows, m->cols);
+    if (m->rows && (!m->w || !m->s)) return g53h_fail("%s: unbound matrix", who);
+    if ((uintptr_t)m->w & 15) return g53h_fail("%s: levels must start at a multiple of 16 bytes", who);
+    return 0;
+}
+
+extern "C" int g53h_mx4_quant(const G53hMx4 *m, const void *x, int dt)
+{
+    const char *who = "g53h_mx4_quant";
+    if (mx_bad(who, m)) return -1;
+    if (!g53_elem_bytes(dt)) return g53h_fail("%s: element type %d", who, dt);
+    if (!m->rows) return 0;
+    if (!x || ((uintptr_t)x & (g53_elem_bytes(dt) - 1))) return g53h_fail("%s: no rows, or not at a multiple of an element", who);
+    if (g53h_ready()) return -1;
+    const long eights = (long)m->rows * m->cols / 8, wgs = (eights + 255) / 256;
+    for (long w0 = 0; w0 < wgs; w0 += G53_MX_WGS) {
+        const dim3 grid((unsigned)(wgs - w0 < G53_MX_WGS ? wgs - w0 : G53_MX_WGS));
+        G53_BY_TYPE(dt, hipLaunchKernelGGL(k_mx4_quant<E>, grid, dim3(256), 0, g53h_stream(), m->w, m->s, (const E *)x, eights, w0));
+        G53_LAUNCHED("k_mx4_quant");
+    }
+    return 0;
+}
+
+extern "C" int g53h_mx4_dequant(void *x, int dt, const G53hMx4 *m)
+{
+    const char *who = "g53h_mx4_dequant";
+    if (mx_bad(who, m)) return -1;
+    if (!g53_elem_bytes(dt)) return g53h_fail("%s: element type %d", who, dt);
+    if (!m->rows) return 0;
+    if (!x || ((uintptr_t)x & (g53_elem_bytes(dt) - 1))) return g53h_fail("%s: no rows, or not at a multiple of an element", who);
+    if (g53h_ready()) return -1;
+    const long eights = (long)m->rows * m->cols / 8, wgs = (eights + 255) / 256;
+    for (long w0 = 0; w0 < wgs; w0 += G53_MX_WGS) {
+        const dim3 grid((unsigned)(wgs - w0 < G53_MX_WGS ? wgs - w0 : G53_MX_WGS));
+        G53_BY_TYPE(dt, hipLaunchKernelGGL(k_mx4_dequant<E>, grid, dim3(256), 0, g53h_stream(), (E *)x, m->w, m->s, eights, w0));
+        G53_LAUNCHED("k_mx4_dequant");
+    }
+    return 0;
+}
+
+/* Both matrices, the type and the limit; fills what a dense and a sorted product share. */
+static int mx_product(const char *who, void *y, int dt, const G53hMx4 *x, const G53hMx4 *m, float limit, G53MxArgs &a)
+{
+    if (mx_bad(who, x) || mx_bad(who, m)) return -1;
+    if (m->rows < 1) return g53h_fail("%s: a matrix of %d rows", who, m->rows);
+    if (x->cols != m->cols) return g53h_fail("%s: rows of %d columns by a matrix of %d", who, x->cols, m->cols);
+    if (!g53_elem_bytes(dt)) return g53h_fail("%s: element type %d", who, dt);
+    if (!(limit >= 0.0f) || limit > 3.0e38f) return g53h_fail("%s: SwiGLU limit %g", who, limit);
+    if (limit > 0.0f && m->rows % 2) return g53h_fail("%s: SwiGLU of %d rows", who, m->rows);
+    if ((uintptr_t)y & (g53_elem_bytes(dt) - 1)) return g53h_fail("%s: results must be at a multiple of an element", who);
+    a = G53MxArgs{};
+    a.x = x->w;
+    a.xs = x->s;
+    a.w = m->w;
+    a.s = m->s;
+    a.out = y;
+    a.NE = 1;
+    a.T = x->rows;
+    a.rows = m->rows;
+    a.cols = m->cols;
+    a.limit = limit;
+    a.half = limit > 0.0f ? m->rows / 2 : m->rows;
+    a.topk = g53_div_of(1);
+    return 0;
+}
+
+template <typename E> static int by_size(const G53MxArgs &a, long n) { return launch<E, 2, 2, 4, 4, 2>(a, n); }
+
+extern "C" int g53h_mm_mx4(void *y, int dt, const G53hMx4 *x, const G53hMx4 *m, float swiglu_limit)
+{
+    G53MxArgs a;
+    if (mx_product("g53h_mm_mx4", y, dt, x, m, swiglu_limit, a)) return -1;
+    if (!a.T) return 0;
+    if (!y) return g53h_fail("g53h_mm_mx4: no results");
+    if (g53h_ready()) return -1;
+    int rc;
+    G53_BY_TYPE(dt, rc = by_size<E>(a, a.T));
+    return rc;
+}
+
+extern "C" int g53h_sorted_mm_mx4(void *ys, int dt, const G53hMx4 *x, int gather, const G53hSort *p, const G53hMx4 *m,
+                                  float swiglu_limit)
+{
+    const char *who = "g53h_sorted_mm_mx4";
+    G53MxArgs a;
+    if (mx_product(who, ys, dt, x, m, swiglu_limit, a)) return -1;
+    if (!p || p->T < 0 || p->topk < 1 || p->topk > 64 || p->n_experts < 1 || p->n_experts > G53_MX_MAXE ||
+        (long)p->T * p->topk > 0x7fffffffl || !p->offsets || (p->T && !p->pair))
+        return g53h_fail("%s: no plan of g53h_sort_tokens", who);
+    const long n = (long)p->T * p->topk;
+    if (x->rows < (gather ? p->T : n)) return g53h_fail("%s: %d rows of x, the plan has %ld", who, x->rows, gather ? (long)p->T : n);
+    if (!p->T) return 0;
+    if (!ys) return g53h_fail("%s: no results", who);
+    if (g53h_ready()) return -1;
+    a.offsets = p->offsets;
+    a.pair = gather ? p->pair : nullptr;
+    a.NE = p->n_experts;
+    a.topk = g53_div_of(p->topk);
+    int rc;
+    G53_BY_TYPE(dt, rc = by_size<E>(a, n));
+    return rc;
+}

@@ -58,6 +58,10 @@ class G53hW4(C.Structure):
                 ("group", C.c_int), ("s_dt", C.c_int)]
 
 
+class G53hMx4(C.Structure):
+    _fields_ = [("w", C.c_void_p), ("s", C.c_void_p), ("rows", C.c_int), ("cols", C.c_int)]
+
+
 class G53hBlockNorm(C.Structure):
     _fields_ = [("T", C.c_int), ("hidden", C.c_int), ("dt", C.c_int), ("gate_kind", C.c_int), ("eps", C.c_float),
                 ("scale", C.c_float), ("post", C.c_void_p), ("next", C.c_void_p), ("gate", C.c_void_p)]
@@ -271,6 +275,11 @@ _SIGS = {
     "g53h_sorted_mm_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                       C.POINTER(G53hSort), C.c_void_p, C.c_int, C.c_int]),
     "g53h_sorted_swiglu_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(G53hSort), C.c_float]),
+    "g53h_mx4_quant": (C.c_int, [C.POINTER(G53hMx4), C.c_void_p, C.c_int]),
+    "g53h_mx4_dequant": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(G53hMx4)]),
+    "g53h_mm_mx4": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(G53hMx4), C.POINTER(G53hMx4), C.c_float]),
+    "g53h_sorted_mm_mx4": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(G53hMx4), C.c_int, C.POINTER(G53hSort), C.POINTER(G53hMx4),
+                                     C.c_float]),
     "g53h_norm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float]),
     "g53h_norm_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                  C.c_float]),

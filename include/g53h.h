@@ -437,6 +437,28 @@ int g53h_sorted_mm_grad(void *dx_d, void *dw_d, int dw_dt, int add, const void *
 int g53h_sorted_swiglu_grad(void *dgu_d, const void *dact_d, const void *gu_d, int dt, int inter, const G53hSort *p,
                             float limit);
 
+/* A microscaled 4-bit matrix: element (r, c) = 2^(s[r][c / 32] - 127) * level. Levels [rows][cols / 2], the even column in
+ * the low nibble, at a multiple of 16 bytes: bit 3 the sign, bits 0 to 2 count 0, 0.5, 1, 1.5, 2, 3, 4, 6. Scales
+ * [rows][cols / 32], one byte each, 255: NaN. cols a multiple of 32, at most 2^24. Several experts' matrices follow each
+ * other; rows is then that of one. */
+typedef struct {
+    uint8_t *w, *s;
+    int rows, cols;
+} G53hMx4;
+/* x [rows][cols] to m's levels and scales: a block's scale is the power of two at or below its largest value, less 2 (at
+ * least 2^-127; a block of zeros has scale 0), levels the nearest, ties to the even one, 6 for all above. A block
+ * with a value that is not finite has scale 255 and levels of zero. _dequant: the values in x, rounded to the type. */
+int g53h_mx4_quant(const G53hMx4 *m, const void *x_d, int dt);
+int g53h_mx4_dequant(void *x_d, int dt, const G53hMx4 *m);
+/* y[x.rows][m.rows] = the products of x's rows with m's, of type dt; swiglu_limit as in g53h_mm_w4 (y [x.rows][m.rows / 2]).
+ * Products are exact and sums fp32; a block whose scale is 255 gives NaN in every result that it enters. */
+int g53h_mm_mx4(void *y_d, int dt, const G53hMx4 *x, const G53hMx4 *m, float swiglu_limit);
+/* The same over the sorted rows of a plan, each with its expert's matrix: m describes expert 0, levels and scales of the
+ * others follow it. x: with gather the tokens [T][cols], else sorted rows [n][cols]. ys [n][rows (/ 2)]; rows behind the last
+ * are left as they were. */
+int g53h_sorted_mm_mx4(void *ys_d, int dt, const G53hMx4 *x, int gather, const G53hSort *p, const G53hMx4 *m,
+                       float swiglu_limit);
+
 /* xn = x / sqrt(mean of x^2 + eps) * gain per row of hidden <= 16384; gain fp32 [hidden]; eps 1e-30 to
  * 1e30; xn may be x. Squares are summed in fp32: a row whose sum leaves it gives zeros (|x| of 1e19 / sqrt(hidden)
  * and more may). _grad: dx (may be dxn) and, where it is not NULL, dgain fp32 [hidden], from dxn and x. */

@@ -149,3 +149,47 @@ def test_expert_products(L):
     refused(L, L.g53h_sorted_mm_grad(None, P, 0, 0, P, None, 1, 0, plan(), P, 8, 8), "no rows")
     refused(L, L.g53h_sorted_mm_grad(None, P + 2, 0, 0, P, P, 1, 0, plan(), P, 8, 8), "multiples of an element")
     refused(L, L.g53h_sorted_swiglu_grad(P, None, P, 1, 8, plan(), 1.0), "no rows")
+
+
+def mx4(w=P, s=P, rows=8, cols=64):
+    return C.byref(glm53h.G53hMx4(w, s, rows, cols))
+
+
+@pytest.mark.parametrize("bad,word", [(dict(w=None), "unbound"), (dict(s=None), "unbound"), (dict(rows=-1), "levels"), (dict(cols=0), "levels"),
+                                      (dict(cols=48), "levels"), (dict(cols=(1 << 24) + 32), "levels"), (dict(cols=-32), "levels"),
+                                      (dict(w=P + 8), "multiple of 16")])
+def test_microscaled_matrices(L, bad, word):
+    refused(L, L.g53h_mx4_quant(mx4(**bad), P, 1), word)
+    refused(L, L.g53h_mx4_dequant(P, 1, mx4(**bad)), word)
+    for x, m in ((bad, {}), ({}, bad)):
+        refused(L, L.g53h_mm_mx4(P, 1, mx4(**x), mx4(**m), 0.0), word)
+        refused(L, L.g53h_sorted_mm_mx4(P, 1, mx4(**x), 1, plan(), mx4(**m), 0.0), word)
+
+
+def test_microscaled_products(L):
+    refused(L, L.g53h_mx4_quant(None, P, 1), "no matrix")
+    refused(L, L.g53h_mx4_quant(mx4(), None, 1), "no rows")
+    refused(L, L.g53h_mx4_quant(mx4(), P + 1, 1), "multiple of an element")
+    refused(L, L.g53h_mx4_dequant(P + 2, 0, mx4()), "multiple of an element")
+    for dt in (-1, 3):
+        refused(L, L.g53h_mx4_quant(mx4(), P, dt), "element type")
+        refused(L, L.g53h_mx4_dequant(P, dt, mx4()), "element type")
+        refused(L, L.g53h_mm_mx4(P, dt, mx4(), mx4(), 0.0), "element type")
+        refused(L, L.g53h_sorted_mm_mx4(P, dt, mx4(), 1, plan(), mx4(), 0.0), "element type")
+    refused(L, L.g53h_mm_mx4(P, 1, mx4(), None, 0.0), "no matrix")
+    refused(L, L.g53h_mm_mx4(P, 1, mx4(), mx4(rows=0), 0.0), "0 rows")
+    refused(L, L.g53h_mm_mx4(P, 1, mx4(cols=32), mx4(), 0.0), "32 columns")
+    refused(L, L.g53h_mm_mx4(P, 1, mx4(), mx4(rows=7), 1.0), "SwiGLU")
+    for limit in (-1.0, float("nan"), float("inf")):
+        refused(L, L.g53h_mm_mx4(P, 1, mx4(), mx4(), limit), "SwiGLU")
+    refused(L, L.g53h_mm_mx4(None, 1, mx4(), mx4(), 0.0), "no results")
+    refused(L, L.g53h_mm_mx4(P + 1, 1, mx4(), mx4(), 0.0), "multiple of an element")
+    refused(L, L.g53h_sorted_mm_mx4(None, 1, mx4(), 1, plan(), mx4(), 0.0), "no results")
+    for bad in (dict(T=-1), dict(topk=0), dict(NE=1025), dict(offsets=None), dict(pair=None)):
+        refused(L, L.g53h_sorted_mm_mx4(P, 1, mx4(), 1, plan(**bad), mx4(), 0.0), "plan")
+    refused(L, L.g53h_sorted_mm_mx4(P, 1, mx4(rows=3), 1, plan(T=4), mx4(), 0.0), "3 rows of x")
+    refused(L, L.g53h_sorted_mm_mx4(P, 1, mx4(rows=7), 0, plan(T=4, topk=2), mx4(), 0.0), "7 rows of x")
+
+
+def test_new_struct_sizes():
+    assert C.sizeof(glm53h.G53hMx4) == 24
