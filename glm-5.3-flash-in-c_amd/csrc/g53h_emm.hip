@@ -34,7 +34,7 @@ struct G53EmArgs {
 
 /* One tile of OP. DMA: operand rows start at multiples of 16 bytes and are whole pieces. */
 template <typename E, int OP, int WR, int WC, int MT, int NT, int NS, bool DMA>
-__global__ void __launch_bounds__(64 * WR * WC, 2) k_emm(G53EmArgs a)
+__global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emm(G53EmArgs a)
 {
     constexpr int NW = WR * WC, BM = 16 * MT * WR, BN = 16 * NT * WC, SLOT = (BM + BN) * 128, KE = 128 / sizeof(E);
     constexpr int IA = BM / (8 * NW), IB = BN / (8 * NW), STEPS = KE / 32;
@@ -75,20 +75,31 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_emm(G53EmArgs a)
         return g53_div(a.pair[r], a.topk);
     };
 
-    /* along: a row's address and what the lane takes of its chunks; across: the lane's row of a chunk and its columns */
+    /* Where a lane's pieces come from. Along: its row, and its place in 128 bytes. Across: its row of a chunk, whose places
+     * repeat after VA or VB instructions; columns behind the last take the last piece (whole pieces) or what is there of
+     * it: their results are not stored. */
+    typedef G53Across<E, BM, MT> Xa;
+    typedef G53Across<E, BN, NT> Xb;
+    constexpr int KA = 64 / Xa::U, KB = 64 / Xb::U, VA = AX ? Xa::template turns<KA * NW>() : IA, VB = BX ? Xb::template turns<KB * NW>() : IB;
     const int u8 = (lane & 7) ^ (lane >> 3);
-    const uint8_t *pa[IA], *pb[IB];
-    if constexpr (!AX) {
+    const long wrow = (long)a.cols * sizeof(E), drow = (long)a.rows * sizeof(E);
+    const uint8_t *pa[VA], *pb[VB];
+    int ca[AX ? VA : 1], cb[BX ? VB : 1];                               /* across: first byte in a row */
 #pragma unroll
-        for (int i = 0; i < IA; i++) {
+    for (int i = 0; i < VA; i++) {
+        if constexpr (!AX) {
             const int r = (i * NW + wv) * 8 + (lane >> 3), s = it.first + (r < live ? r : live - 1);
-            if constexpr (OP == G53_EM_FWD) pa[i] = a.x + token(s) * a.cols * sizeof(E) + u8 * 16;
-            else pa[i] = a.dy + (long)s * a.rows * sizeof(E) + u8 * 16;
+            pa[i] = OP == G53_EM_FWD ? a.x + token(s) * wrow + u8 * 16 : a.dy + s * drow + u8 * 16;
+        } else {
+            const int k = (i * NW + wv) * KA + lane / Xa::U;
+            const long col = (long)m0 * sizeof(E) + ((lane % Xa::U) ^ Xa::place(k)) * 16;
+            ca[i] = (int)(DMA && col > drow - 16 ? drow - 16 : col);
+            pa[i] = a.dy + (it.first + k) * drow + ca[i];
         }
     }
-    if constexpr (!BX) {
 #pragma unroll
-        for (int i = 0; i < IB; i++) {
+    for (int i = 0; i < VB; i++) {
+        if constexpr (!BX) {
             const int r = (i * NW + wv) * 8 + (lane >> 3);
             int at = n0 + r, up = 0;
             if (sw) {               /* a wave's first half of tiles: gate, the others: up */
@@ -97,62 +108,72 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_emm(G53EmArgs a)
                 at = n0 + w * (8 * NT) + (up ? t - NT / 2 : t) * 16 + r % 16;
             }
             at = at < a.half ? at : a.half - 1;
-            pb[i] = we + (long)(at + (up ? a.half : 0)) * a.cols * sizeof(E) + u8 * 16;
+            pb[i] = we + (at + (up ? a.half : 0)) * wrow + u8 * 16;
+        } else {
+            const int k = (i * NW + wv) * KB + lane / Xb::U;
+            const long col = (long)n0 * sizeof(E) + ((lane % Xb::U) ^ Xb::place(k)) * 16;
+            cb[i] = (int)(DMA && col > wrow - 16 ? wrow - 16 : col);
+            pb[i] = (OP == G53_EM_ROWS ? we + k * wrow : a.x) + cb[i];      /* matrices: the row joins it chunk by chunk */
         }
     }
+    /* matrices: the tokens of an instruction's rows of x, asked for as scalars: their counter is not the loads' */
+    int tok[OP == G53_EM_MATS ? IB : 1][KB];
+    auto tokens = [&](int c) {
+        if constexpr (OP == G53_EM_MATS)
+#pragma unroll
+            for (int i = 0; i < IB; i++)
+#pragma unroll
+                for (int r = 0; r < KB; r++) {
+                    const int k = c * KE + (i * NW + wv) * KB + r, s = it.first + (k < live ? k : live - 1);
+                    tok[i][r] = a.pair ? g53_uniform_load(a.pair + s) : s;
+                }
+    };
+    const int kbytes = (int)(K * (long)sizeof(E));                      /* along: of a row */
     auto piece_a = [&](int i, int c) -> G53Piece {
         if constexpr (!AX) {
-            const long at = (long)c * 128;
-            return {pa[i] + at, K * (long)sizeof(E) - at - u8 * 16};
-        } else {
-            typedef G53Across<E, BM, MT> X;
-            const int q = (i * NW + wv) * 64 + lane, k = q / X::U, u = (q % X::U) ^ X::place(k), col = m0 * (int)sizeof(E) + u * 16;
-            const int kk = c * KE + k;
-            return {a.dy + ((long)(it.first + kk) * a.rows * sizeof(E) + col), kk < live ? (long)a.rows * (long)sizeof(E) - col : 0};
-        }
+            const uint8_t *p = pa[i];
+            pa[i] += 128;
+            return {p, kbytes - c * 128 - u8 * 16};
+        } else return {pa[i % VA] + (c * KE + i / VA * (VA * KA * NW)) * drow,
+                     lane / Xa::U < live - c * KE - (i * NW + wv) * KA ? (DMA ? 16 : (int)drow - ca[i % VA]) : 0};
     };
     auto piece_b = [&](int i, int c) -> G53Piece {
         if constexpr (!BX) {
-            const long at = (long)c * 128;
-            return {pb[i] + at, K * (long)sizeof(E) - at - u8 * 16};
-        } else {
-            typedef G53Across<E, BN, NT> X;
-            const int q = (i * NW + wv) * 64 + lane, k = q / X::U, u = (q % X::U) ^ X::place(k);
-            const long col = (long)n0 * sizeof(E) + u * 16, kk = (long)c * KE + k, end = (long)a.cols * sizeof(E) - col;
-            if constexpr (OP == G53_EM_ROWS) {
-                return {we + (kk * a.cols * (long)sizeof(E) + col), kk < K ? end : 0};
-            } else {
-                /* the instruction's rows of x, asked for as scalars: their counter is not the loads' */
-                constexpr int ROWS = 64 / X::U > 0 ? 64 / X::U : 1;
-                const int k0 = c * KE + (i * NW + wv) * 64 / X::U;
-                long t = 0;
-#pragma unroll
-                for (int r = 0; r < ROWS; r++) {
-                    const int s = it.first + (k0 + r < live ? k0 + r : live - 1);
-                    const long tr = a.pair ? g53_div(g53_uniform_load(a.pair + s), a.topk) : s;
-                    t = lane / X::U == r || ROWS == 1 ? tr : t;
-                }
-                return {a.x + (t * a.cols * (long)sizeof(E) + col), kk < live ? end : 0};
-            }
+            const uint8_t *p = pb[i];
+            pb[i] += 128;
+            return {p, kbytes - c * 128 - u8 * 16};
         }
+        const int n = lane / Xb::U < (int)K - c * KE - (i * NW + wv) * KB ? (DMA ? 16 : (int)wrow - cb[i % VB]) : 0;
+        if constexpr (OP == G53_EM_ROWS) {
+            const uint8_t *p = pb[i % VB] + i / VB * (VB * KB * NW) * wrow;
+            if (i == IB - 1)
+#pragma unroll
+                for (int v = 0; v < VB; v++) pb[v] += KE * wrow;
+            return {p, n};
+        }
+        long t = 0;
+#pragma unroll
+        for (int r = 0; r < KB; r++) {
+            const long at = (long)(a.pair ? g53_div(tok[OP == G53_EM_MATS ? i : 0][r], a.topk) : tok[OP == G53_EM_MATS ? i : 0][r]) * wrow;
+            t = r == 0 || lane / Xb::U == r ? at : t;
+        }
+        return {pb[i % VB] + t, n};
     };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    auto ask1 = [&](int c, int slot, int i) {               /* one instruction of a chunk */
+        const G53Piece s = i < IA ? piece_a(i < IA ? i : 0, c) : piece_b(i < IA ? 0 : i - IA, c);
+        const uint8_t *p = s.n > 0 ? s.p : (const uint8_t *)&g53_nothing;
+        g53_to_lds(p, lds0 + slot * SLOT + wv * 1024 + (i < IA ? i * NW * 1024 : BM * 128 + (i - IA) * NW * 1024));
+    };
     auto ask = [&](int c, int slot) {
-        const uint32_t to = lds0 + slot * SLOT + wv * 1024;
+        tokens(c);
 #pragma unroll
-        for (int i = 0; i < IA; i++) {
-            const G53Piece s = piece_a(i, c);
-            g53_to_lds(s.n > 0 ? s.p : (const uint8_t *)&g53_nothing, to + i * NW * 1024);
-        }
-#pragma unroll
-        for (int i = 0; i < IB; i++) {
-            const G53Piece s = piece_b(i, c);
-            g53_to_lds(s.n > 0 ? s.p : (const uint8_t *)&g53_nothing, to + BM * 128 + i * NW * 1024);
-        }
+        for (int i = 0; i < IA + IB; i++) ask1(c, slot, i);
     };
     g53_v4w ra[DMA ? 1 : IA], rb[DMA ? 1 : IB];
     auto fetch = [&](int c) {
         if constexpr (!DMA) {
+            tokens(c);
 #pragma unroll
             for (int i = 0; i < IA; i++) ra[i] = g53_piece<E>(piece_a(i, c));
 #pragma unroll
@@ -169,10 +190,9 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_emm(G53EmArgs a)
         }
     };
 
-    typedef G53Along<E> Al;
-    typename std::conditional<AX, G53Across<E, BM, MT>, Al>::type fa;
-    typename std::conditional<BX, G53Across<E, BN, NT>, Al>::type fb;
-    fa.setup(wr * 16 * MT);
+    typename std::conditional<AX, G53Across<E, BM, MT, WR>, G53Along<E, WR>>::type fa;
+    typename std::conditional<BX, G53Across<E, BN, NT>, G53Along<E>>::type fb;
+    fa.setup(wr * 16);                  /* tile i of wave row wr is the tile's 16 rows i * WR + wr: rows that are there spread over all */
     fb.setup(wc * 16 * NT);
     g53_v4f acc[MT][NT];
 #pragma unroll
@@ -195,7 +215,65 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_emm(G53EmArgs a)
             }
         }
     };
-    if constexpr (DMA) {
+    if constexpr (DMA && STEPS == 2) {
+        /* Operands of one step are in registers while those of the next leave LDS between its products. The slot of chunk c
+         * is free once its second step's operands are read, halfway through the chunk: there one barrier hands it to chunk
+         * c + NS, and says that c + 1 is there, whose first step's operands are read beside the second half's products. */
+        auto run = [&](auto M_) {
+        constexpr int M = decltype(M_)::value;                  /* row tiles of a wave that are there */
+        G53Frag<E> va[2][M], vb[2][NT];
+        auto read1 = [&](int to, int slot, int j, int i) {  /* one fragment of a step */
+            const uint8_t *la = lds + slot * SLOT;
+            if (i < NT) fb.read(vb[to][i], la + BM * 128, i, j);
+            else fa.read(va[to][i - NT], la, i - NT, j);
+        };
+        constexpr int RD = (M + NT + M - 1) / M, IM = AX ? IA : IA * M / MT, AD = (IM + IB + M - 1) / M;
+        if (chunks) {
+#pragma unroll
+            for (int c = 0; c < NS; c++) {
+                tokens(c);
+#pragma unroll
+                for (int i = 0; i < IM + IB; i++) ask1(c, c, i < IM ? i : i - IM + IA);
+            }         /* behind the last chunk: zeros, which nothing uses */
+            g53_loads_left<(NS - 1) * (IM + IB)>();
+            g53_meet();
+#pragma unroll
+            for (int i = 0; i < M + NT; i++) read1(0, 0, 0, i);
+        }
+        int slot = 0;
+        for (int c = 0; c < chunks; c++) {
+            tokens(c + NS);
+#pragma unroll
+            for (int i = 0; i < M; i++) {
+#pragma unroll
+                for (int k = i * RD; k < (i + 1) * RD && k < M + NT; k++) read1(1, slot, 1, k);
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[i][t] = g53_mm<E>(vb[0][t], va[0][i], acc[i][t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            g53_loads_left<(NS - 2) * (IM + IB)>();
+            g53_meet();
+            const int next = slot == NS - 1 ? 0 : slot + 1;
+#pragma unroll
+            for (int i = 0; i < M; i++) {
+#pragma unroll
+                for (int k = i * AD; k < (i + 1) * AD && k < IM + IB; k++) ask1(c + NS, slot, k < IM ? k : k - IM + IA);
+#pragma unroll
+                for (int k = i * RD; k < (i + 1) * RD && k < M + NT; k++) read1(0, next, 0, k);
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[i][t] = g53_mm<E>(vb[1][t], va[1][i], acc[i][t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            slot = next;
+        }
+        g53_loads_left<0>();                                /* no load outlives the workgroup's LDS */
+        };
+        typedef std::integral_constant<int, MT> All;
+        if constexpr (AX || MT < 8) run(All{});
+        else if (live <= BM / 4) run(std::integral_constant<int, MT / 4>{});
+        else if (live <= BM / 2) run(std::integral_constant<int, MT / 2>{});
+        else run(All{});
+    } else if constexpr (DMA) {
         const int ahead = chunks < NS - 1 ? chunks : NS - 1;
         for (int c = 0; c < ahead; c++) ask(c, c);
         int slot = 0;
@@ -222,44 +300,251 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_emm(G53EmArgs a)
         }
     }
 
-    /* lane (m, q) of a tile: columns 4 q .. 4 q + 3 of row m */
-    const int m = lane & 15, q = lane >> 4;
+    /* out: the loads' slots hold the wave's rows on their way */
+    constexpr bool VIA = DMA && STEPS == 2 && OP != G53_EM_MATS;
+    uint8_t *const buf = lds + wv * (16 * 16 * NT * (int)sizeof(E));
+    if (VIA) g53_meet();
+    auto leave = [&](auto &tiles, E *out, int N, int r0, int c0) {      /* 16 rows from r0, columns from c0 of N */
+        constexpr int n = sizeof(tiles) / sizeof(g53_v4f);
+        E *at = out + (long)(it.first + r0) * N + c0;
+        if constexpr (VIA) {
+            g53_rows_out<E, n, false>(buf, at, N, tiles, live - r0, N - c0, false);
+        } else {
+            const int m = lane & 15, q = lane >> 4;
+            if (r0 + m >= live) return;
+#pragma unroll
+            for (int t = 0; t < n; t++) g53_store4(at + (long)m * N + 4 * q, 16 * t, N - c0 - 4 * q, tiles[t], false);
+        }
+    };
 #pragma unroll
     for (int i = 0; i < MT; i++) {
-        const int r = (wr * MT + i) * 16 + m;
+        const int r0 = (i * WR + wr) * 16;
+#pragma unroll
+        for (int t = 0; t < NT; t++) asm volatile("" ::: "memory");
         if constexpr (OP == G53_EM_MATS) {
-            if (m0 + r >= a.rows) continue;
-            const long at = ((long)it.e * a.rows + m0 + r) * a.cols;
+            const int r = m0 + r0 + (lane & 15), c = n0 + wc * NT * 16 + 4 * (lane >> 4);
+            if (r >= a.rows) continue;
+            const long at = ((long)it.e * a.rows + r) * a.cols + c;
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const int c = n0 + (wc * NT + t) * 16 + 4 * q;
-                if (a.w_f32) g53_store4((float *)a.out + at, c, a.cols, acc[i][t], a.add);
-                else g53_store4((E *)a.out + at, c, a.cols, acc[i][t], a.add);
+                if (a.w_f32) g53_store4((float *)a.out + at, 16 * t, a.cols - c, acc[i][t], a.add);
+                else g53_store4((E *)a.out + at, 16 * t, a.cols - c, acc[i][t], a.add);
             }
-        } else {
-            if (r >= live) continue;
-            const long s = it.first + r;
+        } else if (r0 < live) {
             if (OP == G53_EM_ROWS || !sw) {
-                const int N = OP == G53_EM_ROWS ? a.cols : a.half;
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-                    g53_store4((E *)a.out + s * N, n0 + (wc * NT + t) * 16 + 4 * q, N, acc[i][t], false);
+                leave(acc[i], (E *)a.out, OP == G53_EM_ROWS ? a.cols : a.half, r0, n0 + wc * NT * 16);
             } else {
+                g53_v4f v[NT / 2], g[NT / 2], u[NT / 2];
 #pragma unroll
                 for (int t = 0; t < NT / 2; t++) {
-                    const int c = n0 + (wc * NT / 2 + t) * 16 + 4 * q;
-                    g53_v4f v;
+                    g[t] = acc[i][t];
+                    u[t] = acc[i][t + NT / 2];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] = g53_swiglu1(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
-                    g53_store4((E *)a.out + s * a.half, c, a.half, v, false);
-                    if (a.gu) {
-                        g53_store4((E *)a.gu + s * a.rows, c, a.half, acc[i][t], false);
-                        g53_store4((E *)a.gu + s * a.rows + a.half, c, a.half, acc[i][t + NT / 2], false);
+                    for (int k = 0; k < 4; k++) v[t][k] = g53_swiglu1<E>(g[t][k], u[t][k], a.limit);
+                }
+                const int c = n0 + wc * (NT / 2 * 16);
+                leave(v, (E *)a.out, a.half, r0, c);
+                if (a.gu) {                             /* gate, then up: the rows' second halves */
+                    const int most = a.half - c;
+                    E *at = (E *)a.gu + (long)(it.first + r0) * a.rows + c;
+                    if constexpr (VIA) {
+                        g53_rows_out<E, NT / 2, false>(buf, at, a.rows, g, live - r0, most, false);
+                        g53_rows_out<E, NT / 2, false>(buf, at + a.half, a.rows, u, live - r0, most, false);
+                    } else {
+                        const int m = lane & 15, q = lane >> 4;
+                        if (r0 + m < live)
+#pragma unroll
+                            for (int t = 0; t < NT / 2; t++) {
+                                g53_store4(at + (long)m * a.rows + 4 * q, 16 * t, most - 4 * q, g[t], false);
+                                g53_store4(at + a.half + (long)m * a.rows + 4 * q, 16 * t, most - 4 * q, u[t], false);
+                            }
                     }
                 }
             }
         }
     }
+}
+
+/* The matrices' gradient in 16 bits, of whole pieces. An expert's rows are few next to a matrix (a tile of results often
+ * takes less time to sum than to write), so workgroups stay and go from tile to tile: while a tile's last chunks are
+ * multiplied and its results leave, the next one's first chunks are on their way. The stream of chunks passes experts
+ * without rows, whose tiles are zeros. */
+template <typename E, int WR, int WC, int MT, int NT, int NS>
+__global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emats(G53EmArgs a)
+{
+    constexpr int NW = WR * WC, BM = 16 * MT * WR, BN = 16 * NT * WC, SLOT = (BM + BN) * 128, KE = 64;
+    constexpr int IA = BM / (8 * NW), IB = BN / (8 * NW);
+    typedef G53Across<E, BM, MT> Xa;
+    typedef G53Across<E, BN, NT> Xb;
+    constexpr int KA = 64 / Xa::U, KB = 64 / Xb::U;                     /* rows of a wave's instruction */
+    constexpr int VA = Xa::template turns<KA * NW>(), VB = Xb::template turns<KB * NW>();    /* after as many, places repeat */
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wv / WC, wc = wv % WC;
+    const long wrow = (long)a.cols * sizeof(E), drow = (long)a.rows * sizeof(E);
+    const int per = a.across * a.down;
+    const long total = (long)a.NE * per;
+    const int len = total >= 256 ? 32 : total >= 16 ? (int)(total / 8) : 1;
+    /* the tile of a workgroup's turn w: runs of tiles by die, eight tiles down with each across */
+    struct Tile {
+        int e, m0, n0, first, live;
+    };
+    auto tile_of = [&](long w, Tile &t) {
+        const long i = w >> 3, item = ((i / len) * 8 + (w & 7)) * len + i % len;
+        if (item >= total) return false;
+        t.e = (int)(item / per);
+        const int in = (int)(item % per), g = in / (8 * a.across), in_g = in % (8 * a.across);
+        const int of = a.down - 8 * g < 8 ? a.down - 8 * g : 8;
+        t.m0 = (8 * g + in_g % of) * BM;
+        t.n0 = in_g / of * BN;
+        t.first = g53_uniform_load(a.offsets + t.e);
+        t.live = g53_uniform_load(a.offsets + t.e + 1) - t.first;
+        return true;
+    };
+    const long turns = (total + 8l * len - 1) / (8l * len) * (8l * len);
+    /* The stream: the tile and chunk to be asked for (none behind the last: zeros), and the one after it, whose tokens
+     * are asked for a chunk ahead. */
+    struct At {
+        Tile t;
+        int c, chunks, left;            /* left: rows from the chunk's first on, 0 behind the last tile */
+    };
+    At s, nx;
+    long nw = blockIdx.x;
+    auto seek = [&]() {
+        nx.c = nx.chunks = 0;
+        for (; nw < turns; nw += gridDim.x)
+            if (tile_of(nw, nx.t) && nx.t.live) {
+                nx.chunks = (nx.t.live + KE - 1) / KE;
+                break;
+            }
+    };
+    const uint8_t *pa[VA];
+    int cb[VB], tok[IB], tokn[IB];
+    const int ka = wv * KA + lane / Xa::U, kb = wv * KB + lane / Xb::U;
+    auto tokens = [&]() {
+        if (!nx.chunks) return;
+#pragma unroll
+        for (int i = 0; i < IB; i++) {
+            const int k = nx.c * KE + kb + i * KB * NW, r = nx.t.first + (k < nx.t.live ? k : nx.t.live - 1);
+            tokn[i] = a.pair ? a.pair[r] : r;
+        }
+    };
+    auto on = [&]() {                                       /* to the stream's next chunk */
+        s = nx;
+        s.left = s.chunks ? s.t.live - s.c * KE : 0;
+#pragma unroll
+        for (int i = 0; i < IB; i++) tok[i] = tokn[i];
+        if (!s.chunks) return;
+        if (!s.c) {
+#pragma unroll
+            for (int v = 0; v < VA; v++) {
+                const int k = ka + v * KA * NW;
+                long col = (long)s.t.m0 * sizeof(E) + ((lane % Xa::U) ^ Xa::place(k)) * 16;
+                col = col > drow - 16 ? drow - 16 : col;    /* columns behind the last: not stored */
+                pa[v] = a.dy + (long)(s.t.first + k) * drow + col;
+            }
+#pragma unroll
+            for (int v = 0; v < VB; v++) {
+                const long col = (long)s.t.n0 * sizeof(E) + ((lane % Xb::U) ^ Xb::place(kb + v * KB * NW)) * 16;
+                cb[v] = (int)(col > wrow - 16 ? wrow - 16 : col);
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < VA; v++) pa[v] += KE * drow;
+        }
+        if (++nx.c == nx.chunks) {
+            nw += gridDim.x;
+            seek();
+        }
+    };
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    auto ask1 = [&](int slot, int i) {                      /* one instruction of the stream's chunk */
+        const uint32_t to = lds0 + slot * SLOT + wv * 1024;
+        const uint8_t *p = (const uint8_t *)&g53_nothing;
+        if (i < IA) {
+            const uint8_t *at = pa[i % VA] + (i / VA) * (VA * KA * NW) * drow;
+            p = lane / Xa::U < s.left - (i * NW + wv) * KA ? at : p;
+            g53_to_lds(p, to + i * NW * 1024);
+        } else {
+            const int j = i - IA;
+            const uint8_t *at = a.x + (long)g53_div(tok[j], a.topk) * wrow + cb[j % VB];
+            p = lane / Xb::U < s.left - (j * NW + wv) * KB ? at : p;
+            g53_to_lds(p, to + BM * 128 + j * NW * 1024);
+        }
+    };
+    Xa fa;
+    Xb fb;
+    fa.setup(wr * 16 * MT);
+    fb.setup(wc * 16 * NT);
+    G53Frag<E> va[2][MT], vb[2][NT];
+    auto read1 = [&](int to, int slot, int j, int i) {      /* one fragment of a step */
+        const uint8_t *l = lds + slot * SLOT;
+        if (i < NT) fb.read(vb[to][i], l + BM * 128, i, j);
+        else fa.read(va[to][i - NT], l, i - NT, j);
+    };
+    constexpr int RD = (MT + NT + MT - 1) / MT, AD = 2 * ((IA + IB + MT - 1) / MT);
+    seek();
+    tokens();
+    on();
+#pragma unroll
+    for (int c = 0; c < NS; c++) {
+        tokens();
+#pragma unroll
+        for (int i = 0; i < IA + IB; i++) ask1(c, i);
+        on();
+    }
+    g53_loads_left<(NS - 1) * (IA + IB)>();
+    g53_meet();
+#pragma unroll
+    for (int i = 0; i < MT + NT; i++) read1(0, 0, 0, i);
+    int slot = 0;
+    for (long w = blockIdx.x; w < turns; w += gridDim.x) {
+        Tile t;
+        if (!tile_of(w, t) || (a.add && !t.live)) continue;
+        g53_v4f acc[MT][NT];
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[i][j] = (g53_v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        const int chunks = (t.live + KE - 1) / KE;
+        for (int c = 0; c < chunks; c++) {                  /* see k_emm */
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+#pragma unroll
+                for (int k = i * RD; k < (i + 1) * RD && k < MT + NT; k++) read1(1, slot, 1, k);
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[i][j] = g53_mm<E>(vb[0][j], va[0][i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            g53_loads_left<(NS - 2) * (IA + IB)>();
+            g53_meet();
+            const int next = slot == NS - 1 ? 0 : slot + 1;
+            tokens();
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+#pragma unroll
+                for (int k = i * AD; k < (i + 1) * AD && k < IA + IB; k++) ask1(slot, k);
+#pragma unroll
+                for (int k = i * RD; k < (i + 1) * RD && k < MT + NT; k++) read1(0, next, 0, k);
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[i][j] = g53_mm<E>(vb[1][j], va[1][i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            slot = next;
+            on();
+        }
+        const int r0 = t.m0 + wr * 16 * MT, c0 = t.n0 + wc * 16 * NT;
+        uint8_t *const buf = lds + NS * SLOT + wv * (16 * 16 * NT * 4);
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const long at = ((long)t.e * a.rows + r0 + 16 * i) * a.cols + c0;
+#pragma unroll
+            for (int j = 0; j < NT; j++) asm volatile("" : "+v"(acc[i][j]));    /* out of the accumulators one row of tiles at a time */
+            if (a.w_f32) g53_rows_out<float, NT, true>(buf, (float *)a.out + at, a.cols, acc[i], a.rows - r0 - 16 * i, a.cols - c0, a.add);
+            else g53_rows_out<E, NT, true>(buf, (E *)a.out + at, a.cols, acc[i], a.rows - r0 - 16 * i, a.cols - c0, a.add);
+        }
+    }
+    g53_loads_left<0>();                                    /* no load outlives the workgroup's LDS */
 }
 
 /* Threads of a launch are counted in 32 bits. */
@@ -290,6 +575,25 @@ template <typename E, int OP, int WR, int WC, int MT, int NT, int NS, bool DMA> 
     return 0;
 }
 
+template <typename E, int WR, int WC, int MT, int NT, int NS> static int matrices(G53EmArgs a)
+{
+    constexpr int BM = 16 * MT * WR, BN = 16 * NT * WC;
+    constexpr size_t LDS = (size_t)NS * (BM + BN) * 128 + WR * WC * 16 * 16 * NT * 4;
+    static int allowed = 0;
+    if (!allowed) {
+        G53_TRY(hipFuncSetAttribute((const void *)k_emats<E, WR, WC, MT, NT, NS>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)LDS));
+        allowed = 1;
+    }
+    a.across = (a.cols + BN - 1) / BN;
+    a.down = (a.rows + BM - 1) / BM;
+    const long total = (long)a.NE * a.down * a.across, stay = g53h_num_cus() / 8 * 8 * (LDS > 80 * 1024 ? 1 : 2);
+    const dim3 grid((unsigned)(total < stay ? (total + 7) / 8 * 8 : stay));
+    hipLaunchKernelGGL((k_emats<E, WR, WC, MT, NT, NS>), grid, dim3(64 * WR * WC), LDS, g53h_stream(), a);
+    G53_LAUNCHED("k_emats");
+    return 0;
+}
+
 template <typename E, int OP> static int by_size(const G53EmArgs &a, long n)
 {
     /* whole pieces of 16 bytes at multiples of 16 */
@@ -297,6 +601,28 @@ template <typename E, int OP> static int by_size(const G53EmArgs &a, long n)
                          : OP == G53_EM_ROWS ? (uintptr_t)a.dy | (uintptr_t)a.w : (uintptr_t)a.dy | (uintptr_t)a.x;
     const size_t odd = (a.cols * sizeof(E)) | (OP == G53_EM_FWD ? 0 : a.rows * sizeof(E));
     if ((at | odd) & 15) return launch<E, OP, 2, 2, 4, 4, 2, false>(a, n);
+    if constexpr (sizeof(E) == 2 && OP == G53_EM_MATS) return matrices<E, 2, 2, 4, 4, 2>(a);
+    if constexpr (sizeof(E) == 2 && OP != G53_EM_MATS) {
+        /* Experts' rows count as all alike, since the host does not know them. Tiles of 256 x 256 read LDS least for a
+         * product, where there are as many as CUs; of 128 x 128 where there are two a CU; few rows take tiles of 64 x 128 and
+         * 32 x 128, of which two workgroups a CU keep up to 96 KB of matrices on their way. us, bf16, forward / rows:
+         *     4096 x 4096, 64 experts, top-8   256       128       64 x 256  64 x 128  32 x 128
+         *     4096 tokens                  1094/1269 1299/1319 1534/1522 1601/1581 2286/2259
+         *     1024                           423/476   465/469   507/480   518/505   723/697
+         *     256                            307/265   296/267   295/247   284/263   319/291
+         *     1                               74/78     66/66     55/53     50/48     49/48
+         *     2048 x 1024, 32 experts, top-4
+         *     1024                            39/67     46/43     49/54     48/47     60/59
+         *     64                              23/40     21/32     18/26     19/19     18/19                              */
+        const long busy = a.NE < n ? a.NE : n, mean = (n + busy - 1) / busy, cus = g53h_num_cus();
+        const int N = OP == G53_EM_FWD ? a.rows : a.cols;
+        auto tiles = [&](int bm, int bn) { return (n / bm + busy) * ((N + bn - 1) / bn); };
+        if (mean >= 64 && tiles(256, 256) >= cus) return launch<E, OP, 2, 2, 8, 8, 2, true>(a, n);
+        if (mean >= 128 && tiles(128, 128) >= 2 * cus) return launch<E, OP, 2, 2, 4, 4, 2, true>(a, n);
+        if (OP == G53_EM_ROWS && mean > 1 && tiles(64, 256) >= 2 * cus) return launch<E, G53_EM_ROWS, 1, 4, 4, 4, 3, true>(a, n);
+        if (mean > 4 && tiles(64, 128) >= 2 * cus) return launch<E, OP, 1, 4, 4, 2, 3, true>(a, n);
+        return launch<E, OP, 1, 4, 2, 2, 3, true>(a, n);
+    }
     return launch<E, OP, 2, 2, 4, 4, 2, true>(a, n);
 }
 
@@ -316,7 +642,8 @@ __global__ void __launch_bounds__(256) k_swiglu_grad(E *dgu, const E *dact, cons
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const float gc = g[i] > limit ? limit : g[i], uc = u[i] > limit ? limit : (u[i] < -limit ? -limit : u[i]);
-        const float x = expf(-fabsf(gc)), s = (gc >= 0.0f ? 1.0f : x) / (1.0f + x);      /* no overflow: small, not zero */
+        const bool low = gc < -80.0f;       /* there 1 + exp(g) is 1, and exp(-g) may overflow */
+        const float x = expf(low ? gc : -gc), s = low ? x : 1.0f / (1.0f + x);
         const float dg = d[i] * uc * s * (1.0f + gc * (1.0f - s)), du = d[i] * gc * s;
         const bool g_out = g[i] > limit, u_out = u[i] > limit || u[i] < -limit;
         g[i] = g_out ? 0.0f : dg;
@@ -400,6 +727,7 @@ extern "C" int g53h_sorted_mm_grad(void *dx, void *dw, int dw_dt, int add, const
     if (!rc && dw) {
         a.out = dw;
         a.pair = gather ? p->pair : nullptr;
+        if (!gather) a.topk = g53_div_of(1);
         a.w_f32 = dw_dt == G53H_F32;
         a.add = add != 0;
         G53_BY_TYPE(dt, rc = (by_size<E, G53_EM_MATS>(a, n)));

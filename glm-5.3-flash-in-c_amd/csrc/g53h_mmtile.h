@@ -35,7 +35,7 @@ template <class V> __device__ __forceinline__ V g53_uniform_load(const V *p)
 /* 16 bytes per lane from p to LDS byte lds + 16 * lane. M0 holds the LDS address and is written ahead of the load. */
 __device__ __forceinline__ void g53_to_lds(const uint8_t *p, uint32_t lds)
 {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
 }
 /* At most n loads of the wave are on their way behind this; then every wave of the workgroup gets here. */
 template <int n> __device__ __forceinline__ void g53_loads_left()
@@ -49,19 +49,18 @@ __device__ __forceinline__ void g53_meet()
     asm volatile("" ::: "memory");
 }
 
-/* p / topk for a pair number p (below 2^31) by a product: mul = ceil(2^(31 + l) / topk), shift = 31 + l, l = the bits of
- * topk - 1. */
+/* p / topk for a pair number p (below 2^31) by a product: mul = ceil(2^(31 + l) / topk), l = the bits of topk - 1. */
 struct G53Div {
     uint32_t mul;
-    int shift;
+    int l;
 };
 static inline G53Div g53_div_of(int d)
 {
     int l = 0;
     while ((1 << l) < d) l++;
-    return {(uint32_t)(((1ull << (31 + l)) + (unsigned)d - 1) / (unsigned)d), 31 + l};
+    return {(uint32_t)(((1ull << (31 + l)) + (unsigned)d - 1) / (unsigned)d), l};
 }
-__device__ __forceinline__ int g53_div(int p, G53Div d) { return (int)((uint64_t)(uint32_t)p * d.mul >> d.shift); }
+__device__ __forceinline__ int g53_div(int p, G53Div d) { return (int)(__umulhi((uint32_t)p << 1, d.mul) >> d.l); }
 
 /* Rows [first, last) of expert e: the tile `item / across` in the experts' order, tiles of TM rows; n the tile across.
  * Items are dealt to the 8 dies in runs of up to 32, about what a die has in work at a time, so that its cache serves a
@@ -88,7 +87,7 @@ __device__ __forceinline__ bool g53_tile_item(const int *__restrict__ offsets, i
         if (lane >= d) incl += o;
     }
     const long total = (long)__builtin_amdgcn_readlane(incl, 63) * across;
-    const int run = total >= 256 ? 32 : total >= 16 ? (int)(total / 8) : 1;
+    const int run = total >= 256 ? 16 : total >= 16 ? (int)(total / 8) : 1;
     const long i = wg >> 3, item = ((i / run) * 8 + (wg & 7)) * run + i % run;
     if (item >= total) return false;
     const unsigned long long in = __ballot((long)incl * across > item);
@@ -115,7 +114,7 @@ __device__ __forceinline__ bool g53_tile_item(const int *__restrict__ offsets, i
 /* Where a lane's 16 bytes of a chunk come from, and how many of them there are (16 and more: all, 0 and less: none). */
 struct G53Piece {
     const uint8_t *p;
-    long n;
+    int n;
 };
 /* The piece in registers, zeros behind its end, at any alignment of its elements (of type E). */
 template <typename E> __device__ __forceinline__ g53_v4w g53_piece(const G53Piece &s)
@@ -183,8 +182,8 @@ template <typename E> __device__ __forceinline__ g53_v4f g53_mm(const G53Frag<E>
 }
 
 /* Fragments of 32 summed elements (lane (m, q) = (lane % 16, lane / 16): row m, elements 8 q .. 8 q + 7) from a chunk
- * at LDS address `at`, whose rows start at row0 (a multiple of 16), tile t of 16 rows, step j of 32 elements. */
-template <typename E> struct G53Along {
+ * at LDS address `at`, whose rows start at row0 (a multiple of 16), tile t of 16 rows, every STRIDE-th, step j of 32 elements. */
+template <typename E, int STRIDE = 1> struct G53Along {
     int at[2];
     __device__ __forceinline__ void setup(int row0)
     {
@@ -196,49 +195,50 @@ template <typename E> struct G53Along {
     __device__ __forceinline__ void read(G53Frag<E> &o, const uint8_t *lds, int t, int j) const
     {
         if constexpr (sizeof(E) == 4) {
-            const g53_v4f a = *(const g53_v4f *)(lds + at[0] + t * 2048), b = *(const g53_v4f *)(lds + at[1] + t * 2048);
+            const g53_v4f a = *(const g53_v4f *)(lds + at[0] + t * STRIDE * 2048), b = *(const g53_v4f *)(lds + at[1] + t * STRIDE * 2048);
             float v[8];
 #pragma unroll
             for (int i = 0; i < 4; i++) { v[i] = a[i]; v[4 + i] = b[i]; }
             g53_planes(o, v);
         } else {
-            o.v[0] = *(const typename G53Mm<E>::V *)(lds + at[j] + t * 2048);
+            o.v[0] = *(const typename G53Mm<E>::V *)(lds + at[j] + t * STRIDE * 2048);
         }
     }
 };
 /* The same from a chunk of rows of R columns each, whose columns start at col0: NT tiles of 16. */
-template <typename E, int R, int NT> struct G53Across {
+template <typename E, int R, int NT, int STRIDE = 1> struct G53Across {
     static constexpr int RB = R * sizeof(E), U = RB / 16;         /* bytes and pieces of a row */
-    int at[NT];
+    int at0;
     static __device__ __forceinline__ int place(int k)
     {
         return (sizeof(E) == 4 ? 4 * (k >> 3 & 3) : 2 * ((k & 3) | (k >> 3 & 1) << 2)) & (U - 1);
     }
+    /* Of rows k, k + step, k + 2 step, ... how many until places repeat. */
+    template <int step> static constexpr int turns()
+    {
+        constexpr int period = sizeof(E) == 4 ? 32 : 16;
+        static_assert(step % 8 == 0, "rows of eight");
+        return step % period ? period / step : 1;
+    }
+    /* A tile's columns are other bits of a place than col0's: one address, the others by exclusive or. */
     __device__ __forceinline__ void setup(int col0)
     {
         const int m = threadIdx.x & 15, q = threadIdx.x >> 4 & 3;
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int c = col0 + 16 * t;
-            if (sizeof(E) == 4) {
-                const int k = 8 * q, u = (c + m) >> 2;
-                at[t] = k * RB + ((u ^ place(k)) << 4) + (m & 3) * 4;
-            } else {
-                const int k = 8 * q + (m >> 2), u = (c >> 3) + (m >> 1 & 1);
-                at[t] = k * RB + ((u ^ place(k)) << 4) + (m & 1) * 8;
-            }
-        }
+        const int k = sizeof(E) == 4 ? 8 * q : 8 * q + (m >> 2);
+        const int u = sizeof(E) == 4 ? (col0 + m) >> 2 : (col0 >> 3) + (m >> 1 & 1);
+        at0 = k * RB + ((u ^ place(k)) << 4) + (sizeof(E) == 4 ? (m & 3) * 4 : (m & 1) * 8);
     }
     __device__ __forceinline__ void read(G53Frag<E> &o, const uint8_t *lds, int t, int j) const
     {
+        const int at = at0 ^ (16 * STRIDE * t * (int)sizeof(E));
         if constexpr (sizeof(E) == 4) {
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = *(const float *)(lds + at[t] + i * RB);
+            for (int i = 0; i < 8; i++) v[i] = *(const float *)(lds + at + i * RB);
             g53_planes(o, v);
         } else {
-            const g53_v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((G53LdsTr)(lds + at[t] + j * 32 * RB));
-            const g53_v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((G53LdsTr)(lds + at[t] + (j * 32 + 4) * RB));
+            const g53_v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((G53LdsTr)(lds + at + j * 32 * RB));
+            const g53_v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((G53LdsTr)(lds + at + (j * 32 + 4) * RB));
             o.v[0] = __builtin_bit_cast(typename G53Mm<E>::V, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
@@ -266,12 +266,67 @@ template <typename O> __device__ __forceinline__ void g53_store4(O *row, long c,
     }
 }
 
-/* The clamped SwiGLU, as g53h_swiglu's. */
-__device__ __forceinline__ float g53_swiglu1(float g, float u, float limit)
+/* 16 rows of a wave's NT tiles to memory by whole rows, through 16 x NT x 16 elements of LDS of its own: a store of the sums as
+ * they lie would leave 64 bytes of each of 16 rows, and such halves of lines cost twice (see g53h_emm.hip). out: the first
+ * row's first column, ld: elements from row to row; rows, cols: how many there are. PAST:
+ * whole pieces go past the caches. Rows of less than 128 bytes go as they lie. */
+template <typename O, int NT, bool PAST>
+__device__ __forceinline__ void g53_rows_out(uint8_t *buf, O *out, long ld, g53_v4f (&acc)[NT], int rows, long cols, bool old)
+{
+    if constexpr (NT * 16 * sizeof(O) < 128) {
+        const int m = threadIdx.x & 15, q = threadIdx.x >> 4 & 3;
+        if (m < rows)
+#pragma unroll
+            for (int t = 0; t < NT; t++) g53_store4(out + m * ld + 4 * q, 16 * t, cols - 4 * q, acc[t], old);
+        return;
+    } else {
+    constexpr int RB = NT * 16 * sizeof(O), PR = RB / 16, RI = 64 / PR, EP = 16 / sizeof(O), SW = (PR < 8 ? PR : 8) - 1;
+    typedef O V4 __attribute__((ext_vector_type(4)));
+    typedef O VP __attribute__((ext_vector_type(EP)));
+    struct __attribute__((packed, aligned(2))) Any { VP v; };
+    const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int b = (16 * t + 4 * q) * (int)sizeof(O);
+        if (old && sizeof(O) == 2) {                        /* added in fp32: before it is rounded */
+            const O *was = out + m * ld;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (m < rows && 16 * t + 4 * q + k < cols) acc[t][k] += (float)was[16 * t + 4 * q + k];
+        }
+        V4 o;
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[k] = (O)acc[t][k];
+        *(V4 *)(buf + m * RB + (((b >> 4) ^ (m & SW)) << 4) + (b & 15)) = o;
+    }
+#pragma unroll
+    for (int k = 0; k < 16 / RI; k++) {
+        const int r = k * RI + lane / PR, p = lane % PR;
+        VP v = *(const VP *)(buf + r * RB + ((p ^ (r & SW)) << 4));
+        O *to = out + r * ld + p * EP;
+        if (r >= rows) continue;
+        if (p * EP + EP <= cols) {
+            if (old && sizeof(O) == 4) v += ((const Any *)to)->v;
+            if (PAST && !((uintptr_t)to & 15)) __builtin_nontemporal_store(v, (VP *)to);
+            else ((Any *)to)->v = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < EP; i++)
+                if (p * EP + i < cols) to[i] = old && sizeof(O) == 4 ? v[i] + to[i] : v[i];
+        }
+    }
+    }
+}
+
+/* The clamped SwiGLU, as g53h_swiglu's, for a result of type O. One of 16 bits, whose half step is 2^-9 at best, takes the
+ * hardware's exponential and reciprocal (some 2^-20 off together): they take a quarter of the time, and at the end of a
+ * tile nothing covers it. */
+template <typename O> __device__ __forceinline__ float g53_swiglu1(float g, float u, float limit)
 {
     g = g > limit ? limit : g;
     u = u > limit ? limit : (u < -limit ? -limit : u);
-    return g / (1.0f + expf(-g)) * u;
+    if constexpr (sizeof(O) == 2) return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * u;
+    else return g / (1.0f + expf(-g)) * u;
 }
 
 #endif /* G53H_MMTILE_H */

@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
             for (int t = 0; t < NT / 2; t++) {
                 g53_v4f v;
 #pragma unroll
-                for (int k = 0; k < 4; k++) v[k] = g53_swiglu1(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
+                for (int k = 0; k < 4; k++) v[k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
                 g53_store4(row, n0 + (wc * NT / 2 + t) * 16 + 4 * q, a.half, v, false);
             }
         }

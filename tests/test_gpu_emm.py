@@ -257,3 +257,38 @@ def test_matrices_past_32_bits(L):
     at = (NE - 1) * rows * cols
     assert np.array_equal(dec(w.download(np.float16, rows * cols, 2 * at), F16).reshape(rows, cols), dv.T @ xv)
     assert not w.download(np.uint16, 1 << 20, 2 * (at - (1 << 20))).any()
+
+
+# (T, NE, N, K): as many tiles as every form of the kernel takes, with ends of each
+@pytest.mark.parametrize("T,NE,N,K", [(300, 1, 33032, 72), (200, 3, 12296, 136), (300, 1, 22024, 64), (100, 2, 33800, 40), (40, 40, 1800, 88),
+                                      (3, 3, 700, 520)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_every_tile(L, T, NE, N, K, dt):
+    say("tiles", T, NE, N, K, dt)
+    rng = np.random.default_rng(N)
+    idx = rng.integers(0, NE, (T, 1)).astype(np.int32)
+    offsets, pair, _ = sorted_plan(idx, NE)
+    plan = Plan(idx, NE)
+    xv, wv = values(rng, (T, K), dt, True), values(rng, (NE, N, K), dt, True)
+    x, w, ys, gu = Buf(xv, dt), Buf(wv, dt), Buf.out((T, N), dt), Buf.out((T, N), dt)
+    act = Buf.out((T, N // 2), dt)
+    check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, dt, 1, plan.c, w.ptr, N, K, 0.0))
+    check(L.g53h_sorted_mm(act.ptr, gu.ptr, x.ptr, dt, 1, plan.c, w.ptr, N, K, LIMIT))
+    ref = np.concatenate([xv[pair[offsets[e]:offsets[e + 1]]] @ wv[e].T for e in range(NE)])
+    assert np.array_equal(ys.val(), rounded(ref, dt)) and np.array_equal(gu.val(), ys.val())
+    want = swiglu(ref, LIMIT)
+    # sums are exact; the hardware's exponential and reciprocal 2^-20, the products 2^-23
+    close(act.val(), want, (2.0 ** -20 + HALF[dt]) * np.abs(want) + TINY[dt])
+    # the rows' gradient, of matrices the other way round: [K][N], dys [T][K]
+    wt = np.ascontiguousarray(wv.transpose(0, 2, 1))
+    w2, dx = Buf(wt, dt), Buf.out((T, N), dt)
+    dy = Buf(xv[pair], dt)
+    check(L.g53h_sorted_mm_grad(dx.ptr, None, dt, 0, dy.ptr, None, dt, 1, plan.c, w2.ptr, K, N))
+    assert np.array_equal(dx.get(), ys.get())
+    # the matrices' gradient [K][N] of the same rows and others
+    zv = values(rng, (T, N), dt, True)
+    z, dw = Buf(zv, dt), Buf.out((NE, K, N), F32)
+    check(L.g53h_sorted_mm_grad(None, dw.ptr, F32, 0, dy.ptr, z.ptr, dt, 0, plan.c, None, K, N))
+    for e in range(NE):
+        r = slice(offsets[e], offsets[e + 1])
+        assert np.array_equal(dw.val()[e], xv[pair[r]].T @ zv[r])
