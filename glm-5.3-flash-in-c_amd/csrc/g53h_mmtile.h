@@ -325,8 +325,12 @@ template <typename O> __device__ __forceinline__ float g53_swiglu1(float g, floa
 {
     g = g > limit ? limit : g;
     u = u > limit ? limit : (u < -limit ? -limit : u);
-    if constexpr (sizeof(O) == 2) return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * u;
-    else return g / (1.0f + expf(-g)) * u;
+    if constexpr (sizeof(O) == 2) {
+        const float e = __expf(-fabsf(g));                  /* no overflow, so no reciprocal below the normal range */
+        return g * ((g >= 0.0f ? 1.0f : e) * __builtin_amdgcn_rcpf(1.0f + e)) * u;
+    } else {
+        return g / (1.0f + expf(-g)) * u;
+    }
 }
 
 #endif /* G53H_MMTILE_H */
