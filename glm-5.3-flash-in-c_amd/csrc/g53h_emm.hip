@@ -29,7 +29,7 @@ struct G53EmArgs {
     int w_f32, add;                     /* matrices' gradient: fp32, added to what is there      */
     int across, down;                   /* tiles across a row of results; of a matrix's rows     */
     G53Div topk;
-    long wg0;                           /* first workgroup of the launch                         */
+    long wg0, wgs;                      /* first workgroup of the launch, workgroups of all      */
 };
 
 /* One tile of OP. DMA: operand rows start at multiples of 16 bytes and are whole pieces. */
@@ -51,14 +51,12 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emm(G53E
     if constexpr (OP == G53_EM_MATS) {
         const int per = a.across * a.down;
         const long total = (long)a.NE * per;
-        const int run = total >= 256 ? 32 : total >= 16 ? (int)(total / 8) : 1;
-        const long i = wg >> 3, item = ((i / run) * 8 + (wg & 7)) * run + i % run;
+        const long item = g53_deal(wg, total);
         if (item >= total) return;
         it.e = (int)(item / per);
-        const int in = (int)(item % per), g = in / (8 * a.across), in_g = in % (8 * a.across);
-        const int of = a.down - 8 * g < 8 ? a.down - 8 * g : 8;
-        m0 = (8 * g + in_g % of) * BM;
-        it.n = in_g / of;
+        int t;
+        g53_eight(item % per, a.down, a.across, t, it.n);
+        m0 = t * BM;
         it.first = g53_uniform_load(a.offsets + it.e);
         it.last = g53_uniform_load(a.offsets + it.e + 1);
     } else {
@@ -384,24 +382,23 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emats(G5
     const long wrow = (long)a.cols * sizeof(E), drow = (long)a.rows * sizeof(E);
     const int per = a.across * a.down;
     const long total = (long)a.NE * per;
-    const int len = total >= 256 ? 32 : total >= 16 ? (int)(total / 8) : 1;
     /* the tile of a workgroup's turn w: runs of tiles by die, eight tiles down with each across */
     struct Tile {
         int e, m0, n0, first, live;
     };
     auto tile_of = [&](long w, Tile &t) {
-        const long i = w >> 3, item = ((i / len) * 8 + (w & 7)) * len + i % len;
+        const long item = g53_deal(w, total);
         if (item >= total) return false;
         t.e = (int)(item / per);
-        const int in = (int)(item % per), g = in / (8 * a.across), in_g = in % (8 * a.across);
-        const int of = a.down - 8 * g < 8 ? a.down - 8 * g : 8;
-        t.m0 = (8 * g + in_g % of) * BM;
-        t.n0 = in_g / of * BN;
+        int m, n;
+        g53_eight(item % per, a.down, a.across, m, n);
+        t.m0 = m * BM;
+        t.n0 = n * BN;
         t.first = g53_uniform_load(a.offsets + t.e);
         t.live = g53_uniform_load(a.offsets + t.e + 1) - t.first;
         return true;
     };
-    const long turns = (total + 8l * len - 1) / (8l * len) * (8l * len);
+    const long turns = a.wgs;
     /* The stream: the tile and chunk to be asked for (none behind the last: zeros), and the one after it, whose tokens
      * are asked for a chunk ahead. */
     struct At {
@@ -565,7 +562,7 @@ template <typename E, int OP, int WR, int WC, int MT, int NT, int NS, bool DMA> 
     a.down = (a.rows + BM - 1) / BM;
     const long most = a.NE < n ? a.NE : n;              /* experts that can have rows */
     const long items = OP == G53_EM_MATS ? (long)a.NE * a.down * a.across : (n / BM + most) * a.across;
-    const long wgs = (items + 7) / 8 * 8 + (items < 8 ? 8 : items < 256 ? (items + 7) / 8 * 8 : 256);   /* whole runs on every die */
+    const long wgs = g53_deal_wgs(items);
     for (long w0 = 0; w0 < wgs; w0 += G53_EM_WGS) {
         a.wg0 = w0;
         const dim3 grid((unsigned)(wgs - w0 < G53_EM_WGS ? wgs - w0 : G53_EM_WGS));
@@ -588,7 +585,8 @@ template <typename E, int WR, int WC, int MT, int NT, int NS> static int matrice
     a.across = (a.cols + BN - 1) / BN;
     a.down = (a.rows + BM - 1) / BM;
     const long total = (long)a.NE * a.down * a.across, stay = g53h_num_cus() / 8 * 8 * (LDS > 80 * 1024 ? 1 : 2);
-    const dim3 grid((unsigned)(total < stay ? (total + 7) / 8 * 8 : stay));
+    a.wgs = g53_deal_wgs(total);
+    const dim3 grid((unsigned)(a.wgs < stay ? a.wgs : stay));
     hipLaunchKernelGGL((k_emats<E, WR, WC, MT, NT, NS>), grid, dim3(64 * WR * WC), LDS, g53h_stream(), a);
     G53_LAUNCHED("k_emats");
     return 0;

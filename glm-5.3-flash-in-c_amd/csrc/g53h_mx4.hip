@@ -8,6 +8,7 @@
  * row m and block q of four, and their scale. Products and scales are exact; sums are fp32.
  */
 #include <hip/hip_runtime.h>
+#include <type_traits>
 
 #include "g53h.h"
 #include "g53h_elem.h"
@@ -89,13 +90,15 @@ struct G53MxArgs {
     long wg0;
 };
 
-/* One tile: 256 columns a chunk, the scales of two chunks a time. */
-template <typename E, int WR, int WC, int MT, int NT, int NS>
+/* One tile, by the stream of k_emm (g53h_emm.hip): a chunk is 256 columns, two steps of 128. Scales come 16 a row at a time,
+ * those of two chunks, through registers, which turn each quarter's four side by side: asked for in the second half of
+ * an odd chunk, put down in that of the even one behind it, and read in that of the odd one behind that. */
+template <typename E, int WR, int WC, int MT, int NT>
 __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
 {
     constexpr int NW = WR * WC, BM = 16 * MT * WR, BN = 16 * NT * WC, SLOT = (BM + BN) * 128, SEG = (BM + BN) * 16;
     constexpr int IA = BM / (8 * NW), IB = BN / (8 * NW), IS = (BM + BN + 64 * NW - 1) / (64 * NW);
-    static_assert(IA * 8 * NW == BM && IB * 8 * NW == BN && NS == 2, "whole instructions");
+    static_assert(IA * 8 * NW == BM && IB * 8 * NW == BN, "whole instructions");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wv / WC, wc = wv % WC;
@@ -106,15 +109,17 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
     if (a.offsets) {
         if (!g53_tile_item(a.offsets, a.NE, BM, a.across, wg, it)) return;
     } else {
-        const long item = wg / a.across;
-        if (item * BM >= a.T) return;
+        const int tiles = (int)((unsigned)(a.T + BM - 1) / BM);
+        const long total = (long)tiles * a.across, item = g53_deal(wg, total);
+        if (item >= total) return;
+        int t;
+        g53_eight(item, tiles, a.across, t, it.n);
         it.e = 0;
-        it.n = (int)(wg % a.across);
-        it.first = (int)(item * BM);
+        it.first = t * BM;
         it.last = a.T - it.first > BM ? it.first + BM : a.T;
     }
     const int n0 = it.n * cut, live = it.last - it.first, rb = a.cols / 2, sb = a.cols / 32;
-    const int chunks = (rb + 127) / 128, segs = (chunks + 1) / 2;
+    const int chunks = (rb + 127) / 128;
     const long e0 = (long)it.e * a.rows;
     auto x_row = [&](int r) -> long {
         const int s = it.first + (r < live ? r : live - 1);
@@ -142,16 +147,13 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
         ps[i] = r < BM ? a.xs + x_row(r) * sb : a.s + w_row(r - BM < BN ? r - BM : BN - 1) * sb;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    auto ask = [&](int c, int slot) {
+    auto ask1 = [&](int c, int slot, int i) {
         const uint32_t to = lds0 + slot * SLOT + wv * 1024;
-        const bool in = c * 128 + u8 * 16 < rb;
-#pragma unroll
-        for (int i = 0; i < IA; i++) g53_to_lds(in ? pa[i] + (long)c * 128 : (const uint8_t *)&g53_nothing, to + i * NW * 1024);
-#pragma unroll
-        for (int i = 0; i < IB; i++)
-            g53_to_lds(in ? pb[i] + (long)c * 128 : (const uint8_t *)&g53_nothing, to + BM * 128 + i * NW * 1024);
+        const uint8_t *&p = i < IA ? pa[i < IA ? i : 0] : pb[i < IA ? 0 : i - IA];
+        g53_to_lds(u8 * 16 < rb - c * 128 ? p : (const uint8_t *)&g53_nothing, to + (i < IA ? i * NW * 1024 : BM * 128 + (i - IA) * NW * 1024));
+        p += 128;
+        asm volatile("" : "+v"(p));     /* one register pair a piece: else each of the loop's chunks gets its own */
     };
-    /* A row's 16 scales of a segment, each quarter's four side by side. */
     g53_v4w rs[IS];
     auto fetch = [&](int seg) {
         const int n = sb - seg * 16;
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
                 }
         }
     };
-    uint8_t *const lds_s = lds + NS * SLOT;
+    uint8_t *const lds_s = lds + 2 * SLOT;
     auto put = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < IS; i++) {
@@ -182,92 +184,125 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
         }
     };
     const int m = lane & 15, q = lane >> 4;
-    const int fa = (wr * 16 * MT + m) * 128 + ((q ^ (m & 7)) << 4), fb = BM * 128 + (wc * 16 * NT + m) * 128 + ((q ^ (m & 7)) << 4);
-    const int sa = (wr * 16 * MT + m) * 16 + 4 * q, sbt = (BM + wc * 16 * NT + m) * 16 + 4 * q;
+    const int fa = (wr * 16 + m) * 128 + ((q ^ (m & 7)) << 4), fb = BM * 128 + (wc * 16 * NT + m) * 128 + ((q ^ (m & 7)) << 4);
+    const int sa = (wr * 16 + m) * 16 + 4 * q, sw_at = (BM + wc * 16 * NT + m) * 16 + 4 * q;
     g53_v4f acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[i][t] = (g53_v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    auto frag = [&](const uint8_t *p) {
-        const g53_v4w v = *(const g53_v4w *)p;
-        return (g53_v8i){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
-    };
-    auto multiply = [&](int slot, int c) {
-        const uint8_t *l = lds + slot * SLOT, *ls = lds_s + (c >> 1 & 1) * SEG;
-        const int sh = (c & 1) * 16;
-        int wsc[NT], xsc[MT];
+    auto run = [&](auto M_) {
+        constexpr int M = decltype(M_)::value;              /* row tiles of a wave that are there */
+        constexpr int RD = (M + NT + M - 1) / M, IM = IA * M / MT > 0 ? IA * M / MT : 1, AD = (IM + IB + M - 1) / M;
+        g53_v4w va[2][M], vb[2][NT];
+        int xs[M], ws[NT];
+        auto read1 = [&](int to, int slot, int j, int i) {
+            const uint8_t *l = lds + slot * SLOT;
+            if (i < NT) vb[to][i] = *(const g53_v4w *)(l + (fb ^ j * 64) + i * 2048);
+            else va[to][i - NT] = *(const g53_v4w *)(l + (fa ^ j * 64) + (i - NT) * (WR * 2048));
+        };
+        auto scale_x = [&](int buf, int i) { xs[i] = *(const int *)(lds_s + buf * SEG + sa + i * (WR * 256)); };
+        auto scale_w = [&](int buf) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) wsc[t] = *(const int *)(ls + sbt + t * 256) >> sh;
+            for (int t = 0; t < NT; t++) ws[t] = *(const int *)(lds_s + buf * SEG + sw_at + t * 256);
+        };
+#define G53_MX_ROW(i, h, byte)                                                                                          \
+    _Pragma("unroll") for (int t = 0; t < NT; t++) {                                                                    \
+        const g53_v8i b = {(int)vb[h][t][0], (int)vb[h][t][1], (int)vb[h][t][2], (int)vb[h][t][3], 0, 0, 0, 0};        \
+        const g53_v8i v = {(int)va[h][i][0], (int)va[h][i][1], (int)va[h][i][2], (int)va[h][i][3], 0, 0, 0, 0};        \
+        acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, v, acc[i][t], 4, 4, byte, ws[t], byte, xs[i]); \
+    }                                                                                                                   \
+    __builtin_amdgcn_sched_barrier(0)
+        fetch(0);
+        put(0);
 #pragma unroll
-        for (int i = 0; i < MT; i++) xsc[i] = *(const int *)(ls + sa + i * 256) >> sh;
-#define G53_MX_STEP(j)                                                                                                   \
-    do {                                                                                                                 \
-        g53_v8i b[NT];                                                                                                   \
-        _Pragma("unroll") for (int t = 0; t < NT; t++) b[t] = frag(l + (fb ^ (j) * 64) + t * 2048);                      \
-        _Pragma("unroll") for (int i = 0; i < MT; i++) {                                                                 \
-            const g53_v8i v = frag(l + (fa ^ (j) * 64) + i * 2048);                                                      \
-            _Pragma("unroll") for (int t = 0; t < NT; t++) acc[i][t] =                                                   \
-                __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[t], v, acc[i][t], 4, 4, j, wsc[t], j, xsc[i]);        \
-        }                                                                                                                \
-    } while (0)
-        G53_MX_STEP(0);
-        G53_MX_STEP(1);
-#undef G53_MX_STEP
-    };
-    fetch(0);
-    put(0);
-    ask(0, 0);
-    for (int c = 0; c < chunks; c++) {
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int i = 0; i < IM + IB; i++) ask1(c, c, i < IM ? i : i - IM + IA);
+        fetch(1);
         g53_loads_left<0>();
         g53_meet();
-        /* the next segment's scales: asked for with its first chunk's time to spare, put before more loads are asked for */
-        const int seg = c >> 1;
-        if ((c & 1) && seg + 1 < segs) put(seg + 1 & 1);
-        if (!(c & 1) && seg + 1 < segs) fetch(seg + 1);
-        if (c + 1 < chunks) ask(c + 1, c + 1 & 1);
-        multiply(c & 1, c);
-    }
+#pragma unroll
+        for (int i = 0; i < M + NT; i++) read1(0, 0, 0, i);
+#pragma unroll
+        for (int i = 0; i < M; i++) scale_x(0, i);
+        scale_w(0);
+        /* chunk c, in slot c & 1 */
+        auto chunk = [&](int c, auto odd_) {
+            constexpr int odd = decltype(odd_)::value;
+#pragma unroll
+            for (int i = 0; i < M; i++) {
+#pragma unroll
+                for (int k = i * RD; k < (i + 1) * RD && k < M + NT; k++) read1(1, odd, 1, k);
+                G53_MX_ROW(i, 0, 2 * odd);
+            }
+            g53_loads_left<0>();
+            g53_meet();
+            if (odd) fetch((c + 1) / 2 + 1);
+            else put((c / 2 + 1) & 1);
+#pragma unroll
+            for (int i = 0; i < M; i++) {
+#pragma unroll
+                for (int k = i * AD; k < (i + 1) * AD && k < IM + IB; k++) ask1(c + 2, odd, k < IM ? k : k - IM + IA);
+#pragma unroll
+                for (int k = i * RD; k < (i + 1) * RD && k < M + NT; k++) read1(0, odd ^ 1, 0, k);
+                G53_MX_ROW(i, 1, 2 * odd + 1);
+                if (odd) scale_x((c + 1) / 2 & 1, i);       /* the next segment's, each in the place of the one just used */
+            }
+            if (odd) scale_w((c + 1) / 2 & 1);
+        };
+        for (int c = 0;; c += 2) {
+            chunk(c, std::integral_constant<int, 0>{});
+            if (c + 1 >= chunks) break;
+            chunk(c + 1, std::integral_constant<int, 1>{});
+            if (c + 2 >= chunks) break;
+        }
+#undef G53_MX_ROW
+        g53_loads_left<0>();                                /* no load outlives the workgroup's LDS */
+    };
+    if constexpr (MT < 4) run(std::integral_constant<int, MT>{});
+    else if (live <= BM / 4) run(std::integral_constant<int, MT / 4>{});
+    else if (live <= BM / 2) run(std::integral_constant<int, MT / 2>{});
+    else run(std::integral_constant<int, MT>{});
+    g53_meet();
+    uint8_t *const buf = lds + wv * (16 * 16 * NT * (int)sizeof(E));
 #pragma unroll
     for (int i = 0; i < MT; i++) {
-        const int r = (wr * MT + i) * 16 + m;
-        if (r >= live) continue;
-        E *row = (E *)a.out + (long)(it.first + r) * a.half;
+        const int r0 = (i * WR + wr) * 16;
+        asm volatile("" ::: "memory");                      /* out of the accumulators one row of tiles at a time */
+        if (r0 >= live) continue;
+        const int c = n0 + wc * (sw ? NT / 2 : NT) * 16;
+        E *at = (E *)a.out + (long)(it.first + r0) * a.half + c;
         if (!sw) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) g53_store4(row, n0 + (wc * NT + t) * 16 + 4 * q, a.half, acc[i][t], false);
+            g53_rows_out<E, NT, false>(buf, at, a.half, acc[i], live - r0, a.half - c, false);
         } else {
+            g53_v4f v[NT / 2];
 #pragma unroll
-            for (int t = 0; t < NT / 2; t++) {
-                g53_v4f v;
+            for (int t = 0; t < NT / 2; t++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) v[k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
-                g53_store4(row, n0 + (wc * NT / 2 + t) * 16 + 4 * q, a.half, v, false);
-            }
+                for (int k = 0; k < 4; k++) v[t][k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
+            g53_rows_out<E, NT / 2, false>(buf, at, a.half, v, live - r0, a.half - c, false);
         }
     }
 }
 
-template <typename E, int WR, int WC, int MT, int NT, int NS> static int launch(G53MxArgs a, long n)
+template <typename E, int WR, int WC, int MT, int NT> static int launch(G53MxArgs a, long n)
 {
     constexpr int BM = 16 * MT * WR, BN = 16 * NT * WC;
-    constexpr size_t LDS = (size_t)NS * (BM + BN) * 128 + 2 * (BM + BN) * 16;
+    constexpr size_t LDS = 2 * (size_t)(BM + BN) * (128 + 16);
+    static_assert(LDS >= WR * WC * 16 * 16 * NT * sizeof(E), "rows on their way out");
     static int allowed = 0;
     if (!allowed) {
-        G53_TRY(hipFuncSetAttribute((const void *)k_mx4<E, WR, WC, MT, NT, NS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
+        G53_TRY(hipFuncSetAttribute((const void *)k_mx4<E, WR, WC, MT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
         allowed = 1;
     }
     const int cut = a.limit > 0.0f ? BN / 2 : BN;
     a.across = (a.half + cut - 1) / cut;
-    long wgs = ((n + BM - 1) / BM) * a.across;
-    if (a.offsets) {
-        const long items = (n / BM + (a.NE < n ? a.NE : n)) * a.across;
-        wgs = (items + 7) / 8 * 8 + (items < 8 ? 8 : items < 256 ? (items + 7) / 8 * 8 : 256);      /* whole runs on every die */
-    }
+    const long wgs = g53_deal_wgs((a.offsets ? n / BM + (a.NE < n ? a.NE : n) : (n + BM - 1) / BM) * a.across);
     for (long w0 = 0; w0 < wgs; w0 += G53_MX_WGS) {
         a.wg0 = w0;
         const dim3 grid((unsigned)(wgs - w0 < G53_MX_WGS ? wgs - w0 : G53_MX_WGS));
-        hipLaunchKernelGGL((k_mx4<E, WR, WC, MT, NT, NS>), grid, dim3(64 * WR * WC), LDS, g53h_stream(), a);
+        hipLaunchKernelGGL((k_mx4<E, WR, WC, MT, NT>), grid, dim3(64 * WR * WC), LDS, g53h_stream(), a);
         G53_LAUNCHED("k_mx4");
     }
     return 0;
@@ -344,7 +379,19 @@ static int mx_product(const char *who, void *y, int dt, const G53hMx4 *x, const 
     return 0;
 }
 
-template <typename E> static int by_size(const G53MxArgs &a, long n) { return launch<E, 2, 2, 4, 4, 2>(a, n); }
+/* Tiles by the rows that experts have, all alike, as in g53h_emm.hip. us, bf16, tiles of 128 x 128, 64 x 128, 32 x 128 (of
+ * 256 x 128, one workgroup a CU, more than any):
+ *     4096 x 4096, 64 experts, top-8: 1024 tokens 158 210 255, 256 93 98 105, 16 55 54 62, 1 18.5 18.3 18.0
+ *     1024 x 1024, 16 experts, top-4: 1024 tokens 12 16 16, 64 6.5 6.4 5.8
+ *     8192 x 8192: 8192 rows 349 503 661, 512 30 31 48, 64 24 24 22, 1 20.6 20.4 20.5 */
+template <typename E> static int by_size(const G53MxArgs &a, long n)
+{
+    const long busy = a.offsets ? (a.NE < n ? a.NE : n) : 1, mean = (n + busy - 1) / busy, cus = g53h_num_cus();
+    auto tiles = [&](int bm, int bn) { return (a.offsets ? n / bm + busy : (n + bm - 1) / bm) * ((a.rows + bn - 1) / bn); };
+    if (mean >= 32 && tiles(128, 128) >= cus) return launch<E, 2, 2, 4, 4>(a, n);
+    if (mean > 1 && tiles(64, 128) >= 2 * cus) return launch<E, 1, 4, 4, 2>(a, n);
+    return launch<E, 1, 4, 2, 2>(a, n);
+}
 
 extern "C" int g53h_mm_mx4(void *y, int dt, const G53hMx4 *x, const G53hMx4 *m, float swiglu_limit)
 {

@@ -241,3 +241,30 @@ def test_offsets_past_32_bits(L):
     want_lv, want_s = quant(wide(lv, np.full((last, cols // 32), 127, np.uint8)))
     assert np.array_equal(w2.download(np.uint8, last * cols // 2, (part - last) * cols // 2).reshape(last, -1), pack(want_lv))
     assert np.array_equal(s2.download(np.uint8, last * cols // 32, (part - last) * cols // 32).reshape(last, -1), want_s)
+
+
+# as many tiles as every form of the kernel takes, with ends of each
+@pytest.mark.parametrize("T,NE,rows,cols", [(200, 0, 17000, 320), (300, 3, 11000, 96), (70, 0, 34000, 64), (20, 10, 7000, 544), (3, 3, 1000, 1088)])
+def test_every_tile(L, T, NE, rows, cols):
+    say("tiles", T, NE, rows, cols)
+    rng = np.random.default_rng(rows)
+    x, m = Mx4.random(rng, T, cols, low=127, high=128), Mx4.random(rng, rows, cols, max(NE, 1), low=125, high=126)
+    y, act = Buf.out((T, rows), F32), Buf.out((T, rows // 2), BF16)
+    if NE:
+        idx = rng.integers(0, NE, (T, 1)).astype(np.int32)
+        offsets, pair, _ = sorted_plan(idx, NE)
+        plan = Plan(idx, NE)
+        check(L.g53h_sorted_mm_mx4(y.ptr, F32, x.c, 1, plan.c, m.c, 0.0))
+        check(L.g53h_sorted_mm_mx4(act.ptr, BF16, x.c, 1, plan.c, m.c, LIMIT))
+        ref = np.concatenate([x.wide[pair[offsets[e]:offsets[e + 1]]] @ m.wide[e * rows:(e + 1) * rows].T for e in range(NE)])
+    else:
+        check(L.g53h_mm_mx4(y.ptr, F32, x.c, m.c, 0.0))
+        check(L.g53h_mm_mx4(act.ptr, BF16, x.c, m.c, LIMIT))
+        ref = x.wide @ m.wide.T
+    assert np.array_equal(y.val(), ref)                      # multiples of 1 / 16 below 2^20: exact
+    g, u = np.split(ref, 2, 1)
+    with np.errstate(over="ignore"):
+        want = swiglu(ref, LIMIT)
+    # the hardware's exponential and reciprocal 2^-20; the exponential is zero where it lies below 2^-126
+    deep = np.where(g < -87, 2.0 ** -126 * np.abs(g * np.clip(u, -LIMIT, LIMIT)), 0)
+    close(act.val(), want, (2.0 ** -20 + HALF[BF16]) * np.abs(want) + TINY[BF16] + deep)
