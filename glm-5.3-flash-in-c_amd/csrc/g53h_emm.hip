@@ -127,40 +127,49 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emm(G53E
                 }
     };
     const int kbytes = (int)(K * (long)sizeof(E));                      /* along: of a row */
+    /* DMA: a row that is not there may have any address */
     auto piece_a = [&](int i, int c) -> G53Piece {
         if constexpr (!AX) {
             const uint8_t *p = pa[i];
             pa[i] += 128;
-            return {p, kbytes - c * 128 - u8 * 16};
-        } else return {pa[i % VA] + (c * KE + i / VA * (VA * KA * NW)) * drow,
-                     lane / Xa::U < live - c * KE - (i * NW + wv) * KA ? (DMA ? 16 : (int)drow - ca[i % VA]) : 0};
+            return {p, kbytes - c * 128 - u8 * 16, true};
+        } else {
+            const int left = live - c * KE - (i * NW + wv) * KA, k = c * KE + i / VA * (VA * KA * NW);
+            const bool row = lane / Xa::U < left;
+            if constexpr (DMA) return {pa[i % VA] + k * drow, 16, row};
+            return {pa[i % VA] + (row ? k : k + left - 1 - lane / Xa::U) * drow, (int)drow - ca[i % VA], row};
+        }
     };
     auto piece_b = [&](int i, int c) -> G53Piece {
         if constexpr (!BX) {
             const uint8_t *p = pb[i];
             pb[i] += 128;
-            return {p, kbytes - c * 128 - u8 * 16};
-        }
-        const int n = lane / Xb::U < (int)K - c * KE - (i * NW + wv) * KB ? (DMA ? 16 : (int)wrow - cb[i % VB]) : 0;
-        if constexpr (OP == G53_EM_ROWS) {
-            const uint8_t *p = pb[i % VB] + i / VB * (VB * KB * NW) * wrow;
-            if (i == IB - 1)
+            return {p, kbytes - c * 128 - u8 * 16, true};
+        } else {
+            const int left = (int)K - c * KE - (i * NW + wv) * KB, n = DMA ? 16 : (int)wrow - cb[i % VB];
+            const bool row = lane / Xb::U < left;
+            if constexpr (OP == G53_EM_ROWS) {
+                const uint8_t *p = pb[i % VB] + i / VB * (VB * KB * NW) * wrow;
+                if (!DMA && !row) p += (left - 1 - lane / Xb::U) * wrow;
+                if (i == IB - 1)
 #pragma unroll
-                for (int v = 0; v < VB; v++) pb[v] += KE * wrow;
-            return {p, n};
-        }
-        long t = 0;
+                    for (int v = 0; v < VB; v++) pb[v] += KE * wrow;
+                return {p, n, row};
+            }
+            long t = 0;
 #pragma unroll
-        for (int r = 0; r < KB; r++) {
-            const long at = (long)(a.pair ? g53_div(tok[OP == G53_EM_MATS ? i : 0][r], a.topk) : tok[OP == G53_EM_MATS ? i : 0][r]) * wrow;
-            t = r == 0 || lane / Xb::U == r ? at : t;
+            for (int r = 0; r < KB; r++) {
+                const int pr = tok[OP == G53_EM_MATS ? i : 0][r];
+                const long at = (long)(a.pair ? g53_div(pr, a.topk) : pr) * wrow;
+                t = r == 0 || lane / Xb::U == r ? at : t;
+            }
+            return {pb[i % VB] + t, n, row};
         }
-        return {pb[i % VB] + t, n};
     };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
     auto ask1 = [&](int c, int slot, int i) {               /* one instruction of a chunk */
         const G53Piece s = i < IA ? piece_a(i < IA ? i : 0, c) : piece_b(i < IA ? 0 : i - IA, c);
-        const uint8_t *p = s.n > 0 ? s.p : (const uint8_t *)&g53_nothing;
+        const uint8_t *p = s.n > 0 && s.row ? s.p : (const uint8_t *)&g53_nothing;
         g53_to_lds(p, lds0 + slot * SLOT + wv * 1024 + (i < IA ? i * NW * 1024 : BM * 128 + (i - IA) * NW * 1024));
     };
     auto ask = [&](int c, int slot) {
@@ -168,23 +177,35 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emm(G53E
 #pragma unroll
         for (int i = 0; i < IA + IB; i++) ask1(c, slot, i);
     };
-    g53_v4w ra[DMA ? 1 : IA], rb[DMA ? 1 : IB];
-    auto fetch = [&](int c) {
+    /* small tiles: two sets, a chunk's pieces are asked for two chunks ahead (behind the last: somewhere in the rows) and put
+     * down one ahead; large ones, whose registers would not hold them, one */
+    constexpr int SETS = MT * NT <= 8 ? 2 : 1;
+    g53_v4w ra[SETS][DMA ? 1 : IA], rb[SETS][DMA ? 1 : IB];
+    int bya[SETS][DMA ? 1 : IA], byb[SETS][DMA ? 1 : IB];
+    const bool short_a = (AX ? drow : kbytes) < 16, short_b = (BX ? wrow : kbytes) < 16;
+    auto fetch = [&](int c, int set) {
         if constexpr (!DMA) {
             tokens(c);
+            if (short_a || short_b) {
 #pragma unroll
-            for (int i = 0; i < IA; i++) ra[i] = g53_piece<E>(piece_a(i, c));
+                for (int i = 0; i < IA; i++) g53_take_short<E>(ra[set][i], bya[set][i], piece_a(i, c));
 #pragma unroll
-            for (int i = 0; i < IB; i++) rb[i] = g53_piece<E>(piece_b(i, c));
+                for (int i = 0; i < IB; i++) g53_take_short<E>(rb[set][i], byb[set][i], piece_b(i, c));
+            } else {
+#pragma unroll
+                for (int i = 0; i < IA; i++) g53_take(ra[set][i], bya[set][i], piece_a(i, c));
+#pragma unroll
+                for (int i = 0; i < IB; i++) g53_take(rb[set][i], byb[set][i], piece_b(i, c));
+            }
         }
     };
-    auto put = [&](int slot) {
+    auto put = [&](int slot, int set) {
         if constexpr (!DMA) {
             uint8_t *to = lds + slot * SLOT + wv * 1024 + lane * 16;
 #pragma unroll
-            for (int i = 0; i < IA; i++) *(g53_v4w *)(to + i * NW * 1024) = ra[i];
+            for (int i = 0; i < IA; i++) *(g53_v4w *)(to + i * NW * 1024) = g53_moved<E>(ra[set][i], bya[set][i]);
 #pragma unroll
-            for (int i = 0; i < IB; i++) *(g53_v4w *)(to + BM * 128 + i * NW * 1024) = rb[i];
+            for (int i = 0; i < IB; i++) *(g53_v4w *)(to + BM * 128 + i * NW * 1024) = g53_moved<E>(rb[set][i], byb[set][i]);
         }
     };
 
@@ -287,78 +308,70 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emm(G53E
         }
     } else {
         if (chunks) {
-            fetch(0);
-            put(0);
+            fetch(0, 0);
+            if (SETS == 2) fetch(1, SETS - 1);
+            put(0, 0);
         }
-        for (int c = 0; c < chunks; c++) {
-            __syncthreads();
-            if (c + 1 < chunks) fetch(c + 1);
-            multiply(c & 1);
-            if (c + 1 < chunks) put(c + 1 & 1);
+        if constexpr (SETS == 2) {
+            for (int c = 0; c < chunks; c += 2) {
+                __syncthreads();
+                fetch(c + 2, 0);
+                multiply(0);
+                put(1, SETS - 1);
+                if (c + 1 >= chunks) break;
+                __syncthreads();
+                fetch(c + 3, SETS - 1);
+                multiply(1);
+                put(0, 0);
+            }
+        } else {
+            for (int c = 0; c < chunks; c++) {
+                __syncthreads();
+                fetch(c + 1, 0);
+                multiply(c & 1);
+                put(c + 1 & 1, 0);
+            }
         }
     }
 
-    /* out: the loads' slots hold the wave's rows on their way */
-    constexpr bool VIA = DMA && STEPS == 2 && OP != G53_EM_MATS;
-    uint8_t *const buf = lds + wv * (16 * 16 * NT * (int)sizeof(E));
-    if (VIA) g53_meet();
-    auto leave = [&](auto &tiles, E *out, int N, int r0, int c0) {      /* 16 rows from r0, columns from c0 of N */
-        constexpr int n = sizeof(tiles) / sizeof(g53_v4f);
-        E *at = out + (long)(it.first + r0) * N + c0;
-        if constexpr (VIA) {
-            g53_rows_out<E, n, false>(buf, at, N, tiles, live - r0, N - c0, false);
+    /* out: the loads' slots hold the wave's tiles on their way */
+    g53_meet();
+    if constexpr (OP == G53_EM_MATS) {
+        const int r0 = m0 + wr * 16, c0 = n0 + wc * NT * 16;
+        static_assert(NS * SLOT >= NW * MT * NT * 1024, "tiles on their way out");
+        g53_leave_sums<E, WR>(lds + wv * (MT * NT * 1024), a.out, ((long)it.e * a.rows + r0) * a.cols + c0, a.cols, acc, a.rows - r0,
+                              a.cols - c0, a.w_f32, a.add);
+    } else {
+        static_assert(NS * SLOT >= NW * MT * NT * 256 * (int)sizeof(E), "tiles on their way out");
+        uint8_t *const buf = lds + wv * (MT * NT * 256 * (int)sizeof(E));
+        const int r0 = wr * 16, N = OP == G53_EM_ROWS ? a.cols : a.half;
+        const long first = it.first + r0;
+        if (OP == G53_EM_ROWS || !sw) {
+            const int c = n0 + wc * NT * 16;
+            g53_leave<E, WR>(buf, (E *)a.out + first * N + c, N, acc, live - r0, N - c);
         } else {
-            const int m = lane & 15, q = lane >> 4;
-            if (r0 + m >= live) return;
+            const int c = n0 + wc * (NT / 2 * 16), most = a.half - c;
+            g53_v4f v[MT][NT / 2];
+            if (a.gu) {                                     /* gate, then up: the rows' second halves */
+                E *at = (E *)a.gu + first * a.rows + c;
 #pragma unroll
-            for (int t = 0; t < n; t++) g53_store4(at + (long)m * N + 4 * q, 16 * t, N - c0 - 4 * q, tiles[t], false);
-        }
-    };
+                for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-        const int r0 = (i * WR + wr) * 16;
+                    for (int t = 0; t < NT / 2; t++) v[i][t] = acc[i][t];
+                g53_leave<E, WR>(buf, at, a.rows, v, live - r0, most);
 #pragma unroll
-        for (int t = 0; t < NT; t++) asm volatile("" ::: "memory");
-        if constexpr (OP == G53_EM_MATS) {
-            const int r = m0 + r0 + (lane & 15), c = n0 + wc * NT * 16 + 4 * (lane >> 4);
-            if (r >= a.rows) continue;
-            const long at = ((long)it.e * a.rows + r) * a.cols + c;
+                for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                if (a.w_f32) g53_store4((float *)a.out + at, 16 * t, a.cols - c, acc[i][t], a.add);
-                else g53_store4((E *)a.out + at, 16 * t, a.cols - c, acc[i][t], a.add);
+                    for (int t = 0; t < NT / 2; t++) v[i][t] = acc[i][t + NT / 2];
+                g53_leave<E, WR>(buf, at + a.half, a.rows, v, live - r0, most);
             }
-        } else if (r0 < live) {
-            if (OP == G53_EM_ROWS || !sw) {
-                leave(acc[i], (E *)a.out, OP == G53_EM_ROWS ? a.cols : a.half, r0, n0 + wc * NT * 16);
-            } else {
-                g53_v4f v[NT / 2], g[NT / 2], u[NT / 2];
 #pragma unroll
-                for (int t = 0; t < NT / 2; t++) {
-                    g[t] = acc[i][t];
-                    u[t] = acc[i][t + NT / 2];
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) v[t][k] = g53_swiglu1<E>(g[t][k], u[t][k], a.limit);
-                }
-                const int c = n0 + wc * (NT / 2 * 16);
-                leave(v, (E *)a.out, a.half, r0, c);
-                if (a.gu) {                             /* gate, then up: the rows' second halves */
-                    const int most = a.half - c;
-                    E *at = (E *)a.gu + (long)(it.first + r0) * a.rows + c;
-                    if constexpr (VIA) {
-                        g53_rows_out<E, NT / 2, false>(buf, at, a.rows, g, live - r0, most, false);
-                        g53_rows_out<E, NT / 2, false>(buf, at + a.half, a.rows, u, live - r0, most, false);
-                    } else {
-                        const int m = lane & 15, q = lane >> 4;
-                        if (r0 + m < live)
+                for (int t = 0; t < NT / 2; t++)
 #pragma unroll
-                            for (int t = 0; t < NT / 2; t++) {
-                                g53_store4(at + (long)m * a.rows + 4 * q, 16 * t, most - 4 * q, g[t], false);
-                                g53_store4(at + a.half + (long)m * a.rows + 4 * q, 16 * t, most - 4 * q, u[t], false);
-                            }
-                    }
-                }
-            }
+                    for (int k = 0; k < 4; k++) v[i][t][k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
+            g53_leave<E, WR>(buf, (E *)a.out + first * N + c, N, v, live - r0, most);
         }
     }
 }
@@ -531,14 +544,14 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emats(G5
             on();
         }
         const int r0 = t.m0 + wr * 16 * MT, c0 = t.n0 + wc * 16 * NT;
-        uint8_t *const buf = lds + NS * SLOT + wv * (16 * 16 * NT * 4);
+        uint8_t *const buf = lds + NS * SLOT + wv * (NT * 1024);
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
-            const long at = ((long)t.e * a.rows + r0 + 16 * i) * a.cols + c0;
+        for (int i = 0; i < MT; i++) {                      /* LDS beside the slots holds a row of tiles */
+            const int r = r0 + 16 * i;
+            g53_v4f v[1][NT];
 #pragma unroll
-            for (int j = 0; j < NT; j++) asm volatile("" : "+v"(acc[i][j]));    /* out of the accumulators one row of tiles at a time */
-            if (a.w_f32) g53_rows_out<float, NT, true>(buf, (float *)a.out + at, a.cols, acc[i], a.rows - r0 - 16 * i, a.cols - c0, a.add);
-            else g53_rows_out<E, NT, true>(buf, (E *)a.out + at, a.cols, acc[i], a.rows - r0 - 16 * i, a.cols - c0, a.add);
+            for (int j = 0; j < NT; j++) v[0][j] = acc[i][j];
+            g53_leave_sums<E, 1>(buf, a.out, ((long)t.e * a.rows + r) * a.cols + c0, a.cols, v, a.rows - r, a.cols - c0, a.w_f32, a.add);
         }
     }
     g53_loads_left<0>();                                    /* no load outlives the workgroup's LDS */
@@ -575,7 +588,7 @@ template <typename E, int OP, int WR, int WC, int MT, int NT, int NS, bool DMA> 
 template <typename E, int WR, int WC, int MT, int NT, int NS> static int matrices(G53EmArgs a)
 {
     constexpr int BM = 16 * MT * WR, BN = 16 * NT * WC;
-    constexpr size_t LDS = (size_t)NS * (BM + BN) * 128 + WR * WC * 16 * 16 * NT * 4;
+    constexpr size_t LDS = (size_t)NS * (BM + BN) * 128 + WR * WC * NT * 1024;
     static int allowed = 0;
     if (!allowed) {
         G53_TRY(hipFuncSetAttribute((const void *)k_emats<E, WR, WC, MT, NT, NS>, hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -598,9 +611,18 @@ template <typename E, int OP> static int by_size(const G53EmArgs &a, long n)
     const uintptr_t at = OP == G53_EM_FWD ? (uintptr_t)a.x | (uintptr_t)a.w
                          : OP == G53_EM_ROWS ? (uintptr_t)a.dy | (uintptr_t)a.w : (uintptr_t)a.dy | (uintptr_t)a.x;
     const size_t odd = (a.cols * sizeof(E)) | (OP == G53_EM_FWD ? 0 : a.rows * sizeof(E));
-    if ((at | odd) & 15) return launch<E, OP, 2, 2, 4, 4, 2, false>(a, n);
-    if constexpr (sizeof(E) == 2 && OP == G53_EM_MATS) return matrices<E, 2, 2, 4, 4, 2>(a);
-    if constexpr (sizeof(E) == 2 && OP != G53_EM_MATS) {
+    /* Few rows an expert, or few tiles of the matrices: tiles of 32 x 128, of which more are at work at a time. us, 2048 x 1024,
+     * 16 experts, top-4, 1, 32, 256 and 2048 tokens, tiles of 128 x 128 / 32 x 128: forward fp32 56 59 70 240 / 28 34 59 299,
+     * fp16 of 1023 columns 26 31 34 101 / 18 20 31 147; rows fp32 110 111 112 276 / 55 56 76 296; matrices fp32 57 50 58 228 /
+     * 43 34 64 313. */
+    const long busy = a.NE < n ? a.NE : n, mean = busy ? (n + busy - 1) / busy : 0, cus = g53h_num_cus();
+    const bool few = OP == G53_EM_MATS ? (long)a.NE * ((a.rows + 127) / 128) * ((a.cols + 127) / 128) < cus : mean <= 64;
+    if ((at | odd) & 15) return few ? launch<E, OP, 1, 4, 2, 2, 2, false>(a, n) : launch<E, OP, 2, 2, 4, 4, 2, false>(a, n);
+    if constexpr (sizeof(E) == 4) {
+        return few ? launch<E, OP, 1, 4, 2, 2, 4, true>(a, n) : launch<E, OP, 2, 2, 4, 4, 2, true>(a, n);
+    } else if constexpr (OP == G53_EM_MATS) {
+        return matrices<E, 2, 2, 4, 4, 2>(a);
+    } else {
         /* Experts' rows count as all alike, since the host does not know them. Tiles of 256 x 256 read LDS least for a
          * product, where there are as many as CUs; of 128 x 128 where there are two a CU; few rows take tiles of 64 x 128 and
          * 32 x 128, of which two workgroups a CU keep up to 96 KB of matrices on their way. us, bf16, forward / rows:
@@ -612,7 +634,6 @@ template <typename E, int OP> static int by_size(const G53EmArgs &a, long n)
          *     2048 x 1024, 32 experts, top-4
          *     1024                            39/67     46/43     49/54     48/47     60/59
          *     64                              23/40     21/32     18/26     19/19     18/19                              */
-        const long busy = a.NE < n ? a.NE : n, mean = (n + busy - 1) / busy, cus = g53h_num_cus();
         const int N = OP == G53_EM_FWD ? a.rows : a.cols;
         auto tiles = [&](int bm, int bn) { return (n / bm + busy) * ((N + bn - 1) / bn); };
         if (mean >= 64 && tiles(256, 256) >= cus) return launch<E, OP, 2, 2, 8, 8, 2, true>(a, n);
@@ -621,7 +642,6 @@ template <typename E, int OP> static int by_size(const G53EmArgs &a, long n)
         if (mean > 4 && tiles(64, 128) >= 2 * cus) return launch<E, OP, 1, 4, 4, 2, 3, true>(a, n);
         return launch<E, OP, 1, 4, 2, 2, 3, true>(a, n);
     }
-    return launch<E, OP, 2, 2, 4, 4, 2, true>(a, n);
 }
 
 /* ------------------------------------------------------------- SwiGLU's gradient ---- */

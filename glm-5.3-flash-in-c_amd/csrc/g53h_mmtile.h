@@ -16,11 +16,11 @@
 #define G53H_MMTILE_H
 
 #include <hip/hip_runtime.h>
+#include <type_traits>
 
 #include "g53h.h"
 #include "g53h_elem.h"
 
-typedef float g53_v4f_mm __attribute__((ext_vector_type(4)));
 typedef short g53_v4s __attribute__((ext_vector_type(4)));
 typedef g53_v4s __attribute__((address_space(3))) *G53LdsTr;
 
@@ -125,26 +125,44 @@ __device__ __forceinline__ bool g53_tile_item(const int *__restrict__ offsets, i
     return true;
 }
 
-/* Where a lane's 16 bytes of a chunk come from, and how many of them there are (16 and more: all, 0 and less: none). */
+/* Where a lane's 16 bytes of a chunk come from, how many bytes its row has from there on (0 and less: none), and whether
+ * the row is there at all; the address is that of a row in any case. */
 struct G53Piece {
     const uint8_t *p;
     int n;
+    bool row;
 };
-/* The piece in registers, zeros behind its end, at any alignment of its elements (of type E). */
-template <typename E> __device__ __forceinline__ g53_v4w g53_piece(const G53Piece &s)
+/* Pieces through registers, at any alignment of their elements (of type E). All of a thread's are asked for together and
+ * looked at when they are put down: one that meets its row's end is the row's last 16 bytes, moved down by `by` then
+ * (16: nothing is there, zeros). Rows of less than 16 bytes go by elements. */
+__device__ __forceinline__ void g53_take(g53_v4w &o, int &by, const G53Piece &s)
 {
-    if (s.n >= 16) return ((const G53v4w_any *)s.p)->v;
-    g53_v4w o = {0, 0, 0, 0};
-    if (s.n > 0) {
-        const E *p = (const E *)s.p;
-        constexpr int N = 16 / sizeof(E);
-        const int n = (int)s.n / (int)sizeof(E);
-        E v[N];
+    const int back = s.n >= 16 ? 0 : 16 - s.n;
+    o = ((const G53v4w_any *)(s.p - back))->v;
+    by = s.row && back < 16 ? back : 16;
+}
+template <typename E> __device__ __forceinline__ void g53_take_short(g53_v4w &o, int &by, const G53Piece &s)
+{
+    const E *p = (const E *)s.p;
+    constexpr int N = 16 / sizeof(E);
+    const int n = s.row ? s.n / (int)sizeof(E) : 0;
+    E v[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = i < n ? p[i] : (E)0.0f;
-        __builtin_memcpy(&o, v, 16);
-    }
-    return o;
+    for (int i = 0; i < N; i++) v[i] = i < n ? p[i] : (E)0.0f;
+    __builtin_memcpy(&o, v, 16);
+    by = 0;
+}
+template <typename E> __device__ __forceinline__ g53_v4w g53_moved(const g53_v4w &v, int by)
+{
+    unsigned d[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] = by & 8 ? (i < 2 ? d[i + 2] : 0u) : d[i];
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] = by & 4 ? (i < 3 ? d[i + 1] : 0u) : d[i];
+    if (sizeof(E) == 2)
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[i] = by & 2 ? __builtin_amdgcn_alignbyte(i < 3 ? d[i + 1] : 0u, d[i], 2) : d[i];
+    return (g53_v4w){by & 16 ? 0u : d[0], by & 16 ? 0u : d[1], by & 16 ? 0u : d[2], by & 16 ? 0u : d[3]};
 }
 
 /* The 16-bit type of the products and the planes of a value. fp32 enters as three bf16 planes, each the rounded rest of
@@ -169,17 +187,22 @@ template <typename E> struct G53Frag { typename G53Mm<E>::V v[G53Mm<E>::P]; };
 
 __device__ __forceinline__ void g53_planes(G53Frag<float> &o, const float (&v)[8])
 {
-    float r[8];
+    typedef float F2 __attribute__((ext_vector_type(2)));
+    typedef g53_bf16 B2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int i = 0; i < 8; i++) r[i] = v[i];
+    for (int i = 0; i < 4; i++) {
+        float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
-    for (int p = 0; p < 3; p++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const g53_bf16 h = (g53_bf16)r[i];
-            o.v[p][i] = h;
-            if (p < 2) r[i] -= (float)h;          /* exact */
+        for (int p = 0; p < 3; p++) {                       /* two at a time: one conversion */
+            const B2 h = __builtin_convertvector((F2){a, b}, B2);
+            o.v[p][2 * i] = h[0];
+            o.v[p][2 * i + 1] = h[1];
+            if (p == 2) break;
+            const unsigned u = __builtin_bit_cast(unsigned, h);
+            a -= __builtin_bit_cast(float, u << 16);        /* exact */
+            b -= __builtin_bit_cast(float, u & 0xffff0000u);
         }
+    }
 }
 template <typename E> __device__ __forceinline__ g53_v4f g53_mm(const G53Frag<E> &a, const G53Frag<E> &b, g53_v4f c)
 {
@@ -258,78 +281,91 @@ template <typename E, int R, int NT, int STRIDE = 1> struct G53Across {
     }
 };
 
-/* Four neighbours of a row, those below `n` columns of them; rounded once. old: added to what is there. */
-template <typename O> __device__ __forceinline__ void g53_store4(O *row, long c, long n, g53_v4f v, bool old)
+/* A wave's MT x n tiles to memory, each value rounded once. They go through LDS (buf: 16 MT x 16 n elements of the wave's own)
+ * and leave as pieces of 16 bytes, whole rows of the wave's columns: a store of the sums as they lie would leave 64 bytes of
+ * each of 16 rows. The loop over pieces is not unrolled whole: small calls wait for every instruction of it to be fetched.
+ * out: the first row's first column; tile i is 16 STRIDE i rows on. ld: elements from row to row; rows, cols: how many there are. */
+template <typename O, int STRIDE, int MT, int n>
+__device__ __forceinline__ void g53_leave(uint8_t *buf, O *out, long ld, const g53_v4f (&v)[MT][n], int rows, int cols)
 {
-    typedef O V4 __attribute__((ext_vector_type(4)));
-    struct __attribute__((packed, aligned(2))) Any { V4 v; };
-    if (c + 4 <= n) {
-        V4 o;
-        if (old) {
-            const V4 was = ((const Any *)(row + c))->v;
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] += (float)was[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = (O)v[i];
-        ((Any *)(row + c))->v = o;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (c + i < n) row[c + i] = (O)(old ? v[i] + (float)row[c + i] : v[i]);
-    }
-}
-
-/* 16 rows of a wave's NT tiles to memory by whole rows, through 16 x NT x 16 elements of LDS of its own: a store of the sums as
- * they lie would leave 64 bytes of each of 16 rows, and such halves of lines cost twice (see g53h_emm.hip). out: the first
- * row's first column, ld: elements from row to row; rows, cols: how many there are. PAST:
- * whole pieces go past the caches. Rows of less than 128 bytes go as they lie. */
-template <typename O, int NT, bool PAST>
-__device__ __forceinline__ void g53_rows_out(uint8_t *buf, O *out, long ld, g53_v4f (&acc)[NT], int rows, long cols, bool old)
-{
-    if constexpr (NT * 16 * sizeof(O) < 128) {
-        const int m = threadIdx.x & 15, q = threadIdx.x >> 4 & 3;
-        if (m < rows)
-#pragma unroll
-            for (int t = 0; t < NT; t++) g53_store4(out + m * ld + 4 * q, 16 * t, cols - 4 * q, acc[t], old);
-        return;
-    } else {
-    constexpr int RB = NT * 16 * sizeof(O), PR = RB / 16, RI = 64 / PR, EP = 16 / sizeof(O), SW = (PR < 8 ? PR : 8) - 1;
+    constexpr int RB = n * 16 * sizeof(O), PR = RB / 16, RI = 64 / PR, EP = 16 / sizeof(O), SW = (PR < 8 ? PR : 8) - 1;
     typedef O V4 __attribute__((ext_vector_type(4)));
     typedef O VP __attribute__((ext_vector_type(EP)));
     struct __attribute__((packed, aligned(2))) Any { VP v; };
+    static_assert(16 * MT % RI == 0, "whole rounds of rows");
     const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int b = (16 * t + 4 * q) * (int)sizeof(O);
-        if (old && sizeof(O) == 2) {                        /* added in fp32: before it is rounded */
-            const O *was = out + m * ld;
+    for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (m < rows && 16 * t + 4 * q + k < cols) acc[t][k] += (float)was[16 * t + 4 * q + k];
+        for (int t = 0; t < n; t++) {
+            const int b = (16 * t + 4 * q) * (int)sizeof(O);
+            V4 o;
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] = (O)v[i][t][k];
+            *(V4 *)(buf + (16 * i + m) * RB + (((b >> 4) ^ (m & SW)) << 4) + (b & 15)) = o;
         }
-        V4 o;
-#pragma unroll
-        for (int k = 0; k < 4; k++) o[k] = (O)acc[t][k];
-        *(V4 *)(buf + m * RB + (((b >> 4) ^ (m & SW)) << 4) + (b & 15)) = o;
+    const int p = lane % PR, left = cols - p * EP;
+#pragma unroll 4
+    for (int k = 0; k < 16 * MT / RI; k++) {
+        const int r = k * RI + lane / PR, at = (r >> 4) * (16 * STRIDE) + (r & 15);
+        const VP o = *(const VP *)(buf + r * RB + ((p ^ (r & SW)) << 4));
+        O *to = out + at * ld + p * EP;
+        if (at >= rows) continue;
+        if (left >= EP) ((Any *)to)->v = o;
+        else
+            for (int i = 0; i < left; i++) to[i] = ((const O *)(buf + r * RB + ((p ^ (r & SW)) << 4)))[i];
     }
+}
+/* The same for sums that may be added to what is there: they pass LDS (16 MT x 16 n fp32) as they are, are added in fp32 and
+ * rounded then, to fp32 or to O. Whole pieces go past the caches: these results are many, and whoever reads them does so
+ * much later (4.3 GB 1472 us against 1589). */
+template <typename O, int STRIDE, int MT, int n>
+__device__ __forceinline__ void g53_leave_sums(uint8_t *buf, void *out, long first, long ld, const g53_v4f (&v)[MT][n], int rows, int cols,
+                                               bool f32, bool old)
+{
+    constexpr int RB = n * 64;
+    const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
 #pragma unroll
-    for (int k = 0; k < 16 / RI; k++) {
-        const int r = k * RI + lane / PR, p = lane % PR;
-        VP v = *(const VP *)(buf + r * RB + ((p ^ (r & SW)) << 4));
-        O *to = out + r * ld + p * EP;
-        if (r >= rows) continue;
-        if (p * EP + EP <= cols) {
-            if (old && sizeof(O) == 4) v += ((const Any *)to)->v;
-            if (PAST && !((uintptr_t)to & 15)) __builtin_nontemporal_store(v, (VP *)to);
-            else ((Any *)to)->v = v;
-        } else {
+    for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int i = 0; i < EP; i++)
-                if (p * EP + i < cols) to[i] = old && sizeof(O) == 4 ? v[i] + to[i] : v[i];
+        for (int t = 0; t < n; t++) *(g53_v4f *)(buf + (16 * i + m) * RB + (((4 * t + q) ^ (m & 7)) << 4)) = v[i][t];
+    auto all = [&](auto *base) {
+        typedef typename std::remove_pointer<decltype(base)>::type T;
+        constexpr int EP = 16 / sizeof(T), PR = n * 16 / EP, RI = 64 / PR;      /* a lane's 16 bytes of result */
+        typedef T V __attribute__((ext_vector_type(EP)));
+        static_assert(16 * MT % RI == 0, "whole rounds of rows");
+        const int p = lane % PR, left = cols - EP * p;
+#pragma unroll 4
+        for (int k = 0; k < 16 * MT / RI; k++) {
+            const int r = k * RI + lane / PR, at = (r >> 4) * (16 * STRIDE) + (r & 15);
+            if (at >= rows || left <= 0) continue;
+            T *row = base + first + at * ld + EP * p;
+            float o[EP];
+#pragma unroll
+            for (int h = 0; h < EP / 4; h++) {
+                const g53_v4f part = *(const g53_v4f *)(buf + r * RB + (((EP / 4 * p + h) ^ (r & 7)) << 4));
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[4 * h + i] = part[i];
+            }
+            if (left >= EP && !((uintptr_t)row & 15)) {
+                V w;
+                if (old) {
+                    w = *(const V *)row;
+#pragma unroll
+                    for (int i = 0; i < EP; i++) o[i] += (float)w[i];
+                }
+#pragma unroll
+                for (int i = 0; i < EP; i++) w[i] = (T)o[i];
+                __builtin_nontemporal_store(w, (V *)row);
+            } else {
+#pragma unroll
+                for (int i = 0; i < EP; i++)
+                    if (i < left) row[i] = (T)(old ? o[i] + (float)row[i] : o[i]);
+            }
         }
-    }
-    }
+    };
+    if (f32) all((float *)out);
+    else all((O *)out);
 }
 
 /* The clamped SwiGLU, as g53h_swiglu's, for a result of type O. One of 16 bits, whose half step is 2^-9 at best, takes the

@@ -265,24 +265,20 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
     else if (live <= BM / 2) run(std::integral_constant<int, MT / 2>{});
     else run(std::integral_constant<int, MT>{});
     g53_meet();
-    uint8_t *const buf = lds + wv * (16 * 16 * NT * (int)sizeof(E));
+    uint8_t *const buf = lds + wv * (MT * NT * 256 * (int)sizeof(E));
+    const int r0 = wr * 16, c = n0 + wc * (sw ? NT / 2 : NT) * 16;
+    E *at = (E *)a.out + (long)(it.first + r0) * a.half + c;
+    if (!sw) {
+        g53_leave<E, WR>(buf, at, a.half, acc, live - r0, a.half - c);
+    } else {
+        g53_v4f v[MT][NT / 2];
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-        const int r0 = (i * WR + wr) * 16;
-        asm volatile("" ::: "memory");                      /* out of the accumulators one row of tiles at a time */
-        if (r0 >= live) continue;
-        const int c = n0 + wc * (sw ? NT / 2 : NT) * 16;
-        E *at = (E *)a.out + (long)(it.first + r0) * a.half + c;
-        if (!sw) {
-            g53_rows_out<E, NT, false>(buf, at, a.half, acc[i], live - r0, a.half - c, false);
-        } else {
-            g53_v4f v[NT / 2];
+        for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int t = 0; t < NT / 2; t++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) v[t][k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
-            g53_rows_out<E, NT / 2, false>(buf, at, a.half, v, live - r0, a.half - c, false);
-        }
+                for (int k = 0; k < 4; k++) v[i][t][k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
+        g53_leave<E, WR>(buf, at, a.half, v, live - r0, a.half - c);
     }
 }
 
@@ -290,7 +286,7 @@ template <typename E, int WR, int WC, int MT, int NT> static int launch(G53MxArg
 {
     constexpr int BM = 16 * MT * WR, BN = 16 * NT * WC;
     constexpr size_t LDS = 2 * (size_t)(BM + BN) * (128 + 16);
-    static_assert(LDS >= WR * WC * 16 * 16 * NT * sizeof(E), "rows on their way out");
+    static_assert(LDS >= WR * WC * MT * NT * 256 * sizeof(E), "rows on their way out");
     static int allowed = 0;
     if (!allowed) {
         G53_TRY(hipFuncSetAttribute((const void *)k_mx4<E, WR, WC, MT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
