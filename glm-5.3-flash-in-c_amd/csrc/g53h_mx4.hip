@@ -93,7 +93,7 @@ struct G53MxArgs {
 /* One tile, by the stream of k_emm (g53h_emm.hip): a chunk is 256 columns, two steps of 128. Scales come 16 a row at a time,
  * those of two chunks, through registers, which turn each quarter's four side by side: asked for in the second half of
  * an odd chunk, put down in that of the even one behind it, and read in that of the odd one behind that. */
-template <typename E, int WR, int WC, int MT, int NT>
+template <typename E, int WR, int WC, int MT, int NT, int NS>
 __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
 {
     constexpr int NW = WR * WC, BM = 16 * MT * WR, BN = 16 * NT * WC, SLOT = (BM + BN) * 128, SEG = (BM + BN) * 16;
@@ -147,12 +147,15 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
         ps[i] = r < BM ? a.xs + x_row(r) * sb : a.s + w_row(r - BM < BN ? r - BM : BN - 1) * sb;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    auto ask1 = [&](int c, int slot, int i) {
+    /* Behind a row's end its last piece comes again: levels are finite whatever they are, and both scales there are 0, so what
+     * they add is below fp32's steps. */
+    const int end = rb - 16 - u8 * 16;
+    int off = 0;
+    auto to_chunk = [&](int c) { off = c * 128 < end ? c * 128 : end; };
+    auto ask1 = [&](int slot, int i) {
         const uint32_t to = lds0 + slot * SLOT + wv * 1024;
-        const uint8_t *&p = i < IA ? pa[i < IA ? i : 0] : pb[i < IA ? 0 : i - IA];
-        g53_to_lds(u8 * 16 < rb - c * 128 ? p : (const uint8_t *)&g53_nothing, to + (i < IA ? i * NW * 1024 : BM * 128 + (i - IA) * NW * 1024));
-        p += 128;
-        asm volatile("" : "+v"(p));     /* one register pair a piece: else each of the loop's chunks gets its own */
+        g53_to_lds((i < IA ? pa[i < IA ? i : 0] : pb[i < IA ? 0 : i - IA]) + off,
+                   to + (i < IA ? i * NW * 1024 : BM * 128 + (i - IA) * NW * 1024));
     };
     g53_v4w rs[IS];
     auto fetch = [&](int seg) {
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
                 }
         }
     };
-    uint8_t *const lds_s = lds + 2 * SLOT;
+    uint8_t *const lds_s = lds + NS * SLOT;
     auto put = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < IS; i++) {
@@ -216,9 +219,11 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
         fetch(0);
         put(0);
 #pragma unroll
-        for (int c = 0; c < 2; c++)
+        for (int c = 0; c < NS; c++) {
+            to_chunk(c);
 #pragma unroll
-            for (int i = 0; i < IM + IB; i++) ask1(c, c, i < IM ? i : i - IM + IA);
+            for (int i = 0; i < IM + IB; i++) ask1(c, i < IM ? i : i - IM + IA);
+        }
         fetch(1);
         g53_loads_left<0>();
         g53_meet();
@@ -227,29 +232,32 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
 #pragma unroll
         for (int i = 0; i < M; i++) scale_x(0, i);
         scale_w(0);
-        /* chunk c, in slot c & 1 */
+        int slot = 0;
         auto chunk = [&](int c, auto odd_) {
             constexpr int odd = decltype(odd_)::value;
+            const int next = slot == NS - 1 ? 0 : slot + 1;
 #pragma unroll
             for (int i = 0; i < M; i++) {
 #pragma unroll
-                for (int k = i * RD; k < (i + 1) * RD && k < M + NT; k++) read1(1, odd, 1, k);
+                for (int k = i * RD; k < (i + 1) * RD && k < M + NT; k++) read1(1, slot, 1, k);
                 G53_MX_ROW(i, 0, 2 * odd);
             }
-            g53_loads_left<0>();
+            g53_loads_left<(NS - 2) * (IM + IB)>();
             g53_meet();
+            to_chunk(c + NS);
             if (odd) fetch((c + 1) / 2 + 1);
             else put((c / 2 + 1) & 1);
 #pragma unroll
             for (int i = 0; i < M; i++) {
 #pragma unroll
-                for (int k = i * AD; k < (i + 1) * AD && k < IM + IB; k++) ask1(c + 2, odd, k < IM ? k : k - IM + IA);
+                for (int k = i * AD; k < (i + 1) * AD && k < IM + IB; k++) ask1(slot, k < IM ? k : k - IM + IA);
 #pragma unroll
-                for (int k = i * RD; k < (i + 1) * RD && k < M + NT; k++) read1(0, odd ^ 1, 0, k);
+                for (int k = i * RD; k < (i + 1) * RD && k < M + NT; k++) read1(0, next, 0, k);
                 G53_MX_ROW(i, 1, 2 * odd + 1);
                 if (odd) scale_x((c + 1) / 2 & 1, i);       /* the next segment's, each in the place of the one just used */
             }
             if (odd) scale_w((c + 1) / 2 & 1);
+            slot = next;
         };
         for (int c = 0;; c += 2) {
             chunk(c, std::integral_constant<int, 0>{});
@@ -282,14 +290,14 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
     }
 }
 
-template <typename E, int WR, int WC, int MT, int NT> static int launch(G53MxArgs a, long n)
+template <typename E, int WR, int WC, int MT, int NT, int NS> static int launch(G53MxArgs a, long n)
 {
     constexpr int BM = 16 * MT * WR, BN = 16 * NT * WC;
-    constexpr size_t LDS = 2 * (size_t)(BM + BN) * (128 + 16);
+    constexpr size_t LDS = (size_t)(BM + BN) * (NS * 128 + 2 * 16);
     static_assert(LDS >= WR * WC * MT * NT * 256 * sizeof(E), "rows on their way out");
     static int allowed = 0;
     if (!allowed) {
-        G53_TRY(hipFuncSetAttribute((const void *)k_mx4<E, WR, WC, MT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
+        G53_TRY(hipFuncSetAttribute((const void *)k_mx4<E, WR, WC, MT, NT, NS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
         allowed = 1;
     }
     const int cut = a.limit > 0.0f ? BN / 2 : BN;
@@ -298,7 +306,7 @@ template <typename E, int WR, int WC, int MT, int NT> static int launch(G53MxArg
     for (long w0 = 0; w0 < wgs; w0 += G53_MX_WGS) {
         a.wg0 = w0;
         const dim3 grid((unsigned)(wgs - w0 < G53_MX_WGS ? wgs - w0 : G53_MX_WGS));
-        hipLaunchKernelGGL((k_mx4<E, WR, WC, MT, NT>), grid, dim3(64 * WR * WC), LDS, g53h_stream(), a);
+        hipLaunchKernelGGL((k_mx4<E, WR, WC, MT, NT, NS>), grid, dim3(64 * WR * WC), LDS, g53h_stream(), a);
         G53_LAUNCHED("k_mx4");
     }
     return 0;
@@ -376,7 +384,8 @@ static int mx_product(const char *who, void *y, int dt, const G53hMx4 *x, const 
 }
 
 /* Tiles by the rows that experts have, all alike, as in g53h_emm.hip. us, bf16, tiles of 128 x 128, 64 x 128, 32 x 128 (of
- * 256 x 128, one workgroup a CU, more than any):
+ * 256 x 128, one workgroup of four waves a CU, more than any; of 128 x 256, eight waves and three slots, 152 and 90 for the first
+ * two, 328 for 8192 rows, 32 for 512):
  *     4096 x 4096, 64 experts, top-8: 1024 tokens 158 210 255, 256 93 98 105, 16 55 54 62, 1 18.5 18.3 18.0
  *     1024 x 1024, 16 experts, top-4: 1024 tokens 12 16 16, 64 6.5 6.4 5.8
  *     8192 x 8192: 8192 rows 349 503 661, 512 30 31 48, 64 24 24 22, 1 20.6 20.4 20.5 */
@@ -384,9 +393,10 @@ template <typename E> static int by_size(const G53MxArgs &a, long n)
 {
     const long busy = a.offsets ? (a.NE < n ? a.NE : n) : 1, mean = (n + busy - 1) / busy, cus = g53h_num_cus();
     auto tiles = [&](int bm, int bn) { return (a.offsets ? n / bm + busy : (n + bm - 1) / bm) * ((a.rows + bn - 1) / bn); };
-    if (mean >= 32 && tiles(128, 128) >= cus) return launch<E, 2, 2, 4, 4>(a, n);
-    if (mean > 1 && tiles(64, 128) >= 2 * cus) return launch<E, 1, 4, 4, 2>(a, n);
-    return launch<E, 1, 4, 2, 2>(a, n);
+    if (mean >= 32 && tiles(128, 256) >= 2 * cus) return launch<E, 2, 4, 4, 4, 3>(a, n);
+    if (mean >= 32 && tiles(128, 128) >= cus) return launch<E, 2, 2, 4, 4, 2>(a, n);
+    if (mean > 1 && tiles(64, 128) >= 2 * cus) return launch<E, 1, 4, 4, 2, 2>(a, n);
+    return launch<E, 1, 4, 2, 2, 2>(a, n);
 }
 
 extern "C" int g53h_mm_mx4(void *y, int dt, const G53hMx4 *x, const G53hMx4 *m, float swiglu_limit)
