@@ -15,6 +15,7 @@
 
 #define G53_EM_MAXE 1024
 #define G53_EM_MAXD (1 << 24)           /* rows and columns of a matrix */
+#define G53_EM_MAXN (0x80000000l - 1024) /* pairs: chunks behind the last are counted in ints too */
 
 enum { G53_EM_FWD, G53_EM_ROWS, G53_EM_MATS };
 
@@ -394,24 +395,25 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emats(G5
     const int wr = wv / WC, wc = wv % WC;
     const long wrow = (long)a.cols * sizeof(E), drow = (long)a.rows * sizeof(E);
     const int per = a.across * a.down;
-    const long total = (long)a.NE * per;
+    /* tiles: fewer than 2^31 (each has 128 elements of memory and more, or is an expert's only one) */
+    const unsigned total = (unsigned)a.NE * per;
     /* the tile of a workgroup's turn w: runs of tiles by die, eight tiles down with each across */
     struct Tile {
         int e, m0, n0, first, live;
     };
-    auto tile_of = [&](long w, Tile &t) {
-        const long item = g53_deal(w, total);
+    auto tile_of = [&](unsigned w, Tile &t) {
+        const unsigned item = g53_deal(w, total);
         if (item >= total) return false;
         t.e = (int)(item / per);
         int m, n;
-        g53_eight(item % per, a.down, a.across, m, n);
+        g53_eight(item - (unsigned)t.e * per, a.down, a.across, m, n);
         t.m0 = m * BM;
         t.n0 = n * BN;
         t.first = g53_uniform_load(a.offsets + t.e);
         t.live = g53_uniform_load(a.offsets + t.e + 1) - t.first;
         return true;
     };
-    const long turns = a.wgs;
+    const unsigned turns = (unsigned)a.wgs;
     /* The stream: the tile and chunk to be asked for (none behind the last: zeros), and the one after it, whose tokens
      * are asked for a chunk ahead. */
     struct At {
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emats(G5
         int c, chunks, left;            /* left: rows from the chunk's first on, 0 behind the last tile */
     };
     At s, nx;
-    long nw = blockIdx.x;
+    unsigned nw = blockIdx.x;
     auto seek = [&]() {
         nx.c = nx.chunks = 0;
         for (; nw < turns; nw += gridDim.x)
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emats(G5
 #pragma unroll
     for (int i = 0; i < MT + NT; i++) read1(0, 0, 0, i);
     int slot = 0;
-    for (long w = blockIdx.x; w < turns; w += gridDim.x) {
+    for (unsigned w = blockIdx.x; w < turns; w += gridDim.x) {
         Tile t;
         if (!tile_of(w, t) || (a.add && !t.live)) continue;
         g53_v4f acc[MT][NT];
@@ -675,8 +677,8 @@ __global__ void __launch_bounds__(256) k_swiglu_grad(E *dgu, const E *dact, cons
 static int em_plan(const char *who, const G53hSort *p, int dt, int rows, int cols, G53EmArgs &a)
 {
     if (!p || p->T < 0 || p->topk < 1 || p->topk > 64 || p->n_experts < 1 || p->n_experts > G53_EM_MAXE ||
-        (long)p->T * p->topk > 0x7fffffffl || !p->offsets || (p->T && !p->pair))
-        return g53h_fail("%s: no plan of g53h_sort_tokens", who);
+        (long)p->T * p->topk > G53_EM_MAXN || !p->offsets || (p->T && !p->pair))
+        return g53h_fail("%s: no plan of g53h_sort_tokens (of at most 2^31 - 1024 pairs)", who);
     if (!g53_elem_bytes(dt)) return g53h_fail("%s: element type %d", who, dt);
     if (rows < 1 || rows > G53_EM_MAXD || cols < 1 || cols > G53_EM_MAXD)
         return g53h_fail("%s: matrices of %d x %d (1 to 2^24 rows and columns)", who, rows, cols);

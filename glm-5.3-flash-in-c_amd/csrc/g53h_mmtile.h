@@ -69,19 +69,19 @@ __device__ __forceinline__ int g53_div(int p, G53Div d) { return (int)(__umulhi(
 struct G53Item {
     int e, first, last, n;
 };
-__device__ __forceinline__ long g53_deal(long wg, long total)
+template <typename I> __device__ __forceinline__ I g53_deal(I wg, I total)
 {
-    const int run = total >= 256 ? 16 : total >= 16 ? (int)(total / 8) : 1;
-    const long i = wg >> 3;
+    if (total >= 256) return (wg >> 7 << 7) + (wg & 7) * 16 + (wg >> 3 & 15);       /* runs of 16 */
+    const I run = total >= 16 ? total / 8 : 1, i = wg >> 3;
     return ((i / run) * 8 + (wg & 7)) * run + i % run;
 }
 /* The workgroups that cover `total` items so dealt, or fewer. */
 static inline long g53_deal_wgs(long total) { return (total + 7) / 8 * 8 + (total < 8 ? 8 : total < 256 ? (total + 7) / 8 * 8 : 256); }
 /* Item `in` of tiles x across: eight tiles go with each tile across. */
-__device__ __forceinline__ void g53_eight(long in, int tiles, int across, int &t, int &n)
+template <typename I> __device__ __forceinline__ void g53_eight(I in, int tiles, int across, int &t, int &n)
 {
-    const long eight = 8l * across;
-    const int g = (int)(in / eight), in_g = (int)(in % eight), of = tiles - 8 * g < 8 ? tiles - 8 * g : 8;
+    const I eight = (I)8 * across;
+    const int g = (int)(in / eight), in_g = (int)(in - g * eight), of = tiles - 8 * g < 8 ? tiles - 8 * g : 8;
     t = 8 * g + in_g % of;
     n = in_g / of;
 }
@@ -356,34 +356,35 @@ __device__ __forceinline__ void g53_leave_sums(uint8_t *buf, void *out, long fir
         typedef typename std::remove_pointer<decltype(base)>::type T;
         constexpr int EP = 16 / sizeof(T), PR = n * 16 / EP, RI = 64 / PR;      /* a lane's 16 bytes of result */
         typedef T V __attribute__((ext_vector_type(EP)));
-        static_assert(16 * MT % RI == 0, "whole rounds of rows");
-        const int p = lane % PR, left = cols - EP * p;
+        static_assert(16 * MT % RI == 0 && (STRIDE == 1 || RI <= 16), "whole rounds of rows");
+        const int p = lane % PR, left = cols - EP * p, r0 = lane / PR;
+        T *row = base + first + r0 * ld + EP * p;
+        if (rows >= 16 * (STRIDE * (MT - 1) + 1) && cols >= 16 * n && !old && !(((uintptr_t)base | (first | ld) * sizeof(T)) & 15)) {
 #pragma unroll 4
-        for (int k = 0; k < 16 * MT / RI; k++) {
-            const int r = k * RI + lane / PR, at = (r >> 4) * (16 * STRIDE) + (r & 15);
-            if (at >= rows || left <= 0) continue;
-            T *row = base + first + at * ld + EP * p;
-            float o[EP];
-#pragma unroll
-            for (int h = 0; h < EP / 4; h++) {
-                const g53_v4f part = *(const g53_v4f *)(buf + r * RB + (((EP / 4 * p + h) ^ (r & 7)) << 4));
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[4 * h + i] = part[i];
-            }
-            if (left >= EP && !((uintptr_t)row & 15)) {
+            for (int k = 0; k < 16 * MT / RI; k++) {        /* all there, in whole pieces */
+                const int r = k * RI + r0;
                 V w;
-                if (old) {
-                    w = *(const V *)row;
 #pragma unroll
-                    for (int i = 0; i < EP; i++) o[i] += (float)w[i];
+                for (int h = 0; h < EP / 4; h++) {
+                    const g53_v4f part = *(const g53_v4f *)(buf + r * RB + (((EP / 4 * p + h) ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) w[4 * h + i] = (T)part[i];
                 }
-#pragma unroll
-                for (int i = 0; i < EP; i++) w[i] = (T)o[i];
                 __builtin_nontemporal_store(w, (V *)row);
-            } else {
+                row += (RI % 16 == 0 ? RI * STRIDE : (k + 1) * RI % 16 ? RI : RI + 16 * (STRIDE - 1)) * ld;
+            }
+            return;
+        }
+#pragma unroll 1
+        for (int k = 0; k < 16 * MT / RI; k++) {
+            const int r = k * RI + r0, at = (r >> 4) * (16 * STRIDE) + (r & 15);
+            if (at >= rows || left <= 0) continue;
+            row = base + first + at * ld + EP * p;
 #pragma unroll
-                for (int i = 0; i < EP; i++)
-                    if (i < left) row[i] = (T)(old ? o[i] + (float)row[i] : o[i]);
+            for (int i = 0; i < EP; i++) {
+                const int c = EP * p + i;                   /* its fp32 in LDS */
+                const float o = *(const float *)(buf + r * RB + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4);
+                if (i < left) row[i] = (T)(old ? o + (float)row[i] : o);
             }
         }
     };
