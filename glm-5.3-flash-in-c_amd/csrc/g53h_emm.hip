@@ -4,6 +4,24 @@
  *     forward     gu[r] = W[e] . x[r],  ys[r] = gu[r] or silu(min(gate, limit)) * clip(up, -limit, limit)
  *     rows        dx[r] = W[e]^T . dys[r]
  *     matrices    dW[e] = sum over the expert's rows of dys[r] x[r]^T, zeros for an expert without rows
+ *
+ * A tile of results belongs to one expert; a workgroup finds its tile from the plan's offsets, so the host need not know how
+ * many rows an expert has. Operands stream through LDS (g53h_mmtile.h); products are v_mfma_f32_16x16x32 of bf16 or fp16 with
+ * fp32 sums, the matrix's rows as the first operand, so that a lane holds four neighbours of a result's row. With 16 bits the
+ * operands of a step of 32 leave LDS while those before it are multiplied. fp32 enters as three bf16 planes, six products
+ * each: their rate is 6 to 1, and still above the fp32 matrix instructions' (2.4e14 against 1.45e14 a second at the rates of
+ * a large library product); splitting takes vector work of about the products' time.
+ *
+ * Measured (bf16 unless named; a 4 GiB copy moves 4.67 TB/s, a library product of 8192 cubed 1448 TFLOP/s in bf16 with both
+ * operands along the summed dimension, 145 in fp32):
+ *     8192 x 8192 by 8192 rows: forward 843 us, 1305 TFLOP/s, bound by power and LDS; rows 970, 1134; matrices 1250, 880
+ *     gate/up 4096 x 4096 of one token's 8 of 288 experts, SwiGLU: 55.7 us, 4.8 TB/s, HBM
+ *     the same by 4096 tokens, 8 of 64, gate and up kept: 1127 us, 976 TFLOP/s (rows of popular experts 2000, of others none:
+ *     tiles partly empty, dies unevenly loaded at the end)
+ *     gradients of 2048 such tokens, matrices in fp32: SwiGLU 68 us (4.9 TB/s), rows 745, matrices 1450; the last write 4.3 GB,
+ *     which alone take 870, and sum some 400 rows each between: instructions of addresses and of the way out, 6 a product
+ *     fp16 1001 x 1023, 301 tokens of 3 of 37 experts: 21 us, 3.7 TB/s, loads at odd addresses through registers
+ *     fp32 2048 x 1024, 512 tokens of 4 of 16 experts: 91 us, 94 TFLOP/s, one round of tiles
  */
 #include <hip/hip_runtime.h>
 #include <type_traits>
@@ -347,33 +365,34 @@ __global__ void __launch_bounds__(64 * WR * WC, MT * NT > 32 ? 1 : 2) k_emm(G53E
         uint8_t *const buf = lds + wv * (MT * NT * 256 * (int)sizeof(E));
         const int r0 = wr * 16, N = OP == G53_EM_ROWS ? a.cols : a.half;
         const long first = it.first + r0;
-        if (OP == G53_EM_ROWS || !sw) {
-            const int c = n0 + wc * NT * 16;
-            g53_leave<E, WR>(buf, (E *)a.out + first * N + c, N, acc, live - r0, N - c);
-        } else {
-            const int c = n0 + wc * (NT / 2 * 16), most = a.half - c;
-            g53_v4f v[MT][NT / 2];
-            if (a.gu) {                                     /* gate, then up: the rows' second halves */
-                E *at = (E *)a.gu + first * a.rows + c;
+        if constexpr (OP == G53_EM_FWD)
+            if (sw) {
+                const int c = n0 + wc * (NT / 2 * 16), most = a.half - c;
+                g53_v4f v[MT][NT / 2];
+                if (a.gu) {                                     /* gate, then up: the rows' second halves */
+                    E *at = (E *)a.gu + first * a.rows + c;
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int t = 0; t < NT / 2; t++) v[i][t] = acc[i][t];
+                    g53_leave<E, WR>(buf, at, a.rows, v, live - r0, most);
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int t = 0; t < NT / 2; t++) v[i][t] = acc[i][t + NT / 2];
+                    g53_leave<E, WR>(buf, at + a.half, a.rows, v, live - r0, most);
+                }
 #pragma unroll
                 for (int i = 0; i < MT; i++)
 #pragma unroll
-                    for (int t = 0; t < NT / 2; t++) v[i][t] = acc[i][t];
-                g53_leave<E, WR>(buf, at, a.rows, v, live - r0, most);
+                    for (int t = 0; t < NT / 2; t++)
 #pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int t = 0; t < NT / 2; t++) v[i][t] = acc[i][t + NT / 2];
-                g53_leave<E, WR>(buf, at + a.half, a.rows, v, live - r0, most);
+                        for (int k = 0; k < 4; k++) v[i][t][k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
+                g53_leave<E, WR>(buf, (E *)a.out + first * N + c, N, v, live - r0, most);
+                return;
             }
-#pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int t = 0; t < NT / 2; t++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) v[i][t][k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
-            g53_leave<E, WR>(buf, (E *)a.out + first * N + c, N, v, live - r0, most);
-        }
+        const int c = n0 + wc * NT * 16;
+        g53_leave<E, WR>(buf, (E *)a.out + first * N + c, N, acc, live - r0, N - c);
     }
 }
 
@@ -619,6 +638,10 @@ template <typename E, int OP> static int by_size(const G53EmArgs &a, long n)
      * 43 34 64 313. */
     const long busy = a.NE < n ? a.NE : n, mean = busy ? (n + busy - 1) / busy : 0, cus = g53h_num_cus();
     const bool few = OP == G53_EM_MATS ? (long)a.NE * ((a.rows + 127) / 128) * ((a.cols + 127) / 128) < cus : mean <= 64;
+    if constexpr (OP == G53_EM_ROWS) {      /* fewer still: a wave's part of a chunk is what takes time */
+        if (few && (n / 32 + busy) * ((a.cols + 127) / 128) < cus && (sizeof(E) == 4 || (at | odd) & 15))
+            return (at | odd) & 15 ? launch<E, OP, 1, 4, 2, 1, 2, false>(a, n) : launch<E, OP, 1, 4, 2, 1, sizeof(E) == 4 ? 4 : 2, true>(a, n);
+    }
     if ((at | odd) & 15) return few ? launch<E, OP, 1, 4, 2, 2, 2, false>(a, n) : launch<E, OP, 2, 2, 4, 4, 2, false>(a, n);
     if constexpr (sizeof(E) == 4) {
         return few ? launch<E, OP, 1, 4, 2, 2, 4, true>(a, n) : launch<E, OP, 2, 2, 4, 4, 2, true>(a, n);
