@@ -295,3 +295,26 @@ def test_every_tile(L, T, NE, N, K, dt):
     for e in range(NE):
         r = slice(offsets[e], offsets[e + 1])
         assert np.array_equal(dw.val()[e], xv[pair[r]].T @ zv[r])
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("w32", [0, 1])
+def test_results_at_any_element(L, dt, w32):
+    """Operands at multiples of 16 bytes, results that start one element on, odd result columns among them."""
+    say("results off", dt, w32)
+    rng = np.random.default_rng(12)
+    for T, NE, rows, cols in ((70, 2, 137, 64), (5, 3, 72, 136), (200, 2, 264, 72)):
+        idx = rng.integers(0, NE, (T, 1)).astype(np.int32)
+        offsets, pair, _ = sorted_plan(idx, NE)
+        plan, wt = Plan(idx, NE), F32 if w32 else dt
+        xv, wv, dv = values(rng, (T, cols), dt, True), values(rng, (NE, rows, cols), dt, True), values(rng, (T, rows), dt, True)
+        x, w, d = Buf(xv, dt), Buf(wv, dt), Buf(dv, dt)
+        one = 4 if dt == F32 else 2
+        ys, dx, dw = Buf.out((T, rows), dt, one), Buf.out((T, cols), dt, one), Buf.out((NE, rows, cols), wt, 4 if wt == F32 else 2)
+        check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, dt, 1, plan.c, w.ptr, rows, cols, 0.0))
+        check(L.g53h_sorted_mm_grad(dx.ptr, dw.ptr, wt, 0, d.ptr, x.ptr, dt, 1, plan.c, w.ptr, rows, cols))
+        for e in range(NE):
+            r = slice(offsets[e], offsets[e + 1])
+            assert np.array_equal(ys.val()[r], rounded(xv[pair[r]] @ wv[e].T, dt))
+            assert np.array_equal(dx.val()[r], rounded(dv[r] @ wv[e], dt))
+            assert np.array_equal(dw.val()[e], rounded(dv[r].T @ xv[pair[r]], wt))
