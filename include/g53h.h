@@ -361,8 +361,9 @@ int g53h_mtile_i4_host(uint8_t *dst_w, float *dst_s, const uint8_t *src_w, const
  * No counterpart in the reference. What a trunk does around and inside a MoE layer, on the library's
  * stream, so that nothing has to wait between them and, in fp32, g53h_router and g53h_moe, which take no
  * other type (a caller of bf16 or fp16 rows converts the layer's x itself): norms before and after the block with
- * its gate and residual, tokens sorted by expert and back, products with 4-bit matrices of any group
- * width; and the gradients of those that a training step differentiates. Pointers are device memory
+ * its gate and residual, tokens sorted by expert and back, products with matrices of the rows' own type, of
+ * 4-bit levels in groups of any width and of microscaled 4 bits; and the gradients of those that a training step
+ * differentiates. Pointers are device memory
  * of contiguous rows, aligned to one element; activations are of one of the types below, sums are fp32,
  * and results are rounded once. T = 0 is allowed everywhere. Arguments are checked before any work. */
 #define G53H_F32  0
@@ -418,7 +419,7 @@ int g53h_sorted_mm_w4(void *ys_d, const void *x_d, int dt, int gather, const G53
                       float swiglu_limit);
 
 /* Products of a plan's sorted rows with matrices of type dt, for experts that are trained: w [n_experts][rows][cols], any
- * rows and cols (2^24 each at most; rows that are multiples of 16 bytes, in arrays at such multiples, take the faster
+ * rows and cols (2^24 each at most, of plans of at most 2^31 - 1024 pairs; rows that are multiples of 16 bytes, in arrays at such multiples, take the faster
  * loads). x as in g53h_sorted_mm_w4. With swiglu_limit > 0 the matrices are gate over up (rows / 2 each), ys
  * [n][rows / 2] is their SwiGLU from the fp32 sums, and gu [n][rows], where it is not NULL, takes gate and up, which the
  * gradient needs; 0: ys [n][rows], gu NULL. Rows behind the last sorted one are left as they were, here and below.

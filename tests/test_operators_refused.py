@@ -193,3 +193,10 @@ def test_microscaled_products(L):
 
 def test_new_struct_sizes():
     assert C.sizeof(glm53h.G53hMx4) == 24
+
+
+def test_expert_products_most_pairs(L):
+    most = (1 << 31) - 1024
+    refused(L, L.g53h_sorted_mm(P, None, P, 1, 0, plan(T=most + 1, topk=1), P, 8, 8, 0.0), "2^31 - 1024")
+    refused(L, L.g53h_sorted_mm_grad(P, P, 0, 0, P, P, 1, 0, plan(T=most + 1, topk=1), P, 8, 8), "2^31 - 1024")
+    refused(L, L.g53h_sorted_swiglu_grad(P, P, P, 1, 8, plan(T=most + 1, topk=1), 1.0), "2^31 - 1024")
