@@ -93,7 +93,7 @@ __device__ __forceinline__ bool g53_tile_item(const int *__restrict__ offsets, i
     for (int i = 0, at = from; i < per; i++)
         if (e0 + i < NE) {
             const int to = offsets[e0 + i + 1];
-            n += (int)((unsigned)(to - at + TM - 1) / TM);
+            n += (int)(((unsigned)(to - at) + TM - 1) / TM);
             at = to;
         }
     int incl = n;
@@ -111,7 +111,7 @@ __device__ __forceinline__ bool g53_tile_item(const int *__restrict__ offsets, i
     int first = __builtin_amdgcn_readlane(from, l), last, e = l * per, tiles;
     for (;; e++) {                      /* lane l's experts: one of them holds the item */
         last = g53_uniform_load(offsets + e + 1);
-        tiles = (int)((unsigned)(last - first + TM - 1) / TM);
+        tiles = (int)(((unsigned)(last - first) + TM - 1) / TM);
         if (left < (long)tiles * across) break;
         left -= (long)tiles * across;
         first = last;

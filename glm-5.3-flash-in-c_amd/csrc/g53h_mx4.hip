@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
     if (a.offsets) {
         if (!g53_tile_item(a.offsets, a.NE, BM, a.across, wg, it)) return;
     } else {
-        const int tiles = (int)((unsigned)(a.T + BM - 1) / BM);
+        const int tiles = (int)(((unsigned)a.T + BM - 1) / BM);
         const long total = (long)tiles * a.across, item = g53_deal(wg, total);
         if (item >= total) return;
         int t;
@@ -132,13 +132,13 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
         return a.pair ? g53_div(a.pair[s], a.topk) : s;
     };
     auto w_row = [&](int r) -> long {
-        int at = n0 + r, up = 0;
+        unsigned at = n0 + (unsigned)r, up = 0;     /* past a matrix's last row it may pass 2^31 */
         if (sw) {                       /* a wave's first half of tiles: gate, the others: up */
             const int t = r / 16 % NT;
             up = t >= NT / 2;
-            at = n0 + r / (16 * NT) * (8 * NT) + (up ? t - NT / 2 : t) * 16 + r % 16;
+            at = n0 + (unsigned)(r / (16 * NT) * (8 * NT) + (up ? t - NT / 2 : t) * 16 + r % 16);
         }
-        at = at < a.half ? at : a.half - 1;
+        at = at < (unsigned)a.half ? at : a.half - 1;
         return e0 + at + (up ? a.half : 0);
     };
     const int u8 = (lane & 7) ^ (lane >> 3);
@@ -280,10 +280,12 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
     else run(std::integral_constant<int, MT>{});
     g53_meet();
     uint8_t *const buf = lds + wv * (MT * NT * 256 * (int)sizeof(E));
-    const int r0 = wr * 16, c = n0 + wc * (sw ? NT / 2 : NT) * 16;
-    E *at = (E *)a.out + (long)(it.first + r0) * a.half + c;
+    const int r0 = wr * 16;
+    const long c = n0 + (long)(wc * (sw ? NT / 2 : NT) * 16);
+    const int most = (int)(a.half - c);
+    E *at = (E *)a.out + (it.first + (long)r0) * a.half + c;
     if (!sw) {
-        g53_leave<E, WR>(buf, at, a.half, acc, live - r0, a.half - c);
+        g53_leave<E, WR>(buf, at, a.half, acc, live - r0, most);
     } else {
         g53_v4f v[MT][NT / 2];
 #pragma unroll
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) k_mx4(G53MxArgs a)
             for (int t = 0; t < NT / 2; t++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) v[i][t][k] = g53_swiglu1<E>(acc[i][t][k], acc[i][t + NT / 2][k], a.limit);
-        g53_leave<E, WR>(buf, at, a.half, v, live - r0, a.half - c);
+        g53_leave<E, WR>(buf, at, a.half, v, live - r0, most);
     }
 }
 
@@ -307,7 +309,7 @@ template <typename E, int WR, int WC, int MT, int NT, int NS> static int launch(
         allowed = 1;
     }
     const int cut = a.limit > 0.0f ? BN / 2 : BN;
-    a.across = (a.half + cut - 1) / cut;
+    a.across = (int)(((long)a.half + cut - 1) / cut);
     const long wgs = g53_deal_wgs((a.offsets ? n / BM + (a.NE < n ? a.NE : n) : (n + BM - 1) / BM) * a.across);
     for (long w0 = 0; w0 < wgs; w0 += G53_MX_WGS) {
         a.wg0 = w0;
@@ -398,7 +400,7 @@ static int mx_product(const char *who, void *y, int dt, const G53hMx4 *x, const 
 template <typename E> static int by_size(const G53MxArgs &a, long n)
 {
     const long busy = a.offsets ? (a.NE < n ? a.NE : n) : 1, mean = (n + busy - 1) / busy, cus = g53h_num_cus();
-    auto tiles = [&](int bm, int bn) { return (a.offsets ? n / bm + busy : (n + bm - 1) / bm) * ((a.rows + bn - 1) / bn); };
+    auto tiles = [&](int bm, int bn) { return (a.offsets ? n / bm + busy : (n + bm - 1) / bm) * (((long)a.rows + bn - 1) / bn); };
     if (mean >= 32 && tiles(128, 256) >= 2 * cus) return launch<E, 2, 4, 4, 4, 3>(a, n);
     if (mean >= 32 && tiles(128, 128) >= cus) return launch<E, 2, 2, 4, 4, 2>(a, n);
     if (mean > 1 && tiles(64, 128) >= 2 * cus) return launch<E, 1, 4, 4, 2, 2>(a, n);

@@ -268,3 +268,44 @@ def test_every_tile(L, T, NE, rows, cols):
     # the hardware's exponential and reciprocal 2^-20; the exponential is zero where it lies below 2^-126
     deep = np.where(g < -87, 2.0 ** -126 * np.abs(g * np.clip(u, -LIMIT, LIMIT)), 0)
     close(act.val(), want, (2.0 ** -20 + HALF[BF16]) * np.abs(want) + TINY[BF16] + deep)
+
+
+@pytest.mark.parametrize("rows,sw,sort", [((1 << 31) - 1, 0, 0), ((1 << 31) - 1, 0, 1), ((1 << 31) - 2, 1, 0)])
+def test_as_many_rows_as_an_int_holds(L, rows, sw, sort):
+    """Results of a matrix whose last tile ends behind row 2^31 - 1: its first, middle and last ones are right."""
+    say("rows", rows, sw, sort)
+    rng = np.random.default_rng(rows + sort)
+    cols, half, some = 32, rows // 2 if sw else rows, 300
+    # zeros but for `some` rows in a few places, of gate and of up with SwiGLU
+    places = [0, 1 << 20, half // 2 + 5, half - some]
+    w, s = DevBuf(rows * cols // 2), DevBuf(rows)
+    check(L.g53h_memset(w.ptr, 0, w.nbytes))
+    check(L.g53h_memset(s.ptr, 127, s.nbytes))
+    x = Mx4.random(rng, 1, cols, low=127, high=127)
+    y = DevBuf(2 * half)
+    check(L.g53h_memset(y.ptr, 0x55, y.nbytes))
+    want = []
+    for at in places:
+        y1 = []
+        for part in range(2 if sw else 1):
+            lv = rng.integers(0, 16, (some, cols)).astype(np.uint8)
+            bits = pack(lv)
+            check(L.g53h_h2d(w.ptr + (part * half + at) * cols // 2, bits.ctypes.data, bits.nbytes))
+            y1.append(x.wide @ wide(lv, np.full((some, 1), 127, np.uint8)).T)
+        want.append(np.concatenate(y1, 1))
+    m = glm53h.G53hMx4(w.ptr, s.ptr, rows, cols)
+    if sort:
+        plan = Plan(np.zeros((1, 1), np.int32), 1)
+        check(L.g53h_sorted_mm_mx4(y.ptr, F16, x.c, 1, plan.c, m, LIMIT if sw else 0.0))
+    else:
+        check(L.g53h_mm_mx4(y.ptr, F16, x.c, m, LIMIT if sw else 0.0))
+    for at, v in zip(places, want):
+        got = dec(y.download(np.float16, some, 2 * at), F16)
+        if sw:                                               # sums are exact; see test_every_tile
+            act = swiglu(v, LIMIT)[0]
+            assert (np.abs(got - act) <= (2.0 ** -20 + HALF[F16]) * np.abs(act) + TINY[F16] + 2.0 ** -100).all(), at
+        else:
+            assert np.array_equal(got, dec(enc(v[0], F16), F16)), at
+    # between them: products with zeros
+    for at in (some, half // 3, half - some - 1000):
+        assert not dec(y.download(np.float16, 900, 2 * at), F16).any(), at
