@@ -101,7 +101,7 @@ def close(got, want, tol, what=""):
     fine = np.isfinite(want)
     assert np.array_equal(got[~fine], want[~fine], equal_nan=True), what
     off = np.abs(got - want)[fine] - np.broadcast_to(tol, want.shape)[fine]
-    assert not off.size or not (off > 0).any(), (what, "by", off.max(), "over", int((off > 0).sum()), "of", off.size)
+    assert not off.size or (off <= 0).all(), (what, "by", off.max(), "over", int((~(off <= 0)).sum()), "of", off.size)
 
 
 # ---------------------------------------------------------------------- 4-bit matrices ----
