@@ -684,7 +684,10 @@ __global__ void __launch_bounds__(256) k_swiglu_grad(E *dgu, const E *dact, cons
     g53_load8_to(u, gu + r * 2 * H + H, c, H);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float gc = g[i] > limit ? limit : g[i], uc = u[i] > limit ? limit : (u[i] < -limit ? -limit : u[i]);
+        /* below -1000, where the sigmoid is 0, any gate is -1000: with the 0, -inf (as a gate past fp16 is kept) and what
+         * overflows next to the type's lowest value would give NaN */
+        const float gc = g[i] > limit ? limit : (g[i] < -1000.0f ? -1000.0f : g[i]);
+        const float uc = u[i] > limit ? limit : (u[i] < -limit ? -limit : u[i]);
         const bool low = gc < -80.0f;       /* there 1 + exp(g) is 1, and exp(-g) may overflow */
         const float x = expf(low ? gc : -gc), s = low ? x : 1.0f / (1.0f + x);
         const float dg = d[i] * uc * s * (1.0f + gc * (1.0f - s)), du = d[i] * gc * s;

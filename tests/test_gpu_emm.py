@@ -318,3 +318,59 @@ def test_results_at_any_element(L, dt, w32):
             assert np.array_equal(ys.val()[r], rounded(xv[pair[r]] @ wv[e].T, dt))
             assert np.array_equal(dx.val()[r], rounded(dv[r] @ wv[e], dt))
             assert np.array_equal(dw.val()[e], rounded(dv[r].T @ xv[pair[r]], wt))
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+def test_swiglu_grad_of_deep_gates(L, dt):
+    """Gates from -60 down to the type's lowest value and -inf, as a forward pass may store them: gradients that fade to
+    zero; gates and ups above the clamps up to inf have none, NaN stays."""
+    say("deep gates", dt)
+    rng = np.random.default_rng(13)
+    low = {F32: -3.4e38, BF16: -3.38e38, F16: -65504.0}[dt]
+    gates = np.array([-60.0, -79.5, -80.5, -86.0, -88.0, -95.0, -103.0, -110.0, -200.0, -999.0, -1001.0, -5e4, low, -np.inf, np.inf, -0.0])
+    T, inter = 9, gates.size
+    plan = Plan(np.zeros((T, 1), np.int32), 1)
+    gv = np.tile(gates, (T, 2))
+    gv[:, inter:] = rounded(rng.standard_normal((T, inter)), dt)
+    gv[1, inter:], gv[2, inter:] = np.inf, -np.inf
+    gv = rounded(gv, dt)
+    gv[3, 0], gv[3, inter + 1] = np.nan, np.nan
+    dv = rounded(rng.standard_normal((T, inter)), dt)
+    gu, d, out = Buf(gv, dt), Buf(dv, dt), Buf.out((T, 2 * inter), dt)
+    check(L.g53h_sorted_swiglu_grad(out.ptr, d.ptr, gu.ptr, dt, inter, plan.c, LIMIT))
+    g, u = gv[:, :inter], gv[:, inter:]
+    gc, uc = np.maximum(np.minimum(g, LIMIT), -1000.0), np.clip(u, -LIMIT, LIMIT)     # at -1000 s is 0 in fp32
+    with np.errstate(over="ignore"):
+        s = 1.0 / (1.0 + np.exp(-gc))
+    want = np.concatenate([np.where(g > LIMIT, 0, dv * uc * s * (1 + gc * (1 - s))), np.where(np.abs(u) > LIMIT, 0, dv * gc * s)], 1)
+    # as in test_swiglu_grad, whose `deep` counts s below the normal range. The product d u s is rounded there too, to a
+    # multiple of 2^-149, before it is multiplied by 1 + g (1 - s): 2^-150 (1 + |g|) however small d u is
+    size = np.concatenate([np.abs(dv * uc) * s * (1 + np.abs(gc)), np.abs(dv * gc) * s], 1)
+    deep = 2.0 ** -149 * np.concatenate([np.abs(dv * uc) * (1 + np.abs(gc)) + 0.5 * (1 + np.abs(gc)), np.abs(dv * gc)], 1)
+    close(out.val(), want, 16 * 2.0 ** -24 * size + deep + HALF[dt] * np.abs(want) + TINY[dt])
+
+
+def test_gates_past_fp16_forward_and_back(L):
+    """A gate's sum that passes fp16: the activation is 0 or clamped, gate and up are kept as infinities, and no gradient that
+    comes of them is one, or NaN."""
+    say("gates past fp16")
+    rng = np.random.default_rng(14)
+    T, inter, cols = 12, 8, 16
+    xv, wv = rng.integers(-3, 4, (T, cols)).astype(float), rng.integers(-3, 4, (1, 2 * inter, cols)).astype(float)
+    xv[:, 0], wv[0, :, 0] = 300.0, 0.0
+    wv[0, 0, 0], wv[0, 1, 0], wv[0, inter + 2, 0], wv[0, inter + 3, 0] = -300.0, 300.0, -300.0, 300.0
+    x, w, plan = Buf(xv, F16), Buf(wv, F16), Plan(np.zeros((T, 1), np.int32), 1)
+    act, gu = Buf.out((T, inter), F16), Buf.out((T, 2 * inter), F16)
+    check(L.g53h_sorted_mm(act.ptr, gu.ptr, x.ptr, F16, 1, plan.c, w.ptr, 2 * inter, cols, LIMIT))
+    kept = gu.val()
+    assert (kept[:, [0, inter + 2]] == -np.inf).all() and (kept[:, [1, inter + 3]] == np.inf).all()
+    assert np.isfinite(act.val()).all() and not act.val()[:, 0].any()
+    dv = rng.integers(-3, 4, (T, inter)).astype(float)
+    d, dgu, dx, dw = Buf(dv, F16), Buf.out((T, 2 * inter), F16), Buf.out((T, cols), F16), Buf.out((1, 2 * inter, cols), F32)
+    check(L.g53h_sorted_swiglu_grad(dgu.ptr, d.ptr, gu.ptr, F16, inter, plan.c, LIMIT))
+    check(L.g53h_sorted_mm_grad(dx.ptr, dw.ptr, F32, 0, dgu.ptr, x.ptr, F16, 1, plan.c, w.ptr, 2 * inter, cols))
+    v = dgu.val()
+    assert not v[:, [0, 1, inter, inter + 2, inter + 3]].any()           # the two gates, the deep gate's up, the two ups
+    s = 1 / (1 + np.exp(-LIMIT))
+    assert (np.abs(v[:, inter + 1] - np.where(np.abs(kept[:, inter + 1]) <= LIMIT, dv[:, 1] * LIMIT * s, 0)) <= 2.0 ** -10 * 8).all()
+    assert np.isfinite(v).all() and np.isfinite(dx.val()).all() and np.isfinite(dw.val()).all() and not dw.val()[0, [0, inter]].any()
