@@ -168,7 +168,9 @@ template <typename E> __device__ __forceinline__ g53_v4w g53_moved(const g53_v4w
 /* The 16-bit type of the products and the planes of a value. fp32 enters as three bf16 planes, each the rounded rest of
  * those before it: with 8 bits a plane and at most half a step left by each, the three hold every bit of the value
  * (above 2^-109; and values that round past bf16's largest, from 3.39e38, count as infinite). Of the nine products
- * of two values' planes six are taken: the others are below 2^-26 of the value's product together. */
+ * of two values' planes six are taken. The planes of a value in [1, 2) are at most 2^-8 and 2^-17, so the others are below
+ * 2^-24 of the values' product together, fp32's own rounding of one (2^-24.01 for 0x1.00ff8p0 by itself, 2^-28 in the mean of
+ * random values, of either sign). */
 template <typename E> struct G53Mm;
 template <> struct G53Mm<float> { typedef g53_v8b V; static constexpr int P = 3; };
 template <> struct G53Mm<g53_bf16> { typedef g53_v8b V; static constexpr int P = 1; };

@@ -374,3 +374,30 @@ def test_gates_past_fp16_forward_and_back(L):
     s = 1 / (1 + np.exp(-LIMIT))
     assert (np.abs(v[:, inter + 1] - np.where(np.abs(kept[:, inter + 1]) <= LIMIT, dv[:, 1] * LIMIT * s, 0)) <= 2.0 ** -10 * 8).all()
     assert np.isfinite(v).all() and np.isfinite(dx.val()).all() and np.isfinite(dw.val()).all() and not dw.val()[0, [0, inter]].any()
+
+
+@pytest.mark.parametrize("n", [1, 300])
+def test_products_whose_parts_are_largest(L, n):
+    """fp32 values whose second and third bf16 parts are as large as they get, 2^-8 and 2^-17 of them, so that the products
+    of parts that are left out come near their bound, 2^-24 of a product, and of one sign: sums of n."""
+    say("largest parts", n)
+    hard = np.array([float.fromhex(v) for v in ("0x1.00ff8p0", "0x1.01008p0", "0x1.00fe8p0", "0x1.20ff8p0")])
+    T, N = 40, 70
+    scale = np.exp2(np.arange(N) % 5 - 2.0)
+    av = np.repeat(hard[np.arange(T) % 4][:, None], n, 1)                # [T][n]: a row's values alike
+    bv = np.repeat((hard[np.arange(N) % 4] * scale)[:, None], n, 1)       # [N][n]
+    want = av @ bv.T
+    # besides: one product's parts are added in three steps of at most 2^-8 of it and one of its own size, each of 2^-23
+    # (cut); sums of more add what test_forward's do
+    tol = (2.0 ** -24 + 2.0 ** -23 + 3 * 2.0 ** -31) * want if n == 1 else off(n, want, want, F32, False) + 2.0 ** -24 * want
+    plan = Plan(np.zeros((T, 1), np.int32), 1)
+    x, w, ys = Buf(av, F32), Buf(bv[None], F32), Buf.out((T, N), F32)
+    check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, F32, 1, plan.c, w.ptr, N, n, 0.0))
+    close(ys.val(), want, tol, "forward")
+    wt, dx = Buf(np.ascontiguousarray(bv.T)[None], F32), Buf.out((T, N), F32)
+    check(L.g53h_sorted_mm_grad(dx.ptr, None, F32, 0, x.ptr, None, F32, 1, plan.c, wt.ptr, n, N))
+    close(dx.val(), want, tol, "rows")
+    plan = Plan(np.zeros((n, 1), np.int32), 1)
+    d, z, dw = Buf(np.ascontiguousarray(av.T), F32), Buf(np.ascontiguousarray(bv.T), F32), Buf.out((1, T, N), F32)
+    check(L.g53h_sorted_mm_grad(None, dw.ptr, F32, 0, d.ptr, z.ptr, F32, 1, plan.c, None, T, N))
+    close(dw.val()[0], want, tol, "matrices")
