@@ -401,3 +401,37 @@ def test_products_whose_parts_are_largest(L, n):
     d, z, dw = Buf(np.ascontiguousarray(av.T), F32), Buf(np.ascontiguousarray(bv.T), F32), Buf.out((1, T, N), F32)
     check(L.g53h_sorted_mm_grad(None, dw.ptr, F32, 0, d.ptr, z.ptr, F32, 1, plan.c, None, T, N))
     close(dw.val()[0], want, tol, "matrices")
+
+
+@pytest.mark.parametrize("what", ["small", "smaller", "large", "past"])
+def test_fp32_at_the_ends_of_its_range(L, what):
+    say("ends of fp32", what)
+    rng = np.random.default_rng(15)
+    T, N, K = 34, 66, 40
+    one = 1.0 + rng.integers(0, 1 << 23, T) / 2.0 ** 23
+    v = {"small": one * 2.0 ** -109, "smaller": one * np.exp2(-rng.integers(112, 127, T).astype(float)),
+         "large": np.full(T, float.fromhex("0x1.fefffep127")), "past": np.full(T, float.fromhex("0x1.ffp127"))}[what]
+    up = 2.0 ** (-120 if what in ("large", "past") else 100)
+    xv, wv = np.zeros((T, K)), np.zeros((1, N, K))
+    at = np.arange(T) % K
+    xv[np.arange(T), at] = v
+    xv[5] = 0.0                                              # a row of zeros among them
+    wv[0] = up * np.exp2(np.arange(N) % 3)[:, None]
+    want = xv @ wv[0].T
+    plan = Plan(np.zeros((T, 1), np.int32), 1)
+    x, w, ys = Buf(xv, F32), Buf(wv, F32), Buf.out((T, N), F32)
+    check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, F32, 1, plan.c, w.ptr, N, K, 0.0))
+    wt, dx = Buf(np.ascontiguousarray(wv[0].T)[None], F32), Buf.out((T, N), F32)
+    check(L.g53h_sorted_mm_grad(dx.ptr, None, F32, 0, x.ptr, None, F32, 1, plan.c, wt.ptr, K, N))
+    dw = Buf.out((1, K, N), F32)
+    ones = np.broadcast_to(wv[0, :, 0], (T, N))
+    z = Buf(np.ascontiguousarray(ones), F32)
+    check(L.g53h_sorted_mm_grad(None, dw.ptr, F32, 0, x.ptr, z.ptr, F32, 1, plan.c, None, K, N))
+    wantw = xv.T @ ones
+    for got, ref in ((ys.val(), want), (dx.val(), want), (dw.val()[0], wantw)):
+        if what in ("small", "large"):                       # a value times a power of two: exact
+            assert np.array_equal(got, ref)
+        elif what == "smaller":                              # held to half of bf16's smallest step, 2^-133
+            assert (np.abs(got - ref) <= 2.0 ** -134 * up * 4 + 2.0 ** -24 * np.abs(ref)).all()
+        else:
+            assert np.isnan(got[np.abs(ref).max(1) > 0]).all() and not got[np.abs(ref).max(1) == 0].any()
