@@ -396,7 +396,8 @@ static int mx_product(const char *who, void *y, int dt, const G53hMx4 *x, const 
  * two, 328 for 8192 rows, 32 for 512):
  *     4096 x 4096, 64 experts, top-8: 1024 tokens 158 210 255, 256 93 98 105, 16 55 54 62, 1 18.5 18.3 18.0
  *     1024 x 1024, 16 experts, top-4: 1024 tokens 12 16 16, 64 6.5 6.4 5.8
- *     8192 x 8192: 8192 rows 349 503 661, 512 30 31 48, 64 24 24 22, 1 20.6 20.4 20.5 */
+ *     8192 x 8192: 8192 rows 349 503 661, 512 30 31 48, 64 24 24 22, 1 20.6 20.4 20.5
+ * The tests repeat this rule, to name the tile that a size takes. */
 template <typename E> static int by_size(const G53MxArgs &a, long n)
 {
     const long busy = a.offsets ? (a.NE < n ? a.NE : n) : 1, mean = (n + busy - 1) / busy, cus = g53h_num_cus();

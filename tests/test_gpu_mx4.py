@@ -309,3 +309,55 @@ def test_as_many_rows_as_an_int_holds(L, rows, sw, sort):
     # between them: products with zeros
     for at in (some, half // 3, half - some - 1000):
         assert not dec(y.download(np.float16, 900, 2 * at), F16).any(), at
+
+
+def tile(cus, n, NE, rows):
+    """The tile (rows of x, rows of the matrix) that the library takes for n rows, by its rule."""
+    busy = min(NE, n) if NE else 1
+    mean = -(-n // busy)
+    count = lambda bm, bn: (n // bm + busy if NE else -(-n // bm)) * -(-rows // bn)     # noqa: E731
+    if mean >= 32 and count(128, 256) >= 2 * cus:
+        return 128, 256
+    if mean >= 32 and count(128, 128) >= cus:
+        return 128, 128
+    return (64, 128) if mean > 1 and count(64, 128) >= 2 * cus else (32, 128)
+
+
+# rows of x in every expert (one number: a single matrix), columns: one, two and three chunks, with scales to the end of a
+# segment and not; the last tile of an expert has up to a quarter, a half and all of its rows
+@pytest.mark.parametrize("counts,cols", [((300,), 352), ((140,), 96), ((148, 50, 102), 544), ((128, 0, 190), 512), ((33, 64, 97), 32)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_widest_tiles(L, counts, cols, dt):
+    say("widest tiles", counts, cols, dt)
+    rng = np.random.default_rng(sum(counts) + cols)
+    used, NE, cus = sum(counts), len(counts) if len(counts) > 1 else 0, L.g53h_num_cus()
+    n = used + 3 if NE else used                             # three tokens without an expert
+    down = n // 128 + NE if NE else -(-n // 128)
+    rows = 256 * (-(-2 * cus // down) + 1) - 150             # the last tile across: 106 rows
+    assert tile(cus, n, NE, rows) == (128, 256)
+    x, m = Mx4.random(rng, n, cols, low=127, high=128), Mx4.random(rng, rows, cols, max(NE, 1), low=125, high=126)
+    idx = np.concatenate([np.repeat(np.arange(len(counts)), counts), np.full(n - used, -1)]).astype(np.int32)[:, None]
+    rng.shuffle(idx)
+    offsets, pair, _ = sorted_plan(idx, len(counts))
+    plan = Plan(idx, len(counts))
+    for sw in (0, 1):
+        y = Buf.out((n, rows // 2 if sw else rows), dt, shift=2 if dt != F32 else 4)
+        if NE:
+            check(L.g53h_sorted_mm_mx4(y.ptr, dt, x.c, 1, plan.c, m.c, LIMIT if sw else 0.0))
+            ref = np.concatenate([x.wide[pair[offsets[e]:offsets[e + 1]]] @ m.wide[e * rows:(e + 1) * rows].T for e in range(NE)])
+        else:
+            check(L.g53h_mm_mx4(y.ptr, dt, x.c, m.c, LIMIT if sw else 0.0))
+            ref = x.wide @ m.wide.T
+        got = y.val()
+        assert (got[used:] == 77).all()
+        if not sw:
+            assert np.array_equal(got[:used], dec(enc(ref, dt), dt))       # sums are exact, see test_every_tile
+            continue
+        g, u = np.split(ref, 2, 1)
+        with np.errstate(over="ignore"):
+            want = swiglu(ref, LIMIT)
+        deep = np.where(g < -87, 2.0 ** -126 * np.abs(g * np.clip(u, -LIMIT, LIMIT)), 0)
+        # expf, a division and products: 4 steps; the hardware's exponential and reciprocal 2^-20, and half a step of what
+        # the exponential is of, the gate by log2 e
+        rel = 4 * 2.0 ** -23 if dt == F32 else 2.0 ** -20 + np.abs(np.minimum(g, 0)) * 2.0 ** -24
+        close(got[:used], want, (rel + HALF[dt]) * np.abs(want) + TINY[dt] + deep)
