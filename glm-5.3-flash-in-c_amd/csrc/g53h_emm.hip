@@ -635,7 +635,7 @@ template <typename E, int OP> static int by_size(const G53EmArgs &a, long n)
     /* Few rows an expert, or few tiles of the matrices: tiles of 32 x 128, of which more are at work at a time. us, 2048 x 1024,
      * 16 experts, top-4, 1, 32, 256 and 2048 tokens, tiles of 128 x 128 / 32 x 128: forward fp32 56 59 70 240 / 28 34 59 299,
      * fp16 of 1023 columns 26 31 34 101 / 18 20 31 147; rows fp32 110 111 112 276 / 55 56 76 296; matrices fp32 57 50 58 228 /
-     * 43 34 64 313. */
+     * 43 34 64 313. The tests repeat the rules below, to name the tile that a size takes. */
     const long busy = a.NE < n ? a.NE : n, mean = busy ? (n + busy - 1) / busy : 0, cus = g53h_num_cus();
     const bool few = OP == G53_EM_MATS ? (long)a.NE * ((a.rows + 127) / 128) * ((a.cols + 127) / 128) < cus : mean <= 64;
     if constexpr (OP == G53_EM_ROWS) {      /* fewer still: a wave's part of a chunk is what takes time */

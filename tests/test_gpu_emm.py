@@ -435,3 +435,89 @@ def test_fp32_at_the_ends_of_its_range(L, what):
             assert (np.abs(got - ref) <= 2.0 ** -134 * up * 4 + 2.0 ** -24 * np.abs(ref)).all()
         else:
             assert np.isnan(got[np.abs(ref).max(1) > 0]).all() and not got[np.abs(ref).max(1) == 0].any()
+
+
+def tile(cus, op, dt, n, NE, rows, cols, whole):
+    """The tile (rows, columns of the result) that the library takes for n rows, by its rule, or "stream" for the matrices'
+    gradient in 16 bits; whole: operands of whole pieces of 16 bytes."""
+    busy = min(NE, n)
+    mean, size = -(-n // busy), rows if op == "forward" else cols
+    count = lambda bm, bn: (n // bm + busy) * -(-size // bn)                         # noqa: E731
+    few = NE * -(-rows // 128) * -(-cols // 128) < cus if op == "matrices" else mean <= 64
+    if op == "rows" and few and count(32, 128) < cus and (dt == F32 or not whole):
+        return 32, 64
+    if dt == F32 or not whole:
+        return (32, 128) if few else (128, 128)
+    if op == "matrices":
+        return "stream"
+    if mean >= 64 and count(256, 256) >= cus:
+        return 256, 256
+    if mean >= 128 and count(128, 128) >= 2 * cus:
+        return 128, 128
+    if op == "rows" and mean > 1 and count(64, 256) >= 2 * cus:
+        return 64, 256
+    return (64, 128) if mean > 4 and count(64, 128) >= 2 * cus else (32, 128)
+
+
+# rows of every expert, rows and columns of a matrix, bytes off a multiple of 16: the tiles that the other tests' sizes do not take,
+# on 256 CUs, with ends of every kind
+FORMS = [("rows", (64, 256), (BF16, F16), (70, 30), 72, 43768, 0), ("rows", (64, 256), (BF16, F16), (33, 0, 64, 16), 136, 33032, 0),
+         ("rows", (64, 256), (BF16, F16), (48, 47), 40, 44032, 0),
+         ("rows", (32, 128), (F32,), (33, 1, 0, 30), 132, 8196, 0), ("rows", (32, 128), (F32, BF16, F16), (33, 1, 0, 30), 131, 8193, 0),
+         ("rows", (32, 128), (F32, BF16, F16), (40, 24), 64, 13000, 1),
+         ("rows", (256, 256), (BF16, F16), (356, 40, 0, 204), 200, 13320, 0), ("forward", (256, 256), (BF16, F16), (356, 40, 0, 204), 13320, 200, 0),
+         ("rows", (256, 256), (BF16, F16), (65, 384, 128), 136, 16648, 0), ("forward", (256, 256), (BF16, F16), (65, 384, 128), 16648, 136, 0),
+         ("matrices", (128, 128), (F32,), (0, 33, 87), 1004, 1396, 0), ("matrices", (128, 128), (F32, BF16, F16), (1, 70, 128), 1001, 1399, 0),
+         ("matrices", (128, 128), (F32, BF16, F16), (64, 0, 65), 1008, 1400, 1), ("matrices", (128, 128), (F32,), (300,), 2052, 2064, 0)]
+
+
+@pytest.mark.parametrize("op,want_tile,dt,counts,rows,cols,shifted",
+                         [(op, t, dt, *rest) for op, t, dts, *rest in FORMS for dt in dts])
+def test_tiles_of_other_sizes(L, op, want_tile, dt, counts, rows, cols, shifted):
+    say("tiles of other sizes", op, want_tile, dt, counts, rows, cols, shifted)
+    rng = np.random.default_rng(sum(counts) + rows)
+    NE, used, n = len(counts), sum(counts), sum(counts) + 3          # three tokens without an expert
+    one = 4 if dt == F32 else 2
+    whole = not shifted and cols * one % 16 == 0 and (op == "forward" or rows * one % 16 == 0)
+    cus = L.g53h_num_cus()
+    if cus == 256:
+        assert tile(cus, op, dt, n, NE, rows, cols, whole) == want_tile
+    idx = np.concatenate([np.repeat(np.arange(NE), counts), np.full(3, -1)]).astype(np.int32)[:, None]
+    rng.shuffle(idx)
+    offsets, pair, _ = sorted_plan(idx, NE)
+    plan, shift = Plan(idx, NE), one if shifted else 0
+    of = lambda e: slice(offsets[e], offsets[e + 1])                 # noqa: E731
+    xv = values(rng, (n, cols), dt, True)
+    if op == "matrices":
+        dv = values(rng, (n, rows), dt, True)
+        old = values(rng, (NE, rows, cols), dt, True)
+        x, d, dw, da = Buf(xv, dt, shift), Buf(dv, dt, shift), Buf.out((NE, rows, cols), F32), Buf(old, dt, shift)
+        check(L.g53h_sorted_mm_grad(None, dw.ptr, F32, 0, d.ptr, x.ptr, dt, 1, plan.c, None, rows, cols))
+        check(L.g53h_sorted_mm_grad(None, da.ptr, dt, 1, d.ptr, x.ptr, dt, 1, plan.c, None, rows, cols))
+        got, added = dw.val(), da.val()
+        for e in range(NE):
+            ref = dv[of(e)].T @ xv[pair[of(e)]]
+            assert np.array_equal(got[e], ref) and np.array_equal(added[e], rounded(old[e] + ref, dt)), e
+        return
+    wv = values(rng, (NE, rows, cols), dt, True)
+    w = Buf(wv, dt, shift)
+    if op == "rows":
+        dv = values(rng, (n, rows), dt, True)
+        d, dx = Buf(dv, dt, shift), Buf.out((n, cols), dt, shift)
+        check(L.g53h_sorted_mm_grad(dx.ptr, None, dt, 0, d.ptr, None, dt, 1, plan.c, w.ptr, rows, cols))
+        ref = np.concatenate([dv[of(e)] @ wv[e] for e in range(NE)])
+        assert np.array_equal(dx.val()[:used], rounded(ref, dt)) and (dx.val()[used:] == 77).all()
+        return
+    x, ys, gu, act = Buf(xv, dt, shift), Buf.out((n, rows), dt, shift), Buf.out((n, rows), dt, shift), Buf.out((n, rows // 2), dt, shift)
+    check(L.g53h_sorted_mm(ys.ptr, None, x.ptr, dt, 1, plan.c, w.ptr, rows, cols, 0.0))
+    check(L.g53h_sorted_mm(act.ptr, gu.ptr, x.ptr, dt, 1, plan.c, w.ptr, rows, cols, LIMIT))
+    ref = np.concatenate([xv[pair[of(e)]] @ wv[e].T for e in range(NE)])
+    assert np.array_equal(ys.val()[:used], rounded(ref, dt)) and np.array_equal(gu.val(), ys.val())
+    assert (ys.val()[used:] == 77).all() and (act.val()[used:] == 77).all()
+    with np.errstate(over="ignore"):
+        want = swiglu(ref, LIMIT)
+    g, u = np.split(ref, 2, 1)
+    # as in test_every_tile, and half a step of what the exponential is of, the gate by log2 e
+    deep = np.where(g < -87, 2.0 ** -126 * np.abs(g * np.clip(u, -LIMIT, LIMIT)), 0)
+    rel = 2.0 ** -20 + np.abs(np.minimum(g, 0)) * 2.0 ** -24
+    close(act.val()[:used], want, (rel + HALF[dt]) * np.abs(want) + TINY[dt] + deep)
