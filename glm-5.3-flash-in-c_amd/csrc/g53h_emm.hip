@@ -639,8 +639,10 @@ template <typename E, int OP> static int by_size(const G53EmArgs &a, long n)
     const long busy = a.NE < n ? a.NE : n, mean = busy ? (n + busy - 1) / busy : 0, cus = g53h_num_cus();
     const bool few = OP == G53_EM_MATS ? (long)a.NE * ((a.rows + 127) / 128) * ((a.cols + 127) / 128) < cus : mean <= 64;
     if constexpr (OP == G53_EM_ROWS) {      /* fewer still: a wave's part of a chunk is what takes time */
-        if (few && (n / 32 + busy) * ((a.cols + 127) / 128) < cus && (sizeof(E) == 4 || (at | odd) & 15))
-            return (at | odd) & 15 ? launch<E, OP, 1, 4, 2, 1, 2, false>(a, n) : launch<E, OP, 1, 4, 2, 1, sizeof(E) == 4 ? 4 : 2, true>(a, n);
+        if (few && (n / 32 + busy) * ((a.cols + 127) / 128) < cus) {
+            if ((at | odd) & 15) return launch<E, OP, 1, 4, 2, 1, 2, false>(a, n);
+            if constexpr (sizeof(E) == 4) return launch<E, OP, 1, 4, 2, 1, 4, true>(a, n);
+        }
     }
     if ((at | odd) & 15) return few ? launch<E, OP, 1, 4, 2, 2, 2, false>(a, n) : launch<E, OP, 2, 2, 4, 4, 2, false>(a, n);
     if constexpr (sizeof(E) == 4) {
