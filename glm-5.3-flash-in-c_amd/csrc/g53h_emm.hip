@@ -9,19 +9,22 @@
  * many rows an expert has. Operands stream through LDS (g53h_mmtile.h); products are v_mfma_f32_16x16x32 of bf16 or fp16 with
  * fp32 sums, the matrix's rows as the first operand, so that a lane holds four neighbours of a result's row. With 16 bits the
  * operands of a step of 32 leave LDS while those before it are multiplied. fp32 enters as three bf16 planes, six products
- * each: their rate is 6 to 1, and still above the fp32 matrix instructions' (2.4e14 against 1.45e14 a second at the rates of
- * a large library product); splitting takes vector work of about the products' time.
+ * each: at the rates of large library products 2.4e14 a second against 1.45e14 of the fp32 matrix instructions. Splitting takes
+ * vector work of about the products' time, and what is reached is no more than the latter: 1.4e14 by 2048 tokens.
  *
  * Measured (bf16 unless named; a 4 GiB copy moves 4.67 TB/s, a library product of 8192 cubed 1448 TFLOP/s in bf16 with both
  * operands along the summed dimension, 145 in fp32):
- *     8192 x 8192 by 8192 rows: forward 843 us, 1305 TFLOP/s, bound by power and LDS; rows 970, 1134; matrices 1250, 880
- *     gate/up 4096 x 4096 of one token's 8 of 288 experts, SwiGLU: 55.7 us, 4.8 TB/s, HBM
- *     the same by 4096 tokens, 8 of 64, gate and up kept: 1127 us, 976 TFLOP/s (rows of popular experts 2000, of others none:
- *     tiles partly empty, dies unevenly loaded at the end)
- *     gradients of 2048 such tokens, matrices in fp32: SwiGLU 68 us (4.9 TB/s), rows 745, matrices 1450; the last write 4.3 GB,
- *     which alone take 870, and sum some 400 rows each between: instructions of addresses and of the way out, 6 a product
- *     fp16 1001 x 1023, 301 tokens of 3 of 37 experts: 21 us, 3.7 TB/s, loads at odd addresses through registers
- *     fp32 2048 x 1024, 512 tokens of 4 of 16 experts: 91 us, 94 TFLOP/s, one round of tiles
+ *     8192 x 8192 by 8192 rows: forward 858 us, 1282 TFLOP/s, bound by power and LDS; rows 1005, 1094; matrices 1257, 875
+ *     gate/up 4096 x 4096 of one token's 8 of 288 experts, SwiGLU: 52 to 55 us, 4.9 to 5.2 TB/s, HBM
+ *     the same by 4096 tokens, 8 of 64, gate and up kept: 1137 to 1160 us, 950 to 967 TFLOP/s (rows of popular experts 2000, of
+ *     others none: tiles partly empty, dies unevenly loaded at the end)
+ *     gradients of 2048 such tokens, matrices in fp32: SwiGLU 65 us (5.2 TB/s), rows 752, matrices 1446; the last write 4.3 GB,
+ *     which alone take 870, and sum some 400 rows each between: instructions of addresses and of the way out, 5 beside a matrix
+ *     instruction. Added to what is there, element by element: 2679
+ *     fp16 1001 x 1023, 301 tokens of 3 of 37 experts (21 get rows): 21 us, 2.2 TB/s, loads at odd addresses through registers
+ *     fp32 2048 x 1024, 4 of 16 experts: 512 tokens 93 to 97 us, 89 to 93 TFLOP/s, one round of tiles, 27% of the matrix
+ *     instructions on rows that are not there; 2048 tokens 244 us, 141; one token 28 us, 64 workgroups
+ * The rows' gradient in tiles of 256 x 256 spills four registers, outside its loop.
  */
 #include <hip/hip_runtime.h>
 #include <type_traits>

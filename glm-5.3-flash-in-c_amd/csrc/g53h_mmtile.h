@@ -167,7 +167,7 @@ template <typename E> __device__ __forceinline__ g53_v4w g53_moved(const g53_v4w
 
 /* The 16-bit type of the products and the planes of a value. fp32 enters as three bf16 planes, each the rounded rest of
  * those before it: with 8 bits a plane and at most half a step left by each, the three hold every bit of the value
- * (above 2^-109; and values that round past bf16's largest, from 3.39e38, count as infinite). Of the nine products
+ * (above 2^-109; and values that round past bf16's largest, from 3.396e38, count as infinite). Of the nine products
  * of two values' planes six are taken. The planes of a value in [1, 2) are at most 2^-8 and 2^-17, so the others are below
  * 2^-24 of the values' product together, fp32's own rounding of one (2^-24.01 for 0x1.00ff8p0 by itself, 2^-28 in the mean of
  * random values, of either sign). */
@@ -394,9 +394,10 @@ __device__ __forceinline__ void g53_leave_sums(uint8_t *buf, void *out, long fir
     else all((O *)out);
 }
 
-/* The clamped SwiGLU, as g53h_swiglu's, for a result of type O. One of 16 bits, whose half step is 2^-9 at best, takes the
- * hardware's exponential and reciprocal (some 2^-20 off together): they take a quarter of the time, and at the end of a
- * tile nothing covers it. */
+/* The clamped SwiGLU, as g53h_swiglu's, for a result of type O. One of 16 bits, whose half step is 2^-11 of a value and more,
+ * takes the hardware's exponential and reciprocal: they take a quarter of the time, and at the end of a tile nothing covers it.
+ * Off by some 2^-20 together, and |gate| 2^-24 more where the gate is negative (its product with log2 e is rounded); 0 where the
+ * exponential lies below 2^-126, gates of -87.4 and less. */
 template <typename O> __device__ __forceinline__ float g53_swiglu1(float g, float u, float limit)
 {
     g = g > limit ? limit : g;

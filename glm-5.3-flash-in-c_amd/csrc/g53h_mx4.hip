@@ -7,11 +7,12 @@
  * Levels and scales go to v_mfma_scale_f32_16x16x128_f8f6f4 as they lie: lane (m, q) takes the 32 levels, 16 bytes, of
  * row m and block q of four, and their scale. Products and scales are exact; sums are fp32.
  *
- * Measured: 65536 x 4096 bf16 quantised in 112 us and read back in 129, 6.1 and 5.3 TB/s of what passes (a copy 4.67, a fill
- * 6.8); gate/up 4096 x 4096 of one token's 8 of 288 experts 15.7 to 18.7 us, 71 MB, HBM behind a launch and the search of a
- * row's expert; 65536 x 4096 by 5 rows 28.8 us, 4.9 TB/s; 8192 x 8192 by 8192 rows 324 us, 3400 TFLOP/s, and gate/up by 4096
- * tokens, 8 of 64 experts, 435 us, 2530: a chunk of 256 columns is 512 cycles of matrix instructions beside 32 to 48 KB on
- * their way to LDS, and waits for them are 40% of the waves' time (matrix instructions 42% of the CUs').
+ * Measured: 65536 x 4096 bf16 quantised in 114 us and read back in 129, 6.0 and 5.3 TB/s of what passes (a copy 4.67, a fill
+ * 6.8; one behind the other, as the cache holds it, 137 and 123); gate/up 4096 x 4096 of one token's 8 of 288 experts 15.0 to
+ * 18.6 us, 71 MB, HBM behind a launch and the search of a row's expert; 65536 x 4096 by 5 rows 28.6 us, 5.0 TB/s; 8192 x 8192
+ * by 8192 rows 331 us, 3320 TFLOP/s, and gate/up by 4096 tokens, 8 of 64 experts, 448 us, 2450: a chunk of 256 columns is 512
+ * cycles of matrix instructions beside 32 to 48 KB on their way to LDS, and waits are 33 and 41% of the waves' time (matrix
+ * instructions 44 and 28% of the CUs').
  */
 #include <hip/hip_runtime.h>
 #include <type_traits>

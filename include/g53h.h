@@ -424,7 +424,7 @@ int g53h_sorted_mm_w4(void *ys_d, const void *x_d, int dt, int gather, const G53
  * (rows / 2 each), ys [n][rows / 2] is their SwiGLU from the fp32 sums, and gu [n][rows], where it is not NULL, takes gate
  * and up, which the gradient needs; 0: ys [n][rows], gu NULL. Rows behind the last sorted one are left as they were, here and
  * below. Sums are fp32. fp32 values enter the matrix cores as three bf16 parts that hold them whole: products are good to
- * 2^-24, those of values below 2^-109 to less, and one that is not finite, or past 3.38e38, gives NaN.
+ * 2^-24, those of values below 2^-109 to less, and one that is not finite, or from 3.396e38 on, gives NaN.
  * _grad, of dys [n][rows] (with SwiGLU: of gate and up, see below): dx [n][cols], the gradient of the sorted rows of x
  * (g53h_sorted_dispatch_grad takes them to the tokens), and dw [n_experts][rows][cols] of type dw_dt (dt or G53H_F32), that
  * of the matrices, zeros where an expert has no rows; with add it is added to dw, in fp32, rounded once. Either may be
@@ -434,7 +434,7 @@ int g53h_sorted_mm(void *ys_d, void *gu_d, const void *x_d, int dt, int gather, 
 int g53h_sorted_mm_grad(void *dx_d, void *dw_d, int dw_dt, int add, const void *dys_d, const void *x_d, int dt, int gather,
                         const G53hSort *p, const void *w_d, int rows, int cols);
 /* The SwiGLU's gradient: dgu [n][2 inter] of dact [n][inter] and gu [n][2 inter] (dgu may be gu). Clamped values have none;
- * a value at its limit counts as inside. */
+ * a value at its limit counts as inside, and a gate of -inf, as fp16 keeps one of -65520 and less, gives zeros. */
 int g53h_sorted_swiglu_grad(void *dgu_d, const void *dact_d, const void *gu_d, int dt, int inter, const G53hSort *p,
                             float limit);
 
